@@ -147,7 +147,8 @@ void lava_hip_kernel_log_clear(void);
  *  LAVA_HIP_FAMILY_GEMM: 1 the 256 x 256 tile kernel, 2 the 64 x 64 small-product kernel
  *                        without a K split, 3 the staged kernel, 4 the 128 x 128 mid-size kernel
  *                        (f16 / bf16 / int8 / unsigned bytes, any operand layout; the fused
- *                        epilogue for f16 / bf16), not its K-split form.
+ *                        epilogue for f16 / bf16), not its K-split form;
+ *  LAVA_HIP_FAMILY_PAGED: attention over the paged cache: 1 the generic kernel.
  * Unknown families or choices return LAVA_HIP_ERR_INVALID_ARG. */
 /* Reads [src, src + bytes) once with 16-byte nontemporal loads, `unroll` (4, 8 or 16) in flight
  * per thread, `blocks` workgroups of 256 threads, and writes the XOR of what each thread read to
@@ -177,6 +178,7 @@ int lava_hip_mfma_loop(int op, const void* a, const void* b, size_t bytes, int b
 
 #define LAVA_HIP_FAMILY_ATTN 1
 #define LAVA_HIP_FAMILY_GEMM 2
+#define LAVA_HIP_FAMILY_PAGED 3
 int lava_hip_set_kernel_override(int family, int choice);
 
 /* ========================================================================= */
@@ -542,6 +544,106 @@ int lava_hip_gemm_w8a16_noalloc(const void* X, const void* W, const void* scale,
 int lava_hip_flash_attn_fwd_f16(const void* Q, const void* K, const void* V, void* O, int64_t B, int64_t H, int64_t S,
                                 int64_t D, const int64_t* strides, const int64_t* ostrides, float scale, int causal,
                                 void* stream);
+
+/* ========================================================================= */
+/* A paged key/value cache, and the attention of new tokens over it.          */
+/* No counterpart in the reference, whose attention takes whole (E, L, H, B)  */
+/* tensors (src/device/tensor_intrinsics.jl:279-281): the form of             */
+/* lava_hip_flash_attn_fwd_f16 for programs that generate tokens.             */
+/* ========================================================================= */
+
+/* Keys and values in pages of page_size tokens: element e of head h of token l of page p of either is at
+ * e + l * strides[1] + h * strides[2] + p * strides[3] (elements; strides[0] = 1), an (E, L, H, P) tensor.
+ * Offsets within a page are below 2^31 bytes, a page's own offset may pass 32 bits. */
+typedef struct lava_hip_kv_cache {
+    void* k;
+    void* v;
+    int32_t dtype;     /* LAVA_HIP_F16 or LAVA_HIP_BF16; Q, K, V and O of a call have it too */
+    int32_t head_dim;  /* E, 1 .. 256 */
+    int32_t page_size; /* tokens a page, >= 1 */
+    int32_t heads;     /* key (and value) heads */
+    int64_t pages;     /* pages in the cache, below 2^31 */
+    int64_t strides[4];
+} lava_hip_kv_cache;
+
+/* A ragged batch: the new tokens of sequence b are rows q_start[b] .. q_start[b + 1] - 1 of the (E, H, T)
+ * tensors of a call, and the last of its kv_len[b] tokens in the cache (those of this call included); its token
+ * j lies in page table[b * max_pages + j / page_size], row j % page_size.  q_start, kv_len and table are device
+ * memory and are read when the kernels run.  Nothing they hold makes a kernel read or write outside the
+ * buffers: row numbers are cut to [0, tokens], kv_len to [0, max_pages * page_size], and a page number outside
+ * [0, pages) is no page: its keys are masked, and nothing is written to it.  Rows behind the last
+ * sequence's are not written.  Sequences may have no new tokens, and no tokens at all. */
+typedef struct lava_hip_kv_batch {
+    int32_t sequences; /* B */
+    int32_t max_pages; /* entries of a sequence's row of the table */
+    int64_t tokens;    /* T, rows of the (E, H, T) tensors, below 2^31 */
+    int64_t max_q;     /* the most new tokens a sequence has, or 0 if unknown: chooses kernels, never results' validity */
+    const int32_t* q_start; /* B + 1 */
+    const int32_t* kv_len;  /* B */
+    const int32_t* table;   /* B rows of max_pages */
+    /* workspace of the attention calls, lava_hip_paged_workspace_bytes of it; NULL for the library's own of the
+     * stream (see lava_hip_gemm_w8a16).  Two graphs that may run at once need one each. */
+    void* workspace;
+    size_t workspace_bytes;
+} lava_hip_kv_batch;
+
+/* Rotary positions: pairs j < rot_dim / 2 of a head's elements -- (j, j + rot_dim / 2), or (2j, 2j + 1) if
+ * interleaved -- turn by position * inv_freq[j]: (x cos - y sin, y cos + x sin).  The angle is reduced to a turn in
+ * 64 bits, sine, cosine and the products are in 32, rounded once.  Elements from rot_dim on are copied. */
+typedef struct lava_hip_rope {
+    const float* inv_freq;    /* device, rot_dim / 2 */
+    int32_t rot_dim;          /* even, 0 .. head_dim */
+    int32_t interleaved;
+    const int32_t* positions; /* device, one per row of the batch; NULL: offset + place in the sequence */
+    int32_t offset;           /* added where positions is NULL (the length of a shared prefix) */
+} lava_hip_rope;
+
+/* Stores the new tokens' K and V, (E, H, T) tensors of element strides kv_strides = {1, head, token}, in the cache,
+ * K (and Q beside it) turned by `rope` (NULL: as they are).  Q may be NULL; else its q_heads heads (q_strides) go
+ * to Q_out (qo_strides), which may be Q itself with the same strides and otherwise does not overlap it.  K and V do
+ * not overlap the cache, and no two tokens of a call share a slot of it.  The reference's kernels have positions
+ * in none of their tensors; one launch. */
+int lava_hip_kv_append(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, const void* K, const void* V,
+                       const int64_t* kv_strides, const void* Q, void* Q_out, int64_t q_heads, const int64_t* q_strides,
+                       const int64_t* qo_strides, const lava_hip_rope* rope, void* stream);
+
+/* What becomes of a score s = scale * q.k of a query at position i and a key at position j:
+ *   cap > 0:  s = cap * tanh(s / cap);
+ *   slopes:   s -= slopes[query head] * |i - j|;
+ *   masked (no part of the softmax) unless j <= i (causal) or j < bidirectional[b], and, with window > 0,
+ *   only if j > i - window.
+ * A query that sees no key gives zeros and a log-sum-exp of -inf. */
+typedef struct lava_hip_attn_score {
+    float scale;
+    float cap;                    /* 0: none */
+    int32_t causal;
+    int32_t window;               /* 0: none */
+    const float* slopes;          /* device, q_heads, or NULL */
+    const int32_t* bidirectional; /* device, B: leading keys that every query of a sequence sees, or NULL (causal calls) */
+} lava_hip_attn_score;
+
+/* O = softmax(scores of Q with the cached keys) times the cached values, for the new tokens of every sequence:
+ * Q and O are (E, H, T) tensors of q_heads heads, a multiple of the cache's (query head h reads key head
+ * h / (q_heads / heads)).  lse (may be NULL) receives the natural logarithm of each row's sum of exp(score),
+ * lse[token * q_heads + head].  MFMA kernels take head dimensions that are a multiple of 8, pages of a multiple of 8 tokens, 16-byte
+ * aligned Q and cache with strides that are multiples of 8 and O aligned to 8 bytes with strides multiples of 4; a generic kernel
+ * the rest.  P is rounded once to the operands' type before the second product; sums are in 32 bits, in a fixed order. */
+int lava_hip_paged_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, const lava_hip_attn_score* score,
+                        const void* Q, void* O, int64_t q_heads, const int64_t* q_strides, const int64_t* o_strides,
+                        float* lse, void* stream);
+
+/* The same for sequences that all begin with the same prefix_len tokens, held once in the cache, in pages
+ * prefix_pages[0 .. ceil(prefix_len / page_size)) (device memory): the batch's kv_len and table are those of each sequence's own tokens,
+ * whose positions start at prefix_len.  The prefix is read once for many sequences' queries.
+ * `bidirectional` is not taken here. */
+int lava_hip_shared_prefix_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                                const lava_hip_attn_score* score, const int32_t* prefix_pages, int64_t prefix_len,
+                                const void* Q, void* O, int64_t q_heads, const int64_t* q_strides,
+                                const int64_t* o_strides, float* lse, void* stream);
+
+/* The workspace that a call with these descriptors (prefix_len 0: lava_hip_paged_attn) needs, 0 included. */
+int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, int64_t q_heads,
+                                   int64_t prefix_len, size_t* bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,261 @@
+// paged_attn.hip -- attention over the paged cache: checks, choice of kernel, and the generic kernel.
+//
+//  * paged_rows_kernel (paged_attn_rows.hip): rows of a sequence's queries and heads that share a key head,
+//    the work split evenly along the keys over the whole chip;
+//  * paged_any_kernel: any head dimension, page size, strides and alignment; one wavefront a query and head.
+#include "paged_attn.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace lava {
+
+int paged_check(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, PagedCache* c,
+                PagedBatch* b) {
+    LAVA_ARG(cache && batch, "%s: null descriptor", fn);
+    LAVA_REQUIRE(cache->dtype == LAVA_HIP_F16 || cache->dtype == LAVA_HIP_BF16, LAVA_HIP_ERR_UNSUPPORTED,
+                 "%s: the cache's dtype is %d, not f16 or bf16", fn, cache->dtype);
+    LAVA_ARG(cache->head_dim >= 1, "%s: head_dim = %d", fn, cache->head_dim);
+    LAVA_REQUIRE(cache->head_dim <= 256, LAVA_HIP_ERR_UNSUPPORTED, "%s: head_dim = %d > 256 is not supported", fn,
+                 cache->head_dim);
+    LAVA_ARG(cache->page_size >= 1 && cache->heads >= 1 && cache->heads <= 65535,
+             "%s: page_size = %d, heads = %d (at least 1; at most 65535 heads)", fn, cache->page_size, cache->heads);
+    LAVA_ARG(cache->pages >= 0 && cache->pages <= 0x7fffffff, "%s: pages = %lld", fn, (long long)cache->pages);
+    LAVA_ARG(batch->sequences >= 0 && batch->tokens >= 0 && batch->max_pages >= 0 && batch->max_q >= 0,
+             "%s: negative extent", fn);
+    LAVA_ARG(batch->tokens <= 0x7fffffff, "%s: tokens = %lld is too large", fn, (long long)batch->tokens);
+    LAVA_REQUIRE((int64_t)batch->max_pages * cache->page_size <= 0x40000000, LAVA_HIP_ERR_UNSUPPORTED,
+                 "%s: a sequence of up to %lld tokens (max_pages * page_size) is longer than 2^30", fn,
+                 (long long)batch->max_pages * cache->page_size);
+    const int64_t* st = cache->strides;
+    LAVA_ARG(st[0] == 1, "%s: the head dimension (E) of the cache must be contiguous", fn);
+    const int64_t extent[4] = {cache->head_dim, cache->page_size, cache->heads, cache->pages};
+    for (int i = 1; i < 4; ++i) {
+        LAVA_ARG(st[i] >= 0 && st[i] <= ((int64_t)1 << 40), "%s: cache stride %d is %lld", fn, i, (long long)st[i]);
+        LAVA_ARG(extent[i] <= 1 || st[i] >= cache->head_dim, "%s: cache stride %d smaller than head_dim", fn, i);
+    }
+    const int64_t span = (cache->page_size - 1) * st[1] + (cache->heads - 1) * st[2] + cache->head_dim;
+    LAVA_REQUIRE(st[1] <= 0x3fffffff && st[2] <= 0x3fffffff && span <= 0x3fffffff, LAVA_HIP_ERR_UNSUPPORTED,
+                 "%s: a page spans 2^31 bytes or more", fn);
+    *c = {cache->k, cache->v, st[1], st[2], st[3], cache->head_dim, cache->page_size, cache->heads,
+          (int)cache->pages, fast_div((uint32_t)cache->page_size)};
+    *b = {batch->q_start, batch->kv_len, batch->table, batch->sequences, batch->max_pages, (int)batch->tokens,
+          batch->max_pages * cache->page_size};
+    if (batch->sequences == 0 || batch->tokens == 0) return LAVA_HIP_OK;
+    LAVA_ARG(batch->q_start && batch->kv_len && (batch->table || batch->max_pages == 0), "%s: null pointer in the batch", fn);
+    LAVA_ARG((cache->k && cache->v) || cache->pages == 0, "%s: null pointer in the cache", fn);
+    LAVA_ARG(aligned(batch->q_start, 4) && aligned(batch->kv_len, 4) && aligned(batch->table, 4) && aligned(cache->k, 2) &&
+             aligned(cache->v, 2), "%s: misaligned", fn);
+    return LAVA_HIP_OK;
+}
+
+int paged_check_strides(const char* fn, const char* what, const int64_t* st, int64_t D, int64_t heads, int64_t tokens) {
+    LAVA_ARG(st[0] == 1, "%s: %s: the head dimension (E) must be contiguous", fn, what);
+    for (int i = 1; i < 3; ++i) {
+        LAVA_ARG(st[i] >= 0 && st[i] <= ((int64_t)1 << 40), "%s: %s: stride %d is %lld", fn, what, i, (long long)st[i]);
+        LAVA_ARG((i == 1 ? heads : tokens) <= 1 || st[i] >= D, "%s: %s: stride %d smaller than head_dim", fn, what, i);
+    }
+    return LAVA_HIP_OK;
+}
+
+int paged_check_device(const char* fn, const void* ptr, void* stream) {
+    static const int devices = [] {
+        int n = 0;
+        return hipGetDeviceCount(&n) == hipSuccess ? n : 1;
+    }();
+    if (devices <= 1) return LAVA_HIP_OK;
+    int cur = 0;
+    LAVA_HIP_TRY(hipGetDevice(&cur));
+    if (stream) {
+        hipDevice_t dev = 0;
+        LAVA_HIP_TRY(hipStreamGetDevice(as_stream(stream), &dev));
+        LAVA_ARG(dev == cur, "%s: the stream belongs to device %d, the current device is %d", fn, (int)dev, cur);
+    }
+    hipPointerAttribute_t at;
+    if (ptr && hipPointerGetAttributes(&at, ptr) == hipSuccess)
+        LAVA_ARG(at.device == cur, "%s: the cache is on device %d, the current device is %d", fn, at.device, cur);
+    else
+        (void)hipGetLastError();
+    return LAVA_HIP_OK;
+}
+
+// One wavefront a row (query and head): 64 keys at a time, a key a lane for the scores, then the head dimension over
+// the lanes for the sums.  Masked keys are not read at all.
+template <typename T>
+__global__ void __launch_bounds__(64) paged_any_kernel(PaParams p) {
+    __shared__ float q[256];
+    __shared__ float w[64];
+    __shared__ int64_t at[64];
+    const int lane = threadIdx.x;
+    const int t = (int)(blockIdx.x / (unsigned)p.Hq), h = (int)(blockIdx.x % (unsigned)p.Hq), D = p.c.D;
+    const int b = paged_find(p.b, t, lane);
+    if (b >= p.b.B) return;
+    const PagedSeq s = paged_seq(p.b, b);
+    if (t < s.first || t >= s.first + s.n) return;
+    const int end = p.P + s.kv, pos = end - s.n + (t - s.first), bid = p.bidir ? p.bidir[b] : 0;
+    const PaRange r = pa_range(p, pos, end, bid);
+    const float slope = p.slopes ? p.slopes[h] * PA_LOG2E : 0.f;
+    const T* qr = (const T*)p.Q + (int64_t)t * p.qst + (int64_t)h * p.qsh;
+    for (int e = lane; e < D; e += 64) q[e] = (float)qr[e];
+    __syncthreads();
+    const int64_t head = (int64_t)(h / p.G) * p.c.sh;
+    float acc[4] = {}, m = -INFINITY, l = 0.f;
+    for (int j0 = r.lo; j0 <= r.hi; j0 += 64) {
+        const int j = j0 + lane;
+        bool keep = j <= r.hi;
+        int64_t o = 0;
+        float x = -INFINITY;
+        if (keep) {
+            const int k = j < p.P ? j : j - p.P;
+            const int page_no = (int)div_of((uint32_t)k, p.c.by_page);
+            const int page = j < p.P ? p.ppages[page_no] : p.b.table[(int64_t)b * p.b.max_pages + page_no];
+            keep = page >= 0 && page < p.c.pages;
+            if (keep) {
+                o = (int64_t)page * p.c.sp + (int64_t)(k - page_no * p.c.page) * p.c.sl + head;
+                const T* kr = (const T*)p.c.k + o;
+                float d = 0.f;
+                for (int e = 0; e < D; ++e) d = fmaf(q[e], (float)kr[e], d);
+                x = pa_score(d, p.mul, p.cap2) - slope * fabsf((float)(pos - j));
+            }
+        }
+        uint64_t live = __builtin_amdgcn_ballot_w64(keep);
+        float top = x;
+        for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i, 64));
+        const float mn = fmaxf(m, top), sub = mn == -INFINITY ? 0.f : mn;
+        const float alpha = __builtin_amdgcn_exp2f(m - sub);   // m = -inf: 0
+        const float e1 = keep ? __builtin_amdgcn_exp2f(x - sub) : 0.f;
+        __syncthreads();   // the round before has read w and at
+        w[lane] = e1;
+        at[lane] = o;
+        __syncthreads();
+        float sum = e1;
+        for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i, 64);
+        l = l * alpha + sum;
+        m = mn;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] *= alpha;
+        for (; live; live &= live - 1) {
+            const int i = __builtin_ctzll(live);
+            const T* vr = (const T*)p.c.v + at[i];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (lane + 64 * u < D) acc[u] = fmaf(w[i], (float)vr[lane + 64 * u], acc[u]);
+        }
+    }
+    T* orow = (T*)p.O + (int64_t)t * p.ost + (int64_t)h * p.osh;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (lane + 64 * u < D) orow[lane + 64 * u] = (T)(acc[u] * inv);
+    if (p.lse && lane == 0) p.lse[(int64_t)t * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * PA_LN2;
+}
+
+// What both attention entry points check and fill in.  *done: there is nothing to compute.
+static int pa_prepare(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                      const lava_hip_attn_score* score, int64_t q_heads, PaParams* p, bool* done) {
+    *done = true;
+    int rc = paged_check(fn, cache, batch, &p->c, &p->b);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_ARG(q_heads >= 0 && q_heads <= 65535, "%s: q_heads = %lld is outside [0, 65535]", fn, (long long)q_heads);
+    LAVA_ARG(q_heads % p->c.heads == 0, "%s: %lld query heads are not a multiple of the cache's %d", fn,
+             (long long)q_heads, p->c.heads);
+    if (score) {
+        LAVA_ARG(std::isfinite(score->scale) && std::isfinite(score->cap), "%s: scale or cap is not finite", fn);
+        LAVA_ARG(score->cap >= 0.f, "%s: cap = %g is negative", fn, score->cap);
+        LAVA_ARG(score->window >= 0, "%s: window = %d is negative", fn, score->window);
+        LAVA_ARG(aligned(score->slopes, 4) && aligned(score->bidirectional, 4), "%s: slopes or bidirectional misaligned", fn);
+        LAVA_ARG(!score->bidirectional || score->causal, "%s: bidirectional keys need a causal call", fn);
+        p->cap2 = score->cap * PA_LOG2E;
+        p->mul = score->cap > 0.f ? (float)(2.0 * score->scale / score->cap * 1.4426950408889634) : (float)(score->scale * 1.4426950408889634);
+        LAVA_ARG(std::isfinite(p->mul), "%s: scale / cap overflows", fn);
+        p->causal = score->causal != 0;
+        p->window = score->window;
+        p->slopes = score->slopes;
+        p->bidir = score->bidirectional;
+    }
+    p->Hq = (int)q_heads;
+    p->G = (int)(q_heads / p->c.heads);
+    if (p->b.T == 0 || p->b.B == 0 || q_heads == 0) return LAVA_HIP_OK;
+    p->by_g = fast_div((uint32_t)p->G);
+    *done = false;
+    return LAVA_HIP_OK;
+}
+
+// Rows (queries times heads of a key head) that a sequence has at most, as far as the host knows.
+static int64_t pa_max_rows(const PaParams& p, const lava_hip_kv_batch* batch) {
+    const int64_t q = batch->max_q > 0 && batch->max_q < p.b.T ? batch->max_q : p.b.T;
+    return q * p.G;
+}
+
+static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                   const lava_hip_attn_score* score, const int32_t* ppages, int64_t prefix, const void* Q, void* O,
+                   int64_t q_heads, const int64_t* q_strides, const int64_t* o_strides, float* lse, void* stream) {
+    PaParams p = {};
+    bool done;
+    LAVA_ARG(score, "%s: null score", fn);
+    int rc = pa_prepare(fn, cache, batch, score, q_heads, &p, &done);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_ARG(prefix >= 0, "%s: prefix_len is negative", fn);
+    LAVA_REQUIRE(prefix <= 0x3fffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s: prefix_len = %lld is longer than 2^30", fn,
+                 (long long)prefix);
+    if (done) return LAVA_HIP_OK;
+    LAVA_ARG(Q && O && q_strides && o_strides && (ppages || prefix == 0), "%s: null pointer", fn);
+    LAVA_ARG(aligned(Q, 2) && aligned(O, 2) && aligned(lse, 4) && aligned(ppages, 4), "%s: misaligned", fn);
+    rc = paged_check_strides(fn, "q_strides", q_strides, p.c.D, q_heads, p.b.T);
+    if (rc == LAVA_HIP_OK) rc = paged_check_strides(fn, "o_strides", o_strides, p.c.D, q_heads, p.b.T);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_REQUIRE((int64_t)p.b.T * q_heads <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED,
+                 "%s: %lld rows (tokens * q_heads) are 2^31 or more", fn, (long long)p.b.T * q_heads);
+    rc = lava_hip_init();
+    if (rc != LAVA_HIP_OK) return rc;
+    rc = paged_check_device(fn, p.c.k, stream);
+    if (rc != LAVA_HIP_OK) return rc;
+    p.Q = Q;
+    p.O = O;
+    p.lse = lse;
+    p.qsh = q_strides[1];
+    p.qst = q_strides[2];
+    p.osh = o_strides[1];
+    p.ost = o_strides[2];
+    p.ppages = ppages;
+    p.P = (int)prefix;
+    hipStream_t s = as_stream(stream);
+    if (cache->dtype == LAVA_HIP_F16)
+        hipLaunchKernelGGL((paged_any_kernel<f16>), dim3((unsigned)(p.b.T * p.Hq)), dim3(64), 0, s, p);
+    else
+        hipLaunchKernelGGL((paged_any_kernel<bf16>), dim3((unsigned)(p.b.T * p.Hq)), dim3(64), 0, s, p);
+    LAVA_LAUNCH_CHECK("paged_any_kernel");
+    return LAVA_HIP_OK;
+}
+
+}  // namespace lava
+
+using namespace lava;
+
+extern "C" int lava_hip_paged_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                                   const lava_hip_attn_score* score, const void* Q, void* O, int64_t q_heads,
+                                   const int64_t* q_strides, const int64_t* o_strides, float* lse, void* stream) {
+    return pa_attn("paged_attn", cache, batch, score, nullptr, 0, Q, O, q_heads, q_strides, o_strides, lse, stream);
+}
+
+extern "C" int lava_hip_shared_prefix_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                                           const lava_hip_attn_score* score, const int32_t* prefix_pages,
+                                           int64_t prefix_len, const void* Q, void* O, int64_t q_heads,
+                                           const int64_t* q_strides, const int64_t* o_strides, float* lse, void* stream) {
+    LAVA_REQUIRE(!score || !score->bidirectional, LAVA_HIP_ERR_UNSUPPORTED,
+                 "shared_prefix_attn: bidirectional keys are not taken with a shared prefix");
+    return pa_attn("shared_prefix_attn", cache, batch, score, prefix_pages, prefix_len, Q, O, q_heads, q_strides,
+                   o_strides, lse, stream);
+}
+
+extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
+                                              int64_t q_heads, int64_t prefix_len, size_t* bytes) {
+    PaParams p = {};
+    bool done;
+    LAVA_ARG(bytes, "paged_workspace_bytes: null pointer");
+    LAVA_ARG(prefix_len >= 0, "paged_workspace_bytes: prefix_len is negative");
+    const int rc = pa_prepare("paged_workspace_bytes", cache, batch, nullptr, q_heads, &p, &done);
+    if (rc != LAVA_HIP_OK) return rc;
+    *bytes = 0;
+    return LAVA_HIP_OK;
+}

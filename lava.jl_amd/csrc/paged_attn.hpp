@@ -1,0 +1,65 @@
+// paged_attn.hpp -- what the attention kernels over the paged cache share (internal).
+//
+// A query at position i and a key at position j score s = scale q.k, capped (cap tanh(s / cap)), less
+// slope |i - j|, and are kept for j in one interval [lo, hi] of the query's: causal, window, bidirectional
+// prefix and the sequence's end all narrow it, so every kernel masks by one comparison of a row's own
+// two bounds.  Scores are in base 2 throughout (times log2 e).
+//
+// A sequence's keys come from up to two sources: the batch's shared prefix (positions 0 .. P - 1) and its own
+// pages (positions P ..).
+#pragma once
+#include "paged.hpp"
+
+namespace lava {
+
+struct PaParams {
+    PagedCache c;
+    PagedBatch b;
+    const void* Q;
+    void* O;
+    float* lse;
+    int64_t qsh, qst, osh, ost;   // head and token strides
+    int Hq, G;                    // query heads, those of a key head
+    FastDiv by_g;
+    float mul;                    // scores to base 2; with a cap to 2 log2(e) s / cap
+    float cap2;                   // cap log2(e), or 0
+    int causal, window;
+    const float* slopes;
+    const int* bidir;
+    const int* ppages;            // the shared prefix's pages
+    int P;                        // its length, 0: none
+    // the row kernel (paged_attn_rows.hip)
+    int stack;                    // the prefix is attended once, by the rows of many sequences together
+    int row_limit;                // sequences of more rows (new tokens times G) are another kernel's
+    int part;                     // rows of a partial result in the workspace
+    float* ws_o;                  // partial sums [workgroup][2][part][DP], their (m, l)
+    float2* ws_ml;
+    float* row_o;                 // stack: a row's whole results [prefix, own][T * Hq][DP]
+    float2* row_ml;
+};
+
+struct PaRange {
+    int lo, hi;   // positions of the keys a query sees
+};
+// A query at position pos of a sequence whose last key is at end - 1.
+__device__ __forceinline__ PaRange pa_range(const PaParams& p, int pos, int end, int bid) {
+    const int hi = p.causal ? min(max(pos, bid - 1), end - 1) : end - 1;
+    return {p.window > 0 ? max(0, pos - p.window + 1) : 0, hi};
+}
+
+// The score in base 2 from the product q.k.
+__device__ __forceinline__ float pa_score(float s, float mul, float cap2) {
+    const float x = s * mul;
+    if (cap2 == 0.f) return x;
+    // cap tanh(z) = cap (1 - 2 / (1 + e^2z)), with x = 2 z log2 e: +-cap where e^2z leaves the range
+    return fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap2);
+}
+
+constexpr float PA_LN2 = 0.69314718055994530942f;
+constexpr float PA_LOG2E = 1.44269504088896340736f;
+
+int paged_rows_launch(PaParams& p, int dtype, int max_rows, hipStream_t s, void* stream, void* workspace,
+                      size_t workspace_bytes);
+size_t paged_rows_workspace(const PaParams& p, int max_rows);
+
+}  // namespace lava

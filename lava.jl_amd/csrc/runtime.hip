@@ -76,10 +76,10 @@ int check_launch(const char* kernel) {
 }
 
 // Kernel choices pinned by lava_hip_set_kernel_override, per family (0 = automatic).
-static std::atomic<int> g_override[3];
+static std::atomic<int> g_override[4];
 
 int kernel_override(int family) {
-    return family > 0 && family < 3 ? g_override[family].load(std::memory_order_relaxed) : 0;
+    return family > 0 && family < 4 ? g_override[family].load(std::memory_order_relaxed) : 0;
 }
 
 __global__ void fill_bytes_kernel(uint8_t* __restrict__ dst, uint8_t value, size_t n) {
@@ -226,7 +226,8 @@ void lava_hip_kernel_log_clear(void) { g_klaunched = 0; }
 
 int lava_hip_set_kernel_override(int family, int choice) {
     const bool ok = (family == LAVA_HIP_FAMILY_ATTN && (choice == 0 || choice == 3 || choice == 5)) ||
-                    (family == LAVA_HIP_FAMILY_GEMM && choice >= 0 && choice <= 4);
+                    (family == LAVA_HIP_FAMILY_GEMM && choice >= 0 && choice <= 4) ||
+                    (family == LAVA_HIP_FAMILY_PAGED && choice >= 0 && choice <= 1);
     LAVA_ARG(ok, "set_kernel_override: unknown family %d or choice %d", family, choice);
     g_override[family].store(choice, std::memory_order_relaxed);
     return LAVA_HIP_OK;

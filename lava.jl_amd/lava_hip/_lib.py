@@ -56,6 +56,31 @@ u32 = C.c_uint32
 u64 = C.c_uint64
 ci = C.c_int
 
+
+class KVCacheDesc(C.Structure):
+    """lava_hip_kv_cache."""
+    _fields_ = [("k", vp), ("v", vp), ("dtype", C.c_int32), ("head_dim", C.c_int32), ("page_size", C.c_int32),
+                ("heads", C.c_int32), ("pages", i64), ("strides", i64 * 4)]
+
+
+class KVBatchDesc(C.Structure):
+    """lava_hip_kv_batch."""
+    _fields_ = [("sequences", C.c_int32), ("max_pages", C.c_int32), ("tokens", i64), ("max_q", i64), ("q_start", vp),
+                ("kv_len", vp), ("table", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
+class RopeDesc(C.Structure):
+    """lava_hip_rope."""
+    _fields_ = [("inv_freq", vp), ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("positions", vp),
+                ("offset", C.c_int32)]
+
+
+class AttnScoreDesc(C.Structure):
+    """lava_hip_attn_score."""
+    _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int32), ("window", C.c_int32), ("slopes", vp),
+                ("bidirectional", vp)]
+
+
 # name -> (restype, argtypes)
 PROTOTYPES: dict[str, tuple] = {
     "lava_hip_init": (ci, []),
@@ -112,6 +137,14 @@ PROTOTYPES: dict[str, tuple] = {
     "lava_hip_gemm_w8a16_noalloc": (ci, [vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, u32, vp]),
     "lava_hip_flash_attn_fwd_f16": (ci, [vp, vp, vp, vp, i64, i64, i64, i64, C.POINTER(i64),
                                          C.POINTER(i64), C.c_float, ci, vp]),
+    "lava_hip_kv_append": (ci, [C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), vp, vp, C.POINTER(i64), vp, vp, i64,
+                                C.POINTER(i64), C.POINTER(i64), C.POINTER(RopeDesc), vp]),
+    "lava_hip_paged_attn": (ci, [C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), C.POINTER(AttnScoreDesc), vp, vp, i64,
+                                 C.POINTER(i64), C.POINTER(i64), vp, vp]),
+    "lava_hip_shared_prefix_attn": (ci, [C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), C.POINTER(AttnScoreDesc), vp,
+                                         i64, vp, vp, i64, C.POINTER(i64), C.POINTER(i64), vp, vp]),
+    "lava_hip_paged_workspace_bytes": (ci, [C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), i64, i64,
+                                            C.POINTER(C.c_size_t)]),
     "lava_hip_release_workspaces": (ci, []),
     "lava_hip_read_stream": (ci, [vp, C.c_size_t, vp, ci, ci, vp]),
     "lava_hip_mfma_loop": (ci, [ci, vp, vp, C.c_size_t, ci, ci, ci, vp, vp]),
@@ -125,7 +158,7 @@ PROTOTYPES: dict[str, tuple] = {
 }
 
 # kernel families of lava_hip_set_kernel_override
-FAMILY_ATTN, FAMILY_GEMM = 1, 2
+FAMILY_ATTN, FAMILY_GEMM, FAMILY_PAGED = 1, 2, 3
 
 _lib: C.CDLL | None = None
 
