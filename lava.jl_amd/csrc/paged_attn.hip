@@ -187,6 +187,18 @@ static int64_t pa_max_rows(const PaParams& p, const lava_hip_kv_batch* batch) {
     return q * p.G;
 }
 
+// Whether the cache allows 16-byte reads of 8 keys in one page.
+static bool pa_vectors(const PaParams& p) {
+    return p.c.D % 8 == 0 && p.c.page % 8 == 0 && p.c.sl % 8 == 0 && p.c.sh % 8 == 0 && p.c.sp % 8 == 0 &&
+           aligned(p.c.k, 16) && aligned(p.c.v, 16);
+}
+
+// What depends on the batch's size and the prefix alone.
+static void pa_plan(PaParams* p) {
+    p->stack = p->P > 0;
+    p->row_limit = 0x7fffffff;
+}
+
 static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
                    const lava_hip_attn_score* score, const int32_t* ppages, int64_t prefix, const void* Q, void* O,
                    int64_t q_heads, const int64_t* q_strides, const int64_t* o_strides, float* lse, void* stream) {
@@ -220,6 +232,22 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.ppages = ppages;
     p.P = (int)prefix;
     hipStream_t s = as_stream(stream);
+    const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
+    pa_plan(&p);
+    bool fast = pin != 1 && paged_rows_fits(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
+    for (int i = 1; i < 3; ++i) fast = fast && q_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
+    if (fast) {
+        const int64_t rows = pa_max_rows(p, batch);
+        const size_t bytes = paged_rows_workspace(p, rows);
+        if (batch->workspace) {
+            LAVA_ARG(batch->workspace_bytes >= bytes, "%s: the workspace of %zu bytes is smaller than the %zu this call needs",
+                     fn, batch->workspace_bytes, bytes);
+            return paged_rows_launch(p, cache->dtype, rows, batch->workspace, s);
+        }
+        return with_stream_workspace(bytes + STREAM_WS_RESERVED, stream, [&](void* ws) {
+            return paged_rows_launch(p, cache->dtype, rows, (uint8_t*)ws + STREAM_WS_RESERVED, s);
+        });
+    }
     if (cache->dtype == LAVA_HIP_F16)
         hipLaunchKernelGGL((paged_any_kernel<f16>), dim3((unsigned)(p.b.T * p.Hq)), dim3(64), 0, s, p);
     else
@@ -257,5 +285,9 @@ extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, co
     const int rc = pa_prepare("paged_workspace_bytes", cache, batch, nullptr, q_heads, &p, &done);
     if (rc != LAVA_HIP_OK) return rc;
     *bytes = 0;
+    if (done) return LAVA_HIP_OK;
+    p.P = (int)std::min<int64_t>(prefix_len, 0x3fffffff);
+    pa_plan(&p);
+    if (pa_vectors(p) && paged_rows_fits(p)) *bytes = paged_rows_workspace(p, pa_max_rows(p, batch));
     return LAVA_HIP_OK;
 }

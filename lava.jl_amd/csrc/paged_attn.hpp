@@ -31,8 +31,7 @@ struct PaParams {
     // the row kernel (paged_attn_rows.hip)
     int stack;                    // the prefix is attended once, by the rows of many sequences together
     int row_limit;                // sequences of more rows (new tokens times G) are another kernel's
-    int part;                     // rows of a partial result in the workspace
-    float* ws_o;                  // partial sums [workgroup][2][part][DP], their (m, l)
+    float* ws_o;                  // partial sums [workgroup][2][rows of a tile][DP], their (m, l)
     float2* ws_ml;
     float* row_o;                 // stack: a row's whole results [prefix, own][T * Hq][DP]
     float2* row_ml;
@@ -58,8 +57,10 @@ __device__ __forceinline__ float pa_score(float s, float mul, float cap2) {
 constexpr float PA_LN2 = 0.69314718055994530942f;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
-int paged_rows_launch(PaParams& p, int dtype, int max_rows, hipStream_t s, void* stream, void* workspace,
-                      size_t workspace_bytes);
-size_t paged_rows_workspace(const PaParams& p, int max_rows);
+// The row kernel: whether it can count the call's work, the workspace it needs, the launch.  max_rows: rows of
+// a sequence at most, as far as the host knows.
+bool paged_rows_fits(const PaParams& p);
+size_t paged_rows_workspace(const PaParams& p, int64_t max_rows);
+int paged_rows_launch(PaParams& p, int dtype, int64_t max_rows, void* ws, hipStream_t s);
 
 }  // namespace lava

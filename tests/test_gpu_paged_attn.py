@@ -7,7 +7,7 @@ from paged_reference import Case, bad, to_f64
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = {1: "paged_any_kernel"}
+KERNELS = {1: "paged_any_kernel", 2: "paged_rows_kernel"}
 
 
 class Device:
@@ -121,6 +121,14 @@ CASES = {
     "shared_own_empty": dict(lens=((1, 0), (1, 1), (2, 0)), prefix=77, Hq=4, Hkv=2, D=64),
     "shared_long_rows": dict(lens=((90, 90), (1, 4), (17, 30)), prefix=133, Hq=4, Hkv=2, D=128, order="lh"),
     "shared_all_keys": dict(lens=((9, 12), (1, 4)), prefix=70, causal=False, D=256, Hq=2, Hkv=1),
+    # more blocks of work than workgroups: parts of several blocks, sequences that share a workgroup and that are split
+    "split_uneven": dict(lens=tuple((1, 1 + (i * 397) % 1900) for i in range(48)), Hq=16, Hkv=8, D=128),
+    "split_uneven_d64": dict(lens=tuple((1 + i % 3, 4 + (i * 397) % 1900) for i in range(48)), Hq=32, Hkv=16, D=64,
+                             dtype="bf16", page=40),
+    "split_wide": dict(lens=tuple((9, 9 + (i * 397) % 1500) for i in range(24)), Hq=48, Hkv=8, D=128, window=700),
+    "split_shared": dict(lens=tuple((1, 1 + (i * 97) % 300) for i in range(60)), prefix=1999, Hq=32, Hkv=8, D=128),
+    "split_shared_window": dict(lens=tuple((1 + i % 2, 2 + (i * 97) % 300) for i in range(60)), prefix=1999, window=1200,
+                                Hq=32, Hkv=8, D=64, dtype="bf16", slopes=True),
     "many": dict(lens=tuple((1 if i % 5 else 2, 2 + i % 37) for i in range(150)), Hq=2, Hkv=1, D=64),
 }
 
