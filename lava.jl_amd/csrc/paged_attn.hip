@@ -187,6 +187,9 @@ static int64_t pa_max_rows(const PaParams& p, const lava_hip_kv_batch* batch) {
     return q * p.G;
 }
 
+// Sequences of more rows (new tokens times the query heads of a key head) run on the tile kernel.
+constexpr int PA_TILE_ROWS = 64;
+
 // Whether the cache allows 16-byte reads of 8 keys in one page.
 static bool pa_vectors(const PaParams& p) {
     return p.c.D % 8 == 0 && p.c.page % 8 == 0 && p.c.sl % 8 == 0 && p.c.sh % 8 == 0 && p.c.sp % 8 == 0 &&
@@ -194,9 +197,11 @@ static bool pa_vectors(const PaParams& p) {
 }
 
 // What depends on the batch's size and the prefix alone.
-static void pa_plan(PaParams* p) {
-    p->stack = p->P > 0;
-    p->row_limit = 0x7fffffff;
+static void pa_plan(PaParams* p, int64_t max_rows) {
+    const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
+    p->tiles = p->c.D <= 128 && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS));
+    p->row_limit = !p->tiles ? 0x7fffffff : pin == 3 ? 0 : PA_TILE_ROWS;
+    p->stack = p->P > 0 && pin != 3;
 }
 
 static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
@@ -233,11 +238,16 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.P = (int)prefix;
     hipStream_t s = as_stream(stream);
     const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
-    pa_plan(&p);
+    pa_plan(&p, pa_max_rows(p, batch));
     bool fast = pin != 1 && paged_rows_fits(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
     for (int i = 1; i < 3; ++i) fast = fast && q_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
     if (fast) {
-        const int64_t rows = pa_max_rows(p, batch);
+        int64_t rows = pa_max_rows(p, batch);
+        if (p.tiles) {
+            rc = paged_tile_launch(p, cache->dtype, s);
+            if (rc != LAVA_HIP_OK) return rc;
+            rows = std::min<int64_t>(rows, p.row_limit);
+        }
         const size_t bytes = paged_rows_workspace(p, rows);
         if (batch->workspace) {
             LAVA_ARG(batch->workspace_bytes >= bytes, "%s: the workspace of %zu bytes is smaller than the %zu this call needs",
@@ -287,7 +297,7 @@ extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, co
     *bytes = 0;
     if (done) return LAVA_HIP_OK;
     p.P = (int)std::min<int64_t>(prefix_len, 0x3fffffff);
-    pa_plan(&p);
-    if (pa_vectors(p) && paged_rows_fits(p)) *bytes = paged_rows_workspace(p, pa_max_rows(p, batch));
+    pa_plan(&p, pa_max_rows(p, batch));
+    if (pa_vectors(p) && paged_rows_fits(p)) *bytes = paged_rows_workspace(p, std::min<int64_t>(pa_max_rows(p, batch), p.row_limit));
     return LAVA_HIP_OK;
 }

@@ -29,8 +29,9 @@ struct PaParams {
     const int* ppages;            // the shared prefix's pages
     int P;                        // its length, 0: none
     // the row kernel (paged_attn_rows.hip)
+    int tiles;                    // the tile kernel takes sequences of more than row_limit rows
     int stack;                    // the prefix is attended once, by the rows of many sequences together
-    int row_limit;                // sequences of more rows (new tokens times G) are another kernel's
+    int row_limit;                // sequences of more rows (new tokens times G) are the tile kernel's
     float* ws_o;                  // partial sums [workgroup][2][rows of a tile][DP], their (m, l)
     float2* ws_ml;
     float* row_o;                 // stack: a row's whole results [prefix, own][T * Hq][DP]
@@ -62,5 +63,7 @@ constexpr float PA_LOG2E = 1.44269504088896340736f;
 bool paged_rows_fits(const PaParams& p);
 size_t paged_rows_workspace(const PaParams& p, int64_t max_rows);
 int paged_rows_launch(PaParams& p, int dtype, int64_t max_rows, void* ws, hipStream_t s);
+// The tile kernel: sequences of more than row_limit rows, head dimensions up to 128; no workspace.
+int paged_tile_launch(const PaParams& p, int dtype, hipStream_t s);
 
 }  // namespace lava

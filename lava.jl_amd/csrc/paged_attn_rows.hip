@@ -21,26 +21,12 @@
 #include <algorithm>
 
 #include "lds_dma.hpp"
+#include "paged_types.hpp"
 
 namespace lava {
 
 constexpr int PR_BK = 128;      // keys of a block, 32 a wavefront
 constexpr float PR_RESCALE = 8.f;   // the maximum moves when a score exceeds it by more than this: P <= 2^8
-
-template <typename T>
-struct PrType;
-template <>
-struct PrType<f16> {
-    typedef f16x8 v8;
-    typedef f16x4 v4;
-    __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-};
-template <>
-struct PrType<bf16> {
-    typedef bf16x8 v8;
-    typedef bf16x4 v4;
-    __device__ static f32x4 mma(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-};
 
 // ---- the plan -------------------------------------------------------------------------
 
@@ -154,8 +140,6 @@ __device__ __forceinline__ uint32_t pr_per(uint32_t total) { return max(1u, (tot
 
 // ---- the kernel -----------------------------------------------------------------------
 
-typedef const __attribute__((address_space(4))) int* pr_table;
-
 template <int N>
 __device__ __forceinline__ void pr_wait() {
     static_assert(N >= 0 && N < 64, "vmcnt");
@@ -170,13 +154,12 @@ __device__ __forceinline__ float pr_max4(float x) {   // over the four lanes of 
 // DP: the head dimension rounded up to 64, 128 or 256; a tile is 16 NR rows.
 template <typename T, int DP, int NR>
 __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_rows_kernel(PaParams p) {
-    typedef PrType<T> TT;
+    typedef PgType<T> TT;
     typedef typename TT::v8 v8;
     typedef typename TT::v4 v4;
     typedef __attribute__((address_space(3))) v8 lds_v8;
     typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-    typedef short s16x4_ __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4_ lds_s16x4;
+    typedef __attribute__((address_space(3))) pg_s16x4 lds_s16x4;
     constexpr int R = 16 * NR;
     constexpr int CH = DP / 8, RB = DP * 2;        // 16-byte chunks and bytes of a staged row
     constexpr int RPI = 64 / CH;                   // rows a DMA instruction
@@ -308,8 +291,8 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             int pos;                     // position of the first key
             int last;                    // of the source's last key
         };
-        const pr_table own = (pr_table)(uintptr_t)(p.b.table + (int64_t)max(b, 0) * p.b.max_pages);
-        const pr_table shared = (pr_table)(uintptr_t)p.ppages;
+        const pg_table own = (pg_table)(uintptr_t)(p.b.table + (int64_t)max(b, 0) * p.b.max_pages);
+        const pg_table shared = (pg_table)(uintptr_t)p.ppages;
         auto lookup = [&](int j) __attribute__((always_inline)) {
             Tile t;
             const int blk = blk0 + j;
@@ -385,7 +368,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                 for (int kt = 0; kt < 2; ++kt) {
                     const v8 a = *(const lds_v8*)(uintptr_t)(k_rd[ks] + (uint32_t)(16 * kt * RB));
 #pragma unroll
-                    for (int nr = 0; nr < NR; ++nr) st[kt][nr] = TT::mma(a, qf[nr][ks], st[kt][nr]);
+                    for (int nr = 0; nr < NR; ++nr) st[kt][nr] = TT::mma16(a, qf[nr][ks], st[kt][nr]);
                 }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's place is read
             request(next, true);
@@ -440,11 +423,11 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             pr_wait<NI>();   // V is here
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) {
-                const s16x4_ a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)v_rd[dt]);
-                const s16x4_ a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(v_rd[dt] + (uint32_t)(16 * RB)));
+                const pg_s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)v_rd[dt]);
+                const pg_s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(v_rd[dt] + (uint32_t)(16 * RB)));
                 const v8 a = __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr) o[dt][nr] = TT::mma(a, pf[nr], o[dt][nr]);
+                for (int nr = 0; nr < NR; ++nr) o[dt][nr] = TT::mma16(a, pf[nr], o[dt][nr]);
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V's place is read
             request(next, false);
