@@ -518,7 +518,7 @@ enum W8Path { W8_GENERIC = 0, W8_SPLIT = 1, W8_KMAJOR = 2 };
 // Arrival counters at the front of a split-K workspace: the split rule keeps splits * column
 // blocks * row blocks <= 256 with splits >= 2, so at most 128 counters are ever in use.
 constexpr size_t W8_COUNTER_BYTES = STREAM_WS_RESERVED;
-static_assert(W8_COUNTER_BYTES >= 128 * sizeof(unsigned), "counter region");
+static_assert(W8_COUNTER_BYTES >= 128 * sizeof(unsigned) && STREAM_WS_PAGED >= 128 * sizeof(unsigned), "counter region");
 
 struct W8Plan {
     W8Path path = W8_GENERIC;

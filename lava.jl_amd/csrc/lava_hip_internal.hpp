@@ -29,6 +29,9 @@ inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s);
 // STREAM_WS_RESERVED bytes hold the W8A16 split-K arrival counters, which every call leaves at
 // zero; other users write only past them.
 constexpr size_t STREAM_WS_RESERVED = 4096;
+// Of those bytes the W8A16 counters use the first STREAM_WS_PAGED at most; the paged attention's counters, left at zero
+// likewise, lie behind them.
+constexpr size_t STREAM_WS_PAGED = 512;
 // A call on a stream that is capturing a graph does not allocate: it must fit the workspace the
 // stream already has (the buffer is then kept until the process ends, since the graph holds
 // its address).

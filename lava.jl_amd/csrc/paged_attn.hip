@@ -187,21 +187,82 @@ static int64_t pa_max_rows(const PaParams& p, const lava_hip_kv_batch* batch) {
     return q * p.G;
 }
 
-// Sequences of more rows (new tokens times the query heads of a key head) run on the tile kernel.
-constexpr int PA_TILE_ROWS = 64;
-
 // Whether the cache allows 16-byte reads of 8 keys in one page.
 static bool pa_vectors(const PaParams& p) {
     return p.c.D % 8 == 0 && p.c.page % 8 == 0 && p.c.sl % 8 == 0 && p.c.sh % 8 == 0 && p.c.sp % 8 == 0 &&
            aligned(p.c.k, 16) && aligned(p.c.v, 16);
 }
 
-// What depends on the batch's size and the prefix alone.
-static void pa_plan(PaParams* p, int64_t max_rows) {
+// Sequences of more rows (new tokens times the query heads of a key head) run on the tile kernel, of fewer on the row
+// kernel, which splits them along the keys.
+constexpr int PA_TILE_ROWS = 64;
+constexpr size_t PA_ALIGN = 256;
+
+// What depends on the call's sizes alone: which kernels take which sequences.
+static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
-    p->tiles = p->c.D <= 128 && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS));
-    p->row_limit = !p->tiles ? 0x7fffffff : pin == 3 ? 0 : PA_TILE_ROWS;
-    p->stack = p->P > 0 && pin != 3;
+    PaShape sh = {};
+    sh.dp = p->c.D <= 64 ? 64 : p->c.D <= 128 ? 128 : 256;
+    const int64_t rows = (int64_t)p->b.T * p->G;
+    p->row_limit = 0x7fffffff;
+    if (sh.dp <= 128 && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
+        sh.qh = 2;
+        // mostly prompts: the tile kernel takes the few short sequences too, rather than a launch for them
+        p->row_limit = pin == 3 || rows / (128 * sh.qh) >= 4 * (int64_t)p->b.B ? 0 : PA_TILE_ROWS;
+    }
+    p->tiles = sh.qh != 0;
+    if (p->row_limit > 0) {
+        p->stack = p->P > 0 ? 1 : 0;
+        if (p->stack && rows > PA_TILE_ROWS && sh.dp <= 128 && pin != 2) {
+            p->stack = 2;
+            sh.pre_qh = 2;
+        }
+        const int64_t most = std::min<int64_t>(p->stack == 1 ? rows : max_rows, p->stack == 1 ? rows : p->row_limit);
+        sh.nr = most <= 16 ? 1 : most <= 32 || sh.dp == 256 ? 2 : 4;
+        // as many workgroups as fit (LDS: 512 bytes a column of the head, registers)
+        sh.row_grid = (unsigned)(PA_CUS * (sh.dp == 64 && sh.nr <= 2 ? 3 : sh.dp <= 128 && sh.nr <= 2 ? 2 : 1));
+    }
+    const size_t row = sh.dp * sizeof(float) + sizeof(float2);
+    const size_t parts = 2 * std::max<size_t>((size_t)sh.row_grid * 16 * sh.nr, (size_t)PT_GRID * 128 * sh.qh);
+    const size_t pre = 2 * (size_t)PT_GRID * 128 * sh.pre_qh, whole = p->stack ? 2 * (size_t)p->b.T * p->Hq : 0;
+    sh.count_bytes = STREAM_WS_RESERVED;
+    sh.bytes = sh.count_bytes + (parts + pre + whole) * row + 8 * PA_ALIGN;
+    return sh;
+}
+
+// Lays a workspace out: arrivals at `count`, the rest from `at` on.
+static void pa_workspace(PaParams* p, const PaShape& sh, void* count, void* rest) {
+    uint8_t* at = (uint8_t*)rest;
+    auto take = [&](size_t bytes) {
+        at = (uint8_t*)(((uintptr_t)at + PA_ALIGN - 1) & ~(uintptr_t)(PA_ALIGN - 1));
+        uint8_t* q = at;
+        at += bytes;
+        return q;
+    };
+    const size_t parts = 2 * std::max<size_t>((size_t)sh.row_grid * 16 * sh.nr, (size_t)PT_GRID * 128 * sh.qh);
+    const size_t pre = 2 * (size_t)PT_GRID * 128 * sh.pre_qh, whole = p->stack ? 2 * (size_t)p->b.T * p->Hq : 0;
+    p->ws_count = (unsigned*)count;
+    p->ws_o = (float*)take(parts * sh.dp * sizeof(float));
+    p->ws_ml = (float2*)take(parts * sizeof(float2));
+    p->pre_o = (float*)take(pre * sh.dp * sizeof(float));
+    p->pre_ml = (float2*)take(pre * sizeof(float2));
+    p->row_o = (float*)take(whole * sh.dp * sizeof(float));
+    p->row_ml = (float2*)take(whole * sizeof(float2));
+}
+
+static int pa_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {
+    int rc = LAVA_HIP_OK;
+    if (sh.qh) rc = paged_tile_launch(p, sh.qh, false, dtype, s);
+    if (rc == LAVA_HIP_OK && sh.pre_qh) rc = paged_tile_launch(p, sh.pre_qh, true, dtype, s);
+    if (rc == LAVA_HIP_OK && sh.nr) rc = paged_rows_launch(p, sh, dtype, s);
+    return rc;
+}
+
+// Whether the call's blocks of work can be counted in 31 bits.
+static bool pa_countable(const PaParams& p) {
+    const double tiles = (double)p.b.T * p.G / 16 + 2.0 * p.b.B + 1;
+    const double blocks = ((double)p.b.kv_max + p.P) / PT_BK + 4;
+    return tiles * blocks * p.c.heads < 2147483647.0 && (int64_t)p.b.T * p.G <= 0x7fffff00;
 }
 
 static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
@@ -237,25 +298,20 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.ppages = ppages;
     p.P = (int)prefix;
     hipStream_t s = as_stream(stream);
-    const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
-    pa_plan(&p, pa_max_rows(p, batch));
-    bool fast = pin != 1 && paged_rows_fits(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
+    bool fast = kernel_override(LAVA_HIP_FAMILY_PAGED) != 1 && pa_countable(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
     for (int i = 1; i < 3; ++i) fast = fast && q_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
     if (fast) {
-        int64_t rows = pa_max_rows(p, batch);
-        if (p.tiles) {
-            rc = paged_tile_launch(p, cache->dtype, s);
-            if (rc != LAVA_HIP_OK) return rc;
-            rows = std::min<int64_t>(rows, p.row_limit);
-        }
-        const size_t bytes = paged_rows_workspace(p, rows);
+        const PaShape sh = pa_plan_call(&p, pa_max_rows(p, batch));
         if (batch->workspace) {
-            LAVA_ARG(batch->workspace_bytes >= bytes, "%s: the workspace of %zu bytes is smaller than the %zu this call needs",
-                     fn, batch->workspace_bytes, bytes);
-            return paged_rows_launch(p, cache->dtype, rows, batch->workspace, s);
+            LAVA_ARG(batch->workspace_bytes >= sh.bytes, "%s: the workspace of %zu bytes is smaller than the %zu this call needs",
+                     fn, batch->workspace_bytes, sh.bytes);
+            LAVA_ARG(aligned(batch->workspace, 16), "%s: misaligned workspace", fn);
+            pa_workspace(&p, sh, batch->workspace, (uint8_t*)batch->workspace + sh.count_bytes);
+            return pa_launch(p, sh, cache->dtype, s);
         }
-        return with_stream_workspace(bytes + STREAM_WS_RESERVED, stream, [&](void* ws) {
-            return paged_rows_launch(p, cache->dtype, rows, (uint8_t*)ws + STREAM_WS_RESERVED, s);
+        return with_stream_workspace(sh.bytes, stream, [&](void* ws) {
+            pa_workspace(&p, sh, (uint8_t*)ws + STREAM_WS_PAGED, (uint8_t*)ws + sh.count_bytes);
+            return pa_launch(p, sh, cache->dtype, s);
         });
     }
     if (cache->dtype == LAVA_HIP_F16)
@@ -297,7 +353,6 @@ extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, co
     *bytes = 0;
     if (done) return LAVA_HIP_OK;
     p.P = (int)std::min<int64_t>(prefix_len, 0x3fffffff);
-    pa_plan(&p, pa_max_rows(p, batch));
-    if (pa_vectors(p) && paged_rows_fits(p)) *bytes = paged_rows_workspace(p, std::min<int64_t>(pa_max_rows(p, batch), p.row_limit));
+    if (pa_vectors(p) && pa_countable(p)) *bytes = pa_plan_call(&p, pa_max_rows(p, batch)).bytes;
     return LAVA_HIP_OK;
 }

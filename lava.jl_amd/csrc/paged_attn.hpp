@@ -28,13 +28,20 @@ struct PaParams {
     const int* bidir;
     const int* ppages;            // the shared prefix's pages
     int P;                        // its length, 0: none
-    // the row kernel (paged_attn_rows.hip)
-    int tiles;                    // the tile kernel takes sequences of more than row_limit rows
-    int stack;                    // the prefix is attended once, by the rows of many sequences together
-    int row_limit;                // sequences of more rows (new tokens times G) are the tile kernel's
-    float* ws_o;                  // partial sums [workgroup][2][rows of a tile][DP], their (m, l)
+    // how the work is shared out (paged_plan.hpp)
+    int tiles;                    // the tile kernel takes the sequences of more than row_limit rows
+    int row_limit;                // rows: new tokens times G
+    int stack;                    // the prefix is attended once, by the rows of many sequences together: 1 by the row
+                                  // kernel beside the sequences, 2 by the tile kernel in a launch of its own
+    // a launch's workspace: partial sums [workgroup][2][rows of a tile][DP], their (maximum, weight), arrivals of a tile's
+    // parts at the workgroup it starts in (zero between calls)
+    float* ws_o;
     float2* ws_ml;
-    float* row_o;                 // stack: a row's whole results [prefix, own][T * Hq][DP]
+    unsigned* ws_count;
+    // stack: the same for the prefix's launch, and rows' whole results [prefix, own][T * Hq][DP]
+    float* pre_o;
+    float2* pre_ml;
+    float* row_o;
     float2* row_ml;
 };
 
@@ -58,12 +65,23 @@ __device__ __forceinline__ float pa_score(float s, float mul, float cap2) {
 constexpr float PA_LN2 = 0.69314718055994530942f;
 constexpr float PA_LOG2E = 1.44269504088896340736f;
 
-// The row kernel: whether it can count the call's work, the workspace it needs, the launch.  max_rows: rows of
-// a sequence at most, as far as the host knows.
-bool paged_rows_fits(const PaParams& p);
-size_t paged_rows_workspace(const PaParams& p, int64_t max_rows);
-int paged_rows_launch(PaParams& p, int dtype, int64_t max_rows, void* ws, hipStream_t s);
-// The tile kernel: sequences of more than row_limit rows, head dimensions up to 128; no workspace.
-int paged_tile_launch(const PaParams& p, int dtype, hipStream_t s);
+// What a call runs, from what the host knows: sizes, not the lengths on the device.
+struct PaShape {
+    int dp;               // the head dimension rounded up to 64, 128 or 256
+    int nr;               // row kernel: 16 nr rows a tile; 0: no launch
+    unsigned row_grid;
+    int qh;               // tile kernel: 128 qh rows a tile; 0: no launch for sequences
+    int pre_qh;           // the stacked prefix's launch of the tile kernel; 0: none
+    size_t count_bytes, bytes;   // workspace: arrivals, all of it
+};
+PaShape paged_shape(const PaParams& p, int64_t max_rows);
+int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s);
+int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s);
+
+constexpr int PA_CUS = 256;
+constexpr int PR_BK = 128;                       // the row kernel's blocks of keys
+constexpr int PT_BK = 64;                        // the tile kernel's
+constexpr unsigned PA_MAX_GRID = 768;            // workgroups that leave parts
+constexpr unsigned PT_GRID = PA_CUS;             // those of the tile kernel
 
 }  // namespace lava

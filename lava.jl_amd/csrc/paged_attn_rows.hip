@@ -12,131 +12,20 @@
 //  * S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs: a lane owns one row, the score accumulator converts in place to the
 //    second product's operand (k-slot (g, i) is key 4 g + i of the first 16 keys or, from i = 4 on, of the second; V^T comes
 //    in that order from transposing LDS reads);
-//  * a part that does not cover all keys of its rows leaves (sum, max, weight) in the workspace, and a second small
-//    kernel joins the parts in key order, so results do not depend on timing.
+//  * parts that do not cover all keys of their rows are joined in key order by the last workgroup of a row tile to
+//    arrive (paged_plan.hpp), so results do not depend on timing; behind a stacked prefix by a second small kernel.
 // K and V pages are found 8 keys at a time (page sizes are multiples of 8); a page number that is none reads as zeros
 // and is masked, as are rows at and past the sequence's end.
-#include "paged_attn.hpp"
 
 #include <algorithm>
 
 #include "lds_dma.hpp"
+#include "paged_plan.hpp"
 #include "paged_types.hpp"
 
 namespace lava {
 
-constexpr int PR_BK = 128;      // keys of a block, 32 a wavefront
 constexpr float PR_RESCALE = 8.f;   // the maximum moves when a score exceeds it by more than this: P <= 2^8
-
-// ---- the plan -------------------------------------------------------------------------
-
-// A sequence's (or the stacked prefix's) share of the work: key blocks [p0, p0 + np) of the prefix, then
-// [o0, o0 + nb - np) of its own keys, for every row tile and key head.
-struct PrSeq {
-    uint32_t work;
-    int tiles, nb, p0, np, o0;
-};
-
-__device__ __forceinline__ PrSeq pr_seq(const PaParams& p, const PagedSeq& s, int R) {
-    PrSeq w = {};
-    const int64_t rows = (int64_t)s.n * p.G;
-    if (rows == 0 || rows > p.row_limit) return w;
-    const int first = p.P + s.kv - s.n;
-    const int lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    if (p.P > 0 && !p.stack && lo < p.P) {
-        w.p0 = lo / PR_BK;
-        w.np = (p.P + PR_BK - 1) / PR_BK - w.p0;
-    }
-    const int own = max(0, lo - p.P);
-    w.o0 = own / PR_BK;
-    w.nb = max(1, w.np + (s.kv > own ? (s.kv + PR_BK - 1) / PR_BK - w.o0 : 0));   // rows without keys are written too
-    w.tiles = ((int)rows + R - 1) / R;
-    w.work = (uint32_t)w.tiles * (uint32_t)w.nb * (uint32_t)p.c.heads;
-    return w;
-}
-
-__device__ __forceinline__ uint32_t pr_sum(uint32_t x) {
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i, 64);
-    return x;
-}
-__device__ __forceinline__ uint32_t pr_scan(uint32_t x, int lane) {   // inclusive
-    for (int i = 1; i < 64; i *= 2) {
-        const uint32_t y = __shfl_up(x, i, 64);
-        x += lane >= i ? y : 0;
-    }
-    return x;
-}
-
-// What every wavefront knows of the whole call.
-struct PrPlan {
-    uint32_t total, per;    // blocks of work, and of a workgroup
-    PrSeq prefix;           // stack: the prefix for all rows together, in front of the sequences
-    int t0, t1;             // rows of the batch
-    bool plain;             // stack: every row sees the whole prefix
-    uint32_t upto;          // lane i: the work of sequences 0 .. i (i < 64)
-};
-
-__device__ __forceinline__ PrPlan pr_plan(const PaParams& p, int R, int lane) {
-    PrPlan g = {};
-    uint32_t total = 0;
-    int lo = 0x7fffffff;
-    bool plain = p.window == 0;
-    for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-        uint32_t work = 0;
-        if (b0 + lane < p.b.B) {
-            const PagedSeq s = paged_seq(p.b, b0 + lane);
-            work = pr_seq(p, s, R).work;
-            if (s.n > 0) {
-                const int first = p.P + s.kv - s.n;
-                lo = min(lo, p.window > 0 ? max(0, first - p.window + 1) : 0);
-                plain = plain && s.n <= s.kv;
-            }
-        }
-        const uint32_t upto = pr_scan(work, lane);
-        if (b0 == 0) g.upto = upto;
-        total += __builtin_amdgcn_readlane(upto, 63);
-    }
-    if (p.stack) {
-        for (int i = 1; i < 64; i *= 2) lo = min(lo, __shfl_xor(lo, i, 64));
-        lo = __builtin_amdgcn_readfirstlane(lo);
-        g.plain = __builtin_amdgcn_ballot_w64(!plain) == 0;
-        g.t0 = min(max(p.b.q_start[0], 0), p.b.T);
-        g.t1 = min(max(p.b.q_start[p.b.B], g.t0), p.b.T);
-        if (lo < p.P && g.t1 > g.t0) {
-            g.prefix.p0 = lo / PR_BK;
-            g.prefix.np = g.prefix.nb = (p.P + PR_BK - 1) / PR_BK - g.prefix.p0;
-            g.prefix.tiles = ((g.t1 - g.t0) * p.G + R - 1) / R;
-            g.prefix.work = (uint32_t)g.prefix.tiles * (uint32_t)g.prefix.nb * (uint32_t)p.c.heads;
-        }
-    }
-    g.total = total + g.prefix.work;
-    return g;
-}
-
-// The sequence that holds block `w` of the work, and the work in front of it; -1: the stacked prefix.
-__device__ __forceinline__ int pr_locate(const PaParams& p, const PrPlan& g, int R, uint32_t w, int lane, uint32_t& before) {
-    before = 0;
-    if (w < g.prefix.work) return -1;
-    before = g.prefix.work;
-    for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-        uint32_t upto = g.upto;
-        if (b0 > 0) {
-            uint32_t work = 0;
-            if (b0 + lane < p.b.B) work = pr_seq(p, paged_seq(p.b, b0 + lane), R).work;
-            upto = pr_scan(work, lane);
-        }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > w);
-        if (past != 0) {
-            const int i = __builtin_ctzll(past);
-            if (i > 0) before += __builtin_amdgcn_readlane(upto, i - 1);
-            return b0 + i;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    return p.b.B;   // not reached for w < total
-}
-
-__device__ __forceinline__ uint32_t pr_per(uint32_t total) { return max(1u, (total + gridDim.x - 1) / gridDim.x); }
 
 // ---- the kernel -----------------------------------------------------------------------
 
@@ -169,6 +58,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
     constexpr int NKS = DP / 32, NDT = DP / 16;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[4][2][TILE];   // per wavefront: K, V
     __shared__ float2 stat[4][R];
+    __shared__ int arrived;
     auto kswz = [](int row) { return CH == 8 ? ((row & 7) ^ ((row >> 3) & 1)) : (row & 15); };
     auto vswz = [](int row) { return CH == 8 ? 2 * ((row >> 1) & 3) : 2 * (row & 7); };
 
@@ -176,10 +66,10 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
 
-    const PrPlan plan = pr_plan(p, R, lane);
+    const PaPlan plan = pa_plan<PR_BK, false>(p, R, true, p.stack == 1, lane);
     const uint32_t total = __builtin_amdgcn_readfirstlane(plan.total);
-    const uint32_t per = pr_per(total);
-    const uint32_t begin = min(total, blockIdx.x * per), stop = min(total, begin + per);
+    const uint32_t per = pa_per(total, gridDim.x), wg = pa_place(gridDim.x);
+    const uint32_t begin = min(total, wg * per), stop = min(total, begin + per);
     if (begin >= stop) return;
 
     // LDS-DMA: lane offsets within 8 keys, by the parity of the 8 and the instruction
@@ -211,13 +101,13 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
     for (uint32_t at = begin; at < stop;) {
         // ---- the segment: a row tile of a sequence (or of the stacked prefix), some of its blocks
         uint32_t before;
-        const int b = __builtin_amdgcn_readfirstlane(pr_locate(p, plan, R, at, lane, before));
+        const int b = __builtin_amdgcn_readfirstlane(pa_locate<PR_BK, false>(p, plan, R, at, lane, before));
         before = __builtin_amdgcn_readfirstlane(before);
         PagedSeq seq = {plan.t0, plan.t1 - plan.t0, 0};
-        PrSeq sw = plan.prefix;
+        PaSeq sw = plan.prefix;
         if (b >= 0) {
             seq = paged_seq(p.b, b);
-            sw = pr_seq(p, seq, R);
+            sw = pa_seq<PR_BK, false>(p, seq, R);
         }
         const int nb = __builtin_amdgcn_readfirstlane(sw.nb), np = __builtin_amdgcn_readfirstlane(sw.np);
         const int p0 = __builtin_amdgcn_readfirstlane(sw.p0), o0 = __builtin_amdgcn_readfirstlane(sw.o0);
@@ -227,6 +117,12 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
         const int head = (int)(ht / tiles), tile = (int)(ht - (uint32_t)head * tiles);
         const int nblk = min(nb - blk0, (int)(stop - at));
         const int kv = __builtin_amdgcn_readfirstlane(seq.kv);
+
+        // rows of a sequence that another launch takes, prefix and all
+        if (b < 0 && pa_other(p, seq.first + tile * R / p.G, seq.first + min(seq.n - 1, (tile * R + R - 1) / p.G), lane)) {
+            at += (uint32_t)nblk;
+            continue;
+        }
 
         // ---- the rows of this lane
         v8 qf[NR][NKS];
@@ -248,19 +144,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             if (b < 0) {
                 end = p.P;
                 at_pos = p.P;
-                if ((!plan.plain || p.slopes) && live[nr]) {
-                    // the row's sequence: the first whose end lies behind it
-                    int a = 0, z = p.b.B;
-                    while (a < z) {
-                        const int mid = (a + z) >> 1;
-                        if (min(p.b.q_start[mid + 1], p.b.T) <= row_t[nr]) a = mid + 1;
-                        else z = mid;
-                    }
-                    if (a < p.b.B) {
-                        const PagedSeq s = paged_seq(p.b, a);
-                        at_pos = p.P + s.kv - s.n + (row_t[nr] - s.first);
-                    }
-                }
+                if ((!plan.plain || p.slopes) && live[nr]) at_pos = pa_row_pos(p, row_t[nr]);
             }
             if (live[nr]) {
                 const PaRange rg = pa_range(p, at_pos, end, bid);
@@ -478,17 +362,10 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                 const int64_t out_row = (int64_t)row_t[nr] * p.Hq + row_h[nr];
                 const float inv = ll[nr] == 0.f ? 0.f : 1.f / ll[nr];
                 T* orow = (T*)p.O + (int64_t)row_t[nr] * p.ost + (int64_t)row_h[nr] * p.osh + 4 * g;
-                float* prow;
-                float2* pml;
-                if (whole) {
-                    const int64_t i = (b < 0 ? 0 : (int64_t)p.b.T * p.Hq) + out_row;
-                    prow = p.row_o + i * DP;
-                    pml = p.row_ml + i;
-                } else {
-                    const int64_t i = (int64_t)(2 * blockIdx.x + (blk0 == 0 ? 1 : 0)) * R + 16 * nr + r16;
-                    prow = p.ws_o + i * DP;
-                    pml = p.ws_ml + i;
-                }
+                const int64_t part = whole ? (b < 0 ? 0 : (int64_t)p.b.T * p.Hq) + out_row
+                                           : (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * R + 16 * nr + r16;
+                float* prow = (whole ? p.row_o : p.ws_o) + part * DP + 4 * g;
+                float2* pml = (whole ? p.row_ml : p.ws_ml) + part;
 #pragma unroll
                 for (int d4 = 0; d4 < NDT / 4; ++d4) {
                     const int dt = 4 * d4 + w;
@@ -500,28 +377,32 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                         const v4 y = {(T)(x[0] * inv), (T)(x[1] * inv), (T)(x[2] * inv), (T)(x[3] * inv)};
                         if (16 * dt + 4 * g < p.c.D) *reinterpret_cast<v4*>(orow + 16 * dt) = y;
                     } else {
-                        *reinterpret_cast<f32x4*>(prow + 16 * dt + 4 * g) = x;
+                        pa_put(prow + 16 * dt, x[0], x[1]);
+                        pa_put(prow + 16 * dt + 2, x[2], x[3]);
                     }
                 }
                 if (live[nr] && w == 0 && g == 0) {
                     if (direct) {
                         if (p.lse) p.lse[out_row] = ll[nr] == 0.f ? -INFINITY : (ml[nr] + log2f(ll[nr])) * PA_LN2;
                     } else {
-                        *pml = make_float2(ml[nr], ll[nr]);
+                        pa_put((float*)pml, ml[nr], ll[nr]);
                     }
                 }
             }
+        }
+        if (!whole && p.stack == 0) {
+            const uint32_t a = before + ht * (uint32_t)nb;   // the tile's first block
+            pa_arrive<T, DP, 4>(p, a / per, (a + (uint32_t)nb - 1) / per, R, min(R, seq.n * p.G - tile * R), tile * R, seq.first,
+                                head, w, lane, &arrived);
         }
         at += (uint32_t)nblk;
     }
 }
 
-// Joins the parts of every row that has more than one: the prefix's (stacked) and its sequence's, each in the order of
-// its keys.  One wavefront a row; a lane holds DP / 64 columns.
+// Behind a stacked prefix: a row's parts, the prefix's and its sequence's, each in the order of its keys.  One
+// wavefront a row.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, uint32_t parts) {
-    constexpr int NC = DP / 64;
-    typedef float vf __attribute__((ext_vector_type(NC)));
+__global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, uint32_t row_grid, int pre_R) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= (int64_t)p.b.T * p.Hq) return;
@@ -530,116 +411,74 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, uint
     if (b >= p.b.B) return;
     const PagedSeq s = paged_seq(p.b, b);
     if (t < s.first || t >= s.first + s.n || (int64_t)s.n * p.G > p.row_limit) return;
-    const PrPlan plan = pr_plan(p, R, lane);
-    const uint32_t per = max(1u, (plan.total + parts - 1) / parts);
-    const int head = h / p.G;
+    // a tile's parts: whole (one, by row), or those of workgroups i0 .. i0 + n - 1
+    struct Source {
+        const float* o;
+        const float2* ml;
+        uint32_t i0;
+        int n, R, in;
+        __device__ int64_t at(int j) const { return n == 1 ? in : (int64_t)(2 * (i0 + (uint32_t)j) + (j == 0 ? 1u : 0u)) * R + in; }
+    };
+    const int head = h / p.G, g = h - head * p.G;
+    auto source = [&](const PaSeq& sw, uint32_t before, uint32_t per, int tile_rows, uint32_t r, const float* o, const float2* ml,
+                      int which) {
+        const uint32_t tile = r / (uint32_t)tile_rows;
+        const uint32_t a = before + ((uint32_t)head * (uint32_t)sw.tiles + tile) * (uint32_t)sw.nb, z = a + (uint32_t)sw.nb - 1;
+        Source x;
+        x.i0 = a / per;
+        x.n = (int)(z / per - x.i0) + 1;
+        x.R = tile_rows;
+        const bool whole = x.n == 1;
+        x.in = whole ? 0 : (int)(r - tile * (uint32_t)tile_rows);
+        const int64_t i = (int64_t)which * p.b.T * p.Hq + row;
+        x.o = whole ? p.row_o + i * DP : o;
+        x.ml = whole ? p.row_ml + i : ml;
+        return x;
+    };
+    const PaPlan plan = pa_plan<PR_BK, false>(p, R, true, p.stack == 1, lane);
     uint32_t before = plan.prefix.work;
     for (int b0 = 0; b0 < b; b0 += 64) {
         uint32_t upto = plan.upto;
         if (b0 > 0) {
             uint32_t work = 0;
-            if (b0 + lane < p.b.B) work = pr_seq(p, paged_seq(p.b, b0 + lane), R).work;
-            upto = pr_scan(work, lane);
+            if (b0 + lane < p.b.B) work = pa_seq<PR_BK, false>(p, paged_seq(p.b, b0 + lane), R).work;
+            upto = pa_scan(work, lane);
         }
         before += __builtin_amdgcn_readlane(upto, min(b - b0, 64) - 1);
     }
-    float m = -INFINITY, l = 0.f;
-    vf o = {};
-    auto take = [&](const float* po, float2 ml) {
-        const float mn = fmaxf(m, ml.x), sub = mn == -INFINITY ? 0.f : mn;
-        const float a = __builtin_amdgcn_exp2f(m - sub), c = __builtin_amdgcn_exp2f(ml.x - sub);
-        o = o * a + *reinterpret_cast<const vf*>(po + NC * lane) * c;
-        l = l * a + ml.y * c;
-        m = mn;
-    };
-    // one row tile's parts: false if its one part has written O already
-    auto source = [&](const PrSeq& sw, uint32_t w0, uint32_t r, int which) {
-        const uint32_t tile = r / (uint32_t)R, in = r - tile * (uint32_t)R;
-        const uint32_t a = w0 + ((uint32_t)head * (uint32_t)sw.tiles + tile) * (uint32_t)sw.nb, z = a + (uint32_t)sw.nb - 1;
-        const uint32_t i0 = a / per, i1 = z / per;
-        if (i0 == i1) {
-            if (!p.stack) return false;
-            const int64_t i = (int64_t)which * p.b.T * p.Hq + row;
-            take(p.row_o + i * DP, p.row_ml[i]);
-            return true;
-        }
-        for (uint32_t i = i0; i <= i1; ++i) {
-            const int64_t k = (int64_t)(2 * i + (a >= i * per ? 1 : 0)) * R + in;
-            take(p.ws_o + k * DP, p.ws_ml[k]);
-        }
-        return true;
-    };
-    bool any = false;
-    if (plan.prefix.work > 0) any = source(plan.prefix, 0, (uint32_t)((t - plan.t0) * p.G + h % p.G), 0);
-    any = source(pr_seq(p, s, R), before, (uint32_t)((t - s.first) * p.G + h % p.G), 1) || any;
-    if (!any) return;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* orow = (T*)p.O + (int64_t)t * p.ost + (int64_t)h * p.osh + NC * lane;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-        if (NC * lane + i < p.c.D) orow[i] = (T)(o[i] * inv);
-    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * PA_LN2;
+    const uint32_t per = pa_per(plan.total, row_grid);
+    const Source own = source(pa_seq<PR_BK, false>(p, s, R), before, per, R, (uint32_t)((t - s.first) * p.G + g), p.ws_o, p.ws_ml, 1);
+    Source pre = own;
+    pre.n = 0;
+    if (p.stack == 1) {
+        if (plan.prefix.work > 0) pre = source(plan.prefix, 0, per, R, (uint32_t)((t - plan.t0) * p.G + g), p.ws_o, p.ws_ml, 0);
+    } else {
+        const PaPlan pp = pa_plan<PT_BK, true>(p, pre_R, false, true, lane);
+        if (pp.prefix.work > 0)
+            pre = source(pp.prefix, 0, pa_per(pp.total, PT_GRID), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
+    }
+    float o[DP / 64], m, l;
+    pa_join_row<DP>(pre.n + own.n, [&](int j) { return j < pre.n ? pre.ml + pre.at(j) : own.ml + own.at(j - pre.n); },
+                    [&](int j) { return j < pre.n ? pre.o + pre.at(j) * DP : own.o + own.at(j - pre.n) * DP; }, lane, o, m, l);
+    pa_store_row<T, DP>(p, t, h, o, m, l, lane);
 }
 
-// ---- host -----------------------------------------------------------------------------
-
-constexpr int PR_CUS = 256;
-
-struct PrShape {
-    int dp, nr;
-    unsigned grid;
-    size_t slots, rows;    // partial results, whole ones
-};
-
-static PrShape pr_shape(const PaParams& p, int64_t max_rows) {
-    PrShape s;
-    s.dp = p.c.D <= 64 ? 64 : p.c.D <= 128 ? 128 : 256;
-    if (p.stack) max_rows = std::max<int64_t>(max_rows, (int64_t)p.b.T * p.G);
-    s.nr = max_rows <= 16 ? 1 : max_rows <= 32 || s.dp == 256 ? 2 : 4;
-    const int wgs = s.dp == 64 && s.nr <= 2 ? 4 : s.dp <= 128 && s.nr <= 2 ? 2 : 1;
-    s.grid = (unsigned)(PR_CUS * wgs);
-    s.slots = (size_t)s.grid * 2 * 16 * s.nr;
-    s.rows = p.stack ? (size_t)2 * p.b.T * p.Hq : 0;
-    return s;
-}
-
-size_t paged_rows_workspace(const PaParams& p, int64_t max_rows) {
-    const PrShape s = pr_shape(p, max_rows);
-    return (s.slots + s.rows) * (s.dp * sizeof(float) + sizeof(float2)) + 512;
-}
-
-// Whether the call's blocks of work can be counted in 31 bits.
-bool paged_rows_fits(const PaParams& p) {
-    const double tiles = (double)p.b.T * p.G / 16 + 2.0 * p.b.B + 1;
-    const double blocks = ((double)p.b.kv_max + p.P) / PR_BK + 4;
-    return tiles * blocks * p.c.heads < 2147483647.0 && (int64_t)p.b.T * p.G <= 0x7fffff00;
-}
-
-int paged_rows_launch(PaParams& p, int dtype, int64_t max_rows, void* ws, hipStream_t s) {
-    const PrShape sh = pr_shape(p, max_rows);
-    uint8_t* at = (uint8_t*)(((uintptr_t)ws + 255) & ~(uintptr_t)255);
-    auto take = [&](size_t bytes) {
-        uint8_t* q = at;
-        at += bytes;
-        return q;
-    };
-    p.ws_o = (float*)take(sh.slots * sh.dp * sizeof(float));
-    p.row_o = (float*)take(sh.rows * sh.dp * sizeof(float));
-    p.ws_ml = (float2*)take(sh.slots * sizeof(float2));
-    p.row_ml = (float2*)take(sh.rows * sizeof(float2));
+int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {
     auto by_type = [&](auto tag) {
         typedef decltype(tag) T;
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(sh.grid), dim3(256), 0, s, p); };
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(sh.row_grid), dim3(256), 0, s, p); };
         if (sh.dp == 64)
             sh.nr == 1 ? go(paged_rows_kernel<T, 64, 1>) : sh.nr == 2 ? go(paged_rows_kernel<T, 64, 2>) : go(paged_rows_kernel<T, 64, 4>);
         else if (sh.dp == 128)
             sh.nr == 1 ? go(paged_rows_kernel<T, 128, 1>) : sh.nr == 2 ? go(paged_rows_kernel<T, 128, 2>) : go(paged_rows_kernel<T, 128, 4>);
         else
             sh.nr == 1 ? go(paged_rows_kernel<T, 256, 1>) : go(paged_rows_kernel<T, 256, 2>);
-        const int rc = check_launch("paged_rows_kernel");
-        if (rc != LAVA_HIP_OK) return rc;
+        int rc = check_launch("paged_rows_kernel");
+        if (rc != LAVA_HIP_OK || p.stack == 0) return rc;
         const unsigned rows = (unsigned)(((int64_t)p.b.T * p.Hq + 3) / 4);
-        auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, sh.grid); };
+        auto join = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, sh.row_grid, 128 * sh.pre_qh);
+        };
         sh.dp == 64 ? join(paged_join_kernel<T, 64>) : sh.dp == 128 ? join(paged_join_kernel<T, 128>) : join(paged_join_kernel<T, 256>);
         return check_launch("paged_join_kernel");
     };

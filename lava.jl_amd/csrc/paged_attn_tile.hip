@@ -11,23 +11,22 @@
 //  * MODE 0 (f16, 0 < scale log2 e <= 1, no cap or slopes): the scale is folded into Q (one rounding) and the maximum
 //    enters the product as a bias k-step, so that P = exp2 of the accumulator; 1 (bf16, positive scale): P = exp2(fma(S, c,
 //    -m)), since bf16 would lose 2^-8 of q c; 2: caps, slopes, any scale.
-#include "paged_attn.hpp"
 
 #include <algorithm>
 
 #include "lds_dma.hpp"
+#include "paged_plan.hpp"
 #include "paged_types.hpp"
 
 namespace lava {
 
 constexpr int PT_PAIRS = 4;
-constexpr int PT_BK = 64;
 constexpr int PT_KST = 3, PT_VST = 2;   // LDS stages
 constexpr int PT_PF = 4;                // fragments read ahead of their MFMA
 constexpr float PT_RESCALE = 8.f;
 
 template <typename T, int DE, int QH, int MODE>
-__global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams p) {
+__global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams p, int prefix) {
     typedef PgType<T> TT;
     typedef typename TT::v8 v8;
     typedef typename TT::v4 v4;
@@ -47,6 +46,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
     __shared__ int fbuf[2][PT_PAIRS];
     __shared__ __attribute__((aligned(16))) int nbuf[PT_KST][4];   // keys without a page, 2 bits of 8 keys each
     __shared__ float mbuf[PT_PAIRS][PQ];
+    __shared__ int arrived;
 
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -54,71 +54,110 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
     const int pr = w & (PT_PAIRS - 1);
     const int r32 = lane & 31, h = lane >> 5;
 
-    // ---- the tile: key heads innermost, so that an XCD's workgroups share few heads' keys; a sequence's last tiles,
-    // which see the most keys, first
-    const int head = (int)(blockIdx.x % (unsigned)p.c.heads);
-    int idx = (int)(blockIdx.x / (unsigned)p.c.heads);
-    int b = -1, tile = 0;
-    for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-        int tiles = 0;
-        if (b0 + lane < p.b.B) {
-            const PagedSeq s = paged_seq(p.b, b0 + lane);
-            const int64_t rows = (int64_t)s.n * p.G;
-            tiles = rows > p.row_limit ? (int)((rows + BQ - 1) / BQ) : 0;
+    // ---- which part of the work.  Tiles one by one, a workgroup each, where the longest does not outlast the rest by more
+    // than splitting costs (parts written and joined, about 12 blocks' time, and blocks that only a sequence's
+    // last tiles see counted for all); else the even split over PT_GRID workgroups.
+    const PaPlan plan = pa_plan<PT_BK, true>(p, BQ, !prefix, prefix, lane);
+    const bool by_tile = !prefix && plan.longest / 2 <= 12 + (int)((plan.total - min(plan.total, plan.seen)) / PA_CUS);
+    uint32_t at = 0, stop = 1, per = 1, wg = 0, before = 0;
+    int tb = -1, t_head = 0, t_tile = 0;
+    if (by_tile) {
+        // key heads innermost, so that an XCD's workgroups share few heads' keys; a sequence's last tiles, which
+        // see the most keys, first
+        t_head = (int)(blockIdx.x % (unsigned)p.c.heads);
+        int idx = (int)(blockIdx.x / (unsigned)p.c.heads);
+        for (int b0 = 0; b0 < p.b.B; b0 += 64) {
+            int tiles = 0;
+            if (b0 + lane < p.b.B) tiles = pa_seq<PT_BK, true>(p, paged_seq(p.b, b0 + lane), BQ).tiles;
+            const int upto = (int)pa_scan((uint32_t)tiles, lane);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(upto > idx);
+            if (past != 0) {
+                const int i = __builtin_ctzll(past);
+                const int lower = i > 0 ? __builtin_amdgcn_readlane(upto, i - 1) : 0;
+                tb = b0 + i;
+                t_tile = __builtin_amdgcn_readlane(upto, i) - 1 - (idx - lower) - lower;   // from the last one down
+                break;
+            }
+            idx -= __builtin_amdgcn_readlane(upto, 63);
         }
-        int upto = tiles;
-        for (int i = 1; i < 64; i *= 2) {
-            const int y = __shfl_up(upto, i, 64);
-            upto += lane >= i ? y : 0;
-        }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(upto > idx);
-        if (past != 0) {
-            const int i = __builtin_ctzll(past);
-            b = b0 + i;
-            tile = __builtin_amdgcn_readlane(upto, i) - 1 - idx;   // from the last one down
-            break;
-        }
-        idx -= __builtin_amdgcn_readlane(upto, 63);
+        if (tb < 0) return;
+    } else {
+        if (blockIdx.x >= PT_GRID) return;
+        per = pa_per(plan.total, PT_GRID);
+        wg = pa_place(PT_GRID);
+        at = min(plan.total, wg * per);
+        stop = min(plan.total, at + per);
     }
-    if (b < 0) return;
+
+    for (; at < stop;) {
+    // ---- the segment: some key blocks of a row tile
+    int b = tb;
+    PagedSeq seq = {plan.t0, plan.t1 - plan.t0, 0};
+    PaSeq sw = plan.prefix;
+    if (!by_tile) b = pa_locate<PT_BK, true>(p, plan, BQ, at, lane, before);
     b = __builtin_amdgcn_readfirstlane(b);
-    PagedSeq seq = paged_seq(p.b, b);
+    if (b >= 0) {
+        seq = paged_seq(p.b, b);
+        sw = pa_seq<PT_BK, true>(p, seq, BQ);
+    }
     seq.first = __builtin_amdgcn_readfirstlane(seq.first);
     seq.n = __builtin_amdgcn_readfirstlane(seq.n);
     seq.kv = __builtin_amdgcn_readfirstlane(seq.kv);
-    const int end = p.P + seq.kv;
-    const int bid = p.bidir ? p.bidir[b] : 0;
-    // positions that some row of the tile sees: rows are in order of their positions
-    const int i_lo = (int)div_of((uint32_t)(tile * BQ), p.by_g);
-    const int i_hi = min(seq.n - 1, (int)div_of((uint32_t)(tile * BQ + BQ - 1), p.by_g));
-    const int see_lo = pa_range(p, end - seq.n + i_lo, end, bid).lo;
-    const int see_hi = __builtin_amdgcn_readfirstlane(pa_range(p, end - seq.n + i_hi, end, bid).hi);
-    // key blocks: of the prefix [p0, p0 + np), then of the sequence's own keys from o0 on
-    int p0 = 0, np = 0;
-    if (see_lo < p.P && see_hi >= see_lo) {
-        p0 = see_lo / PT_BK;
-        np = min(see_hi, p.P - 1) / PT_BK - p0 + 1;
+    const int nb = __builtin_amdgcn_readfirstlane(sw.nb), np = __builtin_amdgcn_readfirstlane(sw.np);
+    const int p0 = __builtin_amdgcn_readfirstlane(sw.p0), o0 = __builtin_amdgcn_readfirstlane(sw.o0);
+    int head = t_head, tile = t_tile, blk0 = 0, nseg = nb;
+    if (!by_tile) {
+        const uint32_t rel = at - before, ht = rel / (uint32_t)nb;
+        blk0 = (int)(rel - ht * (uint32_t)nb);
+        head = (int)(ht / (uint32_t)sw.tiles);
+        tile = (int)(ht - (uint32_t)head * (uint32_t)sw.tiles);
+        nseg = min(nb - blk0, (int)(stop - at));
     }
-    int o0 = max(0, see_lo - p.P) / PT_BK;
-    const int no = see_hi >= p.P && see_hi >= see_lo ? (see_hi - p.P) / PT_BK - o0 + 1 : 0;
-    p0 = __builtin_amdgcn_readfirstlane(p0);
-    np = __builtin_amdgcn_readfirstlane(np);
-    o0 = __builtin_amdgcn_readfirstlane(o0);
-    const int nblk = __builtin_amdgcn_readfirstlane(np + no);
+    head = __builtin_amdgcn_readfirstlane(head);
+    tile = __builtin_amdgcn_readfirstlane(tile);
+    blk0 = __builtin_amdgcn_readfirstlane(blk0);
+    nseg = __builtin_amdgcn_readfirstlane(nseg);
+    const bool whole = nseg == nb;
+    const int rows = seq.n * p.G;
+    // rows of a sequence that another launch takes, prefix and all
+    if (b < 0 && pa_other(p, seq.first + tile * BQ / p.G, seq.first + min(seq.n - 1, (tile * BQ + BQ - 1) / p.G), lane)) {
+        at += (uint32_t)nseg;
+        continue;
+    }
+    const int end = b < 0 ? p.P : p.P + seq.kv;
+    const int bid = b >= 0 && p.bidir ? p.bidir[b] : 0;
     auto block_of = [&](int pos) { return pos < p.P ? pos / PT_BK - p0 : np + (pos - p.P) / PT_BK - o0; };
     auto first_pos = [&](int blk) { return blk < np ? (p0 + blk) * PT_BK : p.P + (o0 + blk - np) * PT_BK; };
-    // this pair's rows and blocks
-    const int row0 = tile * BQ + pr * PQ;
-    const int rows = seq.n * p.G;
-    int jf = 0, jl = -1;
-    if (row0 < rows && nblk > 0) {
-        const int a = (int)div_of((uint32_t)row0, p.by_g), z = (int)div_of((uint32_t)min(row0 + PQ - 1, rows - 1), p.by_g);
+    // of rows [r0, r1], in order of their positions, the blocks that some row sees
+    auto sees = [&](int r0, int r1, int& f, int& l) {
+        const int a = (int)div_of((uint32_t)r0, p.by_g), z = (int)div_of((uint32_t)min(r1, rows - 1), p.by_g);
         const int lo = pa_range(p, end - seq.n + a, end, bid).lo, hi = pa_range(p, end - seq.n + z, end, bid).hi;
-        if (hi >= lo) {
-            jf = __builtin_amdgcn_readfirstlane(max(0, block_of(lo)));
-            jl = __builtin_amdgcn_readfirstlane(min(nblk - 1, block_of(hi)));
+        f = 0;
+        l = -1;
+        if (r0 < rows && hi >= lo) {
+            f = max(0, block_of(lo));
+            l = min(nb - 1, block_of(hi));
         }
+    };
+    int e0 = blk0, e1 = blk0 + nseg - 1;
+    if (b >= 0) {
+        int f, l;
+        sees(tile * BQ, tile * BQ + BQ - 1, f, l);
+        e0 = max(e0, f);
+        e1 = min(e1, l);
     }
+    e0 = __builtin_amdgcn_readfirstlane(e0);
+    const int nblk = __builtin_amdgcn_readfirstlane(max(0, e1 - e0 + 1));
+    // this pair's rows and blocks, from e0 on
+    const int row0 = tile * BQ + pr * PQ;
+    int jf = 0, jl = row0 < rows ? nblk - 1 : -1;
+    if (b >= 0) {
+        sees(row0, row0 + PQ - 1, jf, jl);
+        jf = max(0, jf - e0);
+        jl = min(nblk - 1, jl - e0);
+    }
+    jf = __builtin_amdgcn_readfirstlane(jf);
+    jl = __builtin_amdgcn_readfirstlane(jl);
     // this lane's rows
     int row_t[QH], row_h[QH], r_lo[QH], r_hi[QH];
     float r_pos[QH];
@@ -130,10 +169,15 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
         live[qh] = row < rows;
         row_t[qh] = seq.first + i;
         row_h[qh] = head * p.G + row - i * p.G;
-        const PaRange rg = pa_range(p, end - seq.n + i, end, bid);
+        int pos = end - seq.n + i;
+        if (b < 0) {
+            pos = p.P;
+            if ((!plan.plain || p.slopes) && live[qh]) pos = pa_row_pos(p, row_t[qh]);
+        }
+        const PaRange rg = pa_range(p, pos, end, bid);
         r_lo[qh] = live[qh] ? rg.lo : 0;
         r_hi[qh] = live[qh] ? rg.hi : 0x7fffffff;
-        r_pos[qh] = (float)(end - seq.n + i);
+        r_pos[qh] = (float)pos;
     }
 
     const uint32_t p_lane = lds_addr(&pbuf[0][0][0]) + (uint32_t)pr * PBUF + 16u * lane;
@@ -219,8 +263,8 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
                 __builtin_amdgcn_sched_barrier(0);
             }
             const int none = __builtin_amdgcn_readfirstlane(nn.x | nn.y << 2 | nn.z << 4 | nn.w << 6);
-            const int pos0 = __builtin_amdgcn_readfirstlane(first_pos(j));
-            const int src_hi = j < np ? p.P - 1 : end - 1;
+            const int pos0 = __builtin_amdgcn_readfirstlane(first_pos(e0 + j));
+            const int src_hi = e0 + j < np ? p.P - 1 : end - 1;
             if constexpr (MODE == 2) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -349,12 +393,13 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
         struct Src {
             int page[2], row[2], n[2];   // per 8 keys: the page (-1: none), the row in it, keys below the end
         };
-        const pg_table own = (pg_table)(uintptr_t)(p.b.table + (int64_t)b * p.b.max_pages);
+        const pg_table own = (pg_table)(uintptr_t)(p.b.table + (int64_t)max(b, 0) * p.b.max_pages);
         const pg_table shared = (pg_table)(uintptr_t)p.ppages;
         auto lookup = [&](int j) __attribute__((always_inline)) {
             Src t;
-            const bool pre = j < np;
-            const int key0 = (pre ? p0 + j : o0 + j - np) * PT_BK + 16 * pr;
+            const int blk = e0 + j;
+            const bool pre = blk < np;
+            const int key0 = (pre ? p0 + blk : o0 + blk - np) * PT_BK + 16 * pr;
             const int len = j < nblk ? (pre ? p.P : seq.kv) : 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -488,46 +533,65 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
             pg_xor32_pair(l[qh], a, c);
             const float sum = a + c, inv = sum == 0.f ? 0.f : 1.f / sum;
             if (!live[qh]) continue;
-            T* orow = (T*)p.O + (int64_t)row_t[qh] * p.ost + (int64_t)row_h[qh] * p.osh;
+            const int64_t out_row = (int64_t)row_t[qh] * p.Hq + row_h[qh];
+            if (whole && b >= 0) {
+                T* orow = (T*)p.O + (int64_t)row_t[qh] * p.ost + (int64_t)row_h[qh] * p.osh;
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
+                for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) {
-                    const int d = 32 * dt + 8 * g4 + 4 * h;
-                    const v4 v = {(T)(o[dt][qh][4 * g4] * inv), (T)(o[dt][qh][4 * g4 + 1] * inv), (T)(o[dt][qh][4 * g4 + 2] * inv),
-                                  (T)(o[dt][qh][4 * g4 + 3] * inv)};
-                    if (d < p.c.D) *reinterpret_cast<v4*>(orow + d) = v;
+                    for (int g4 = 0; g4 < 4; ++g4) {
+                        const int d = 32 * dt + 8 * g4 + 4 * h;
+                        const v4 v = {(T)(o[dt][qh][4 * g4] * inv), (T)(o[dt][qh][4 * g4 + 1] * inv), (T)(o[dt][qh][4 * g4 + 2] * inv),
+                                      (T)(o[dt][qh][4 * g4 + 3] * inv)};
+                        if (d < p.c.D) *reinterpret_cast<v4*>(orow + d) = v;
+                    }
+                if (p.lse && h == 0) p.lse[out_row] = sum == 0.f ? -INFINITY : (mbuf[pr][32 * qh + r32] + log2f(sum)) * PA_LN2;
+            } else {
+                const int64_t part = whole ? out_row : (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * BQ + pr * PQ + 32 * qh + r32;
+                float* prow = (whole ? p.row_o : prefix ? p.pre_o : p.ws_o) + part * DE + 4 * h;
+                if (sum != 0.f) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int g4 = 0; g4 < 4; ++g4) {
+                            pa_put(prow + 32 * dt + 8 * g4, o[dt][qh][4 * g4], o[dt][qh][4 * g4 + 1]);
+                            pa_put(prow + 32 * dt + 8 * g4 + 2, o[dt][qh][4 * g4 + 2], o[dt][qh][4 * g4 + 3]);
+                        }
                 }
-            if (p.lse && h == 0)
-                p.lse[(int64_t)row_t[qh] * p.Hq + row_h[qh]] =
-                    sum == 0.f ? -INFINITY : (mbuf[pr][32 * qh + r32] + log2f(sum)) * PA_LN2;
+                if (h == 0) pa_put((float*)((whole ? p.row_ml : prefix ? p.pre_ml : p.ws_ml) + part), mbuf[pr][32 * qh + r32], sum);
+            }
         }
+    }
+    if (!whole && !prefix) {
+        const uint32_t a = before + ((uint32_t)head * (uint32_t)sw.tiles + (uint32_t)tile) * (uint32_t)nb;   // the tile's first block
+        pa_arrive<T, DE, 2 * PT_PAIRS>(p, a / per, (a + (uint32_t)nb - 1) / per, BQ, min(BQ, rows - tile * BQ), tile * BQ, seq.first,
+                                       head, w, lane, &arrived);
+    }
+    at += (uint32_t)nseg;
     }
 }
 
 // ---- host -----------------------------------------------------------------------------
 
-int paged_tile_launch(const PaParams& p, int dtype, hipStream_t s) {
+int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s) {
     const bool plain = p.cap2 == 0.f && !p.slopes && p.mul > 0.f;
-    const int64_t rows = (int64_t)p.b.T * p.G;
-    const bool narrow = false;
-    const int bq = (narrow ? 32 : 64) * PT_PAIRS;
-    const int64_t blocks = (rows / bq + p.b.B) * p.c.heads;
-    LAVA_REQUIRE(blocks <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "paged attention: problem too large");
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(128 * PT_PAIRS), 0, s, p); };
-    auto by_d = [&](auto type, auto qh, auto mode) {
+    const int64_t tiles = ((int64_t)p.b.T * p.G / (128 * qh) + p.b.B) * p.c.heads;   // no fewer than there are
+    LAVA_REQUIRE(tiles <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "paged attention: problem too large");
+    const unsigned grid = prefix ? PT_GRID : (unsigned)std::max<int64_t>(tiles, PT_GRID);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(128 * PT_PAIRS), 0, s, p, prefix ? 1 : 0); };
+    auto by_d = [&](auto type, auto q, auto mode) {
         typedef decltype(type) T;
-        constexpr int QH = decltype(qh)::value, MODE = decltype(mode)::value;
+        constexpr int QH = decltype(q)::value, MODE = decltype(mode)::value;
         p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE>) : go(paged_tile_kernel<T, 128, QH, MODE>);
     };
-    auto by_mode = [&](auto qh) {
+    auto by_mode = [&](auto q) {
         if (dtype == LAVA_HIP_F16)
-            plain && p.mul <= 1.f ? by_d(f16{}, qh, pg_int<0>{}) : by_d(f16{}, qh, pg_int<2>{});
+            plain && p.mul <= 1.f ? by_d(f16{}, q, pg_int<0>{}) : by_d(f16{}, q, pg_int<2>{});
         else
-            plain ? by_d(bf16{}, qh, pg_int<1>{}) : by_d(bf16{}, qh, pg_int<2>{});
+            plain ? by_d(bf16{}, q, pg_int<1>{}) : by_d(bf16{}, q, pg_int<2>{});
     };
-    narrow ? by_mode(pg_int<1>{}) : by_mode(pg_int<2>{});
-    return check_launch(narrow ? "paged_tile_kernel+paged_tile_kernel<32>" : "paged_tile_kernel");
+    qh == 1 ? by_mode(pg_int<1>{}) : by_mode(pg_int<2>{});
+    return check_launch(qh == 1 ? "paged_tile_kernel+paged_tile_kernel<32>" : "paged_tile_kernel");
 }
 
 }  // namespace lava
