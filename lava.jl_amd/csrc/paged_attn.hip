@@ -205,7 +205,7 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     sh.dp = p->c.D <= 64 ? 64 : p->c.D <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)p->b.T * p->G;
     p->row_limit = 0x7fffffff;
-    if (sh.dp <= 128 && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
+    if (paged_tile_takes(*p) && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
         sh.qh = 2;
         // mostly prompts: the tile kernel takes the few short sequences too, rather than a launch for them
         p->row_limit = pin == 3 || rows / (128 * sh.qh) >= 4 * (int64_t)p->b.B ? 0 : PA_TILE_ROWS;
@@ -213,7 +213,7 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     p->tiles = sh.qh != 0;
     if (p->row_limit > 0) {
         p->stack = p->P > 0 ? 1 : 0;
-        if (p->stack && rows > PA_TILE_ROWS && sh.dp <= 128 && pin != 2) {
+        if (p->stack && rows > PA_TILE_ROWS && paged_tile_takes(*p) && pin != 2) {
             p->stack = 2;
             sh.pre_qh = 2;
         }
@@ -222,6 +222,8 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
         // as many workgroups as fit (LDS: 512 bytes a column of the head, registers)
         sh.row_grid = (unsigned)(PA_CUS * (sh.dp == 64 && sh.nr <= 2 ? 3 : sh.dp <= 128 && sh.nr <= 2 ? 2 : 1));
     }
+    p->by_rows = fast_div(std::max(1u, sh.row_grid));
+    p->by_tiles = fast_div(PT_GRID);
     const size_t row = sh.dp * sizeof(float) + sizeof(float2);
     const size_t parts = 2 * std::max<size_t>((size_t)sh.row_grid * 16 * sh.nr, (size_t)PT_GRID * 128 * sh.qh);
     const size_t pre = 2 * (size_t)PT_GRID * 128 * sh.pre_qh, whole = p->stack ? 2 * (size_t)p->b.T * p->Hq : 0;
@@ -295,6 +297,7 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.qst = q_strides[2];
     p.osh = o_strides[1];
     p.ost = o_strides[2];
+    p.o16 = aligned(O, 16) && p.osh % 8 == 0 && p.ost % 8 == 0;
     p.ppages = ppages;
     p.P = (int)prefix;
     hipStream_t s = as_stream(stream);

@@ -20,6 +20,7 @@ struct PaParams {
     float* lse;
     int64_t qsh, qst, osh, ost;   // head and token strides
     int Hq, G;                    // query heads, those of a key head
+    int o16;                      // O and its strides allow 16-byte stores
     FastDiv by_g;
     float mul;                    // scores to base 2; with a cap to 2 log2(e) s / cap
     float cap2;                   // cap log2(e), or 0
@@ -33,6 +34,7 @@ struct PaParams {
     int row_limit;                // rows: new tokens times G
     int stack;                    // the prefix is attended once, by the rows of many sequences together: 1 by the row
                                   // kernel beside the sequences, 2 by the tile kernel in a launch of its own
+    FastDiv by_rows, by_tiles;    // workgroups of the row kernel's launch, of the tile kernel's that split
     // a launch's workspace: partial sums [workgroup][2][rows of a tile][DP], their (maximum, weight), arrivals of a tile's
     // parts at the workgroup it starts in (zero between calls)
     float* ws_o;
@@ -76,6 +78,7 @@ struct PaShape {
 };
 PaShape paged_shape(const PaParams& p, int64_t max_rows);
 int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s);
+bool paged_tile_takes(const PaParams& p);
 int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s);
 
 constexpr int PA_CUS = 256;

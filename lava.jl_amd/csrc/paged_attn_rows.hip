@@ -41,8 +41,8 @@ __device__ __forceinline__ float pr_max4(float x) {   // over the four lanes of 
 }
 
 // DP: the head dimension rounded up to 64, 128 or 256; a tile is 16 NR rows.
-template <typename T, int DP, int NR>
-__global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_rows_kernel(PaParams p) {
+template <typename T, int DP, int NR, bool PRE>
+__global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_rows_kernel(PaParams) {
     typedef PgType<T> TT;
     typedef typename TT::v8 v8;
     typedef typename TT::v4 v4;
@@ -66,10 +66,12 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r16 = lane & 15, g = lane >> 4;
 
-    const PaPlan plan = pa_plan<PR_BK, false>(p, R, true, p.stack == 1, lane);
-    const uint32_t total = __builtin_amdgcn_readfirstlane(plan.total);
-    const uint32_t per = pa_per(total, gridDim.x), wg = pa_place(gridDim.x);
-    const uint32_t begin = min(total, wg * per), stop = min(total, begin + per);
+    PaArgs args;
+    args.load(lane);
+    const PaParams p = args.get();
+    const PaPlan plan = pa_plan<PR_BK, false, PRE>(p, R, true, PRE && p.stack == 1, lane);
+    const uint32_t per = pa_per(plan.total, p.by_rows), wg = blockIdx.x;
+    const uint32_t begin = min(plan.total, wg * per), stop = min(plan.total, begin + per);
     if (begin >= stop) return;
 
     // LDS-DMA: lane offsets within 8 keys, by the parity of the 8 and the instruction
@@ -100,61 +102,51 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
 
     for (uint32_t at = begin; at < stop;) {
         // ---- the segment: a row tile of a sequence (or of the stacked prefix), some of its blocks
-        uint32_t before;
-        const int b = __builtin_amdgcn_readfirstlane(pa_locate<PR_BK, false>(p, plan, R, at, lane, before));
-        before = __builtin_amdgcn_readfirstlane(before);
-        PagedSeq seq = {plan.t0, plan.t1 - plan.t0, 0};
-        PaSeq sw = plan.prefix;
-        if (b >= 0) {
-            seq = paged_seq(p.b, b);
-            sw = pa_seq<PR_BK, false>(p, seq, R);
-        }
-        const int nb = __builtin_amdgcn_readfirstlane(sw.nb), np = __builtin_amdgcn_readfirstlane(sw.np);
-        const int p0 = __builtin_amdgcn_readfirstlane(sw.p0), o0 = __builtin_amdgcn_readfirstlane(sw.o0);
-        const uint32_t tiles = __builtin_amdgcn_readfirstlane(sw.tiles);
-        const uint32_t rel = at - before, ht = rel / (uint32_t)nb;
-        const int blk0 = (int)(rel - ht * (uint32_t)nb);
-        const int head = (int)(ht / tiles), tile = (int)(ht - (uint32_t)head * tiles);
+        const PaParams p = args.get();
+        const PaSegment sg = pa_segment<PR_BK, false, PRE>(p, plan, R, at, lane);
+        const int b = sg.b, nb = sg.sw.nb, np = PRE ? sg.sw.np : 0, p0 = sg.sw.p0, o0 = sg.sw.o0;
+        const int head = sg.head, tile = sg.tile, blk0 = sg.blk0, kv = sg.seq.kv, rows = sg.seq.n * p.G;
         const int nblk = min(nb - blk0, (int)(stop - at));
-        const int kv = __builtin_amdgcn_readfirstlane(seq.kv);
-
         // rows of a sequence that another launch takes, prefix and all
-        if (b < 0 && pa_other(p, seq.first + tile * R / p.G, seq.first + min(seq.n - 1, (tile * R + R - 1) / p.G), lane)) {
+        if (PRE && b < 0 && pa_other(p, sg.seq.first + tile * R / p.G, sg.seq.first + min(sg.seq.n - 1, (tile * R + R - 1) / p.G), lane)) {
             at += (uint32_t)nblk;
             continue;
         }
 
-        // ---- the rows of this lane
+        // ---- the rows of this lane; the last position that the first row sees and the first that the last one does
+        // bound what needs comparing (rows are in order of their positions)
         v8 qf[NR][NKS];
         int row_t[NR], row_h[NR], lo[NR], hi[NR];
         float pos[NR], slope[NR];
         bool live[NR];
-        int lo_max = 0, hi_min = 0x7fffffff;
-        const int bid = (b >= 0 && p.bidir) ? p.bidir[b] : 0;
+        const int bid = p.bidir && b >= 0 ? p.bidir[b] : 0;
+        const int end = PRE ? p.P + kv : kv, pos0 = end - sg.seq.n;   // of a prefix tile: P
+        int lo_max = pa_range(p, pos0 + (int)div_of((uint32_t)min(tile * R + R - 1, rows - 1), p.by_g), end, bid).lo;
+        int hi_min = pa_range(p, pos0 + (int)div_of((uint32_t)(tile * R), p.by_g), end, bid).hi;
+        if (PRE && b < 0) {
+            lo_max = plan.plain ? 0 : 0x7fffffff;
+            hi_min = p.P - 1;
+        }
+        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+        hi_min = __builtin_amdgcn_readfirstlane(hi_min);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             const uint32_t row = (uint32_t)(tile * R + 16 * nr + r16);
             const int i = (int)div_of(row, p.by_g);
-            live[nr] = i < seq.n;
-            row_t[nr] = seq.first + i;
-            row_h[nr] = head * p.G + (int)(row - (uint32_t)(i * p.G));
-            int end = p.P + kv, at_pos = end - seq.n + i;
-            lo[nr] = 0;
-            hi[nr] = 0x7fffffff;
-            if (b < 0) {
-                end = p.P;
+            live[nr] = (int)row < rows;
+            row_t[nr] = sg.seq.first + i;
+            row_h[nr] = head * p.G + (int)row - i * p.G;
+            int at_pos = pos0 + i;
+            if (PRE && b < 0) {
                 at_pos = p.P;
                 if ((!plan.plain || p.slopes) && live[nr]) at_pos = pa_row_pos(p, row_t[nr]);
             }
-            if (live[nr]) {
-                const PaRange rg = pa_range(p, at_pos, end, bid);
-                lo[nr] = rg.lo;
-                hi[nr] = rg.hi;
-            }
+            const PaRange rg = pa_range(p, at_pos, end, bid);
+            lo[nr] = rg.lo;
+            hi[nr] = rg.hi;
             pos[nr] = (float)at_pos;
-            slope[nr] = (p.slopes && live[nr]) ? p.slopes[row_h[nr]] * PA_LOG2E : 0.f;
-            lo_max = max(lo_max, lo[nr]);
-            hi_min = min(hi_min, hi[nr]);
+            slope[nr] = 0.f;
+            if (p.slopes && live[nr]) slope[nr] = p.slopes[row_h[nr]] * PA_LOG2E;
             const T* qr = (const T*)p.Q + (int64_t)row_t[nr] * p.qst + (int64_t)row_h[nr] * p.qsh + 8 * g;
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
@@ -162,58 +154,6 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                 if (live[nr] && 32 * ks + 8 * g < p.c.D) qf[nr][ks] = *reinterpret_cast<const v8*>(qr + 32 * ks);
             }
         }
-        for (int i = 1; i < 16; i *= 2) {
-            lo_max = max(lo_max, __shfl_xor(lo_max, i, 64));
-            hi_min = min(hi_min, __shfl_xor(hi_min, i, 64));
-        }
-        lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-        hi_min = __builtin_amdgcn_readfirstlane(hi_min);
-
-        // ---- this wavefront's tile of block j: where its keys are
-        struct Tile {
-            int page[4], row[4], n[4];   // per 8 keys: the page (-1: none), the row in it, keys below the end
-            int pos;                     // position of the first key
-            int last;                    // of the source's last key
-        };
-        const pg_table own = (pg_table)(uintptr_t)(p.b.table + (int64_t)max(b, 0) * p.b.max_pages);
-        const pg_table shared = (pg_table)(uintptr_t)p.ppages;
-        auto lookup = [&](int j) __attribute__((always_inline)) {
-            Tile t;
-            const int blk = blk0 + j;
-            const bool pre = blk < np;
-            const int key0 = (pre ? p0 + blk : o0 + blk - np) * PR_BK + 32 * w;
-            const int len = j < nblk ? (pre ? p.P : kv) : 0;
-            t.pos = key0 + (pre ? 0 : p.P);
-            t.last = pre ? p.P - 1 : p.P + kv - 1;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = key0 + 8 * i;
-                t.n[i] = min(max(len - k, 0), 8);
-                t.page[i] = 0;
-                t.row[i] = 0;
-                if (t.n[i] > 0) {
-                    const int no = (int)div_of((uint32_t)k, p.c.by_page);
-                    t.row[i] = k - no * p.c.page;
-                    const int pg = pre ? shared[no] : own[no];
-                    t.page[i] = (uint32_t)pg < (uint32_t)p.c.pages ? pg : -1;
-                }
-            }
-            return t;
-        };
-        auto request = [&](const Tile& t, bool is_k) __attribute__((always_inline)) {
-            const T* base = (const T*)(is_k ? p.c.k : p.c.v) + (int64_t)head * p.c.sh;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool none = t.page[i] < 0 || t.n[i] == 0;
-                const T* at8 = base + (none ? 0 : (int64_t)t.page[i] * p.c.sp + (int64_t)t.row[i] * p.c.sl);
-                const uint32_t bytes = none ? 0u : (uint32_t)(t.n[i] - 1) * row_bytes + 2u * (uint32_t)p.c.D;
-                const v4i rs = make_rsrc(at8, bytes);
-#pragma unroll
-                for (int u = 0; u < IPG; ++u)
-                    dma16(rs, is_k ? ofs_k[i & 1][u] : ofs_v[u], 0u,
-                          __builtin_amdgcn_readfirstlane((is_k ? lds_k : lds_v) + 1024u * (uint32_t)(i * IPG + u)));
-            }
-        };
 
         // Q and the slopes are used here, so that the compiler waits for their loads now and not in the loop, where its
         // wait (it does not count the DMAs) would be for everything in flight
@@ -236,6 +176,49 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             for (int dt = 0; dt < NDT; ++dt) o[dt][nr] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         __syncthreads();   // the segment before has left the ring and the statistics
+        {
+        const PaParams p = args.get();
+        // ---- this wavefront's tiles, 32 keys of a block
+        PaPages<4, PRE> pages;
+        auto where = [&](int j, int i, int& k, bool& pre) {
+            const int blk = blk0 + j;
+            pre = PRE && blk < np;
+            k = (pre ? p0 + blk : o0 + blk - np) * PR_BK + 32 * w + 8 * i;
+            return j < nblk && k < (pre ? p.P : kv);
+        };
+        pages.load(p, b, 0, lane, where);
+        pages.ofs[1] = -1;
+        if (nblk + 1 >= decltype(pages)::TPC) pages.load(p, b, 1, lane, where);   // lookups run two tiles ahead
+        struct Tile {
+            int64_t at[4];   // per 8 keys, -1: none
+            int left;        // keys from the first to the end of the source
+            int pos;         // position of the first key
+        };
+        auto lookup = [&](int j) __attribute__((always_inline)) {
+            Tile t;
+            const int blk = blk0 + j;
+            const bool pre = PRE && blk < np;
+            const int key0 = (pre ? p0 + blk : o0 + blk - np) * PR_BK + 32 * w;
+            t.pos = key0 + (pre || !PRE ? 0 : p.P);
+            t.left = (pre ? p.P : kv) - key0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t.at[i] = pages.get(j, i);
+            return t;
+        };
+        auto request = [&](const Tile& t, bool is_k) __attribute__((always_inline)) {
+            const T* base = (const T*)(is_k ? p.c.k : p.c.v) + (int64_t)head * p.c.sh;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t o = t.at[i];
+                const uint32_t bytes = o < 0 ? 0u : (uint32_t)(min(t.left - 8 * i, 8) - 1) * row_bytes + 2u * (uint32_t)p.c.D;
+                const v4i rs = make_rsrc(base + o, bytes);   // none: nothing in range
+#pragma unroll
+                for (int u = 0; u < IPG; ++u)
+                    dma16(rs, is_k ? ofs_k[i & 1][u] : ofs_v[u], 0u,
+                          __builtin_amdgcn_readfirstlane((is_k ? lds_k : lds_v) + 1024u * (uint32_t)(i * IPG + u)));
+            }
+        };
+
         Tile now = lookup(0), next = lookup(1);
         request(now, true);
         request(now, false);
@@ -257,14 +240,15 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K's place is read
             request(next, true);
 
-            const int first = now.pos, none = (now.page[0] < 0) | (now.page[1] < 0) << 1 | (now.page[2] < 0) << 2 | (now.page[3] < 0) << 3;
-            const bool cut = none != 0 || first < lo_max || first + 31 > min(hi_min, now.last);
+            const int first = now.pos, none = (now.at[0] < 0) | (now.at[1] < 0) << 1 | (now.at[2] < 0) << 2 | (now.at[3] < 0) << 3;
+            const int end_pos = first + now.left - 1;   // the source's last key
+            const bool cut = none != 0 || first < lo_max || first + 31 > min(hi_min, end_pos);
             float up[NR];
             bool move = false;
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
                 float top = -INFINITY;
-                const int last = min(hi[nr], now.last);
+                const int last = min(hi[nr], end_pos);
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -316,7 +300,11 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // V's place is read
             request(next, false);
             now = next;
+            if ((j + 2) % decltype(pages)::TPC == 0 && j + 2 >= decltype(pages)::TPC)
+                pages.load(p, b, (j + 2) / decltype(pages)::TPC + 1, lane, where);   // into the place of the chunk just left
             next = lookup(j + 2);
+        }
+
         }
 
         // ---- the four wavefronts' parts together, two row sixteens at a time through the ring
@@ -344,7 +332,8 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             for (int i = 0; i < 4; ++i) ll[nr] += s4[i].y * __builtin_amdgcn_exp2f(s4[i].x - sub);
             f[nr] = __builtin_amdgcn_exp2f(m[nr] - sub);
         }
-        const bool whole = nblk == nb, direct = whole && !p.stack;
+        const PaParams e = args.get();
+        const bool whole = nblk == nb, direct = whole && !(PRE && e.stack);
         constexpr int NH = NR < 2 ? 1 : 2;
         const uint32_t box = lds_addr(&ring[0][0][0]) + 16u * (uint32_t)lane;
 #pragma unroll
@@ -359,13 +348,13 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
 #pragma unroll
             for (int u = 0; u < NH; ++u) {
                 const int nr = n0 + u;
-                const int64_t out_row = (int64_t)row_t[nr] * p.Hq + row_h[nr];
+                const int64_t out_row = (int64_t)row_t[nr] * e.Hq + row_h[nr];
                 const float inv = ll[nr] == 0.f ? 0.f : 1.f / ll[nr];
-                T* orow = (T*)p.O + (int64_t)row_t[nr] * p.ost + (int64_t)row_h[nr] * p.osh + 4 * g;
-                const int64_t part = whole ? (b < 0 ? 0 : (int64_t)p.b.T * p.Hq) + out_row
+                T* orow = (T*)e.O + (int64_t)row_t[nr] * e.ost + (int64_t)row_h[nr] * e.osh + 4 * g;
+                const int64_t part = whole ? (b < 0 ? 0 : (int64_t)e.b.T * e.Hq) + out_row
                                            : (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * R + 16 * nr + r16;
-                float* prow = (whole ? p.row_o : p.ws_o) + part * DP + 4 * g;
-                float2* pml = (whole ? p.row_ml : p.ws_ml) + part;
+                float* prow = (whole ? e.row_o : e.ws_o) + part * DP + 4 * g;
+                float2* pml = (whole ? e.row_ml : e.ws_ml) + part;
 #pragma unroll
                 for (int d4 = 0; d4 < NDT / 4; ++d4) {
                     const int dt = 4 * d4 + w;
@@ -375,7 +364,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                     if (!live[nr]) continue;
                     if (direct) {
                         const v4 y = {(T)(x[0] * inv), (T)(x[1] * inv), (T)(x[2] * inv), (T)(x[3] * inv)};
-                        if (16 * dt + 4 * g < p.c.D) *reinterpret_cast<v4*>(orow + 16 * dt) = y;
+                        if (16 * dt + 4 * g < e.c.D) *reinterpret_cast<v4*>(orow + 16 * dt) = y;
                     } else {
                         pa_put(prow + 16 * dt, x[0], x[1]);
                         pa_put(prow + 16 * dt + 2, x[2], x[3]);
@@ -383,16 +372,16 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                 }
                 if (live[nr] && w == 0 && g == 0) {
                     if (direct) {
-                        if (p.lse) p.lse[out_row] = ll[nr] == 0.f ? -INFINITY : (ml[nr] + log2f(ll[nr])) * PA_LN2;
+                        if (e.lse) e.lse[out_row] = ll[nr] == 0.f ? -INFINITY : (ml[nr] + log2f(ll[nr])) * PA_LN2;
                     } else {
                         pa_put((float*)pml, ml[nr], ll[nr]);
                     }
                 }
             }
         }
-        if (!whole && p.stack == 0) {
-            const uint32_t a = before + ht * (uint32_t)nb;   // the tile's first block
-            pa_arrive<T, DP, 4>(p, a / per, (a + (uint32_t)nb - 1) / per, R, min(R, seq.n * p.G - tile * R), tile * R, seq.first,
+        if (!whole && !(PRE && e.stack)) {
+            const uint32_t a = at - (uint32_t)blk0;   // the tile's first block
+            pa_arrive<T, DP, 4>(e, a / per, (a + (uint32_t)nb - 1) / per, R, min(R, rows - tile * R), tile * R, sg.seq.first,
                                 head, w, lane, &arrived);
         }
         at += (uint32_t)nblk;
@@ -402,7 +391,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
 // Behind a stacked prefix: a row's parts, the prefix's and its sequence's, each in the order of its keys.  One
 // wavefront a row.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, uint32_t row_grid, int pre_R) {
+__global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, int pre_R) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= (int64_t)p.b.T * p.Hq) return;
@@ -435,27 +424,23 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, uint
         x.ml = whole ? p.row_ml + i : ml;
         return x;
     };
-    const PaPlan plan = pa_plan<PR_BK, false>(p, R, true, p.stack == 1, lane);
-    uint32_t before = plan.prefix.work;
+    const PaPlan plan = pa_plan<PR_BK, false, true>(p, R, true, p.stack == 1, lane);
+    uint32_t before = plan.pre_work;
     for (int b0 = 0; b0 < b; b0 += 64) {
-        uint32_t upto = plan.upto;
-        if (b0 > 0) {
-            uint32_t work = 0;
-            if (b0 + lane < p.b.B) work = pa_seq<PR_BK, false>(p, paged_seq(p.b, b0 + lane), R).work;
-            upto = pa_scan(work, lane);
-        }
+        const uint32_t upto =
+            b0 == 0 ? plan.upto : pa_scan(pa_work(p, pa_seq<PR_BK, false, true>(p, pa_lane_seq(p, b0 + lane), R)));
         before += __builtin_amdgcn_readlane(upto, min(b - b0, 64) - 1);
     }
-    const uint32_t per = pa_per(plan.total, row_grid);
-    const Source own = source(pa_seq<PR_BK, false>(p, s, R), before, per, R, (uint32_t)((t - s.first) * p.G + g), p.ws_o, p.ws_ml, 1);
+    const uint32_t per = pa_per(plan.total, p.by_rows);
+    const Source own = source(pa_seq<PR_BK, false, true>(p, s, R), before, per, R, (uint32_t)((t - s.first) * p.G + g), p.ws_o, p.ws_ml, 1);
     Source pre = own;
     pre.n = 0;
     if (p.stack == 1) {
-        if (plan.prefix.work > 0) pre = source(plan.prefix, 0, per, R, (uint32_t)((t - plan.t0) * p.G + g), p.ws_o, p.ws_ml, 0);
+        if (plan.pre_work > 0) pre = source(plan.prefix, 0, per, R, (uint32_t)((t - plan.t0) * p.G + g), p.ws_o, p.ws_ml, 0);
     } else {
-        const PaPlan pp = pa_plan<PT_BK, true>(p, pre_R, false, true, lane);
-        if (pp.prefix.work > 0)
-            pre = source(pp.prefix, 0, pa_per(pp.total, PT_GRID), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
+        const PaPlan pp = pa_plan<PT_BK, true, true>(p, pre_R, false, true, lane);
+        if (pp.pre_work > 0)
+            pre = source(pp.prefix, 0, pa_per(pp.total, p.by_tiles), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
     }
     float o[DP / 64], m, l;
     pa_join_row<DP>(pre.n + own.n, [&](int j) { return j < pre.n ? pre.ml + pre.at(j) : own.ml + own.at(j - pre.n); },
@@ -467,17 +452,25 @@ int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream
     auto by_type = [&](auto tag) {
         typedef decltype(tag) T;
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(sh.row_grid), dim3(256), 0, s, p); };
-        if (sh.dp == 64)
-            sh.nr == 1 ? go(paged_rows_kernel<T, 64, 1>) : sh.nr == 2 ? go(paged_rows_kernel<T, 64, 2>) : go(paged_rows_kernel<T, 64, 4>);
-        else if (sh.dp == 128)
-            sh.nr == 1 ? go(paged_rows_kernel<T, 128, 1>) : sh.nr == 2 ? go(paged_rows_kernel<T, 128, 2>) : go(paged_rows_kernel<T, 128, 4>);
-        else
-            sh.nr == 1 ? go(paged_rows_kernel<T, 256, 1>) : go(paged_rows_kernel<T, 256, 2>);
+        auto by_shape = [&](auto pre) {
+            constexpr bool PRE = decltype(pre)::value;
+            if (sh.dp == 64)
+                sh.nr == 1   ? go(paged_rows_kernel<T, 64, 1, PRE>)
+                : sh.nr == 2 ? go(paged_rows_kernel<T, 64, 2, PRE>)
+                             : go(paged_rows_kernel<T, 64, 4, PRE>);
+            else if (sh.dp == 128)
+                sh.nr == 1   ? go(paged_rows_kernel<T, 128, 1, PRE>)
+                : sh.nr == 2 ? go(paged_rows_kernel<T, 128, 2, PRE>)
+                             : go(paged_rows_kernel<T, 128, 4, PRE>);
+            else
+                sh.nr == 1 ? go(paged_rows_kernel<T, 256, 1, PRE>) : go(paged_rows_kernel<T, 256, 2, PRE>);
+        };
+        p.P > 0 ? by_shape(pg_tag<true>{}) : by_shape(pg_tag<false>{});
         int rc = check_launch("paged_rows_kernel");
         if (rc != LAVA_HIP_OK || p.stack == 0) return rc;
         const unsigned rows = (unsigned)(((int64_t)p.b.T * p.Hq + 3) / 4);
         auto join = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, sh.row_grid, 128 * sh.pre_qh);
+            hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, 128 * sh.pre_qh);
         };
         sh.dp == 64 ? join(paged_join_kernel<T, 64>) : sh.dp == 128 ? join(paged_join_kernel<T, 128>) : join(paged_join_kernel<T, 256>);
         return check_launch("paged_join_kernel");

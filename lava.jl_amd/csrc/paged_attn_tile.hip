@@ -25,8 +25,8 @@ constexpr int PT_KST = 3, PT_VST = 2;   // LDS stages
 constexpr int PT_PF = 4;                // fragments read ahead of their MFMA
 constexpr float PT_RESCALE = 8.f;
 
-template <typename T, int DE, int QH, int MODE>
-__global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams p, int prefix) {
+template <typename T, int DE, int QH, int MODE, bool PRE>
+__global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams, int stacked) {
     typedef PgType<T> TT;
     typedef typename TT::v8 v8;
     typedef typename TT::v4 v4;
@@ -54,36 +54,65 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
     const int pr = w & (PT_PAIRS - 1);
     const int r32 = lane & 31, h = lane >> 5;
 
+    const bool prefix = PRE && stacked != 0;   // the launch for the stacked prefix
     // ---- which part of the work.  Tiles one by one, a workgroup each, where the longest does not outlast the rest by more
     // than splitting costs (parts written and joined, about 12 blocks' time, and blocks that only a sequence's
     // last tiles see counted for all); else the even split over PT_GRID workgroups.
-    const PaPlan plan = pa_plan<PT_BK, true>(p, BQ, !prefix, prefix, lane);
-    const bool by_tile = !prefix && plan.longest / 2 <= 12 + (int)((plan.total - min(plan.total, plan.seen)) / PA_CUS);
-    uint32_t at = 0, stop = 1, per = 1, wg = 0, before = 0;
-    int tb = -1, t_head = 0, t_tile = 0;
+    PaArgs args;
+    args.load(lane);
+    const PaParams p = args.get();
+    const PaPlan plan = pa_plan<PT_BK, true, PRE>(p, BQ, !prefix, prefix, lane);
+    bool by_tile = false;
+    int tiles_upto = 0;   // lane i: row tiles of sequences 0 .. i
+    if (!prefix) {
+        int longest = 0;
+        uint32_t seen = 0;
+        for (int b0 = 0; b0 < p.b.B; b0 += 64) {
+            const PagedSeq s = b0 == 0 ? plan.mine : pa_lane_seq(p, b0 + lane);
+            const PaSeq q = pa_seq<PT_BK, true, PRE>(p, s, BQ);
+            longest = max(longest, q.nb);
+            seen += q.tiles > 0 ? (uint32_t)q.tiles * (uint32_t)(q.nb + pa_first_nb<PT_BK>(p, s, q)) / 2u * (uint32_t)p.c.heads : 0u;
+            if (b0 == 0) tiles_upto = (int)pa_scan((uint32_t)q.tiles);
+        }
+        longest = pa_wave_max(longest);
+        by_tile = longest <= 24;
+        if (!by_tile) {
+            seen = __builtin_amdgcn_readlane(pa_scan(seen), 63);
+            by_tile = longest / 2 <= 12 + (int)((plan.total - min(plan.total, seen)) / PA_CUS);
+        }
+    }
+    uint32_t at = 0, stop = 1, per = 1, wg = 0;
+    PaSegment sg = {};
     if (by_tile) {
         // key heads innermost, so that an XCD's workgroups share few heads' keys; a sequence's last tiles, which
         // see the most keys, first
-        t_head = (int)(blockIdx.x % (unsigned)p.c.heads);
         int idx = (int)(blockIdx.x / (unsigned)p.c.heads);
-        for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-            int tiles = 0;
-            if (b0 + lane < p.b.B) tiles = pa_seq<PT_BK, true>(p, paged_seq(p.b, b0 + lane), BQ).tiles;
-            const int upto = (int)pa_scan((uint32_t)tiles, lane);
+        sg.head = (int)blockIdx.x - idx * p.c.heads;
+        sg.b = -1;
+        int upto = tiles_upto;
+        PagedSeq s = plan.mine;
+        for (int b0 = 0;;) {
             const uint64_t past = __builtin_amdgcn_ballot_w64(upto > idx);
             if (past != 0) {
                 const int i = __builtin_ctzll(past);
-                const int lower = i > 0 ? __builtin_amdgcn_readlane(upto, i - 1) : 0;
-                tb = b0 + i;
-                t_tile = __builtin_amdgcn_readlane(upto, i) - 1 - (idx - lower) - lower;   // from the last one down
+                sg.b = b0 + i;
+                sg.tile = __builtin_amdgcn_readlane(upto, i) - 1 - idx;   // from the last one down
+                sg.seq.first = __builtin_amdgcn_readlane(s.first, i);
+                sg.seq.n = __builtin_amdgcn_readlane(s.n, i);
+                sg.seq.kv = __builtin_amdgcn_readlane(s.kv, i);
                 break;
             }
             idx -= __builtin_amdgcn_readlane(upto, 63);
+            b0 += 64;
+            if (b0 >= p.b.B) break;
+            s = pa_lane_seq(p, b0 + lane);
+            upto = (int)pa_scan((uint32_t)pa_seq<PT_BK, true, PRE>(p, s, BQ).tiles);
         }
-        if (tb < 0) return;
+        if (sg.b < 0) return;
+        sg.sw = pa_seq<PT_BK, true, PRE>(p, sg.seq, BQ);
     } else {
         if (blockIdx.x >= PT_GRID) return;
-        per = pa_per(plan.total, PT_GRID);
+        per = pa_per(plan.total, p.by_tiles);
         wg = pa_place(PT_GRID);
         at = min(plan.total, wg * per);
         stop = min(plan.total, at + per);
@@ -91,43 +120,24 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
 
     for (; at < stop;) {
     // ---- the segment: some key blocks of a row tile
-    int b = tb;
-    PagedSeq seq = {plan.t0, plan.t1 - plan.t0, 0};
-    PaSeq sw = plan.prefix;
-    if (!by_tile) b = pa_locate<PT_BK, true>(p, plan, BQ, at, lane, before);
-    b = __builtin_amdgcn_readfirstlane(b);
-    if (b >= 0) {
-        seq = paged_seq(p.b, b);
-        sw = pa_seq<PT_BK, true>(p, seq, BQ);
-    }
-    seq.first = __builtin_amdgcn_readfirstlane(seq.first);
-    seq.n = __builtin_amdgcn_readfirstlane(seq.n);
-    seq.kv = __builtin_amdgcn_readfirstlane(seq.kv);
-    const int nb = __builtin_amdgcn_readfirstlane(sw.nb), np = __builtin_amdgcn_readfirstlane(sw.np);
-    const int p0 = __builtin_amdgcn_readfirstlane(sw.p0), o0 = __builtin_amdgcn_readfirstlane(sw.o0);
-    int head = t_head, tile = t_tile, blk0 = 0, nseg = nb;
-    if (!by_tile) {
-        const uint32_t rel = at - before, ht = rel / (uint32_t)nb;
-        blk0 = (int)(rel - ht * (uint32_t)nb);
-        head = (int)(ht / (uint32_t)sw.tiles);
-        tile = (int)(ht - (uint32_t)head * (uint32_t)sw.tiles);
-        nseg = min(nb - blk0, (int)(stop - at));
-    }
-    head = __builtin_amdgcn_readfirstlane(head);
-    tile = __builtin_amdgcn_readfirstlane(tile);
-    blk0 = __builtin_amdgcn_readfirstlane(blk0);
-    nseg = __builtin_amdgcn_readfirstlane(nseg);
+    const PaParams p = args.get();
+    if (!by_tile) sg = pa_segment<PT_BK, true, PRE>(p, plan, BQ, at, lane);
+    const PagedSeq seq = sg.seq;
+    const int b = sg.b, nb = sg.sw.nb, np = PRE ? sg.sw.np : 0, p0 = sg.sw.p0, o0 = sg.sw.o0;
+    const int head = __builtin_amdgcn_readfirstlane(sg.head), tile = __builtin_amdgcn_readfirstlane(sg.tile), blk0 = sg.blk0;
+    const int nseg = by_tile ? nb : min(nb - blk0, (int)(stop - at));
     const bool whole = nseg == nb;
     const int rows = seq.n * p.G;
     // rows of a sequence that another launch takes, prefix and all
-    if (b < 0 && pa_other(p, seq.first + tile * BQ / p.G, seq.first + min(seq.n - 1, (tile * BQ + BQ - 1) / p.G), lane)) {
+    if (PRE && b < 0 && pa_other(p, seq.first + tile * BQ / p.G, seq.first + min(seq.n - 1, (tile * BQ + BQ - 1) / p.G), lane)) {
         at += (uint32_t)nseg;
         continue;
     }
-    const int end = b < 0 ? p.P : p.P + seq.kv;
+    const int P = PRE ? p.P : 0;
+    const int end = P + (b < 0 ? 0 : seq.kv);
     const int bid = b >= 0 && p.bidir ? p.bidir[b] : 0;
-    auto block_of = [&](int pos) { return pos < p.P ? pos / PT_BK - p0 : np + (pos - p.P) / PT_BK - o0; };
-    auto first_pos = [&](int blk) { return blk < np ? (p0 + blk) * PT_BK : p.P + (o0 + blk - np) * PT_BK; };
+    auto block_of = [&](int pos) { return PRE && pos < P ? pos / PT_BK - p0 : np + (pos - P) / PT_BK - o0; };
+    auto first_pos = [&](int blk) { return PRE && blk < np ? (p0 + blk) * PT_BK : P + (o0 + blk - np) * PT_BK; };
     // of rows [r0, r1], in order of their positions, the blocks that some row sees
     auto sees = [&](int r0, int r1, int& f, int& l) {
         const int a = (int)div_of((uint32_t)r0, p.by_g), z = (int)div_of((uint32_t)min(r1, rows - 1), p.by_g);
@@ -158,28 +168,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
     }
     jf = __builtin_amdgcn_readfirstlane(jf);
     jl = __builtin_amdgcn_readfirstlane(jl);
-    // this lane's rows
-    int row_t[QH], row_h[QH], r_lo[QH], r_hi[QH];
-    float r_pos[QH];
-    bool live[QH];
-#pragma unroll
-    for (int qh = 0; qh < QH; ++qh) {
-        const int row = row0 + 32 * qh + r32;
-        const int i = (int)div_of((uint32_t)row, p.by_g);
-        live[qh] = row < rows;
-        row_t[qh] = seq.first + i;
-        row_h[qh] = head * p.G + row - i * p.G;
-        int pos = end - seq.n + i;
-        if (b < 0) {
-            pos = p.P;
-            if ((!plan.plain || p.slopes) && live[qh]) pos = pa_row_pos(p, row_t[qh]);
-        }
-        const PaRange rg = pa_range(p, pos, end, bid);
-        r_lo[qh] = live[qh] ? rg.lo : 0;
-        r_hi[qh] = live[qh] ? rg.hi : 0x7fffffff;
-        r_pos[qh] = (float)pos;
-    }
-
     const uint32_t p_lane = lds_addr(&pbuf[0][0][0]) + (uint32_t)pr * PBUF + 16u * lane;
     auto paddr = [&](int buf, int kt, int ks, int qh) __attribute__((always_inline)) -> uint32_t {
         return p_lane + (uint32_t)(buf * PT_PAIRS * PBUF + ((kt * 2 + ks) * QH + qh) * 1024);
@@ -187,38 +175,78 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
 
     if (is_s) {
         // ================= score wavefront =================
-        v8 qf[QH][NKS];
-        float slope[QH] = {};
+        // The pair's rows of Q by LDS-DMA, 4 whole rows an instruction, into its P buffers (free until the first block's P), in
+        // the K tile's layout; 32 rows x 32 bytes a load straight into the fragments took 8 us a tile.  Row offsets from
+        // the tile's first token and head fit 31 bits (paged_tile_takes).
+        const uint32_t qbuf = lds_addr(&pbuf[0][pr][0]);
+        auto q_row = [&](int r) { return qbuf + (uint32_t)(r / (16 * QH) * PT_PAIRS * PBUF + r % (16 * QH) * RB); };
+        {
+            const PaParams p = args.get();
+            const int lane = pa_again(threadIdx.x & 63);
+            const int i0 = (int)div_of((uint32_t)row0, p.by_g);
+            const T* base = (const T*)p.Q + (int64_t)(seq.first + i0) * p.qst + (int64_t)(head * p.G) * p.qsh;
+            const v4i rs = make_rsrc(base, 0x7fffffffu);
+            const uint32_t st = (uint32_t)p.qst * 2u, sh = (uint32_t)p.qsh * 2u;
 #pragma unroll
-        for (int qh = 0; qh < QH; ++qh) {
-            const T* qr = (const T*)p.Q + (int64_t)row_t[qh] * p.qst + (int64_t)row_h[qh] * p.qsh + 8 * h;
+            for (int i = 0; i < 8 * QH; ++i) {
+                const int r = 4 * i + lane / CH, row = row0 + r, c = (lane % CH) ^ (r & 15);
+                const int t = (int)div_of((uint32_t)row, p.by_g);
+                const uint32_t o = (uint32_t)(t - i0) * st + (uint32_t)(row - t * p.G) * sh + 16u * (uint32_t)c;
+                dma16(rs, row < rows && 8 * c < p.c.D ? o : OOB_OFS, 0u, __builtin_amdgcn_readfirstlane(q_row(4 * i)));
+            }
+        }
+        // this lane's rows: the positions that they see
+        int r_lo[QH], r_hi[QH];
+        float r_pos[QH], slope[QH];
+        {
+            const PaParams p = args.get();
+#pragma unroll
+            for (int qh = 0; qh < QH; ++qh) {
+                const int row = row0 + 32 * qh + r32, i = (int)div_of((uint32_t)row, p.by_g);
+                int pos = end - seq.n + i;
+                if (PRE && b < 0) {
+                    pos = P;
+                    if ((!plan.plain || p.slopes) && row < rows) pos = pa_row_pos(p, seq.first + i);
+                }
+                const PaRange rg = pa_range(p, pos, end, bid);
+                r_lo[qh] = rg.lo;
+                r_hi[qh] = rg.hi;
+                r_pos[qh] = (float)pos;
+                slope[qh] = 0.f;
+                if (MODE == 2 && p.slopes && row < rows) slope[qh] = p.slopes[head * p.G + row - i * p.G] * PA_LOG2E;
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        v8 qf[QH][NKS];   // Q^T: row row0 + 32 qh + r32, d = 16 ks + 8 h + [0, 8)
+#pragma unroll
+        for (int qh = 0; qh < QH; ++qh)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks)
+                qf[qh][ks] = *(const lds_v8*)(uintptr_t)(q_row(32 * qh + (r32 & 16)) + (uint32_t)((r32 & 15) * RB + (((2 * ks + h) ^ (r32 & 15)) << 4)));
+#pragma unroll
+        for (int qh = 0; qh < QH; ++qh)
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {
-                qf[qh][ks] = v8{};
-                if (live[qh] && 16 * ks + 8 * h < p.c.D) qf[qh][ks] = *reinterpret_cast<const v8*>(qr + 16 * ks);
+                const uint4 u = __builtin_bit_cast(uint4, qf[qh][ks]);
+                asm volatile("" ::"v"(u.x), "v"(u.y), "v"(u.z), "v"(u.w) : "memory");
             }
-            if (MODE == 2 && p.slopes && live[qh]) slope[qh] = p.slopes[row_h[qh]] * PA_LOG2E;
-        }
         if constexpr (MODE == 0) {
 #pragma unroll
             for (int qh = 0; qh < QH; ++qh)
 #pragma unroll
                 for (int ks = 0; ks < NKS; ++ks) pg_scale_f16(qf[qh][ks], p.mul);
         }
-        // bounds that every row of the pair shares: inside them no comparison
-        int in_lo = 0, in_hi = 0x7fffffff;
-#pragma unroll
-        for (int qh = 0; qh < QH; ++qh) {
-            in_lo = max(in_lo, r_lo[qh]);
-            in_hi = min(in_hi, r_hi[qh]);
-        }
-        for (int i = 1; i < 32; i *= 2) {
-            in_lo = max(in_lo, __shfl_xor(in_lo, i, 64));
-            in_hi = min(in_hi, __shfl_xor(in_hi, i, 64));
+        // between the first position that the pair's last row sees and the last that its first one does, no comparison
+        int in_lo = pa_range(p, end - seq.n + (int)div_of((uint32_t)min(row0 + PQ - 1, rows - 1), p.by_g), end, bid).lo;
+        int in_hi = pa_range(p, end - seq.n + (int)div_of((uint32_t)row0, p.by_g), end, bid).hi;
+        if (PRE && b < 0) {
+            in_lo = plan.plain ? 0 : 0x7fffffff;
+            in_hi = P - 1;
         }
         in_lo = __builtin_amdgcn_readfirstlane(in_lo);
         in_hi = __builtin_amdgcn_readfirstlane(in_hi);
 
+        const PaParams p = args.get();
         bool fast = MODE == 0;   // the maximum comes in through the product (wavefront-uniform)
         v8 ones{};
         ones[0] = h == 0 ? (T)1.f : (T)0.f;
@@ -264,7 +292,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
             }
             const int none = __builtin_amdgcn_readfirstlane(nn.x | nn.y << 2 | nn.z << 4 | nn.w << 6);
             const int pos0 = __builtin_amdgcn_readfirstlane(first_pos(e0 + j));
-            const int src_hi = e0 + j < np ? p.P - 1 : end - 1;
+            const int src_hi = PRE && e0 + j < np ? P - 1 : end - 1;
             if constexpr (MODE == 2) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -381,6 +409,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
         __syncthreads();
     } else {
         // ================= output wavefront =================
+        const PaParams p = args.get();
         const uint32_t row_bytes = (uint32_t)(p.c.sl * 2);
         uint32_t ofs_k[4], ofs_v[2];   // rows 4 i + lane / 16 of this wavefront's 16
 #pragma unroll
@@ -390,56 +419,42 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
             ofs_k[i] = 8 * ck < p.c.D ? (uint32_t)in8 * row_bytes + 16u * (uint32_t)ck : OOB_OFS;
             if (i < 2) ofs_v[i] = 8 * cv < p.c.D ? (uint32_t)in8 * row_bytes + 16u * (uint32_t)cv : OOB_OFS;
         }
-        struct Src {
-            int page[2], row[2], n[2];   // per 8 keys: the page (-1: none), the row in it, keys below the end
-        };
-        const pg_table own = (pg_table)(uintptr_t)(p.b.table + (int64_t)max(b, 0) * p.b.max_pages);
-        const pg_table shared = (pg_table)(uintptr_t)p.ppages;
-        auto lookup = [&](int j) __attribute__((always_inline)) {
-            Src t;
+        // blocks of 16 keys of this wavefront's
+        PaPages<2, PRE> pages;
+        auto where = [&](int j, int i, int& k, bool& pre) {
             const int blk = e0 + j;
-            const bool pre = blk < np;
-            const int key0 = (pre ? p0 + blk : o0 + blk - np) * PT_BK + 16 * pr;
-            const int len = j < nblk ? (pre ? p.P : seq.kv) : 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int k = key0 + 8 * i;
-                t.n[i] = min(max(len - k, 0), 8);
-                t.page[i] = 0;
-                t.row[i] = 0;
-                if (t.n[i] > 0) {
-                    const int no_ = (int)div_of((uint32_t)k, p.c.by_page);
-                    t.row[i] = k - no_ * p.c.page;
-                    const int pg = pre ? shared[no_] : own[no_];
-                    t.page[i] = (uint32_t)pg < (uint32_t)p.c.pages ? pg : -1;
-                }
-            }
-            return t;
+            pre = PRE && blk < np;
+            k = (pre ? p0 + blk : o0 + blk - np) * PT_BK + 16 * pr + 8 * i;
+            return j < nblk && k < (pre ? P : seq.kv);
         };
-        auto request = [&](const Src& t, bool is_k, int j) __attribute__((always_inline)) {
+        pages.load(p, b, 0, lane, where);
+        pages.ofs[1] = -1;
+        if (nblk + 3 > decltype(pages)::TPC) pages.load(p, b, 1, lane, where);   // requests run three blocks ahead
+        auto request = [&](bool is_k, int j) __attribute__((always_inline)) {
             const T* base = (const T*)(is_k ? p.c.k : p.c.v) + (int64_t)head * p.c.sh;
+            const int blk = e0 + j;
+            const bool pre = PRE && blk < np;
+            const int left = (pre ? P : seq.kv) - (pre ? p0 + blk : o0 + blk - np) * PT_BK - 16 * pr;   // keys to the end
             const uint32_t dst = lds_addr(is_k ? &kbuf[0][0] : &vbuf[0][0]) + (uint32_t)pr * 16 * RB +
                                  (uint32_t)(j % (is_k ? PT_KST : PT_VST)) * TILE;
+            int none = 0;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bool none = t.page[i] < 0 || t.n[i] == 0;
-                const T* at8 = base + (none ? 0 : (int64_t)t.page[i] * p.c.sp + (int64_t)t.row[i] * p.c.sl);
-                const v4i rs = make_rsrc(at8, none ? 0u : (uint32_t)(t.n[i] - 1) * row_bytes + 2u * (uint32_t)p.c.D);
+                const int64_t o = pages.get(j, i);
+                const uint32_t bytes = o < 0 ? 0u : (uint32_t)(min(left - 8 * i, 8) - 1) * row_bytes + 2u * (uint32_t)p.c.D;
+                const v4i rs = make_rsrc(base + o, bytes);   // none: nothing in range
+                none |= o < 0 ? 1 << i : 0;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     dma16(rs, is_k ? ofs_k[2 * i + u] : ofs_v[u], 0u,
                           __builtin_amdgcn_readfirstlane(dst + 1024u * (uint32_t)(2 * i + u)));
             }
-            if (is_k && lane == 0) nbuf[j % PT_KST][pr] = (t.page[0] < 0 ? 1 : 0) | (t.page[1] < 0 ? 2 : 0);
+            if (is_k && lane == 0) nbuf[j % PT_KST][pr] = none;
         };
-        Src sv = lookup(0), s1 = lookup(1), s2 = lookup(2);
-        request(sv, true, 0);
-        request(s1, true, 1);
-        request(s2, true, 2);
-        request(sv, false, 0);
-        Src sk = lookup(3);   // K of block j + 3 is next, V of block j + 1
-        sv = s1;
-        s1 = s2;
+        request(true, 0);
+        request(true, 1);
+        request(true, 2);
+        request(false, 0);
 
         uint32_t vb0[NDT];
         {
@@ -464,11 +479,10 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
         for (int j = 0; j < nblk; ++j) {
             const int buf = j & 1;
             // K_{j+3} into K_j's stage, V_{j+1} into V_{j-1}'s, both read in iteration j - 1
-            request(sk, true, j + 3);
-            request(sv, false, j + 1);
-            sv = s1;
-            s1 = sk;
-            sk = lookup(j + 4);
+            request(true, j + 3);
+            request(false, j + 1);
+            // V of chunk c - 1 is past when K is two blocks into chunk c
+            if ((j + 3) % decltype(pages)::TPC == 2 && j + 3 > decltype(pages)::TPC) pages.load(p, b, (j + 3) / decltype(pages)::TPC + 1, lane, where);
             if (j >= jf && j <= jl) {
                 if (fbuf[buf][pr] != 0) {   // the maximum moved at block j
                     float al[QH];
@@ -527,44 +541,105 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
             __syncthreads();
         }
         __syncthreads();   // the maxima are published
+        const PaParams e = args.get();
+        const int lane = pa_again(threadIdx.x & 63), r32 = lane & 31, h = lane >> 5;
+        // Rows leave through LDS, so that stores are of whole rows: 16 rows of 256 bytes at a time in each of this wavefront's
+        // parts of the K stages and the first V stage, which only it requests into again
+        auto o_row = [&](int r) {   // of 64 (32) rows in 16 bits; r / 16: the part
+            return (r < 48 ? lds_addr(&kbuf[0][0]) + (uint32_t)(r / 16 * TILE) : lds_addr(&vbuf[0][0])) + (uint32_t)((16 * pr + r % 16) * RB);
+        };
+        auto live = [&](int qh) { return row0 + 32 * qh + r32 < rows; };
+        auto out_row = [&](int row) {   // token * Hq + head
+            const int t = (int)div_of((uint32_t)row, e.by_g);
+            return (int64_t)(seq.first + t) * e.Hq + head * e.G + row - t * e.G;
+        };
+        float sum[QH];
 #pragma unroll
         for (int qh = 0; qh < QH; ++qh) {
             float a, c;
             pg_xor32_pair(l[qh], a, c);
-            const float sum = a + c, inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (!live[qh]) continue;
-            const int64_t out_row = (int64_t)row_t[qh] * p.Hq + row_h[qh];
-            if (whole && b >= 0) {
-                T* orow = (T*)p.O + (int64_t)row_t[qh] * p.ost + (int64_t)row_h[qh] * p.osh;
+            sum[qh] = a + c;
+        }
+        typedef __attribute__((address_space(3))) v4 lds_v4;
+        typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+        typedef float f2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) f2 lds_f2;
+        if (whole && b >= 0) {
+#pragma unroll
+            for (int qh = 0; qh < QH; ++qh) {
+                const float inv = sum[qh] == 0.f ? 0.f : 1.f / sum[qh];
+                const uint32_t to = o_row(32 * qh + (r32 & 16)) + (uint32_t)((r32 & 15) * RB + 8 * h);
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
-                        const int d = 32 * dt + 8 * g4 + 4 * h;
                         const v4 v = {(T)(o[dt][qh][4 * g4] * inv), (T)(o[dt][qh][4 * g4 + 1] * inv), (T)(o[dt][qh][4 * g4 + 2] * inv),
                                       (T)(o[dt][qh][4 * g4 + 3] * inv)};
-                        if (d < p.c.D) *reinterpret_cast<v4*>(orow + d) = v;
+                        *(lds_v4*)(uintptr_t)(to + (uint32_t)(((4 * dt + g4) ^ (r32 & 15)) << 4)) = v;
                     }
-                if (p.lse && h == 0) p.lse[out_row] = sum == 0.f ? -INFINITY : (mbuf[pr][32 * qh + r32] + log2f(sum)) * PA_LN2;
-            } else {
-                const int64_t part = whole ? out_row : (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * BQ + pr * PQ + 32 * qh + r32;
-                float* prow = (whole ? p.row_o : prefix ? p.pre_o : p.ws_o) + part * DE + 4 * h;
-                if (sum != 0.f) {
+                if (e.lse && live(qh) && h == 0)
+                    e.lse[out_row(row0 + 32 * qh + r32)] =
+                        sum[qh] == 0.f ? -INFINITY : (mbuf[pr][32 * qh + r32] + log2f(sum[qh])) * PA_LN2;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            const int cc = lane % CH;
+            const bool o16 = e.o16;   // rows of 16-byte pieces, else of 8
 #pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                        for (int g4 = 0; g4 < 4; ++g4) {
-                            pa_put(prow + 32 * dt + 8 * g4, o[dt][qh][4 * g4], o[dt][qh][4 * g4 + 1]);
-                            pa_put(prow + 32 * dt + 8 * g4 + 2, o[dt][qh][4 * g4 + 2], o[dt][qh][4 * g4 + 3]);
-                        }
+            for (int i = 0; i < 8 * QH; ++i) {
+                const int r = 4 * i + lane / CH, row = row0 + r;
+                const v8 v = *(const lds_v8*)(uintptr_t)(o_row(4 * i) + (uint32_t)((lane / CH) * RB + ((cc ^ (r & 15)) << 4)));
+                if (row < rows && 8 * cc < e.c.D) {
+                    const int t = (int)div_of((uint32_t)row, e.by_g);
+                    T* orow = (T*)e.O + (int64_t)(seq.first + t) * e.ost + (int64_t)(head * e.G + row - t * e.G) * e.osh + 8 * cc;
+                    if (o16) {
+                        *reinterpret_cast<v8*>(orow) = v;
+                    } else {
+                        *reinterpret_cast<v4*>(orow) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+                        *reinterpret_cast<v4*>(orow + 4) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+                    }
                 }
-                if (h == 0) pa_put((float*)((whole ? p.row_ml : prefix ? p.pre_ml : p.ws_ml) + part), mbuf[pr][32 * qh + r32], sum);
+            }
+        } else {
+            float* po = whole ? e.row_o : prefix ? e.pre_o : e.ws_o;
+            float2* pml = whole ? e.row_ml : prefix ? e.pre_ml : e.ws_ml;
+            const int64_t part0 = (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * BQ + pr * PQ;
+#pragma unroll
+            for (int qh = 0; qh < QH; ++qh) {
+                // 32 rows of sums, DE x 4 bytes: two rows' worth of LDS a row (8 rows a part at DE = 128)
+                constexpr int RF = DE * 4, RPP = 16 * RB / RF;
+                auto f_row = [&](int r) { return o_row(r / RPP * 16) + (uint32_t)(r % RPP * RF); };
+                constexpr int GO = RPP * 4 < 32 ? RPP * 4 : 32;   // rows the four parts hold
+                static_assert(GO == 32, "32 rows of sums fit the four parts");
+                const uint32_t to = f_row(r32) + 16u * (uint32_t)h;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int g4 = 0; g4 < 4; ++g4)   // 32-byte pieces, ^ row % 8 against bank conflicts
+                        *(lds_f32x4*)(uintptr_t)(to + (uint32_t)(((4 * dt + g4) ^ (r32 & 7)) << 5)) =
+                            f32x4{o[dt][qh][4 * g4], o[dt][qh][4 * g4 + 1], o[dt][qh][4 * g4 + 2], o[dt][qh][4 * g4 + 3]};
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                // a row (DE = 128) or two (64) an instruction, 8 bytes a lane; rows of no weight are not read again
+                constexpr int LPR = DE / 2, RPS = 64 / LPR;
+                const uint64_t some = __builtin_amdgcn_ballot_w64(sum[qh] != 0.f && live(qh));
+#pragma unroll 8
+                for (int r0 = 0; r0 < 32; r0 += RPS) {
+                    const int r = r0 + lane / LPR, x = lane % LPR;
+                    const f2 v = *(const lds_f2*)(uintptr_t)(f_row(r) + (uint32_t)(((x >> 2) ^ (r & 7)) << 5) + 8u * (uint32_t)(x & 3));
+                    const int row = row0 + 32 * qh + r;
+                    if ((some >> r) & 1) {
+                        const int64_t part = whole ? out_row(row) : part0 + 32 * qh + r;
+                        pa_put(po + part * DE + 2 * x, v.x, v.y);
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (live(qh) && h == 0)
+                    pa_put((float*)(pml + (whole ? out_row(row0 + 32 * qh + r32) : part0 + 32 * qh + r32)), mbuf[pr][32 * qh + r32], sum[qh]);
             }
         }
     }
     if (!whole && !prefix) {
-        const uint32_t a = before + ((uint32_t)head * (uint32_t)sw.tiles + (uint32_t)tile) * (uint32_t)nb;   // the tile's first block
-        pa_arrive<T, DE, 2 * PT_PAIRS>(p, a / per, (a + (uint32_t)nb - 1) / per, BQ, min(BQ, rows - tile * BQ), tile * BQ, seq.first,
+        const uint32_t a = at - (uint32_t)blk0;   // the tile's first block
+        pa_arrive<T, DE, 2 * PT_PAIRS>(args.get(), a / per, (a + (uint32_t)nb - 1) / per, BQ, min(BQ, rows - tile * BQ), tile * BQ, seq.first,
                                        head, w, lane, &arrived);
     }
     at += (uint32_t)nseg;
@@ -572,6 +647,11 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams 
 }
 
 // ---- host -----------------------------------------------------------------------------
+
+// Whether Q's offsets within a tile fit the addressing of its DMA.
+bool paged_tile_takes(const PaParams& p) {
+    return p.c.D <= 128 && (double)(128 * 2 / p.G + 2) * p.qst * 2.0 + (double)p.G * p.qsh * 2.0 + 256 < 2147483647.0;
+}
 
 int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s) {
     const bool plain = p.cap2 == 0.f && !p.slopes && p.mul > 0.f;
@@ -582,7 +662,10 @@ int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStre
     auto by_d = [&](auto type, auto q, auto mode) {
         typedef decltype(type) T;
         constexpr int QH = decltype(q)::value, MODE = decltype(mode)::value;
-        p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE>) : go(paged_tile_kernel<T, 128, QH, MODE>);
+        if (p.P > 0)
+            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE, true>) : go(paged_tile_kernel<T, 128, QH, MODE, true>);
+        else
+            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE, false>) : go(paged_tile_kernel<T, 128, QH, MODE, false>);
     };
     auto by_mode = [&](auto q) {
         if (dtype == LAVA_HIP_F16)

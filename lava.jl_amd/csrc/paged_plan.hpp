@@ -11,147 +11,212 @@
 
 namespace lava {
 
+// The kernel's parameters, its first argument, held in two registers' lanes: loaded once, and read back a lane a dword
+// where a phase of the kernel needs them.  Kept in scalar registers throughout they spill, and scalar loads of the kernel's
+// arguments at each phase, each of which goes to the host's memory, took 2 to 10 us a workgroup.
+struct PaArgs {
+    uint32_t a, b;   // lane i: dwords i and 64 + i
+    __device__ __forceinline__ void load(int lane) {
+        constexpr int N = sizeof(PaParams) / 4;
+        static_assert(sizeof(PaParams) % 4 == 0 && N > 64 && N <= 128, "two dwords a lane hold the parameters");
+        auto q = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+        a = q[lane];
+        b = q[64 + min(lane, N - 65)];
+    }
+    // as read in this phase: not hoisted from the loops around it
+    __device__ __forceinline__ PaParams get() {
+        constexpr int N = sizeof(PaParams) / 4;
+        struct {
+            uint32_t d[N];
+        } x;
+        asm volatile("" : "+v"(a), "+v"(b));
+#pragma unroll
+        for (int i = 0; i < N; ++i) x.d[i] = (uint32_t)__builtin_amdgcn_readlane((int)(i < 64 ? a : b), i & 63);
+        return __builtin_bit_cast(PaParams, x);
+    }
+};
+
+// x, as if newly computed: addresses made from it in one phase of a segment are not hoisted out of the loop over segments,
+// where they would take registers from the others.
+__device__ __forceinline__ int pa_again(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A sequence's (or the stacked prefix's) share: key blocks [p0, p0 + np) of the prefix, then [o0, o0 + nb - np) of its
 // own keys, for every row tile and key head.
 struct PaSeq {
-    uint32_t work;
     int tiles, nb, p0, np, o0;
-    int first_nb;   // blocks that the first row tile sees, about (a causal sequence's tiles see more and more)
 };
 
-// ABOVE: the launch takes the sequences of more than row_limit rows (and reads the prefix for each of them),
-// else those of at most that many.
-template <int BK, bool ABOVE>
+// BK: keys of a block.  ABOVE: the launch takes the sequences of more than row_limit rows (and reads the prefix for each of
+// them), else those of at most that many.  PRE: the call has a shared prefix.
+template <int BK, bool ABOVE, bool PRE>
 __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, const PagedSeq& s, int R) {
     PaSeq w = {};
-    const int64_t rows = (int64_t)s.n * p.G;
+    const int rows = s.n * p.G;   // below 2^31, as all rows of the batch are
     if (rows == 0 || (rows > p.row_limit) != ABOVE) return w;
-    const int first = p.P + s.kv - s.n;
-    const int lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
-    if (p.P > 0 && (ABOVE || p.stack == 0) && lo < p.P) {
-        w.p0 = lo / BK;
-        w.np = (p.P + BK - 1) / BK - w.p0;
+    w.nb = (s.kv + BK - 1) / BK;
+    if (p.window > 0 || PRE) {
+        const int P = PRE ? p.P : 0, lo = p.window > 0 ? max(0, P + s.kv - s.n - p.window + 1) : 0;   // first position seen
+        if (PRE && (ABOVE || p.stack == 0) && lo < P) {
+            w.p0 = lo / BK;
+            w.np = (P + BK - 1) / BK - w.p0;
+        }
+        const int own = min(max(0, lo - P), s.kv);
+        w.o0 = own / BK;
+        w.nb = w.np + w.nb - w.o0;
     }
-    const int own = max(0, lo - p.P);
-    w.o0 = own / BK;
-    w.nb = max(1, w.np + (s.kv > own ? (s.kv + BK - 1) / BK - w.o0 : 0));   // rows without keys are written too
-    w.first_nb = p.causal && !p.bidir ? max(1, w.nb - (s.n + BK - 1) / BK) : w.nb;
-    w.tiles = ((int)rows + R - 1) / R;
-    w.work = (uint32_t)w.tiles * (uint32_t)w.nb * (uint32_t)p.c.heads;
+    w.nb = max(1, w.nb);   // rows without keys are written too
+    w.tiles = (rows + R - 1) / R;
     return w;
 }
+// Blocks that the first row tile sees, about: a causal sequence's tiles see more and more.
+template <int BK>
+__device__ __forceinline__ int pa_first_nb(const PaParams& p, const PagedSeq& s, const PaSeq& w) {
+    return p.causal && !p.bidir ? max(1, w.nb - (s.n + BK - 1) / BK) : w.nb;
+}
+__device__ __forceinline__ uint32_t pa_work(const PaParams& p, const PaSeq& w) {
+    return (uint32_t)w.tiles * (uint32_t)w.nb * (uint32_t)p.c.heads;
+}
 
-__device__ __forceinline__ uint32_t pa_scan(uint32_t x, int lane) {   // inclusive, over the wavefront
-    for (int i = 1; i < 64; i *= 2) {
-        const uint32_t y = __shfl_up(x, i, 64);
-        x += lane >= i ? y : 0;
-    }
+// Scans and reductions over the wavefront by DPP: shifts within 16 lanes, then the last lane of 16 (of 32) to the
+// lanes behind it; lanes that receive nothing combine with `id`.  Some 50 cycles, against 700 for six LDS-pipe shuffles, and a
+// workgroup starts with several.
+template <typename F>
+__device__ __forceinline__ int pa_scan_with(int x, int id, F f) {   // inclusive
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x111, 0xf, 0xf, false));   // row_shr 1, 2, 4, 8
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x112, 0xf, 0xf, false));
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x114, 0xf, 0xf, false));
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x118, 0xf, 0xf, false));
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x142, 0xa, 0xf, false));   // row_bcast 15 into rows 1 and 3
+    x = f(x, __builtin_amdgcn_update_dpp(id, x, 0x143, 0xc, 0xf, false));   // row_bcast 31 into rows 2 and 3
     return x;
 }
+__device__ __forceinline__ uint32_t pa_scan(uint32_t x) {
+    return (uint32_t)pa_scan_with((int)x, 0, [](int a, int b) { return (int)((uint32_t)a + (uint32_t)b); });
+}
+__device__ __forceinline__ int pa_wave_max(int x) {
+    return __builtin_amdgcn_readlane(pa_scan_with(x, (int)0x80000000, [](int a, int b) { return max(a, b); }), 63);
+}
+__device__ __forceinline__ int pa_wave_min(int x) {
+    return __builtin_amdgcn_readlane(pa_scan_with(x, 0x7fffffff, [](int a, int b) { return min(a, b); }), 63);
+}
+__device__ __forceinline__ float pa_as_float(int x) { return __builtin_bit_cast(float, x); }
+__device__ __forceinline__ int pa_as_int(float x) { return __builtin_bit_cast(int, x); }
 __device__ __forceinline__ float pa_wave_max(float x) {
-    for (int i = 1; i < 64; i *= 2) x = fmaxf(x, __shfl_xor(x, i, 64));
-    return x;
+    const int r = pa_scan_with(pa_as_int(x), pa_as_int(-INFINITY),
+                               [](int a, int b) { return pa_as_int(fmaxf(pa_as_float(a), pa_as_float(b))); });
+    return pa_as_float(__builtin_amdgcn_readlane(r, 63));
 }
 __device__ __forceinline__ float pa_wave_sum(float x) {
-    for (int i = 1; i < 64; i *= 2) x += __shfl_xor(x, i, 64);
-    return x;
+    const int r = pa_scan_with(pa_as_int(x), 0, [](int a, int b) { return pa_as_int(pa_as_float(a) + pa_as_float(b)); });
+    return pa_as_float(__builtin_amdgcn_readlane(r, 63));
 }
 
-// What every wavefront knows of the whole call.
+// What every wavefront knows of the whole call.  The first 64 sequences stay in its lanes.
 struct PaPlan {
-    uint32_t total;
-    PaSeq prefix;       // the stacked prefix, in front of the sequences (work 0: none)
+    uint32_t total;     // blocks of work
+    uint32_t upto;      // lane i: those of sequences 0 .. i
+    PagedSeq mine;      // lane i: sequence i
+    // a call with a shared prefix: its stacked share, in front of the sequences (no tiles: none)
+    PaSeq prefix;
+    uint32_t pre_work;
     int t0, t1;         // rows of the batch
     bool plain;         // every row sees the whole prefix
-    uint32_t upto;      // lane i: the work of sequences 0 .. i (i < 64)
-    uint32_t seen;      // ABOVE: blocks that rows see, about (total counts every tile like its sequence's last)
-    int longest;        // ABOVE: the most blocks of a tile
 };
 
-// The stacked prefix for the rows of all sequences; lo: the first position that one of them sees.
-template <int BK>
-__device__ __forceinline__ void pa_plan_prefix(const PaParams& p, PaPlan& g, int R, int lo) {
-    g.t0 = min(max(p.b.q_start[0], 0), p.b.T);
-    g.t1 = min(max(p.b.q_start[p.b.B], g.t0), p.b.T);
-    if (lo < p.P && g.t1 > g.t0) {
-        g.prefix.p0 = lo / BK;
-        g.prefix.np = g.prefix.nb = (p.P + BK - 1) / BK - g.prefix.p0;
-        g.prefix.tiles = ((g.t1 - g.t0) * p.G + R - 1) / R;
-        g.prefix.work = (uint32_t)g.prefix.tiles * (uint32_t)g.prefix.nb * (uint32_t)p.c.heads;
-    }
+__device__ __forceinline__ PagedSeq pa_lane_seq(const PaParams& p, int b) {
+    PagedSeq s = {0, 0, 0};
+    if (b < p.b.B) s = paged_seq(p.b, b);
+    return s;
 }
 
-// SEQS: the launch takes sequences; PREFIX: it takes the stacked prefix.
-template <int BK, bool ABOVE>
+// seqs: the launch takes sequences; prefix: it takes the stacked prefix.
+template <int BK, bool ABOVE, bool PRE>
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, int R, bool seqs, bool prefix, int lane) {
     PaPlan g = {};
     int lo = 0x7fffffff;
     bool plain = p.window == 0;
-    uint32_t seen = 0;
-    int longest = 0;
     for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-        uint32_t work = 0;
-        if (b0 + lane < p.b.B) {
-            const PagedSeq s = paged_seq(p.b, b0 + lane);
-            if (seqs) {
-                const PaSeq q = pa_seq<BK, ABOVE>(p, s, R);
-                work = q.work;
-                seen += (uint32_t)q.tiles * (uint32_t)(q.nb + q.first_nb) / 2u * (uint32_t)p.c.heads;
-                longest = max(longest, q.tiles > 0 ? q.nb : 0);
-            }
-            if (s.n > 0) {
-                lo = min(lo, p.window > 0 ? max(0, p.P + s.kv - s.n - p.window + 1) : 0);
-                plain = plain && s.n <= s.kv;
-            }
+        const PagedSeq s = pa_lane_seq(p, b0 + lane);
+        const uint32_t upto = pa_scan(seqs ? pa_work(p, pa_seq<BK, ABOVE, PRE>(p, s, R)) : 0u);
+        if (b0 == 0) {
+            g.mine = s;
+            g.upto = upto;
         }
-        const uint32_t upto = pa_scan(work, lane);
-        if (b0 == 0) g.upto = upto;
+        if (PRE && s.n > 0) {
+            lo = min(lo, p.window > 0 ? max(0, p.P + s.kv - s.n - p.window + 1) : 0);
+            plain = plain && s.n <= s.kv;
+        }
         g.total += __builtin_amdgcn_readlane(upto, 63);
     }
-    if constexpr (ABOVE) {
-        for (int i = 1; i < 64; i *= 2) {
-            seen += __shfl_xor(seen, i, 64);
-            longest = max(longest, __shfl_xor(longest, i, 64));
-        }
-        g.seen = __builtin_amdgcn_readfirstlane(seen);
-        g.longest = __builtin_amdgcn_readfirstlane(longest);
-    }
-    if (prefix) {
-        for (int i = 1; i < 64; i *= 2) lo = min(lo, __shfl_xor(lo, i, 64));
+    if (PRE && prefix) {
+        lo = pa_wave_min(lo);
         g.plain = __builtin_amdgcn_ballot_w64(!plain) == 0;
-        pa_plan_prefix<BK>(p, g, R, __builtin_amdgcn_readfirstlane(lo));
-        g.total += g.prefix.work;
+        g.t0 = min(max(p.b.q_start[0], 0), p.b.T);
+        g.t1 = min(max(p.b.q_start[p.b.B], g.t0), p.b.T);
+        if (lo < p.P && g.t1 > g.t0) {
+            g.prefix.p0 = lo / BK;
+            g.prefix.np = g.prefix.nb = (p.P + BK - 1) / BK - g.prefix.p0;
+            g.prefix.tiles = ((g.t1 - g.t0) * p.G + R - 1) / R;
+            g.pre_work = pa_work(p, g.prefix);
+        }
+        g.total += g.pre_work;
     }
     return g;
 }
 
-// The sequence that holds block `w` of the work, and the work in front of it; -1: the stacked prefix.
-template <int BK, bool ABOVE>
-__device__ __forceinline__ int pa_locate(const PaParams& p, const PaPlan& g, int R, uint32_t w, int lane, uint32_t& before) {
-    before = 0;
-    if (w < g.prefix.work) return -1;
-    before = g.prefix.work;
-    for (int b0 = 0; b0 < p.b.B; b0 += 64) {
+// The segment at block `at` of the work: its sequence (b = -1: the stacked prefix), the work in front of that, and
+// what of it the tile and head are.
+struct PaSegment {
+    int b;
+    PagedSeq seq;
+    PaSeq sw;
+    uint32_t before;
+    int head, tile, blk0;
+};
+template <int BK, bool ABOVE, bool PRE>
+__device__ __forceinline__ PaSegment pa_segment(const PaParams& p, const PaPlan& g, int R, uint32_t at, int lane) {
+    PaSegment x = {};
+    if (PRE && at < g.pre_work) {
+        x.b = -1;
+        x.seq = {g.t0, g.t1 - g.t0, 0};
+        x.sw = g.prefix;
+    } else {
+        x.before = PRE ? g.pre_work : 0;
         uint32_t upto = g.upto;
-        if (b0 > 0) {
-            uint32_t work = 0;
-            if (b0 + lane < p.b.B) work = pa_seq<BK, ABOVE>(p, paged_seq(p.b, b0 + lane), R).work;
-            upto = pa_scan(work, lane);
+        PagedSeq s = g.mine;
+        for (int b0 = 0;;) {
+            const uint64_t past = __builtin_amdgcn_ballot_w64(x.before + upto > at);
+            if (past != 0) {
+                const int i = __builtin_ctzll(past);
+                if (i > 0) x.before += __builtin_amdgcn_readlane(upto, i - 1);
+                x.b = b0 + i;
+                x.seq.first = __builtin_amdgcn_readlane(s.first, i);
+                x.seq.n = __builtin_amdgcn_readlane(s.n, i);
+                x.seq.kv = __builtin_amdgcn_readlane(s.kv, i);
+                break;
+            }
+            x.before += __builtin_amdgcn_readlane(upto, 63);
+            b0 += 64;
+            if (b0 >= p.b.B) break;   // not reached for at < total
+            s = pa_lane_seq(p, b0 + lane);
+            upto = pa_scan(pa_work(p, pa_seq<BK, ABOVE, PRE>(p, s, R)));
         }
-        const uint64_t past = __builtin_amdgcn_ballot_w64(before + upto > w);
-        if (past != 0) {
-            const int i = __builtin_ctzll(past);
-            if (i > 0) before += __builtin_amdgcn_readlane(upto, i - 1);
-            return b0 + i;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
+        x.sw = pa_seq<BK, ABOVE, PRE>(p, x.seq, R);
     }
-    return p.b.B;   // not reached for w < total
+    const uint32_t rel = at - x.before, ht = rel / (uint32_t)x.sw.nb;
+    x.blk0 = __builtin_amdgcn_readfirstlane((int)(rel - ht * (uint32_t)x.sw.nb));
+    x.head = __builtin_amdgcn_readfirstlane((int)(x.sw.tiles == 1 ? ht : ht / (uint32_t)x.sw.tiles));
+    x.tile = (int)ht - x.head * x.sw.tiles;
+    x.tile = __builtin_amdgcn_readfirstlane(x.tile);
+    return x;
 }
 
 // A workgroup's place among `n` (a multiple of 8): consecutive parts on one XCD, which share keys in its L2.
 __device__ __forceinline__ uint32_t pa_place(uint32_t n) { return (blockIdx.x & 7) * (n >> 3) + (blockIdx.x >> 3); }
-__device__ __forceinline__ uint32_t pa_per(uint32_t total, uint32_t n) { return max(1u, (total + n - 1) / n); }
+__device__ __forceinline__ uint32_t pa_per(uint32_t total, const FastDiv& n) { return max(1u, div_of(total + n.d - 1, n)); }
 
 // The position of row `t` of the batch behind the stacked prefix: of the sequence whose end is the first behind it.
 __device__ __forceinline__ int pa_row_pos(const PaParams& p, int t) {
@@ -174,6 +239,38 @@ __device__ __forceinline__ bool pa_other(const PaParams& p, int t0, int t1, int 
     const PagedSeq s = paged_seq(p.b, b);
     return (int64_t)s.n * p.G > p.row_limit && t1 < s.first + s.n;
 }
+
+// Where a wavefront's keys are, 8 at a time: its tiles (GPT eights each) 64 / GPT at a time in one register, an eight a lane,
+// and the next as many in another.  One load round trip finds them all, and a lane read each gives them back as
+// scalars; page numbers by scalar loads in the loop, which LDS reads then wait for, cost 2 us a workgroup's start and 0.3
+// a block in the tile kernel.
+template <int GPT, bool PRE>
+struct PaPages {
+    static constexpr int TPC = 64 / GPT;
+    int64_t ofs[2];   // elements from the cache's begin, head 0; -1: no page, or no key
+    // chunk c.  where(tile, eight, k, pre): the eight's first key of the prefix (pre) or of the sequence; false: past the end
+    template <typename F>
+    __device__ __forceinline__ void load(const PaParams& p, int b, int c, int lane, F where) {
+        int k;
+        bool pre;
+        int64_t o = -1;
+        if (where(c * TPC + lane / GPT, lane % GPT, k, pre)) {
+            const int no = (int)div_of((uint32_t)k, p.c.by_page);
+            const int* table = p.b.table + (int64_t)max(b, 0) * p.b.max_pages;
+            const int pg = PRE && pre ? p.ppages[no] : table[no];
+            if ((uint32_t)pg < (uint32_t)p.c.pages) o = (int64_t)pg * p.c.sp + (int64_t)(k - no * p.c.page) * p.c.sl;
+        }
+        if (c & 1) ofs[1] = o;
+        else ofs[0] = o;
+    }
+    __device__ __forceinline__ int64_t get(int tile, int i) const {
+        const int at = (tile % TPC) * GPT + i;
+        const int64_t v = (tile / TPC) & 1 ? ofs[1] : ofs[0];
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, at);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at);
+        return (int64_t)((uint64_t)hi << 32 | lo);
+    }
+};
 
 // ---- parts ----------------------------------------------------------------------------
 // Partial results are written and read as device-wide relaxed atomics of 8 bytes: they pass the XCDs' L2 caches

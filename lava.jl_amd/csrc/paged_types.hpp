@@ -16,7 +16,6 @@ struct pg_tag {
 };
 
 typedef short pg_s16x4 __attribute__((ext_vector_type(4)));
-typedef const __attribute__((address_space(4))) int* pg_table;   // read by scalar loads
 
 template <typename T>
 struct PgType;

@@ -130,6 +130,10 @@ CASES = {
     "split_shared": dict(lens=tuple((1, 1 + (i * 97) % 300) for i in range(60)), prefix=1999, Hq=32, Hkv=8, D=128),
     "split_shared_window": dict(lens=tuple((1 + i % 2, 2 + (i * 97) % 300) for i in range(60)), prefix=1999, window=1200,
                                 Hq=32, Hkv=8, D=64, dtype="bf16", slopes=True),
+    # more keys than a wavefront finds the pages of at once (16 and 32 blocks), ends at and around them
+    "long_keys": dict(lens=((1, 2047), (1, 2048), (1, 2049), (3, 4100), (70, 4200)), Hq=2, Hkv=1, D=64, page=8),
+    "long_keys_one_head": dict(lens=((1, 200001),), Hq=1, Hkv=1, D=64, page=64),
+    "long_prefix": dict(lens=((1, 30), (2, 2060), (40, 40)), prefix=6200, Hq=4, Hkv=2, D=64, page=24),
     "many": dict(lens=tuple((1 if i % 5 else 2, 2 + i % 37) for i in range(150)), Hq=2, Hkv=1, D=64),
 }
 
