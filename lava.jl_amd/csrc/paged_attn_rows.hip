@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
         {
         const PaParams p = args.get();
         // ---- this wavefront's tiles, 32 keys of a block
-        PaPages<4, PRE> pages;
+        PaPages<4, PRE> pages = {-1, -1};
         auto where = [&](int j, int i, int& k, bool& pre) {
             const int blk = blk0 + j;
             pre = PRE && blk < np;
@@ -187,7 +187,6 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             return j < nblk && k < (pre ? p.P : kv);
         };
         pages.load(p, b, 0, lane, where);
-        pages.ofs[1] = -1;
         if (nblk + 1 >= decltype(pages)::TPC) pages.load(p, b, 1, lane, where);   // lookups run two tiles ahead
         struct Tile {
             int64_t at[4];   // per 8 keys, -1: none

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             if (i < 2) ofs_v[i] = 8 * cv < p.c.D ? (uint32_t)in8 * row_bytes + 16u * (uint32_t)cv : OOB_OFS;
         }
         // blocks of 16 keys of this wavefront's
-        PaPages<2, PRE> pages;
+        PaPages<2, PRE> pages = {-1, -1};
         auto where = [&](int j, int i, int& k, bool& pre) {
             const int blk = e0 + j;
             pre = PRE && blk < np;
@@ -428,7 +428,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             return j < nblk && k < (pre ? P : seq.kv);
         };
         pages.load(p, b, 0, lane, where);
-        pages.ofs[1] = -1;
         if (nblk + 3 > decltype(pages)::TPC) pages.load(p, b, 1, lane, where);   // requests run three blocks ahead
         auto request = [&](bool is_k, int j) __attribute__((always_inline)) {
             const T* base = (const T*)(is_k ? p.c.k : p.c.v) + (int64_t)head * p.c.sh;

@@ -32,7 +32,16 @@ struct PaArgs {
         asm volatile("" : "+v"(a), "+v"(b));
 #pragma unroll
         for (int i = 0; i < N; ++i) x.d[i] = (uint32_t)__builtin_amdgcn_readlane((int)(i < 64 ? a : b), i & 63);
-        return __builtin_bit_cast(PaParams, x);
+        PaParams p = __builtin_bit_cast(PaParams, x);
+        global(p.c.k), global(p.c.v), global(p.b.q_start), global(p.b.kv_len), global(p.b.table), global(p.Q), global(p.O);
+        global(p.lse), global(p.slopes), global(p.bidir), global(p.ppages), global(p.ws_o), global(p.ws_ml), global(p.ws_count);
+        global(p.pre_o), global(p.pre_ml), global(p.row_o), global(p.row_ml);
+        return p;
+    }
+    // says that a pointer made of register contents is to global memory
+    template <typename T>
+    __device__ __forceinline__ static void global(T*& q) {
+        q = (T*)(__attribute__((address_space(1))) T*)(uintptr_t)q;
     }
 };
 
@@ -247,7 +256,9 @@ __device__ __forceinline__ bool pa_other(const PaParams& p, int t0, int t1, int 
 template <int GPT, bool PRE>
 struct PaPages {
     static constexpr int TPC = 64 / GPT;
-    int64_t ofs[2];   // elements from the cache's begin, head 0; -1: no page, or no key
+    // elements from the cache's begin, head 0, of even chunks and of odd ones; -1: no page, or no key.  (Two members: of an array
+    // indexed by the chunk the compiler makes LDS, whose place it finds in the dispatch packet, in the host's memory: 2 to 10 us.)
+    int64_t even, odd;
     // chunk c.  where(tile, eight, k, pre): the eight's first key of the prefix (pre) or of the sequence; false: past the end
     template <typename F>
     __device__ __forceinline__ void load(const PaParams& p, int b, int c, int lane, F where) {
@@ -260,15 +271,20 @@ struct PaPages {
             const int pg = PRE && pre ? p.ppages[no] : table[no];
             if ((uint32_t)pg < (uint32_t)p.c.pages) o = (int64_t)pg * p.c.sp + (int64_t)(k - no * p.c.page) * p.c.sl;
         }
-        if (c & 1) ofs[1] = o;
-        else ofs[0] = o;
+        const bool to_odd = (c & 1) != 0;
+        even = to_odd ? even : o;
+        odd = to_odd ? o : odd;
     }
-    __device__ __forceinline__ int64_t get(int tile, int i) const {
-        const int at = (tile % TPC) * GPT + i;
-        const int64_t v = (tile / TPC) & 1 ? ofs[1] : ofs[0];
+    __device__ __forceinline__ static int64_t lane_of(int64_t v, int at) {
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, at);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), at);
         return (int64_t)((uint64_t)hi << 32 | lo);
+    }
+    __device__ __forceinline__ int64_t get(int tile, int i) const {
+        const int at = (tile % TPC) * GPT + i;
+        const bool of_odd = ((tile / TPC) & 1) != 0;
+        const int64_t a = lane_of(even, at), b = lane_of(odd, at);
+        return of_odd ? b : a;
     }
 };
 
