@@ -149,7 +149,7 @@ void lava_hip_kernel_log_clear(void);
  *                        (f16 / bf16 / int8 / unsigned bytes, any operand layout; the fused
  *                        epilogue for f16 / bf16), not its K-split form;
  *  LAVA_HIP_FAMILY_PAGED: attention over the paged cache: 1 the generic kernel, 2 the row kernel,
- *                        3 the tile kernel (D <= 128).
+ *                        3 the tile kernel (D <= 128) with 256 rows a tile, 4 with 128.
  * Unknown families or choices return LAVA_HIP_ERR_INVALID_ARG. */
 /* Reads [src, src + bytes) once with 16-byte nontemporal loads, `unroll` (4, 8 or 16) in flight
  * per thread, `blocks` workgroups of 256 threads, and writes the XOR of what each thread read to

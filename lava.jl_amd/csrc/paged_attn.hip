@@ -168,6 +168,19 @@ static int pa_prepare(const char* fn, const lava_hip_kv_cache* cache, const lava
         p->cap2 = score->cap * PA_LOG2E;
         p->mul = score->cap > 0.f ? (float)(2.0 * score->scale / score->cap * 1.4426950408889634) : (float)(score->scale * 1.4426950408889634);
         LAVA_ARG(std::isfinite(p->mul), "%s: scale / cap overflows", fn);
+        if (score->cap > 0.f) {
+            // tanh(z) = z (c0 + c1 z^2 + ..) for |z| <= 1/2, z = q.k scale / cap
+            const double c[5] = {0.9999999316221511, -0.33332776175690243, 0.13320570647011903, -0.052762128916049526,
+                                 0.01673756352440004};
+            const double z = (double)score->scale / score->cap;
+            double power = (double)score->cap * 1.4426950408889634 * z;
+            p->near = (float)std::min(0.5 / std::fabs(z), 1e30);
+            for (int i = 0; i < 5; ++i, power *= z * z) p->a[i] = (float)(c[i] * power);
+            // powers of a large scale / cap leave 32 bits: then the exact form always
+            for (int i = 0; i < 5; ++i)
+                if (!std::isfinite(p->a[i])) p->near = -1.f;
+            if (p->near > 1e15f) p->near = 1e15f;   // u = s^2 stays in range
+        }
         p->causal = score->causal != 0;
         p->window = score->window;
         p->slopes = score->slopes;
@@ -205,10 +218,10 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     sh.dp = p->c.D <= 64 ? 64 : p->c.D <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)p->b.T * p->G;
     p->row_limit = 0x7fffffff;
-    if (paged_tile_takes(*p) && (pin == 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
-        sh.qh = 2;
+    if (paged_tile_takes(*p) && (pin >= 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
+        sh.qh = pin == 4 ? 1 : 2;
         // mostly prompts: the tile kernel takes the few short sequences too, rather than a launch for them
-        p->row_limit = pin == 3 || rows / (128 * sh.qh) >= 4 * (int64_t)p->b.B ? 0 : PA_TILE_ROWS;
+        p->row_limit = pin >= 3 || rows / (128 * sh.qh) >= 4 * (int64_t)p->b.B ? 0 : PA_TILE_ROWS;
     }
     p->tiles = sh.qh != 0;
     if (p->row_limit > 0) {

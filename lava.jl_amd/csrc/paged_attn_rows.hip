@@ -242,6 +242,15 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
             const int first = now.pos, none = (now.at[0] < 0) | (now.at[1] < 0) << 1 | (now.at[2] < 0) << 2 | (now.at[3] < 0) << 3;
             const int end_pos = first + now.left - 1;   // the source's last key
             const bool cut = none != 0 || first < lo_max || first + 31 > min(hi_min, end_pos);
+            bool near = false;   // with a cap: every score in the polynomial's range
+            if (p.cap2 != 0.f) {
+                float far = 0.f;
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) far = fmaxf(far, fabsf(st[e >> 2][nr][e & 3]));
+                near = __builtin_amdgcn_ballot_w64(far > p.near) == 0;
+            }
             float up[NR];
             bool move = false;
 #pragma unroll
@@ -253,7 +262,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int key = first + 16 * kt + 4 * g + r;
-                        float x = pa_score(st[kt][nr][r], p.mul, p.cap2);
+                        float x = near ? pa_cap_near(st[kt][nr][r], p.a) : pa_score(st[kt][nr][r], p.mul, p.cap2);
                         if (p.slopes) x = fmaf(-slope[nr], fabsf(pos[nr] - (float)key), x);
                         if (cut) {
                             const bool keep = key >= lo[nr] && key <= last && !((none >> (2 * kt + (g >> 1))) & 1);

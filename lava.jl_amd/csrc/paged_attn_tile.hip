@@ -10,7 +10,8 @@
 //    compare, blocks that none sees are skipped, and a pair whose rows see nothing yet has no maximum (unset, -inf);
 //  * MODE 0 (f16, 0 < scale log2 e <= 1, no cap or slopes): the scale is folded into Q (one rounding) and the maximum
 //    enters the product as a bias k-step, so that P = exp2 of the accumulator; 1 (bf16, positive scale): P = exp2(fma(S, c,
-//    -m)), since bf16 would lose 2^-8 of q c; 2: caps, slopes, any scale.
+//    -m)), since bf16 would lose 2^-8 of q c; 2: caps (a polynomial where a block's scores are small, pa_cap_near), slopes,
+//    any scale.
 
 #include <algorithm>
 
@@ -253,24 +254,18 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         v8 qm[QH];
 #pragma unroll
         for (int qh = 0; qh < QH; ++qh) qm[qh] = v8{};
-        uint32_t kb0[NKS];
-#pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
-            kb0[ks] = lds_addr(&kbuf[0][0]) + (uint32_t)(r32 * RB + (((2 * ks + h) ^ (r32 & 15)) << 4));
+        // K fragment (kt, ks): row 32 kt + r32, chunk (2 ks + h) ^ (r32 % 16), which is ks in bits 1 and up of the rest
+        const uint32_t kb0 = lds_addr(&kbuf[0][0]) + (uint32_t)(r32 * RB + ((h ^ (r32 & 15)) << 4));
         f32x16 st[2][QH];   // register r: key 32 kt + 8 (r / 4) + 4 h + r % 4
         float m[QH];        // the running maximum, -inf: unset
 #pragma unroll
         for (int qh = 0; qh < QH; ++qh) m[qh] = -INFINITY;
 
         auto block = [&](int j, int buf) __attribute__((always_inline)) {
-            uint32_t ka[NKS];
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                ka[ks] = kb0[ks] + (uint32_t)((j % PT_KST) * TILE);
-                asm("; lds address" : "+v"(ka[ks]));
-            }
+            uint32_t ka = kb0 + (uint32_t)((j % PT_KST) * TILE);
+            asm("; lds address" : "+v"(ka));
             auto kread = [&](int f) __attribute__((always_inline)) -> v8 {   // f = 2 ks + kt
-                return *(const lds_v8*)(uintptr_t)(ka[f >> 1] + (uint32_t)((f & 1) * 32 * RB));
+                return *(const lds_v8*)(uintptr_t)((ka ^ (uint32_t)(32 * (f >> 1))) + (uint32_t)((f & 1) * 32 * RB));
             };
             v8 fr[PT_PF];
 #pragma unroll
@@ -293,20 +288,49 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             const int none = __builtin_amdgcn_readfirstlane(nn.x | nn.y << 2 | nn.z << 4 | nn.w << 6);
             const int pos0 = __builtin_amdgcn_readfirstlane(first_pos(e0 + j));
             const int src_hi = PRE && e0 + j < np ? P - 1 : end - 1;
-            if constexpr (MODE == 2) {
+            // scores relative to the maximum (to 0 while it is unset), as in MODE 0 the product gives them
+            const bool fast_blk = MODE != 0 || fast;
+            float ref[QH];
+#pragma unroll
+            for (int qh = 0; qh < QH; ++qh) ref[qh] = m[qh] == -INFINITY ? 0.f : m[qh];
+            auto each = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int qh = 0; qh < QH; ++qh)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            float x = pa_score(st[kt][qh][r], p.mul, p.cap2);
-                            if (p.slopes) {
-                                const float key = (float)(pos0 + 4 * h) + (float)(32 * kt + 8 * (r >> 2) + (r & 3));
-                                x = fmaf(-slope[qh], fabsf(r_pos[qh] - key), x);
-                            }
-                            st[kt][qh][r] = x;
-                        }
+                        for (int r = 0; r < 16; ++r) st[kt][qh][r] = f(st[kt][qh][r], qh, 32 * kt + 8 * (r >> 2) + (r & 3));
+            };
+            if constexpr (MODE == 1) each([&](float x, int qh, int) { return fmaf(x, p.mul, -ref[qh]); });
+            if constexpr (MODE == 2) {
+                if (p.cap2 == 0.f) {
+                    each([&](float x, int qh, int) { return fmaf(x, p.mul, -ref[qh]); });
+                } else {
+                    float far = 0.f;   // NaN: the exact form carries it as well as the other
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int qh = 0; qh < QH; ++qh)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(st[kt][qh][r]));
+                    if (__builtin_amdgcn_ballot_w64(far > p.near) != 0)
+                        each([&](float x, int qh, int) { return pa_score(x, p.mul, p.cap2) - ref[qh]; });
+                    else
+                        each([&](float x, int qh, int) {
+                            const float u = x * x;
+                            return fmaf(x, fmaf(fmaf(fmaf(fmaf(p.a[4], u, p.a[3]), u, p.a[2]), u, p.a[1]), u, p.a[0]), -ref[qh]);
+                        });
+                }
+                if (p.slopes) {
+                    float d0[QH];
+#pragma unroll
+                    for (int qh = 0; qh < QH; ++qh) d0[qh] = (float)(pos0 + 4 * h) - r_pos[qh];   // whole numbers below 2^31: each exact
+                                                                                                  // to 2^24, of use to the slopes that far
+                    each([&](float x, int qh, int k) { return fmaf(-slope[qh], fabsf(d0[qh] + (float)k), x); });
+                }
+            }
+            if constexpr (MODE == 0) {
+                if (!fast_blk) each([&](float x, int qh, int) { return x - ref[qh]; });
             }
             if (none != 0 || pos0 < in_lo || pos0 + PT_BK - 1 > min(in_hi, src_hi)) {
 #pragma unroll
@@ -323,10 +347,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                         }
                 }
             }
-            // how far the largest score lies above the maximum (above 0 while it is unset)
-            const bool fast_blk = fast;
-            const float cm = MODE == 1 ? p.mul : 1.f;
-            float vl[QH], ref[QH];
+            float vl[QH];   // how far the largest score lies above the maximum
             bool up = false;
 #pragma unroll
             for (int qh = 0; qh < QH; ++qh) {
@@ -335,15 +356,11 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) v = fmaxf(v, st[kt][qh][r]);
-                const bool unset = m[qh] == -INFINITY;
-                ref[qh] = unset ? 0.f : m[qh];
-                vl[qh] = MODE == 0 && fast_blk ? v : fmaf(v, cm, -ref[qh]);
-                up = up || vl[qh] > (unset ? -INFINITY : PT_RESCALE);
+                vl[qh] = v;
+                up = up || v > (m[qh] == -INFINITY ? -INFINITY : PT_RESCALE);
             }
             const bool rescale = __builtin_amdgcn_ballot_w64(up) != 0;
-            float sub[QH];   // what P = exp2(score - sub) takes off
-#pragma unroll
-            for (int qh = 0; qh < QH; ++qh) sub[qh] = MODE == 0 && fast_blk ? 0.f : ref[qh];
+            float sub[QH] = {};   // what P = exp2(score - sub) takes off
             if (rescale) {
                 float mn[QH];
                 bool far = false;
@@ -364,7 +381,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                     const bool unset = m[qh] == -INFINITY, still = mn[qh] == -INFINITY;
                     const float alpha = unset ? 1.f : __builtin_amdgcn_exp2f(m[qh] - mn[qh]);
                     const float to = still ? 0.f : mn[qh];
-                    sub[qh] = MODE == 0 && fast_blk ? to - ref[qh] : to;
+                    sub[qh] = to - ref[qh];
                     m[qh] = mn[qh];
                     if constexpr (MODE == 0) qm[qh][0] = (fast && h == 0) ? (T)(-to) : (T)0.f;
                     if (h == 0) abuf[buf][pr][32 * qh + r32] = alpha;
@@ -383,13 +400,13 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 float x = st[kt][qh][8 * ks + k];
-                                if constexpr (!decltype(plain)::value) x = MODE == 1 ? fmaf(x, cm, msub) : x + msub;
+                                if constexpr (!decltype(plain)::value) x += msub;
                                 u[k] = (T)__builtin_amdgcn_exp2f(x);
                             }
                             *(lds_v8*)(uintptr_t)paddr(buf, kt, ks, qh) = u;
                         }
             };
-            if (MODE == 0 && fast_blk && !rescale)
+            if (!rescale)
                 pstore(pg_tag<true>{});
             else
                 pstore(pg_tag<false>{});
@@ -455,14 +472,10 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         request(true, 2);
         request(false, 0);
 
-        uint32_t vb0[NDT];
-        {
-            const int jj = (lane & 15) >> 2, q = lane & 3, dh = (lane >> 4) & 1;
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt)
-                vb0[dt] = lds_addr(&vbuf[0][0]) +
-                          (uint32_t)((4 * h + jj) * RB + (((4 * dt + 2 * dh + (q >> 1)) ^ (4 * jj)) << 4) + ((q & 1) << 3));
-        }
+        // V^T fragment (dt, key step kk): two transposing reads at keys kk + 4 h + jj and + 8; the chunk
+        // (4 dt + 2 dh + q / 2) ^ 4 jj is dt in bits 2 and up of the rest
+        const int jj = (lane & 15) >> 2, vq = lane & 3, dh = (lane >> 4) & 1;
+        const uint32_t vb0 = lds_addr(&vbuf[0][0]) + (uint32_t)((4 * h + jj) * RB + (((2 * dh + (vq >> 1)) ^ (4 * jj)) << 4) + ((vq & 1) << 3));
         f32x16 o[NDT][QH];
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
@@ -496,16 +509,13 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
                     for (int qh = 0; qh < QH; ++qh) l[qh] *= al[qh];
                 }
-                uint32_t va[NDT];
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) {
-                    va[dt] = vb0[dt] + (uint32_t)((j % PT_VST) * TILE);
-                    asm("; lds address" : "+v"(va[dt]));
-                }
+                uint32_t va = vb0 + (uint32_t)((j % PT_VST) * TILE);
+                asm("; lds address" : "+v"(va));
                 auto vread = [&](int f) __attribute__((always_inline)) -> v8 {   // f = NDT kk + dt
                     const int kk = 16 * (f / NDT), dt = f % NDT;
-                    const pg_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(va[dt] + (uint32_t)(kk * RB)));
-                    const pg_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(va[dt] + (uint32_t)((kk + 8) * RB)));
+                    const uint32_t at = (va ^ (uint32_t)(64 * dt)) + (uint32_t)(kk * RB);
+                    const pg_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)at);
+                    const pg_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(at + 8 * RB));
                     return __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                 };
                 auto pread = [&](int kk, int qh) __attribute__((always_inline)) -> v8 {
@@ -583,13 +593,16 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             const int cc = lane % CH;
             const bool o16 = e.o16;   // rows of 16-byte pieces, else of 8
+            const int i0 = (int)div_of((uint32_t)row0, e.by_g);
+            uint8_t* const obase = (uint8_t*)((T*)e.O + (int64_t)(seq.first + i0) * e.ost + (int64_t)(head * e.G) * e.osh);
+            const uint32_t ost = (uint32_t)e.ost * 2u, osh = (uint32_t)e.osh * 2u;   // offsets fit 31 bits, as Q's
 #pragma unroll
             for (int i = 0; i < 8 * QH; ++i) {
                 const int r = 4 * i + lane / CH, row = row0 + r;
                 const v8 v = *(const lds_v8*)(uintptr_t)(o_row(4 * i) + (uint32_t)((lane / CH) * RB + ((cc ^ (r & 15)) << 4)));
                 if (row < rows && 8 * cc < e.c.D) {
                     const int t = (int)div_of((uint32_t)row, e.by_g);
-                    T* orow = (T*)e.O + (int64_t)(seq.first + t) * e.ost + (int64_t)(head * e.G + row - t * e.G) * e.osh + 8 * cc;
+                    T* orow = (T*)(obase + ((uint32_t)(t - i0) * ost + (uint32_t)(row - t * e.G) * osh + 16u * (uint32_t)cc));
                     if (o16) {
                         *reinterpret_cast<v8*>(orow) = v;
                     } else {
@@ -647,9 +660,10 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 
 // ---- host -----------------------------------------------------------------------------
 
-// Whether Q's offsets within a tile fit the addressing of its DMA.
+// Whether Q's and O's offsets within a tile fit 31 bits.
 bool paged_tile_takes(const PaParams& p) {
-    return p.c.D <= 128 && (double)(128 * 2 / p.G + 2) * p.qst * 2.0 + (double)p.G * p.qsh * 2.0 + 256 < 2147483647.0;
+    auto fits = [&](int64_t st, int64_t sh) { return (256.0 / p.G + 2) * st * 2.0 + (double)p.G * sh * 2.0 + 512 < 2147483647.0; };
+    return p.c.D <= 128 && fits(p.qst, p.qsh) && fits(p.ost, p.osh);
 }
 
 int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s) {

@@ -7,7 +7,7 @@ from paged_reference import Case, bad, to_f64
 
 pytestmark = pytest.mark.gpu
 
-KERNELS = {1: "paged_any_kernel", 2: "paged_rows_kernel", 3: "paged_tile_kernel"}
+KERNELS = {1: "paged_any_kernel", 2: "paged_rows_kernel", 3: "paged_tile_kernel", 4: "paged_tile_kernel"}
 
 
 class Device:
