@@ -207,9 +207,32 @@ static bool pa_vectors(const PaParams& p) {
 }
 
 // Sequences of more rows (new tokens times the query heads of a key head) run on the tile kernel, of fewer on the row
-// kernel, which splits them along the keys.
-constexpr int PA_TILE_ROWS = 64;
+// kernel.  (us, row / tile kernel: 16 x 17 tokens of 4 heads over 2000 keys, 68 rows 75 / 44; 8 x 32 over 3000, 128 rows 69 / 48; one of
+// 16 over 2000, 64 rows 30 / 33.)
+constexpr int PA_TILE_ROWS = 32;
+// Behind a shared prefix those of more rows, which fill a tile by themselves, read it by themselves.
+constexpr int PA_SHARE_ROWS = 256;
 constexpr size_t PA_ALIGN = 256;
+
+// Rows a tile of the tile kernel: 128 take 0.6 of the time of 256 (a fragment read feeds one product, not two), so they pay
+// where tiles of 256 would be half empty, or too few for the CUs and over short keys (over long keys the split fills them).
+// Measured (us, 256 / 128 rows; 32 heads, 8 key heads, D = 128): one prompt of 256 15.9 / 12.0, 1024 32 / 26, 2048 63 / 61, 4096
+// 147 / 189; 4 of 512 24 / 30; 64 tokens over 8000 keys 69 / 44, 256 over 16000 102 / 108, 2 x 512 over 20000 340 / 387.
+static int pa_tile_width(const PaParams& p, int64_t sequences) {
+    const int64_t rows = (int64_t)p.b.T * p.G;
+    const bool few = rows / 256 * p.c.heads < 200 && (int64_t)p.b.kv_max + p.P <= 8192;
+    return rows <= 160 * sequences || few ? 1 : 2;
+}
+
+// Rows that the workspace holds: of parts, of the stacked prefix's parts, whole ones behind it.
+struct PaRows {
+    size_t parts, pre, whole;
+};
+static PaRows pa_rows(const PaParams& p, const PaShape& sh) {
+    auto launch = [](size_t grid, size_t rows) { return 2 * grid * rows; };
+    return {std::max(launch(sh.row_grid, 16 * sh.nr), launch(PT_GRID, 128 * sh.qh)), launch(PT_GRID, 128 * sh.pre_qh),
+            p.stack ? 2 * (size_t)p.b.T * p.Hq : 0};
+}
 
 // What depends on the call's sizes alone: which kernels take which sequences.
 static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
@@ -218,32 +241,39 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     sh.dp = p->c.D <= 64 ? 64 : p->c.D <= 128 ? 128 : 256;
     const int64_t rows = (int64_t)p->b.T * p->G;
     p->row_limit = 0x7fffffff;
-    if (paged_tile_takes(*p) && (pin >= 3 || (pin == 0 && max_rows > PA_TILE_ROWS))) {
-        sh.qh = pin == 4 ? 1 : 2;
-        // mostly prompts: the tile kernel takes the few short sequences too, rather than a launch for them
-        p->row_limit = pin >= 3 || rows / (128 * sh.qh) >= 4 * (int64_t)p->b.B ? 0 : PA_TILE_ROWS;
+    const int limit = p->P > 0 ? PA_SHARE_ROWS : PA_TILE_ROWS;
+    if (paged_tile_takes(*p) && (pin >= 3 || (pin == 0 && max_rows > limit))) {
+        sh.qh = pin == 4 ? 1 : pin == 3 ? 2 : pa_tile_width(*p, p->b.B);
+        // where the sequences' mean is above the limit the tile kernel takes the short ones too (it reads their keys as
+        // fast) rather than a launch for them
+        p->row_limit = pin >= 3 || rows > limit * (int64_t)p->b.B ? 0 : limit;
+        // tiles enough for the CUs over few keys, or keys fewer than a split costs: never split, so no launch to join parts
+        const int64_t blocks = ((int64_t)p->b.kv_max + p->P + PT_BK - 1) / PT_BK;
+        p->whole = blocks <= PT_SPLIT || (blocks <= 32 && rows / (128 * sh.qh) * p->c.heads >= 128);
     }
     p->tiles = sh.qh != 0;
     if (p->row_limit > 0) {
-        p->stack = p->P > 0 ? 1 : 0;
-        if (p->stack && rows > PA_TILE_ROWS && paged_tile_takes(*p) && pin != 2) {
-            p->stack = 2;
-            sh.pre_qh = 2;
+        if (p->P > 0) {   // the prefix once for all: beside the sequences, or on the tile kernel for many rows
+            const bool many = rows > PA_TILE_ROWS && paged_tile_takes(*p) && pin != 2;
+            p->stack = many ? 2 : 1;
+            sh.pre_qh = many ? (rows <= 320 ? 1 : 2) : 0;
         }
-        const int64_t most = std::min<int64_t>(p->stack == 1 ? rows : max_rows, p->stack == 1 ? rows : p->row_limit);
-        sh.nr = most <= 16 ? 1 : most <= 32 || sh.dp == 256 ? 2 : 4;
-        // as many workgroups as fit (LDS: 512 bytes a column of the head, registers)
-        sh.row_grid = (unsigned)(PA_CUS * (sh.dp == 64 && sh.nr <= 2 ? 3 : sh.dp <= 128 && sh.nr <= 2 ? 2 : 1));
+        const int64_t most = p->stack == 1 ? rows : std::min<int64_t>(max_rows, p->row_limit);
+        sh.nr = most <= 16 ? 1 : 2;
+        // as many workgroups as fit (LDS: 512 bytes a column of the head)
+        sh.row_grid = (unsigned)(PA_CUS * (sh.dp == 64 ? 3 : sh.dp == 128 ? 2 : 1));
     }
     p->by_rows = fast_div(std::max(1u, sh.row_grid));
     p->by_tiles = fast_div(PT_GRID);
     const size_t row = sh.dp * sizeof(float) + sizeof(float2);
-    const size_t parts = 2 * std::max<size_t>((size_t)sh.row_grid * 16 * sh.nr, (size_t)PT_GRID * 128 * sh.qh);
-    const size_t pre = 2 * (size_t)PT_GRID * 128 * sh.pre_qh, whole = p->stack ? 2 * (size_t)p->b.T * p->Hq : 0;
+    const PaRows n = pa_rows(*p, sh);
     sh.count_bytes = STREAM_WS_RESERVED;
-    sh.bytes = sh.count_bytes + (parts + pre + whole) * row + 8 * PA_ALIGN;
+    sh.bytes = sh.count_bytes + (n.parts + n.pre + n.whole) * row + PA_MAX_GRID * sizeof(PaOpen) + 8 * PA_ALIGN;
     return sh;
 }
+
+static_assert(STREAM_WS_PAGED + PA_MAX_GRID * sizeof(unsigned) <= STREAM_WS_RESERVED, "the arrivals lie in the reserved part");
+static_assert(PT_GRID <= PA_MAX_GRID && 3 * PA_CUS <= PA_MAX_GRID, "every launch's workgroups have a place");
 
 // Lays a workspace out: arrivals at `count`, the rest from `at` on.
 static void pa_workspace(PaParams* p, const PaShape& sh, void* count, void* rest) {
@@ -254,15 +284,15 @@ static void pa_workspace(PaParams* p, const PaShape& sh, void* count, void* rest
         at += bytes;
         return q;
     };
-    const size_t parts = 2 * std::max<size_t>((size_t)sh.row_grid * 16 * sh.nr, (size_t)PT_GRID * 128 * sh.qh);
-    const size_t pre = 2 * (size_t)PT_GRID * 128 * sh.pre_qh, whole = p->stack ? 2 * (size_t)p->b.T * p->Hq : 0;
+    const PaRows n = pa_rows(*p, sh);
     p->ws_count = (unsigned*)count;
-    p->ws_o = (float*)take(parts * sh.dp * sizeof(float));
-    p->ws_ml = (float2*)take(parts * sizeof(float2));
-    p->pre_o = (float*)take(pre * sh.dp * sizeof(float));
-    p->pre_ml = (float2*)take(pre * sizeof(float2));
-    p->row_o = (float*)take(whole * sh.dp * sizeof(float));
-    p->row_ml = (float2*)take(whole * sizeof(float2));
+    p->ws_open = (PaOpen*)take(PA_MAX_GRID * sizeof(PaOpen));
+    p->ws_o = (float*)take(n.parts * sh.dp * sizeof(float));
+    p->ws_ml = (float2*)take(n.parts * sizeof(float2));
+    p->pre_o = (float*)take(n.pre * sh.dp * sizeof(float));
+    p->pre_ml = (float2*)take(n.pre * sizeof(float2));
+    p->row_o = (float*)take(n.whole * sh.dp * sizeof(float));
+    p->row_ml = (float2*)take(n.whole * sizeof(float2));
 }
 
 static int pa_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {

@@ -33,19 +33,27 @@ struct PaParams {
     // how the work is shared out (paged_plan.hpp)
     int tiles;                    // the tile kernel takes the sequences of more than row_limit rows
     int row_limit;                // rows: new tokens times G
+    int whole;                    // it never splits them
     int stack;                    // the prefix is attended once, by the rows of many sequences together: 1 by the row
                                   // kernel beside the sequences, 2 by the tile kernel in a launch of its own
     FastDiv by_rows, by_tiles;    // workgroups of the row kernel's launch, of the tile kernel's that split
-    // a launch's workspace: partial sums [workgroup][2][rows of a tile][DP], their (maximum, weight), arrivals of a tile's
+    // a launch's workspace: partial sums [workgroup][2 rows of a tile][DP], their (maximum, weight), arrivals of a tile's
     // parts at the workgroup it starts in (zero between calls)
     float* ws_o;
     float2* ws_ml;
     unsigned* ws_count;
+    struct PaOpen* ws_open;       // per workgroup: the tile that starts in its share and leaves it
     // stack: the same for the prefix's launch, and rows' whole results [prefix, own][T * Hq][DP]
     float* pre_o;
     float2* pre_ml;
     float* row_o;
     float2* row_ml;
+};
+
+// A row tile in parts: those of the workgroup that keeps this and of the ones behind it (0: none).
+struct PaOpen {
+    int parts, live, row0, first, head;   // its rows, the first of them in the sequence, the sequence's first token, the key head
+    int unused[3];
 };
 
 struct PaRange {
@@ -93,6 +101,8 @@ int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStre
 constexpr int PA_CUS = 256;
 constexpr int PR_BK = 128;                       // the row kernel's blocks of keys
 constexpr int PT_BK = 64;                        // the tile kernel's
+constexpr unsigned PT_LEAST = 8;                  // blocks of a workgroup that splits: what writing and reading a part's bytes costs
+constexpr int PT_SPLIT = 20;                     // blocks' time that splitting its tiles costs, about
 constexpr unsigned PA_MAX_GRID = 768;            // workgroups that leave parts
 constexpr unsigned PT_GRID = PA_CUS;             // those of the tile kernel
 

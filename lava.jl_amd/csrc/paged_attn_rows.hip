@@ -12,8 +12,8 @@
 //  * S^T = K Q^T and O^T = V^T P^T on 16x16x32 MFMAs: a lane owns one row, the score accumulator converts in place to the
 //    second product's operand (k-slot (g, i) is key 4 g + i of the first 16 keys or, from i = 4 on, of the second; V^T comes
 //    in that order from transposing LDS reads);
-//  * parts that do not cover all keys of their rows are joined in key order by the last workgroup of a row tile to
-//    arrive (paged_plan.hpp), so results do not depend on timing; behind a stacked prefix by a second small kernel.
+//  * parts that do not cover all keys of their rows are joined in key order (paged_plan.hpp), so results do not depend on
+//    timing: those of tiles of 16 rows by the last workgroup of a tile to arrive, others by a second small kernel.
 // K and V pages are found 8 keys at a time (page sizes are multiples of 8); a page number that is none reads as zeros
 // and is masked, as are rows at and past the sequence's end.
 
@@ -40,9 +40,9 @@ __device__ __forceinline__ float pr_max4(float x) {   // over the four lanes of 
     return fmaxf(x, __shfl_xor(x, 32, 64));
 }
 
-// DP: the head dimension rounded up to 64, 128 or 256; a tile is 16 NR rows.
+// DP: the head dimension rounded up to 64, 128 or 256; a tile is 16 NR rows, NR 1 or 2.
 template <typename T, int DP, int NR, bool PRE>
-__global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_rows_kernel(PaParams) {
+__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaParams) {
     typedef PgType<T> TT;
     typedef typename TT::v8 v8;
     typedef typename TT::v4 v4;
@@ -70,9 +70,13 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
     args.load(lane);
     const PaParams p = args.get();
     const PaPlan plan = pa_plan<PR_BK, false, PRE>(p, R, true, PRE && p.stack == 1, lane);
-    const uint32_t per = pa_per(plan.total, p.by_rows), wg = blockIdx.x;
+    const uint32_t per = pa_per(plan.total, p.by_rows, 1), wg = blockIdx.x;
     const uint32_t begin = min(plan.total, wg * per), stop = min(plan.total, begin + per);
-    if (begin >= stop) return;
+    PaOpen open = {};
+    if (begin >= stop) {
+        if (!(NR == 1 && !PRE)) pa_leave_open(p.ws_open + wg, open);
+        return;
+    }
 
     // LDS-DMA: lane offsets within 8 keys, by the parity of the 8 and the instruction
     const uint32_t row_bytes = (uint32_t)(p.c.sl * 2);
@@ -342,7 +346,9 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
         }
         const PaParams e = args.get();
         const bool whole = nblk == nb, direct = whole && !(PRE && e.stack);
+        const PaParts parts = pa_parts(at - (uint32_t)blk0, nb, per);
         constexpr int NH = NR < 2 ? 1 : 2;
+        constexpr bool LIVE = NR == 1 && !PRE;   // parts are read in this launch
         const uint32_t box = lds_addr(&ring[0][0][0]) + 16u * (uint32_t)lane;
 #pragma unroll
         for (int n0 = 0; n0 < NR; n0 += NH) {
@@ -360,7 +366,7 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                 const float inv = ll[nr] == 0.f ? 0.f : 1.f / ll[nr];
                 T* orow = (T*)e.O + (int64_t)row_t[nr] * e.ost + (int64_t)row_h[nr] * e.osh + 4 * g;
                 const int64_t part = whole ? (b < 0 ? 0 : (int64_t)e.b.T * e.Hq) + out_row
-                                           : (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * R + 16 * nr + r16;
+                                           : pa_part(parts, (int)(wg - parts.i0), 16 * nr + r16, R);
                 float* prow = (whole ? e.row_o : e.ws_o) + part * DP + 4 * g;
                 float2* pml = (whole ? e.row_ml : e.ws_ml) + part;
 #pragma unroll
@@ -374,59 +380,71 @@ __global__ void __launch_bounds__(256, (DP <= 128 && NR <= 2) ? 2 : 1) paged_row
                         const v4 y = {(T)(x[0] * inv), (T)(x[1] * inv), (T)(x[2] * inv), (T)(x[3] * inv)};
                         if (16 * dt + 4 * g < e.c.D) *reinterpret_cast<v4*>(orow + 16 * dt) = y;
                     } else {
-                        pa_put(prow + 16 * dt, x[0], x[1]);
-                        pa_put(prow + 16 * dt + 2, x[2], x[3]);
+                        if constexpr (LIVE) {
+                            pa_put(prow + 16 * dt, x[0], x[1]);
+                            pa_put(prow + 16 * dt + 2, x[2], x[3]);
+                        } else {
+                            *reinterpret_cast<f32x4*>(prow + 16 * dt) = x;
+                        }
                     }
                 }
                 if (live[nr] && w == 0 && g == 0) {
                     if (direct) {
                         if (e.lse) e.lse[out_row] = ll[nr] == 0.f ? -INFINITY : (ml[nr] + log2f(ll[nr])) * PA_LN2;
                     } else {
-                        pa_put((float*)pml, ml[nr], ll[nr]);
+                        if constexpr (LIVE) pa_put((float*)pml, ml[nr], ll[nr]);
+                        else *pml = make_float2(ml[nr], ll[nr]);
                     }
                 }
             }
         }
         if (!whole && !(PRE && e.stack)) {
-            const uint32_t a = at - (uint32_t)blk0;   // the tile's first block
-            pa_arrive<T, DP, 4>(e, a / per, (a + (uint32_t)nb - 1) / per, R, min(R, rows - tile * R), tile * R, sg.seq.first,
-                                head, w, lane, &arrived);
+            if constexpr (LIVE)
+                pa_arrive<T, DP, 4>(e, parts, R, min(R, rows - tile * R), tile * R, sg.seq.first, head, w, lane, &arrived);
+            else if (blk0 == 0)
+                open = {parts.n, min(R, rows - tile * R), tile * R, sg.seq.first, head, {}};
         }
         at += (uint32_t)nblk;
     }
+    if (!(NR == 1 && !PRE)) pa_leave_open(args.get().ws_open + wg, open);
 }
 
-// Behind a stacked prefix: a row's parts, the prefix's and its sequence's, each in the order of its keys.  One
-// wavefront a row.
+// Behind a stacked prefix: a row's parts, the prefix's and its sequence's, each in the order of its keys.  256 / DP rows a
+// wavefront, heads of one token.
 template <typename T, int DP>
-__global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, int pre_R) {
+__global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pre_R) {
     const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)p.b.T * p.Hq) return;
-    const int t = __builtin_amdgcn_readfirstlane((int)(row / p.Hq)), h = __builtin_amdgcn_readfirstlane((int)(row % p.Hq));
+    PaArgs args;
+    args.load(lane);
+    const PaParams p = args.get();
+    constexpr int RPW = 256 / DP;
+    const int per_token = (p.Hq + RPW - 1) / RPW;   // wavefronts a token
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int t = wave / per_token, h0 = (wave - t * per_token) * RPW;
+    if (t >= p.b.T) return;
+    const int h = min(h0 + lane / (DP / 4), p.Hq - 1);
     const int b = paged_find(p.b, t, lane);
     if (b >= p.b.B) return;
     const PagedSeq s = paged_seq(p.b, b);
-    if (t < s.first || t >= s.first + s.n || (int64_t)s.n * p.G > p.row_limit) return;
-    // a tile's parts: whole (one, by row), or those of workgroups i0 .. i0 + n - 1
+    if (t < s.first || t >= s.first + s.n || s.n * p.G > p.row_limit) return;
+    // a tile's parts: whole (one, by row), or in the workspace
     struct Source {
         const float* o;
         const float2* ml;
-        uint32_t i0;
-        int n, R, in;
-        __device__ int64_t at(int j) const { return n == 1 ? in : (int64_t)(2 * (i0 + (uint32_t)j) + (j == 0 ? 1u : 0u)) * R + in; }
+        PaParts parts;
+        int R, in;
+        __device__ int64_t at(int j) const { return parts.n == 1 ? 0 : pa_part(parts, j, in, R); }
     };
     const int head = h / p.G, g = h - head * p.G;
+    const int64_t row = (int64_t)t * p.Hq + h;
     auto source = [&](const PaSeq& sw, uint32_t before, uint32_t per, int tile_rows, uint32_t r, const float* o, const float2* ml,
                       int which) {
         const uint32_t tile = r / (uint32_t)tile_rows;
-        const uint32_t a = before + ((uint32_t)head * (uint32_t)sw.tiles + tile) * (uint32_t)sw.nb, z = a + (uint32_t)sw.nb - 1;
         Source x;
-        x.i0 = a / per;
-        x.n = (int)(z / per - x.i0) + 1;
+        x.parts = pa_parts(before + ((uint32_t)head * (uint32_t)sw.tiles + tile) * (uint32_t)sw.nb, sw.nb, per);
         x.R = tile_rows;
-        const bool whole = x.n == 1;
-        x.in = whole ? 0 : (int)(r - tile * (uint32_t)tile_rows);
+        x.in = (int)(r - tile * (uint32_t)tile_rows);
+        const bool whole = x.parts.n == 1;
         const int64_t i = (int64_t)which * p.b.T * p.Hq + row;
         x.o = whole ? p.row_o + i * DP : o;
         x.ml = whole ? p.row_ml + i : ml;
@@ -439,21 +457,26 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams p, int R, int 
             b0 == 0 ? plan.upto : pa_scan(pa_work(p, pa_seq<PR_BK, false, true>(p, pa_lane_seq(p, b0 + lane), R)));
         before += __builtin_amdgcn_readlane(upto, min(b - b0, 64) - 1);
     }
-    const uint32_t per = pa_per(plan.total, p.by_rows);
+    const uint32_t per = pa_per(plan.total, p.by_rows, 1);
     const Source own = source(pa_seq<PR_BK, false, true>(p, s, R), before, per, R, (uint32_t)((t - s.first) * p.G + g), p.ws_o, p.ws_ml, 1);
     Source pre = own;
-    pre.n = 0;
+    pre.parts.n = 0;
     if (p.stack == 1) {
         if (plan.pre_work > 0) pre = source(plan.prefix, 0, per, R, (uint32_t)((t - plan.t0) * p.G + g), p.ws_o, p.ws_ml, 0);
     } else {
         const PaPlan pp = pa_plan<PT_BK, true, true>(p, pre_R, false, true, lane);
         if (pp.pre_work > 0)
-            pre = source(pp.prefix, 0, pa_per(pp.total, p.by_tiles), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
+            pre = source(pp.prefix, 0, pa_per(pp.total, p.by_tiles, PT_LEAST), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
     }
-    float o[DP / 64], m, l;
-    pa_join_row<DP>(pre.n + own.n, [&](int j) { return j < pre.n ? pre.ml + pre.at(j) : own.ml + own.at(j - pre.n); },
-                    [&](int j) { return j < pre.n ? pre.o + pre.at(j) * DP : own.o + own.at(j - pre.n) * DP; }, lane, o, m, l);
-    pa_store_row<T, DP>(p, t, h, o, m, l, lane);
+    f32x4 o;
+    float m, l;
+    pa_join_rows<DP, false>(pre.parts.n + own.parts.n, [&](int j, const float2*& ml, const float*& q) {
+        const bool first = j < pre.parts.n;
+        const int64_t at = first ? pre.at(j) : own.at(j - pre.parts.n);
+        ml = (first ? pre.ml : own.ml) + at;
+        q = (first ? pre.o : own.o) + at * DP;
+    }, lane, o, m, l);
+    if (h0 + lane / (DP / 4) < p.Hq) pa_store_row<T, DP>(p, t, h, o, m, l, lane);
 }
 
 int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {
@@ -463,20 +486,25 @@ int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream
         auto by_shape = [&](auto pre) {
             constexpr bool PRE = decltype(pre)::value;
             if (sh.dp == 64)
-                sh.nr == 1   ? go(paged_rows_kernel<T, 64, 1, PRE>)
-                : sh.nr == 2 ? go(paged_rows_kernel<T, 64, 2, PRE>)
-                             : go(paged_rows_kernel<T, 64, 4, PRE>);
+                sh.nr == 1 ? go(paged_rows_kernel<T, 64, 1, PRE>) : go(paged_rows_kernel<T, 64, 2, PRE>);
             else if (sh.dp == 128)
-                sh.nr == 1   ? go(paged_rows_kernel<T, 128, 1, PRE>)
-                : sh.nr == 2 ? go(paged_rows_kernel<T, 128, 2, PRE>)
-                             : go(paged_rows_kernel<T, 128, 4, PRE>);
+                sh.nr == 1 ? go(paged_rows_kernel<T, 128, 1, PRE>) : go(paged_rows_kernel<T, 128, 2, PRE>);
             else
                 sh.nr == 1 ? go(paged_rows_kernel<T, 256, 1, PRE>) : go(paged_rows_kernel<T, 256, 2, PRE>);
         };
         p.P > 0 ? by_shape(pg_tag<true>{}) : by_shape(pg_tag<false>{});
         int rc = check_launch("paged_rows_kernel");
-        if (rc != LAVA_HIP_OK || p.stack == 0) return rc;
-        const unsigned rows = (unsigned)(((int64_t)p.b.T * p.Hq + 3) / 4);
+        if (rc != LAVA_HIP_OK) return rc;
+        if (p.stack == 0) {
+            if (sh.nr == 1 && p.P == 0) return rc;   // joined by the last workgroup of a tile to arrive
+            auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(sh.row_grid * 4), dim3(256), 0, s, p, 16 * sh.nr, 4); };
+            sh.dp == 64    ? join(paged_join_tiles_kernel<T, 64>)
+            : sh.dp == 128 ? join(paged_join_tiles_kernel<T, 128>)
+                           : join(paged_join_tiles_kernel<T, 256>);
+            return check_launch("paged_join_tiles_kernel");
+        }
+        const int per_wave = 256 / sh.dp;
+        const unsigned rows = (unsigned)(((int64_t)p.b.T * ((p.Hq + per_wave - 1) / per_wave) + 3) / 4);
         auto join = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, 128 * sh.pre_qh);
         };

@@ -47,7 +47,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     __shared__ int fbuf[2][PT_PAIRS];
     __shared__ __attribute__((aligned(16))) int nbuf[PT_KST][4];   // keys without a page, 2 bits of 8 keys each
     __shared__ float mbuf[PT_PAIRS][PQ];
-    __shared__ int arrived;
 
     const int lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -56,32 +55,15 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     const int r32 = lane & 31, h = lane >> 5;
 
     const bool prefix = PRE && stacked != 0;   // the launch for the stacked prefix
-    // ---- which part of the work.  Tiles one by one, a workgroup each, where the longest does not outlast the rest by more
-    // than splitting costs (parts written and joined, about 12 blocks' time, and blocks that only a sequence's
-    // last tiles see counted for all); else the even split over PT_GRID workgroups.
+    // ---- which part of the work
     PaArgs args;
     args.load(lane);
     const PaParams p = args.get();
     const PaPlan plan = pa_plan<PT_BK, true, PRE>(p, BQ, !prefix, prefix, lane);
-    bool by_tile = false;
-    int tiles_upto = 0;   // lane i: row tiles of sequences 0 .. i
-    if (!prefix) {
-        int longest = 0;
-        uint32_t seen = 0;
-        for (int b0 = 0; b0 < p.b.B; b0 += 64) {
-            const PagedSeq s = b0 == 0 ? plan.mine : pa_lane_seq(p, b0 + lane);
-            const PaSeq q = pa_seq<PT_BK, true, PRE>(p, s, BQ);
-            longest = max(longest, q.nb);
-            seen += q.tiles > 0 ? (uint32_t)q.tiles * (uint32_t)(q.nb + pa_first_nb<PT_BK>(p, s, q)) / 2u * (uint32_t)p.c.heads : 0u;
-            if (b0 == 0) tiles_upto = (int)pa_scan((uint32_t)q.tiles);
-        }
-        longest = pa_wave_max(longest);
-        by_tile = longest <= 24;
-        if (!by_tile) {
-            seen = __builtin_amdgcn_readlane(pa_scan(seen), 63);
-            by_tile = longest / 2 <= 12 + (int)((plan.total - min(plan.total, seen)) / PA_CUS);
-        }
-    }
+    int tiles_upto = 0;
+    const bool by_tile = !prefix && pa_by_tile<PRE>(p, plan, BQ, lane, tiles_upto);
+    PaOpen open = {};
+    if (by_tile && blockIdx.x < PT_GRID) pa_leave_open(p.ws_open + blockIdx.x, open);
     uint32_t at = 0, stop = 1, per = 1, wg = 0;
     PaSegment sg = {};
     if (by_tile) {
@@ -113,7 +95,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         sg.sw = pa_seq<PT_BK, true, PRE>(p, sg.seq, BQ);
     } else {
         if (blockIdx.x >= PT_GRID) return;
-        per = pa_per(plan.total, p.by_tiles);
+        per = pa_per(plan.total, p.by_tiles, PT_LEAST);
         wg = pa_place(PT_GRID);
         at = min(plan.total, wg * per);
         stop = min(plan.total, at + per);
@@ -571,8 +553,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         }
         typedef __attribute__((address_space(3))) v4 lds_v4;
         typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-        typedef float f2 __attribute__((ext_vector_type(2)));
-        typedef __attribute__((address_space(3))) f2 lds_f2;
         if (whole && b >= 0) {
 #pragma unroll
             for (int qh = 0; qh < QH; ++qh) {
@@ -614,7 +594,8 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         } else {
             float* po = whole ? e.row_o : prefix ? e.pre_o : e.ws_o;
             float2* pml = whole ? e.row_ml : prefix ? e.pre_ml : e.ws_ml;
-            const int64_t part0 = (int64_t)(2 * wg + (blk0 == 0 ? 1 : 0)) * BQ + pr * PQ;
+            const PaParts parts = pa_parts(at - (uint32_t)blk0, nb, per);
+            const int mine = (int)(wg - parts.i0);
 #pragma unroll
             for (int qh = 0; qh < QH; ++qh) {
                 // 32 rows of sums, DE x 4 bytes: two rows' worth of LDS a row (8 rows a part at DE = 128)
@@ -630,32 +611,30 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                         *(lds_f32x4*)(uintptr_t)(to + (uint32_t)(((4 * dt + g4) ^ (r32 & 7)) << 5)) =
                             f32x4{o[dt][qh][4 * g4], o[dt][qh][4 * g4 + 1], o[dt][qh][4 * g4 + 2], o[dt][qh][4 * g4 + 3]};
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                // a row (DE = 128) or two (64) an instruction, 8 bytes a lane; rows of no weight are not read again
-                constexpr int LPR = DE / 2, RPS = 64 / LPR;
+                // two rows (DE = 128) or four (64) an instruction; rows of no weight are not read again
+                constexpr int LPR = DE / 4, RPS = 64 / LPR;
                 const uint64_t some = __builtin_amdgcn_ballot_w64(sum[qh] != 0.f && live(qh));
 #pragma unroll 8
                 for (int r0 = 0; r0 < 32; r0 += RPS) {
                     const int r = r0 + lane / LPR, x = lane % LPR;
-                    const f2 v = *(const lds_f2*)(uintptr_t)(f_row(r) + (uint32_t)(((x >> 2) ^ (r & 7)) << 5) + 8u * (uint32_t)(x & 3));
+                    const f32x4 v = *(const lds_f32x4*)(uintptr_t)(f_row(r) + (uint32_t)(((x >> 1) ^ (r & 7)) << 5) + 16u * (uint32_t)(x & 1));
                     const int row = row0 + 32 * qh + r;
                     if ((some >> r) & 1) {
-                        const int64_t part = whole ? out_row(row) : part0 + 32 * qh + r;
-                        pa_put(po + part * DE + 2 * x, v.x, v.y);
+                        const int64_t part = whole ? out_row(row) : pa_part(parts, mine, pr * PQ + 32 * qh + r, BQ);
+                        *reinterpret_cast<f32x4*>(po + part * DE + 4 * x) = v;
                     }
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 if (live(qh) && h == 0)
-                    pa_put((float*)(pml + (whole ? out_row(row0 + 32 * qh + r32) : part0 + 32 * qh + r32)), mbuf[pr][32 * qh + r32], sum[qh]);
+                    pml[whole ? out_row(row0 + 32 * qh + r32) : pa_part(parts, mine, pr * PQ + 32 * qh + r32, BQ)] = make_float2(mbuf[pr][32 * qh + r32], sum[qh]);
             }
         }
     }
-    if (!whole && !prefix) {
-        const uint32_t a = at - (uint32_t)blk0;   // the tile's first block
-        pa_arrive<T, DE, 2 * PT_PAIRS>(args.get(), a / per, (a + (uint32_t)nb - 1) / per, BQ, min(BQ, rows - tile * BQ), tile * BQ, seq.first,
-                                       head, w, lane, &arrived);
-    }
+    if (!whole && blk0 == 0 && !prefix)
+        open = {pa_parts(at, nb, per).n, min(BQ, rows - tile * BQ), tile * BQ, seq.first, head, {}};
     at += (uint32_t)nseg;
     }
+    if (!by_tile && !prefix) pa_leave_open(args.get().ws_open + wg, open);
 }
 
 // ---- host -----------------------------------------------------------------------------
@@ -687,7 +666,15 @@ int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStre
             plain ? by_d(bf16{}, q, pg_int<1>{}) : by_d(bf16{}, q, pg_int<2>{});
     };
     qh == 1 ? by_mode(pg_int<1>{}) : by_mode(pg_int<2>{});
-    return check_launch(qh == 1 ? "paged_tile_kernel+paged_tile_kernel<32>" : "paged_tile_kernel");
+    const int rc = check_launch(qh == 1 ? "paged_tile_kernel+paged_tile_kernel<32>" : "paged_tile_kernel");
+    if (rc != LAVA_HIP_OK || prefix || p.whole) return rc;
+    auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(PT_GRID * 8), dim3(256), 0, s, p, 128 * qh, 8); };
+    auto join_type = [&](auto type) {
+        typedef decltype(type) T;
+        p.c.D <= 64 ? join(paged_join_tiles_kernel<T, 64>) : join(paged_join_tiles_kernel<T, 128>);
+    };
+    dtype == LAVA_HIP_F16 ? join_type(f16{}) : join_type(bf16{});
+    return check_launch("paged_join_tiles_kernel");
 }
 
 }  // namespace lava

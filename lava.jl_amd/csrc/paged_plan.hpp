@@ -5,8 +5,11 @@
 // itself, by one scan over the sequences.  A part is a run of segments, each some blocks of one row tile.  A
 // segment of all of its tile's blocks gives the result; another leaves (sums, maximum, weight) in the
 // workspace -- of a workgroup's segments only the first can continue a tile and only the last can leave one open,
-// so two slots a workgroup hold them -- and the last workgroup of a tile to arrive joins its parts in key order.
+// so two tiles' rows a workgroup hold them -- and a tile's parts are joined in key order, by the last of its
+// workgroups to arrive (16 rows) or by a launch of their own (more rows, which would keep one workgroup for long).
 #pragma once
+#include <algorithm>
+
 #include "paged_attn.hpp"
 
 namespace lava {
@@ -34,7 +37,7 @@ struct PaArgs {
         for (int i = 0; i < N; ++i) x.d[i] = (uint32_t)__builtin_amdgcn_readlane((int)(i < 64 ? a : b), i & 63);
         PaParams p = __builtin_bit_cast(PaParams, x);
         global(p.c.k), global(p.c.v), global(p.b.q_start), global(p.b.kv_len), global(p.b.table), global(p.Q), global(p.O);
-        global(p.lse), global(p.slopes), global(p.bidir), global(p.ppages), global(p.ws_o), global(p.ws_ml), global(p.ws_count);
+        global(p.lse), global(p.slopes), global(p.bidir), global(p.ppages), global(p.ws_o), global(p.ws_ml), global(p.ws_count), global(p.ws_open);
         global(p.pre_o), global(p.pre_ml), global(p.row_o), global(p.row_ml);
         return p;
     }
@@ -223,9 +226,34 @@ __device__ __forceinline__ PaSegment pa_segment(const PaParams& p, const PaPlan&
     return x;
 }
 
+// The tile kernel's choice: tiles one by one, a workgroup each, or the even split over PT_GRID workgroups.  Whole tiles take
+// the longest one's time, or the CUs' share and, at the end, half the longest on some; the split takes the share that counts
+// a sequence's every tile as long as its last, and PT_SPLIT blocks more (parts written, a launch that joins them).
+// tiles_upto: lane i: row tiles of sequences 0 .. i.
+template <bool PRE>
+__device__ __forceinline__ bool pa_by_tile(const PaParams& p, const PaPlan& g, int R, int lane, int& tiles_upto) {
+    int longest = 0;
+    uint32_t seen = 0;   // blocks that rows see, about
+    tiles_upto = 0;
+    for (int b0 = 0; b0 < p.b.B; b0 += 64) {
+        const PagedSeq s = b0 == 0 ? g.mine : pa_lane_seq(p, b0 + lane);
+        const PaSeq q = pa_seq<PT_BK, true, PRE>(p, s, R);
+        longest = max(longest, q.nb);
+        seen += q.tiles > 0 ? (uint32_t)q.tiles * (uint32_t)(q.nb + pa_first_nb<PT_BK>(p, s, q)) / 2u * (uint32_t)p.c.heads : 0u;
+        if (b0 == 0) tiles_upto = (int)pa_scan((uint32_t)q.tiles);
+    }
+    if (p.whole) return true;
+    longest = pa_wave_max(longest);
+    seen = __builtin_amdgcn_readlane(pa_scan(seen), 63);
+    return max(longest, (int)(seen / PA_CUS) + longest / 2) <= (int)(g.total / PA_CUS) + PT_SPLIT;
+}
+
 // A workgroup's place among `n` (a multiple of 8): consecutive parts on one XCD, which share keys in its L2.
 __device__ __forceinline__ uint32_t pa_place(uint32_t n) { return (blockIdx.x & 7) * (n >> 3) + (blockIdx.x >> 3); }
-__device__ __forceinline__ uint32_t pa_per(uint32_t total, const FastDiv& n) { return max(1u, div_of(total + n.d - 1, n)); }
+// Blocks a workgroup, at least `least`.
+__device__ __forceinline__ uint32_t pa_per(uint32_t total, const FastDiv& n, uint32_t least) {
+    return max(least, div_of(total + n.d - 1, n));
+}
 
 // The position of row `t` of the batch behind the stacked prefix: of the sequence whose end is the first behind it.
 __device__ __forceinline__ int pa_row_pos(const PaParams& p, int t) {
@@ -288,9 +316,27 @@ struct PaPages {
     }
 };
 
+// A tile in parts: those of workgroups i0 .. i0 + n - 1 of its launch.
+struct PaParts {
+    uint32_t i0;
+    int n;
+};
+// a: the tile's first block of work.
+__device__ __forceinline__ PaParts pa_parts(uint32_t a, int nb, uint32_t per) {
+    const uint32_t i0 = a / per;
+    return {i0, (int)((a + (uint32_t)nb - 1) / per - i0) + 1};
+}
+// The place of row `row` of part j, tiles of R rows: 2 R rows of place a workgroup, of which the tile has those from the second
+// half of i0's to the first half of the last one's.  A row's parts lie one behind the other, in one page (part by part they were
+// 128 KB apart, and a round trip to sixteen of them took 4 us).
+__device__ __forceinline__ int64_t pa_part(const PaParts& t, int j, int row, int R) {
+    return ((int64_t)2 * t.i0 + 1) * R + (int64_t)row * t.n + j;
+}
+
 // ---- parts ----------------------------------------------------------------------------
-// Partial results are written and read as device-wide relaxed atomics of 8 bytes: they pass the XCDs' L2 caches
-// without a fence that would write those back, and a wait for the stores before the arrival is counted orders them.
+// Parts that are joined in the launch that makes them are written and read as device-wide relaxed atomics of 8 bytes: they
+// pass the XCDs' L2 caches without a fence that would write those back, and a wait for the stores before the
+// arrival is counted orders them.  Parts for a later launch are plain stores.
 
 __device__ __forceinline__ void pa_put(float* p, float a, float b) {
     const float2 v = make_float2(a, b);
@@ -300,93 +346,125 @@ __device__ __forceinline__ float2 pa_get(const float* p) {
     return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// A row's parts joined by a wavefront: part j's (maximum, weight) at ml(j), its sums at o(j); DP columns, DP / 64 a lane.
-// Parts of no weight have no sums.
-template <int DP, typename ML, typename OF>
-__device__ __forceinline__ void pa_join_row(int n, ML ml, OF of, int lane, float (&o)[DP / 64], float& m, float& l) {
-    constexpr int NC = DP / 64;
+// Rows joined by a wavefront, 256 / DP of them at once: DP / 4 lanes a row, 4 columns a lane.  Part j of the lane's row has its
+// (maximum, weight) and sums at part(j, ml, o); n parts (at least one).  Sums are requested beside the weights, one round trip for
+// both: those of a part of no weight are not written, and what is read of them is dropped.  LIVE: the parts come from
+// workgroups of this launch (device-wide loads).
+template <int DP, bool LIVE, typename F>
+__device__ __forceinline__ void pa_join_rows(int n, F part, int lane, f32x4& o, float& m, float& l) {
+    constexpr int U = 16;   // parts in flight: a round trip to what other workgroups wrote takes 1 to 2 us
+    const int most = pa_wave_max(n), c = lane % (DP / 4);
     m = -INFINITY;
-    for (int j0 = 0; j0 < n; j0 += 64)
-        if (j0 + lane < n) m = fmaxf(m, pa_get((const float*)ml(j0 + lane)).x);
-    m = pa_wave_max(m);
-    const float sub = m == -INFINITY ? 0.f : m;
     l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < most; j0 += U) {
+        float2 x[U];
+        f32x4 v[U];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) o[c] = 0.f;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        float f = 0.f;
-        if (j0 + lane < n) {
-            const float2 x = pa_get((const float*)ml(j0 + lane));
-            f = x.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(x.x - sub);
-            l += x.y * f;
-        }
-        const int k = min(n - j0, 64);
-        constexpr int U = NC == 4 ? 4 : 8;   // loads in flight
-        for (int j = 0; j < k; j += U) {
-            float2 v[U][(NC + 1) / 2];
-            float w[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                w[u] = j + u < k ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(j + u, 63))) : 0.f;
-#pragma unroll
-                for (int c = 0; c < (NC + 1) / 2; ++c) {
-                    v[u][c] = make_float2(0.f, 0.f);
-                    if (w[u] != 0.f) {
-                        const float* q = of(j0 + j + u);
-                        if constexpr (NC == 1)
-                            v[u][c].x = __hip_atomic_load(q + lane, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                        else
-                            v[u][c] = pa_get(q + NC * lane + 2 * c);
-                    }
-                }
+        for (int u = 0; u < U; ++u) {
+            const float2* ml;
+            const float* q;
+            part(min(j0 + u, n - 1), ml, q);
+            q += 4 * c;
+            if constexpr (LIVE) {
+                x[u] = pa_get((const float*)ml);
+                const float2 a = pa_get(q), b = pa_get(q + 2);
+                v[u] = f32x4{a.x, a.y, b.x, b.y};
+            } else {
+                x[u] = *ml;
+                v[u] = *reinterpret_cast<const f32x4*>(q);
             }
+        }
+        __builtin_amdgcn_sched_barrier(0);   // all requests before the first use
+        float top = m;
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            if (j0 + u >= n) x[u] = make_float2(-INFINITY, 0.f);
+            top = fmaxf(top, x[u].x);
+        }
+        const float sub = top == -INFINITY ? 0.f : top, a = __builtin_amdgcn_exp2f(m - sub);
+        m = top;
+        l *= a;
+        o *= a;
 #pragma unroll
-                for (int c = 0; c < NC; ++c) o[c] = fmaf(w[u], c & 1 ? v[u][c / 2].y : v[u][c / 2].x, o[c]);
+        for (int u = 0; u < U; ++u) {
+            const float f = __builtin_amdgcn_exp2f(x[u].x - sub);
+            l = fmaf(f, x[u].y, l);
+            const bool some = x[u].y != 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = some ? fmaf(f, v[u][e], o[e]) : o[e];
         }
     }
-    l = pa_wave_sum(l);
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void pa_store_row(const PaParams& p, int t, int h, const float (&o)[DP / 64], float m, float l, int lane) {
-    constexpr int NC = DP / 64;
+__device__ __forceinline__ void pa_store_row(const PaParams& p, int t, int h, f32x4 o, float m, float l, int lane) {
+    const int d = 4 * (lane % (DP / 4));
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* orow = (T*)p.O + (int64_t)t * p.ost + (int64_t)h * p.osh + NC * lane;
-    typedef T vt __attribute__((ext_vector_type(NC)));
-    if (NC * lane < p.c.D) {   // D is a multiple of 8
-        vt v;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) v[c] = (T)(o[c] * inv);
-        *reinterpret_cast<vt*>(orow) = v;
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    if (d < p.c.D) {   // D is a multiple of 8
+        const v4 v = {(T)(o[0] * inv), (T)(o[1] * inv), (T)(o[2] * inv), (T)(o[3] * inv)};
+        *reinterpret_cast<v4*>((T*)p.O + (int64_t)t * p.ost + (int64_t)h * p.osh + d) = v;
     }
-    if (p.lse && lane == 0) p.lse[(int64_t)t * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * PA_LN2;
+    if (p.lse && d == 0) p.lse[(int64_t)t * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * PA_LN2;
 }
 
-// The end of a segment that left a part: the last workgroup of the tile to come here joins its parts, those of
-// workgroups i0 .. i1.  Every wavefront of the workgroup calls it, its stores made.
+// Rows r .. r + 256 / DP - 1 (below live) of a tile in parts: joined and written.
+template <typename T, int DP, bool LIVE>
+__device__ __forceinline__ void pa_join_tile_rows(const PaParams& p, const PaParts& t, int R, int r, int live, int row0, int first,
+                                                  int head, int lane) {
+    const int mine = r + lane / (DP / 4), in = min(mine, live - 1);
+    f32x4 o;
+    float m, l;
+    pa_join_rows<DP, LIVE>(t.n, [&](int j, const float2*& ml, const float*& q) {
+        const int64_t at = pa_part(t, j, in, R);
+        ml = p.ws_ml + at;
+        q = p.ws_o + at * DP;
+    }, lane, o, m, l);
+    const int i = (int)div_of((uint32_t)(row0 + in), p.by_g);
+    if (mine < live) pa_store_row<T, DP>(p, first + i, head * p.G + row0 + in - i * p.G, o, m, l, lane);
+}
+
+// The end of a segment that left a part: the last workgroup of the tile to come here joins its parts.  Every wavefront of the
+// workgroup calls it, its stores made.
 template <typename T, int DP, int WAVES>
-__device__ __forceinline__ void pa_arrive(const PaParams& p, uint32_t i0, uint32_t i1, int R, int live, int row0, int first,
+__device__ __forceinline__ void pa_arrive(const PaParams& p, const PaParts& t, int R, int live, int row0, int first,
                                           int head, int w, int lane, int* flag) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        const unsigned before = __hip_atomic_fetch_add(p.ws_count + i0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const bool last = before == i1 - i0;
-        if (last) __hip_atomic_store(p.ws_count + i0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const unsigned before = __hip_atomic_fetch_add(p.ws_count + t.i0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const bool last = before == (unsigned)(t.n - 1);
+        if (last) __hip_atomic_store(p.ws_count + t.i0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         *flag = last;
     }
     __syncthreads();
     if (!*flag) return;
-    for (int r = w; r < live; r += WAVES) {
-        auto at = [&](int j) { return (int64_t)(2 * (i0 + (uint32_t)j) + (j == 0 ? 1u : 0u)) * R + r; };
-        float o[DP / 64], m, l;
-        pa_join_row<DP>((int)(i1 - i0 + 1), [&](int j) { return p.ws_ml + at(j); }, [&](int j) { return p.ws_o + at(j) * DP; }, lane, o,
-                        m, l);
-        const int i = (int)div_of((uint32_t)(row0 + r), p.by_g);
-        pa_store_row<T, DP>(p, first + i, head * p.G + row0 + r - i * p.G, o, m, l, lane);
-    }
+    constexpr int RPW = 256 / DP;
+    for (int r = w * RPW; r < live; r += WAVES * RPW) pa_join_tile_rows<T, DP, true>(p, t, R, r, live, row0, first, head, lane);
+}
+
+// The end of a workgroup of a launch whose parts paged_join_tiles_kernel joins: its open tile, if it has one.
+__device__ __forceinline__ void pa_leave_open(PaOpen* at, const PaOpen& x) {
+    if (threadIdx.x == 0) *at = x;
+}
+
+// Joins the parts of tiles of many rows, which one workgroup would be at for long (256 rows in 32 parts: 80 us): block
+// i `shares` + y takes share y of the rows of the tile that workgroup i left open, if it did.  A tile's shares lie on
+// different XCDs (with the tiles' first workgroups 32 apart and a tile a workgroup column, all were on one, at its 0.9 TB/s).
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) paged_join_tiles_kernel(PaParams, int R, int shares) {
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    PaArgs args;
+    args.load(lane);
+    const PaParams p = args.get();
+    const uint32_t i0 = blockIdx.x / (unsigned)shares;
+    const int share = (int)(blockIdx.x - i0 * (unsigned)shares);
+    const PaOpen x = p.ws_open[i0];
+    if (x.parts == 0) return;
+    constexpr int RPW = 256 / DP;
+    for (int r = (4 * share + w) * RPW; r < x.live; r += 4 * shares * RPW)
+        pa_join_tile_rows<T, DP, false>(p, {i0, x.parts}, R, r, x.live, x.row0, x.first, x.head, lane);
 }
 
 }  // namespace lava
