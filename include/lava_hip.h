@@ -572,8 +572,9 @@ typedef struct lava_hip_kv_cache {
  * j lies in page table[b * max_pages + j / page_size], row j % page_size.  q_start, kv_len and table are device
  * memory and are read when the kernels run.  Nothing they hold makes a kernel read or write outside the
  * buffers: row numbers are cut to [0, tokens], kv_len to [0, max_pages * page_size], and a page number outside
- * [0, pages) is no page: its keys are masked, and nothing is written to it.  Rows behind the last
- * sequence's are not written.  Sequences may have no new tokens, and no tokens at all. */
+ * [0, pages) is no page: its keys are masked, and nothing is written to it.  q_start does not decrease (where it does, which rows
+ * a call writes is open).  Rows behind the last sequence's are not written.  Sequences may have no new tokens, and no
+ * tokens at all. */
 typedef struct lava_hip_kv_batch {
     int32_t sequences; /* B */
     int32_t max_pages; /* entries of a sequence's row of the table */
@@ -582,8 +583,10 @@ typedef struct lava_hip_kv_batch {
     const int32_t* q_start; /* B + 1 */
     const int32_t* kv_len;  /* B */
     const int32_t* table;   /* B rows of max_pages */
-    /* workspace of the attention calls, lava_hip_paged_workspace_bytes of it; NULL for the library's own of the
-     * stream (see lava_hip_gemm_w8a16).  Two graphs that may run at once need one each. */
+    /* workspace of the attention calls, 16-byte aligned, lava_hip_paged_workspace_bytes of it, its first 4096 bytes zeros
+     * before its first use (every call leaves them so); NULL for the library's own of the stream (see
+     * lava_hip_gemm_w8a16), which a graph capture uses if it is large enough and is refused otherwise.  Calls
+     * that may run at once, two replayed graphs' too, need one each. */
     void* workspace;
     size_t workspace_bytes;
 } lava_hip_kv_batch;
@@ -613,7 +616,8 @@ int lava_hip_kv_append(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* 
  *   slopes:   s -= slopes[query head] * |i - j|;
  *   masked (no part of the softmax) unless j <= i (causal) or j < bidirectional[b], and, with window > 0,
  *   only if j > i - window.
- * A query that sees no key gives zeros and a log-sum-exp of -inf. */
+ * A query that sees no key gives zeros and a log-sum-exp of -inf.  What masked places of the cache hold, infinities and NaN
+ * too, has no part in a result. */
 typedef struct lava_hip_attn_score {
     float scale;
     float cap;                    /* 0: none */

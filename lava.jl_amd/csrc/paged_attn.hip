@@ -2,6 +2,7 @@
 //
 //  * paged_rows_kernel (paged_attn_rows.hip): rows of a sequence's queries and heads that share a key head,
 //    the work split evenly along the keys over the whole chip;
+//  * paged_tile_kernel (paged_attn_tile.hip): tiles of 128 or 256 such rows, for prompts;
 //  * paged_any_kernel: any head dimension, page size, strides and alignment; one wavefront a query and head.
 #include "paged_attn.hpp"
 
@@ -319,8 +320,8 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     int rc = pa_prepare(fn, cache, batch, score, q_heads, &p, &done);
     if (rc != LAVA_HIP_OK) return rc;
     LAVA_ARG(prefix >= 0, "%s: prefix_len is negative", fn);
-    LAVA_REQUIRE(prefix <= 0x3fffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s: prefix_len = %lld is longer than 2^30", fn,
-                 (long long)prefix);
+    LAVA_REQUIRE(prefix <= 0x3ffffe00, LAVA_HIP_ERR_UNSUPPORTED, "%s: prefix_len = %lld is longer than 2^30 - 512", fn,
+                 (long long)prefix);   // positions and the block behind the last fit 31 bits
     if (done) return LAVA_HIP_OK;
     LAVA_ARG(Q && O && q_strides && o_strides && (ppages || prefix == 0), "%s: null pointer", fn);
     LAVA_ARG(aligned(Q, 2) && aligned(O, 2) && aligned(lse, 4) && aligned(ppages, 4), "%s: misaligned", fn);
@@ -398,7 +399,13 @@ extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, co
     if (rc != LAVA_HIP_OK) return rc;
     *bytes = 0;
     if (done) return LAVA_HIP_OK;
-    p.P = (int)std::min<int64_t>(prefix_len, 0x3fffffff);
-    if (pa_vectors(p) && pa_countable(p)) *bytes = pa_plan_call(&p, pa_max_rows(p, batch)).bytes;
+    p.P = (int)std::min<int64_t>(prefix_len, 0x3ffffe00);
+    if (!pa_vectors(p) || !pa_countable(p)) return LAVA_HIP_OK;
+    // whatever Q's and O's strides are: with those that the tile kernel takes, and without
+    for (const int64_t stride : {(int64_t)0, (int64_t)1 << 40}) {
+        PaParams q = p;
+        q.qst = stride;
+        *bytes = std::max(*bytes, pa_plan_call(&q, pa_max_rows(q, batch)).bytes);
+    }
     return LAVA_HIP_OK;
 }

@@ -245,7 +245,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
 
             const int first = now.pos, none = (now.at[0] < 0) | (now.at[1] < 0) << 1 | (now.at[2] < 0) << 2 | (now.at[3] < 0) << 3;
             const int end_pos = first + now.left - 1;   // the source's last key
-            const bool cut = none != 0 || first < lo_max || first + 31 > min(hi_min, end_pos);
+            // keys that some row does not see and that have values (those past the end read as zeros)
+            const bool part_seen = first < lo_max || min(first + 31, end_pos) > hi_min;
+            const bool cut = part_seen || none != 0 || first + 31 > end_pos;
             bool near = false;   // with a cap: every score in the polynomial's range
             if (p.cap2 != 0.f) {
                 float far = 0.f;
@@ -301,11 +303,28 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
                 }
             }
             pr_wait<NI>();   // V is here
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) {
+            auto vread = [&](int dt) __attribute__((always_inline)) -> v8 {
                 const pg_s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)v_rd[dt]);
                 const pg_s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(v_rd[dt] + (uint32_t)(16 * RB)));
-                const v8 a = __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+                return __builtin_bit_cast(v8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            if (__builtin_expect(part_seen, 0) && __builtin_expect(pg_not_finite<T, TILE>(lds_v, lane), 0)) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) {
+                    v8 up, down;
+                    pg_split<T>(vread(dt), up, down);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        pg_add_not_finite(o[dt][nr], TT::mma16(up, pf[nr], f32x4{0.f, 0.f, 0.f, 0.f}), 1.f);
+                        pg_add_not_finite(o[dt][nr], TT::mma16(down, pf[nr], f32x4{0.f, 0.f, 0.f, 0.f}), -1.f);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                pg_drop_not_finite<T, TILE>(lds_v, lane);
+            }
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                const v8 a = vread(dt);
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) o[dt][nr] = TT::mma16(a, pf[nr], o[dt][nr]);
             }
@@ -451,6 +470,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pr
         return x;
     };
     const PaPlan plan = pa_plan<PR_BK, false, true>(p, R, true, p.stack == 1, lane);
+    if (plan.falls) return;
     uint32_t before = plan.pre_work;
     for (int b0 = 0; b0 < b; b0 += 64) {
         const uint32_t upto =

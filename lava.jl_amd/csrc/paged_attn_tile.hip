@@ -8,10 +8,10 @@
 //  * 8 keys at a time are found through the page table, a block ahead of their request;
 //  * every row has its own interval of visible positions: only blocks that some row of a pair does not see whole
 //    compare, blocks that none sees are skipped, and a pair whose rows see nothing yet has no maximum (unset, -inf);
-//  * MODE 0 (f16, 0 < scale log2 e <= 1, no cap or slopes): the scale is folded into Q (one rounding) and the maximum
-//    enters the product as a bias k-step, so that P = exp2 of the accumulator; 1 (bf16, positive scale): P = exp2(fma(S, c,
-//    -m)), since bf16 would lose 2^-8 of q c; 2: caps (a polynomial where a block's scores are small, pa_cap_near), slopes,
-//    any scale.
+//  * the scale and the maximum are one fma a score, P = exp2(fma(S, c, -m)); ANY: caps (a polynomial where a block's scores
+//    are small, pa_cap_near), slopes, a scale that is not positive.  Folding the scale into Q and the maximum into the
+//    product, as flash_fwd5_kernel does for f16, is 3.5 % faster on f16 prompts (4 of 4096 tokens: 655 against 679 us)
+//    and rounds each q once more: 3.8e-4 off against 2.9e-4, of which the results' own rounding is 2.1e-4.
 
 #include <algorithm>
 
@@ -26,7 +26,7 @@ constexpr int PT_KST = 3, PT_VST = 2;   // LDS stages
 constexpr int PT_PF = 4;                // fragments read ahead of their MFMA
 constexpr float PT_RESCALE = 8.f;
 
-template <typename T, int DE, int QH, int MODE, bool PRE>
+template <typename T, int DE, int QH, bool ANY, bool PRE>
 __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams, int stacked) {
     typedef PgType<T> TT;
     typedef typename TT::v8 v8;
@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     __shared__ __attribute__((aligned(1024))) uint8_t pbuf[2][PT_PAIRS][PBUF];
     __shared__ float abuf[2][PT_PAIRS][PQ];
     __shared__ int fbuf[2][PT_PAIRS];
+    __shared__ int nan_sums[PT_PAIRS];
     __shared__ __attribute__((aligned(16))) int nbuf[PT_KST][4];   // keys without a page, 2 bits of 8 keys each
     __shared__ float mbuf[PT_PAIRS][PQ];
 
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     const PaParams p = args.get();
     const PaPlan plan = pa_plan<PT_BK, true, PRE>(p, BQ, !prefix, prefix, lane);
     int tiles_upto = 0;
-    const bool by_tile = !prefix && pa_by_tile<PRE>(p, plan, BQ, lane, tiles_upto);
+    const bool by_tile = !prefix && !plan.falls && pa_by_tile<PRE>(p, plan, BQ, lane, tiles_upto);
     PaOpen open = {};
     if (by_tile && blockIdx.x < PT_GRID) pa_leave_open(p.ws_open + blockIdx.x, open);
     uint32_t at = 0, stop = 1, per = 1, wg = 0;
@@ -101,6 +102,10 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         stop = min(plan.total, at + per);
     }
 
+    // 0 times a value that is not finite is NaN, also in rows that do not see its key: a segment with sums that are NaN is done
+    // once more with the values' finite parts apart (pg_split).  That costs inputs without such values 1 %; a look at the
+    // values of blocks that not all rows see whole, in the loop, cost 5 to 10.
+    bool careful = false;
     for (; at < stop;) {
     // ---- the segment: some key blocks of a row tile
     const PaParams p = args.get();
@@ -156,6 +161,11 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         return p_lane + (uint32_t)(buf * PT_PAIRS * PBUF + ((kt * 2 + ks) * QH + qh) * 1024);
     };
 
+    auto again = [&]() {
+        careful = !careful && __builtin_amdgcn_readfirstlane(nan_sums[0] | nan_sums[1] | nan_sums[2] | nan_sums[3]) != 0;
+        return careful;
+    };
+
     if (is_s) {
         // ================= score wavefront =================
         // The pair's rows of Q by LDS-DMA, 4 whole rows an instruction, into its P buffers (free until the first block's P), in
@@ -196,7 +206,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 r_hi[qh] = rg.hi;
                 r_pos[qh] = (float)pos;
                 slope[qh] = 0.f;
-                if (MODE == 2 && p.slopes && row < rows) slope[qh] = p.slopes[head * p.G + row - i * p.G] * PA_LOG2E;
+                if (ANY && p.slopes && row < rows) slope[qh] = p.slopes[head * p.G + row - i * p.G] * PA_LOG2E;
             }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -213,12 +223,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 const uint4 u = __builtin_bit_cast(uint4, qf[qh][ks]);
                 asm volatile("" ::"v"(u.x), "v"(u.y), "v"(u.z), "v"(u.w) : "memory");
             }
-        if constexpr (MODE == 0) {
-#pragma unroll
-            for (int qh = 0; qh < QH; ++qh)
-#pragma unroll
-                for (int ks = 0; ks < NKS; ++ks) pg_scale_f16(qf[qh][ks], p.mul);
-        }
         // between the first position that the pair's last row sees and the last that its first one does, no comparison
         int in_lo = pa_range(p, end - seq.n + (int)div_of((uint32_t)min(row0 + PQ - 1, rows - 1), p.by_g), end, bid).lo;
         int in_hi = pa_range(p, end - seq.n + (int)div_of((uint32_t)row0, p.by_g), end, bid).hi;
@@ -230,12 +234,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         in_hi = __builtin_amdgcn_readfirstlane(in_hi);
 
         const PaParams p = args.get();
-        bool fast = MODE == 0;   // the maximum comes in through the product (wavefront-uniform)
-        v8 ones{};
-        ones[0] = h == 0 ? (T)1.f : (T)0.f;
-        v8 qm[QH];
-#pragma unroll
-        for (int qh = 0; qh < QH; ++qh) qm[qh] = v8{};
         // K fragment (kt, ks): row 32 kt + r32, chunk (2 ks + h) ^ (r32 % 16), which is ks in bits 1 and up of the rest
         const uint32_t kb0 = lds_addr(&kbuf[0][0]) + (uint32_t)(r32 * RB + ((h ^ (r32 & 15)) << 4));
         f32x16 st[2][QH];   // register r: key 32 kt + 8 (r / 4) + 4 h + r % 4
@@ -253,25 +251,18 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
             for (int f = 0; f < PT_PF; ++f) fr[f] = kread(f);
             const i4 nn = *(const lds_i4*)(uintptr_t)lds_addr(&nbuf[j % PT_KST][0]);
-            if constexpr (MODE == 0) {
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int qh = 0; qh < QH; ++qh) st[kt][qh] = TT::mma32(ones, qm[qh], f32x16{});
-            }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < QH * NSF; ++i) {
                 const int f = i / QH, qh = i % QH, ks = f >> 1, kt = f & 1;
-                st[kt][qh] = TT::mma32(fr[f % PT_PF], qf[qh][ks], MODE != 0 && ks == 0 ? f32x16{} : st[kt][qh]);
+                st[kt][qh] = TT::mma32(fr[f % PT_PF], qf[qh][ks], ks == 0 ? f32x16{} : st[kt][qh]);
                 if (qh == QH - 1 && f + PT_PF < NSF) fr[f % PT_PF] = kread(f + PT_PF);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const int none = __builtin_amdgcn_readfirstlane(nn.x | nn.y << 2 | nn.z << 4 | nn.w << 6);
             const int pos0 = __builtin_amdgcn_readfirstlane(first_pos(e0 + j));
             const int src_hi = PRE && e0 + j < np ? P - 1 : end - 1;
-            // scores relative to the maximum (to 0 while it is unset), as in MODE 0 the product gives them
-            const bool fast_blk = MODE != 0 || fast;
+            // scores relative to the maximum, to 0 while it is unset
             float ref[QH];
 #pragma unroll
             for (int qh = 0; qh < QH; ++qh) ref[qh] = m[qh] == -INFINITY ? 0.f : m[qh];
@@ -283,8 +274,8 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
                         for (int r = 0; r < 16; ++r) st[kt][qh][r] = f(st[kt][qh][r], qh, 32 * kt + 8 * (r >> 2) + (r & 3));
             };
-            if constexpr (MODE == 1) each([&](float x, int qh, int) { return fmaf(x, p.mul, -ref[qh]); });
-            if constexpr (MODE == 2) {
+            if constexpr (!ANY) each([&](float x, int qh, int) { return fmaf(x, p.mul, -ref[qh]); });
+            if constexpr (ANY) {
                 if (p.cap2 == 0.f) {
                     each([&](float x, int qh, int) { return fmaf(x, p.mul, -ref[qh]); });
                 } else {
@@ -310,9 +301,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                                                                                                   // to 2^24, of use to the slopes that far
                     each([&](float x, int qh, int k) { return fmaf(-slope[qh], fabsf(d0[qh] + (float)k), x); });
                 }
-            }
-            if constexpr (MODE == 0) {
-                if (!fast_blk) each([&](float x, int qh, int) { return x - ref[qh]; });
             }
             if (none != 0 || pos0 < in_lo || pos0 + PT_BK - 1 > min(in_hi, src_hi)) {
 #pragma unroll
@@ -345,7 +333,6 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             float sub[QH] = {};   // what P = exp2(score - sub) takes off
             if (rescale) {
                 float mn[QH];
-                bool far = false;
 #pragma unroll
                 for (int qh = 0; qh < QH; ++qh) {
                     float a, c;
@@ -353,19 +340,14 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                     const float t = fmaxf(a, c);
                     const bool unset = m[qh] == -INFINITY;
                     mn[qh] = unset ? t : m[qh] + fmaxf(t, 0.f);
-                    far = far || (mn[qh] != -INFINITY && !(fabsf(mn[qh]) <= 32768.f));
                 }
-                // m is kept f16-representable while it enters the product; beyond +-32768 it would be too coarse
-                if (MODE == 0 && fast && __builtin_amdgcn_ballot_w64(far) != 0) fast = false;
 #pragma unroll
                 for (int qh = 0; qh < QH; ++qh) {
-                    if (MODE == 0 && fast) mn[qh] = (float)(T)mn[qh];
                     const bool unset = m[qh] == -INFINITY, still = mn[qh] == -INFINITY;
                     const float alpha = unset ? 1.f : __builtin_amdgcn_exp2f(m[qh] - mn[qh]);
                     const float to = still ? 0.f : mn[qh];
                     sub[qh] = to - ref[qh];
                     m[qh] = mn[qh];
-                    if constexpr (MODE == 0) qm[qh][0] = (fast && h == 0) ? (T)(-to) : (T)0.f;
                     if (h == 0) abuf[buf][pr][32 * qh + r32] = alpha;
                 }
             }
@@ -406,6 +388,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
             for (int qh = 0; qh < QH; ++qh) mbuf[pr][32 * qh + r32] = m[qh];
         }
         __syncthreads();
+        if (again()) continue;
     } else {
         // ================= output wavefront =================
         const PaParams p = args.get();
@@ -470,7 +453,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();   // K_0 .. K_2, V_0 in LDS
         __syncthreads();   // P_0 published
-        for (int j = 0; j < nblk; ++j) {
+        auto step = [&](int j, auto slow) __attribute__((always_inline)) {
             const int buf = j & 1;
             // K_{j+3} into K_j's stage, V_{j+1} into V_{j-1}'s, both read in iteration j - 1
             request(true, j + 3);
@@ -503,35 +486,75 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 auto pread = [&](int kk, int qh) __attribute__((always_inline)) -> v8 {
                     return *(const lds_v8*)(uintptr_t)paddr(buf, kk >> 1, kk & 1, qh);
                 };
-                v8 fr[PT_PF + 1], pp[2][QH];
+                if constexpr (decltype(slow)::value) {
+#pragma unroll 1
+                    for (int kk = 0; kk < 4; ++kk) {
+                        v8 x[QH];
 #pragma unroll
-                for (int qh = 0; qh < QH; ++qh) pp[0][qh] = pread(0, qh);
+                        for (int qh = 0; qh < QH; ++qh) {
+                            x[qh] = pread(kk, qh);
 #pragma unroll
-                for (int f = 0; f < PT_PF + 1; ++f) fr[f] = vread(f);
-                __builtin_amdgcn_sched_barrier(0);
+                            for (int e = 0; e < 4; ++e) l[qh] = TT::dot2(v2{x[qh][2 * e], x[qh][2 * e + 1]}, l[qh]);
+                        }
 #pragma unroll
-                for (int i = 0; i < QH * NVF; ++i) {
-                    const int f = i / QH, qh = i % QH, kk = f / NDT, dt = f % NDT;
-                    if (i % (QH * NDT) == 0 && kk < 3) {
+                        for (int dt = 0; dt < NDT; ++dt) {
+                            v8 up, down;
+                            const v8 a = pg_split<T>(vread(NDT * kk + dt), up, down);
 #pragma unroll
-                        for (int qq = 0; qq < QH; ++qq) pp[(kk + 1) & 1][qq] = pread(kk + 1, qq);
+                            for (int qh = 0; qh < QH; ++qh) {
+                                o[dt][qh] = TT::mma32(a, x[qh], o[dt][qh]);
+                                pg_add_not_finite(o[dt][qh], TT::mma32(up, x[qh], f32x16{}), 1.f);
+                                pg_add_not_finite(o[dt][qh], TT::mma32(down, x[qh], f32x16{}), -1.f);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                        }
                     }
-                    if (i % (QH * NDT) == QH * NDT / 2) {   // row sums of what is multiplied
+                } else {
+                    v8 fr[PT_PF + 1], pp[2][QH];
 #pragma unroll
-                        for (int qq = 0; qq < QH; ++qq)
+                    for (int qh = 0; qh < QH; ++qh) pp[0][qh] = pread(0, qh);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                l[qq] = TT::dot2(v2{pp[kk & 1][qq][2 * e], pp[kk & 1][qq][2 * e + 1]}, l[qq]);
-                    }
-                    o[dt][qh] = TT::mma32(fr[f % (PT_PF + 1)], pp[kk & 1][qh], o[dt][qh]);
-                    if (qh == QH - 1 && f + PT_PF + 1 < NVF) fr[f % (PT_PF + 1)] = vread(f + PT_PF + 1);
+                    for (int f = 0; f < PT_PF + 1; ++f) fr[f] = vread(f);
                     __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int i = 0; i < QH * NVF; ++i) {
+                        const int f = i / QH, qh = i % QH, kk = f / NDT, dt = f % NDT;
+                        if (i % (QH * NDT) == 0 && kk < 3) {
+#pragma unroll
+                            for (int qq = 0; qq < QH; ++qq) pp[(kk + 1) & 1][qq] = pread(kk + 1, qq);
+                        }
+                        if (i % (QH * NDT) == QH * NDT / 2) {   // row sums of what is multiplied
+#pragma unroll
+                            for (int qq = 0; qq < QH; ++qq)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    l[qq] = TT::dot2(v2{pp[kk & 1][qq][2 * e], pp[kk & 1][qq][2 * e + 1]}, l[qq]);
+                        }
+                        o[dt][qh] = TT::mma32(fr[f % (PT_PF + 1)], pp[kk & 1][qh], o[dt][qh]);
+                        if (qh == QH - 1 && f + PT_PF + 1 < NVF) fr[f % (PT_PF + 1)] = vread(f + PT_PF + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // K_{j+3}, V_{j+1} are here
             __syncthreads();
+        };
+        if (__builtin_expect(!careful, 1)) {
+            for (int j = 0; j < nblk; ++j) step(j, pg_tag<false>{});
+            float zero[4] = {};
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int qh = 0; qh < QH; ++qh)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) zero[r & 3] = fmaf(o[dt][qh][r], 0.f, zero[r & 3]);
+            const bool some = __builtin_amdgcn_ballot_w64(!(zero[0] + zero[1] + zero[2] + zero[3] == 0.f)) != 0;
+            if (lane == 0) nan_sums[pr] = some;
+        } else {
+            for (int j = 0; j < nblk; ++j) step(j, pg_tag<true>{});
         }
-        __syncthreads();   // the maxima are published
+        __syncthreads();   // the maxima and whether sums are NaN are published
+        if (again()) continue;
         const PaParams e = args.get();
         const int lane = pa_again(threadIdx.x & 63), r32 = lane & 31, h = lane >> 5;
         // Rows leave through LDS, so that stores are of whole rows: 16 rows of 256 bytes at a time in each of this wavefront's
@@ -651,21 +674,18 @@ int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStre
     LAVA_REQUIRE(tiles <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "paged attention: problem too large");
     const unsigned grid = prefix ? PT_GRID : (unsigned)std::max<int64_t>(tiles, PT_GRID);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(128 * PT_PAIRS), 0, s, p, prefix ? 1 : 0); };
-    auto by_d = [&](auto type, auto q, auto mode) {
+    auto by_d = [&](auto type, auto q, auto any) {
         typedef decltype(type) T;
-        constexpr int QH = decltype(q)::value, MODE = decltype(mode)::value;
+        constexpr int QH = decltype(q)::value;
+        constexpr bool ANY = decltype(any)::value;
         if (p.P > 0)
-            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE, true>) : go(paged_tile_kernel<T, 128, QH, MODE, true>);
+            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, ANY, true>) : go(paged_tile_kernel<T, 128, QH, ANY, true>);
         else
-            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, MODE, false>) : go(paged_tile_kernel<T, 128, QH, MODE, false>);
+            p.c.D <= 64 ? go(paged_tile_kernel<T, 64, QH, ANY, false>) : go(paged_tile_kernel<T, 128, QH, ANY, false>);
     };
-    auto by_mode = [&](auto q) {
-        if (dtype == LAVA_HIP_F16)
-            plain && p.mul <= 1.f ? by_d(f16{}, q, pg_int<0>{}) : by_d(f16{}, q, pg_int<2>{});
-        else
-            plain ? by_d(bf16{}, q, pg_int<1>{}) : by_d(bf16{}, q, pg_int<2>{});
-    };
-    qh == 1 ? by_mode(pg_int<1>{}) : by_mode(pg_int<2>{});
+    auto by_score = [&](auto type, auto q) { plain ? by_d(type, q, pg_tag<false>{}) : by_d(type, q, pg_tag<true>{}); };
+    auto by_rows = [&](auto type) { qh == 1 ? by_score(type, pg_int<1>{}) : by_score(type, pg_int<2>{}); };
+    dtype == LAVA_HIP_F16 ? by_rows(f16{}) : by_rows(bf16{});
     const int rc = check_launch(qh == 1 ? "paged_tile_kernel+paged_tile_kernel<32>" : "paged_tile_kernel");
     if (rc != LAVA_HIP_OK || prefix || p.whole) return rc;
     auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(PT_GRID * 8), dim3(256), 0, s, p, 128 * qh, 8); };

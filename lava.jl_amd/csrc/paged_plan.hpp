@@ -136,6 +136,7 @@ struct PaPlan {
     uint32_t pre_work;
     int t0, t1;         // rows of the batch
     bool plain;         // every row sees the whole prefix
+    bool falls;         // q_start does
 };
 
 __device__ __forceinline__ PagedSeq pa_lane_seq(const PaParams& p, int b) {
@@ -149,9 +150,10 @@ template <int BK, bool ABOVE, bool PRE>
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, int R, bool seqs, bool prefix, int lane) {
     PaPlan g = {};
     int lo = 0x7fffffff;
-    bool plain = p.window == 0;
+    bool plain = p.window == 0, falls = false;
     for (int b0 = 0; b0 < p.b.B; b0 += 64) {
         const PagedSeq s = pa_lane_seq(p, b0 + lane);
+        if (b0 + lane < p.b.B) falls = falls || p.b.q_start[b0 + lane + 1] < p.b.q_start[b0 + lane];
         const uint32_t upto = pa_scan(seqs ? pa_work(p, pa_seq<BK, ABOVE, PRE>(p, s, R)) : 0u);
         if (b0 == 0) {
             g.mine = s;
@@ -175,6 +177,11 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, int R, bool seqs, b
             g.pre_work = pa_work(p, g.prefix);
         }
         g.total += g.pre_work;
+    }
+    // sequences that overlap would be more rows than T, whose blocks the host has counted in 31 bits: no work
+    if (__builtin_amdgcn_ballot_w64(falls) != 0) {
+        g.total = g.pre_work = 0;
+        g.falls = true;
     }
     return g;
 }

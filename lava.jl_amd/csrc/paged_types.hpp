@@ -45,22 +45,70 @@ struct PgType<bf16> {
     }
 };
 
-// q = f16(q c) in place, rounded once: the mixed-precision FMA on either half of a register.  The s_nop is for
-// an MFMA that reads q next.  (bf16 has no such instruction, and no use for it: one rounding of q c would cost 2^-8.)
-__device__ __forceinline__ void pg_scale_f16(f16x8& q, float c) {
-    uint4 u = __builtin_bit_cast(uint4, q);
-    asm("v_fma_mixlo_f16 %0, %0, %4, 0 op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixhi_f16 %0, %0, %4, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixlo_f16 %1, %1, %4, 0 op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixhi_f16 %1, %1, %4, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixlo_f16 %2, %2, %4, 0 op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixhi_f16 %2, %2, %4, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixlo_f16 %3, %3, %4, 0 op_sel_hi:[1,0,0]\n\t"
-        "v_fma_mixhi_f16 %3, %3, %4, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]\n\t"
-        "s_nop 1"
-        : "+v"(u.x), "+v"(u.y), "+v"(u.z), "+v"(u.w)
-        : "v"(c));
-    q = __builtin_bit_cast(f16x8, u);
+// Values that are not finite, at keys that only some rows of a tile see: P V is a matrix product and 0 times infinity is
+// NaN, in rows that do not see the key.  Where a tile of values has any, they enter as zeros, and what they are worth to
+// each row comes from products of P with where they are.
+
+typedef uint16_t pg_u16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t pg_u16x8 __attribute__((ext_vector_type(8)));
+template <typename T>
+constexpr uint16_t PG_EXPONENT = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80 : 0x7c00;
+
+// Whether one of `bytes` bytes of LDS from `at` on is of a value that is not finite (by a wavefront together, 1024 at a time).
+template <typename T, int BYTES>
+__device__ __forceinline__ bool pg_not_finite(uint32_t at, int lane) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) const u4 lds_u4;
+    pg_u16x2 top = {0, 0};
+#pragma unroll 8
+    for (int i = 0; i < BYTES / 1024; ++i) {
+        const u4 u = *(lds_u4*)(uintptr_t)(at + 16u * (uint32_t)lane + 1024u * (uint32_t)i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = __builtin_elementwise_max(top, __builtin_bit_cast(pg_u16x2, u[k] & 0x7fff7fffu));
+    }
+    return __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= PG_EXPONENT<T>) != 0;
+}
+
+// 0 in place of such values there.
+template <typename T, int BYTES>
+__device__ __forceinline__ void pg_drop_not_finite(uint32_t at, int lane) {
+    typedef __attribute__((address_space(3))) pg_u16x8 lds_u16x8;
+#pragma unroll 1
+    for (int i = 0; i < BYTES / 1024; ++i) {
+        lds_u16x8* const x = (lds_u16x8*)(uintptr_t)(at + 16u * (uint32_t)lane + 1024u * (uint32_t)i);
+        pg_u16x8 v = *x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (v[e] & 0x7fff) >= PG_EXPONENT<T> ? (uint16_t)0 : v[e];
+        *x = v;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
+// 1 where a is +infinity or NaN (up), where it is -infinity or NaN (down).  Returns a with 0 in their place.
+template <typename T, typename V>
+__device__ __forceinline__ V pg_split(V a, V& up, V& down) {
+    pg_u16x8 x = __builtin_bit_cast(pg_u16x8, a);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint16_t b = x[e] & 0x7fff;
+        const bool off = b >= PG_EXPONENT<T>, nan = b > PG_EXPONENT<T>, minus = (x[e] >> 15) != 0;
+        up[e] = off && (nan || !minus) ? (T)1.f : (T)0.f;
+        down[e] = off && (nan || minus) ? (T)1.f : (T)0.f;
+        x[e] = off ? (uint16_t)0 : x[e];
+    }
+    return __builtin_bit_cast(V, x);
+}
+
+// What infinities of the sign add to the sums o by `weight`, P's product with where they are: 2^254 times it, which is infinite
+// for every P but 0.
+template <typename F>
+__device__ __forceinline__ void pg_add_not_finite(F& o, const F& weight, float sign) {
+#pragma unroll
+    for (int r = 0; r < (int)(sizeof(F) / 4); ++r) {
+#pragma clang fp contract(off)   // a fused product would stay finite, and infinity minus it infinite
+        const float x = weight[r] * 0x1p127f * (sign * 0x1p127f);
+        o[r] = o[r] + x;
+    }
 }
 
 // x of lanes 0-31 and of lanes 32-63, to all (two copies of x: one register swapped with itself gives no halves)

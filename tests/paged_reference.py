@@ -5,8 +5,7 @@ Everything of a cache that holds no token is NaN, so whatever a kernel reads of 
 Bound of |O - reference|, element by element, for weights w (summing to 1) and u = eps / 2 of the operands' type:
   * P is rounded to that type, and the sum that divides is of the rounded P: 2 u sum(w |v|);
   * a score is off by ds: at most (D + 2) roundings of 2^-24 of sum |q k| scale, the cap's and the slope's at 2^-22 of the
-    score's size, exp2's 2^-22, and, where a kernel folds the scale into Q (`folded`), u sum |q k| scale; the
-    weights are off by that share, numerator and sum: 2 ds sum(w |v|);
+    score's size, exp2's 2^-22; the weights are off by that share, numerator and sum: 2 ds sum(w |v|);
   * f16 holds no P below 2^-25 of the row's largest: 2^-24 sum |v| over the row's keys (m lies at or below the largest
     score, so the sum is at least 1);
   * O's own rounding: u |O|, and half of f16's smallest number;
@@ -95,7 +94,7 @@ class Case:
         h, l, d = self.Hkv, self.page, self.D
         return (1, d, l * d, h * l * d) if self.order == "hl" else (1, h * d, d, h * l * d)
 
-    def reference(self, dead=(), folded=False):
+    def reference(self, dead=()):
         """(O, lse, bound of O, bound of lse), rows of no sequence NaN.  dead: (b, token) of keys on pages that
         are none."""
         T, Hq, D, P = self.T, self.Hq, self.D, self.prefix
@@ -127,7 +126,7 @@ class Case:
                 with np.errstate(all="ignore"):
                     s = (q @ kh.T) * self.scale
                     size = (np.abs(q) @ np.abs(kh).T) * abs(self.scale)
-                    ds = size * (D + 2) * 2.0 ** -24 + (size * u if folded else 0) + 2.0 ** -22
+                    ds = size * (D + 2) * 2.0 ** -24 + 2.0 ** -22
                     if self.cap:
                         s = self.cap * np.tanh(s / self.cap)
                         ds = ds + self.cap * 2.0 ** -22

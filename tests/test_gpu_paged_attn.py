@@ -71,8 +71,7 @@ def check(lh, case, kernel, dead=(), **more):
         lh.set_kernel_override(lh.FAMILY_PAGED, 0)
     if kernel:
         assert log[0] == (KERNELS[kernel] if kernel < 3 or case.D <= 128 else KERNELS[2]), log
-    # the tile kernel folds the scale into f16 queries
-    want, wlse, bound, lbound = case.reference(dead=dead, folded="paged_tile_kernel" in log and case.dtype == "f16")
+    want, wlse, bound, lbound = case.reference(dead=dead)
     off = bad(got, want, bound)
     assert not off.any(), (np.argwhere(off)[:5], got[off][:5], want[off][:5], bound[off][:5])
     off = bad(lse, wlse, lbound)
