@@ -94,8 +94,8 @@ int lava_hip_stream_synchronize(void* stream);
 /* A non-blocking stream (hipStreamNonBlocking, default priority). */
 int lava_hip_stream_create(void** stream);
 /* Waits for the stream's work, frees the workspace the library kept for it (W8A16 and
- * small-product GEMM split-K; buffers a graph captured on the stream may still use are kept
- * until the process ends), then destroys it. */
+ * small-product GEMM split-K, paged attention; buffers a graph captured on the stream may still use are
+ * kept until the process ends), then destroys it. */
 int lava_hip_stream_destroy(void* stream);
 int lava_hip_event_create(void** event);
 int lava_hip_event_destroy(void* event);
@@ -117,7 +117,7 @@ const char* lava_hip_last_error(void);
 /* Library version as MAJOR*10000 + MINOR*100 + PATCH. */
 int lava_hip_version(void);
 /* Frees every workspace the library keeps (W8A16 split-K partials or the row-major copy of X,
- * small-product GEMM split-K partials), after waiting for each device that holds one
+ * small-product GEMM split-K partials, paged attention's parts), after waiting for each device that holds one
  * (hipDeviceSynchronize): the release path of the NULL stream's workspaces, which
  * lava_hip_stream_destroy does not reach, and of streams created outside the library.  Buffers
  * that a graph captured on a stream may still use are kept until the process ends.  No
@@ -135,7 +135,8 @@ int lava_hip_release_workspaces(void);
  * separate form has its own name behind the kernel's: gemm_mid_ksplit_kernel behind gemm_mid_kernel (the
  * K-split form), gemm_small_kernel<any> behind gemm_small_kernel and gemm_small_kernel<u8,any> behind
  * gemm_small_kernel<u8> (operands of any alignment), flash_fwd5_kernel<32> and flash_fwd6_kernel<32>
- * behind the name without <32> (32 queries a wavefront pair or group instead of 64). */
+ * behind the name without <32> (32 queries a wavefront pair or group instead of 64), paged_tile_kernel<32>
+ * behind paged_tile_kernel (32 rows a wavefront pair, 128 a tile). */
 const char* lava_hip_kernel_log(void);
 void lava_hip_kernel_log_clear(void);
 

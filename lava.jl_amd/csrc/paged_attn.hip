@@ -252,7 +252,6 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
         const int64_t blocks = ((int64_t)p->b.kv_max + p->P + PT_BK - 1) / PT_BK;
         p->whole = blocks <= PT_SPLIT || (blocks <= 32 && rows / (128 * sh.qh) * p->c.heads >= 128);
     }
-    p->tiles = sh.qh != 0;
     if (p->row_limit > 0) {
         if (p->P > 0) {   // the prefix once for all: beside the sequences, or on the tile kernel for many rows
             const bool many = rows > PA_TILE_ROWS && paged_tile_takes(*p) && pin != 2;
@@ -344,6 +343,7 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.o16 = aligned(O, 16) && p.osh % 8 == 0 && p.ost % 8 == 0;
     p.ppages = ppages;
     p.P = (int)prefix;
+    if (p.window >= (int64_t)p.P + p.b.kv_max) p.window = 0;   // hides nothing (and positions less it stay in 32 bits)
     hipStream_t s = as_stream(stream);
     bool fast = kernel_override(LAVA_HIP_FAMILY_PAGED) != 1 && pa_countable(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
     for (int i = 1; i < 3; ++i) fast = fast && q_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;

@@ -31,9 +31,8 @@ struct PaParams {
     const int* ppages;            // the shared prefix's pages
     int P;                        // its length, 0: none
     // how the work is shared out (paged_plan.hpp)
-    int tiles;                    // the tile kernel takes the sequences of more than row_limit rows
-    int row_limit;                // rows: new tokens times G
-    int whole;                    // it never splits them
+    int row_limit;                // the tile kernel takes the sequences of more rows (new tokens times G)
+    int whole;                    // and never splits them
     int stack;                    // the prefix is attended once, by the rows of many sequences together: 1 by the row
                                   // kernel beside the sequences, 2 by the tile kernel in a launch of its own
     FastDiv by_rows, by_tiles;    // workgroups of the row kernel's launch, of the tile kernel's that split
@@ -53,7 +52,6 @@ struct PaParams {
 // A row tile in parts: those of the workgroup that keeps this and of the ones behind it (0: none).
 struct PaOpen {
     int parts, live, row0, first, head;   // its rows, the first of them in the sequence, the sequence's first token, the key head
-    int unused[3];
 };
 
 struct PaRange {
@@ -93,7 +91,6 @@ struct PaShape {
     int pre_qh;           // the stacked prefix's launch of the tile kernel; 0: none
     size_t count_bytes, bytes;   // workspace: arrivals, all of it
 };
-PaShape paged_shape(const PaParams& p, int64_t max_rows);
 int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s);
 bool paged_tile_takes(const PaParams& p);
 int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s);

@@ -114,17 +114,6 @@ __device__ __forceinline__ int pa_wave_max(int x) {
 __device__ __forceinline__ int pa_wave_min(int x) {
     return __builtin_amdgcn_readlane(pa_scan_with(x, 0x7fffffff, [](int a, int b) { return min(a, b); }), 63);
 }
-__device__ __forceinline__ float pa_as_float(int x) { return __builtin_bit_cast(float, x); }
-__device__ __forceinline__ int pa_as_int(float x) { return __builtin_bit_cast(int, x); }
-__device__ __forceinline__ float pa_wave_max(float x) {
-    const int r = pa_scan_with(pa_as_int(x), pa_as_int(-INFINITY),
-                               [](int a, int b) { return pa_as_int(fmaxf(pa_as_float(a), pa_as_float(b))); });
-    return pa_as_float(__builtin_amdgcn_readlane(r, 63));
-}
-__device__ __forceinline__ float pa_wave_sum(float x) {
-    const int r = pa_scan_with(pa_as_int(x), 0, [](int a, int b) { return pa_as_int(pa_as_float(a) + pa_as_float(b)); });
-    return pa_as_float(__builtin_amdgcn_readlane(r, 63));
-}
 
 // What every wavefront knows of the whole call.  The first 64 sequences stay in its lanes.
 struct PaPlan {
