@@ -14,7 +14,7 @@
 //    and rounds each q once more: 3.8e-4 off against 2.9e-4, of which the results' own rounding is 2.1e-4.
 
 // Measured (back to back): 4 prompts of 4096 tokens, 32 heads on 8, D = 128, 675 us, 815 TFLOP/s; 12 sequences' chunks and decode
-// steps behind 777 to 6000 keys, capped, 365; 8 prompts of 301 to 1537 tokens, 12 heads of D = 64, 52; a prompt of 64 tokens 9.
+// steps behind 777 to 6000 keys, capped, 343; 8 prompts of 301 to 1537 tokens, 12 heads of D = 64, 52; a prompt of 64 tokens 9.
 
 #include <algorithm>
 

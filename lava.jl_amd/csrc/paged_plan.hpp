@@ -342,18 +342,25 @@ __device__ __forceinline__ float2 pa_get(const float* p) {
     return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
+template <int N>
+struct PaInt {
+    static constexpr int value = N;
+};
+
 // Rows joined by a wavefront, 256 / DP of them at once: DP / 4 lanes a row, 4 columns a lane.  Part j of the lane's row has its
 // (maximum, weight) and sums at part(j, ml, o); n parts (at least one).  Sums are requested beside the weights, one round trip for
 // both: those of a part of no weight are not written, and what is read of them is dropped.  LIVE: the parts come from
 // workgroups of this launch (device-wide loads).
 template <int DP, bool LIVE, typename F>
 __device__ __forceinline__ void pa_join_rows(int n, F part, int lane, f32x4& o, float& m, float& l) {
-    constexpr int U = 16;   // parts in flight: a round trip to what other workgroups wrote takes 1 to 2 us
     const int most = pa_wave_max(n), c = lane % (DP / 4);
     m = -INFINITY;
     l = 0.f;
     o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int j0 = 0; j0 < most; j0 += U) {
+    // parts in flight: a round trip to what other workgroups wrote takes 1 to 2 us; 4 where those are all (of places past
+    // the last part the last one is read again: 16 for tiles of 2 parts: 40 us, now 17, on 12 chunks behind 777 to 6000 keys)
+    auto some_of = [&](int j0, auto in_flight) __attribute__((always_inline)) {
+        constexpr int U = decltype(in_flight)::value;
         float2 x[U];
         f32x4 v[U];
 #pragma unroll
@@ -390,6 +397,11 @@ __device__ __forceinline__ void pa_join_rows(int n, F part, int lane, f32x4& o, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = some ? fmaf(f, v[u][e], o[e]) : o[e];
         }
+    };
+    if (most <= 4) {
+        some_of(0, PaInt<4>{});
+    } else {
+        for (int j0 = 0; j0 < most; j0 += 16) some_of(j0, PaInt<16>{});
     }
 }
 
