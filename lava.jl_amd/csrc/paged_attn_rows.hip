@@ -491,13 +491,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pr
         if (pp.pre_work > 0)
             pre = source(pp.prefix, 0, pa_per(pp.total, p.by_tiles, PT_LEAST), pre_R, (uint32_t)((t - pp.t0) * p.G + g), p.pre_o, p.pre_ml, 0);
     }
+    // a row's parts lie one behind the other.  (Values, not the two structures: chosen between by j those went to scratch memory.)
+    const int pre_n = pre.parts.n, own_n = own.parts.n;
+    const int64_t pre_at = pre.at(0), own_at = own.at(0);
+    const float *const pre_o = pre.o, *const own_o = own.o;
+    const float2 *const pre_ml = pre.ml, *const own_ml = own.ml;
     f32x4 o;
     float m, l;
-    pa_join_rows<DP, false>(pre.parts.n + own.parts.n, [&](int j, const float2*& ml, const float*& q) {
-        const bool first = j < pre.parts.n;
-        const int64_t at = first ? pre.at(j) : own.at(j - pre.parts.n);
-        ml = (first ? pre.ml : own.ml) + at;
-        q = (first ? pre.o : own.o) + at * DP;
+    pa_join_rows<DP, false>(pre_n + own_n, [&](int j, const float2*& ml, const float*& q) {
+        const bool first = j < pre_n;
+        const int64_t at = (first ? pre_at : own_at) + (first ? j : j - pre_n);
+        ml = (first ? pre_ml : own_ml) + at;
+        q = (first ? pre_o : own_o) + at * DP;
     }, lane, o, m, l);
     if (h0 + lane / (DP / 4) < p.Hq) pa_store_row<T, DP>(p, t, h, o, m, l, lane);
 }
