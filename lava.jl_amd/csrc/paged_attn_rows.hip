@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
         // bound what needs comparing (rows are in order of their positions)
         v8 qf[NR][NKS];
         int row_t[NR], row_h[NR], lo[NR], hi[NR];
-        float pos[NR], slope[NR];
+        int pos[NR];
+        float slope[NR];
         bool live[NR];
         const int bid = p.bidir && b >= 0 ? p.bidir[b] : 0;
         const int end = PRE ? p.P + kv : kv, pos0 = end - sg.seq.n;   // of a prefix tile: P
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
             const PaRange rg = pa_range(p, at_pos, end, bid);
             lo[nr] = rg.lo;
             hi[nr] = rg.hi;
-            pos[nr] = (float)at_pos;
+            pos[nr] = at_pos;
             slope[nr] = 0.f;
             if (p.slopes && live[nr]) slope[nr] = p.slopes[row_h[nr]] * PA_LOG2E;
             const T* qr = (const T*)p.Q + (int64_t)row_t[nr] * p.qst + (int64_t)row_h[nr] * p.qsh + 8 * g;
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
                     for (int r = 0; r < 4; ++r) {
                         const int key = first + 16 * kt + 4 * g + r;
                         float x = near ? pa_cap_near(st[kt][nr][r], p.a) : pa_score(st[kt][nr][r], p.mul, p.cap2);
-                        if (p.slopes) x = fmaf(-slope[nr], fabsf(pos[nr] - (float)key), x);
+                        if (p.slopes) x = fmaf(-slope[nr], fabsf((float)(pos[nr] - key)), x);
                         if (cut) {
                             const bool keep = key >= lo[nr] && key <= last && !((none >> (2 * kt + (g >> 1))) & 1);
                             x = keep ? x : -INFINITY;

@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         }
         // this lane's rows: the positions that they see
         int r_lo[QH], r_hi[QH];
-        float r_pos[QH], slope[QH];
+        int r_pos[QH];
+        float slope[QH];
         {
             const PaParams p = args.get();
 #pragma unroll
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 const PaRange rg = pa_range(p, pos, end, bid);
                 r_lo[qh] = rg.lo;
                 r_hi[qh] = rg.hi;
-                r_pos[qh] = (float)pos;
+                r_pos[qh] = pos;
                 slope[qh] = 0.f;
                 if (ANY && p.slopes && row < rows) slope[qh] = p.slopes[head * p.G + row - i * p.G] * PA_LOG2E;
             }
@@ -300,8 +301,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 if (p.slopes) {
                     float d0[QH];
 #pragma unroll
-                    for (int qh = 0; qh < QH; ++qh) d0[qh] = (float)(pos0 + 4 * h) - r_pos[qh];   // whole numbers below 2^31: each exact
-                                                                                                  // to 2^24, of use to the slopes that far
+                    for (int qh = 0; qh < QH; ++qh) d0[qh] = (float)(pos0 + 4 * h - r_pos[qh]);
                     each([&](float x, int qh, int k) { return fmaf(-slope[qh], fabsf(d0[qh] + (float)k), x); });
                 }
             }

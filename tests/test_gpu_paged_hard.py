@@ -253,6 +253,31 @@ def test_offsets_past_32_bits(gpu, kernel):
     assert not bad(got, want, bound).any()
 
 
+@pytest.mark.parametrize("kernel", [0] + list(KERNELS))
+@pytest.mark.parametrize("shift", [2 ** 24, 2 ** 29])
+def test_slopes_at_positions_past_24_bits(gpu, kernel, shift):
+    """A window at the end of a long sequence, its earlier pages gone: distances are exact wherever they lie."""
+    announce(f"slopes at positions past 24 bits kernel={kernel} shift={shift}")
+    page = 2048
+    case = Case(lens=((70, 400), (1, 300)), window=200, slopes=True, Hq=4, Hkv=2, D=64, page=page, seed=22)
+    dev = Device(gpu, case)
+    table = np.full((case.B, shift // page + case.max_pages), -1, np.int32)
+    table[:, shift // page:] = case.table
+    TB = gpu.HIPDeviceArray.from_numpy(table.ravel(), "i32")
+    dev.kv_len.copy_from(case.kv_len + np.int32(shift))
+    dev.batch = gpu.paged_batch_raw(case.B, case.T, dev.q_start.ptr, dev.kv_len.ptr, TB.ptr, table.shape[1], max_q=70)
+    pinned(gpu, kernel)
+    try:
+        dev.clear()
+        dev.launch()
+        gpu.synchronize()
+    finally:
+        pinned(gpu, 0)
+    got, lse, _ = dev.result()
+    want, wlse, bound, lbound = case.reference()
+    assert not bad(got, want, bound).any() and not bad(lse, wlse, lbound).any()
+
+
 # ---- streams, workspaces, graphs --------------------------------------------------------------------------------
 
 SERVED = {
