@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(AppendParams p) {
     typedef T v8 __attribute__((ext_vector_type(8)));
     extern __shared__ float2 turn[];   // rot / 2
     const int tid = threadIdx.x, lane = tid & 63;
-    const int t = (int)blockIdx.x;
+    const int t = (int)pg_block();
     const KaToken k = ka_token(p, t, lane);   // by every wavefront: the same
     if (!k.live) return;
     for (int j = tid; j < p.rot / 2; j += KA_THREADS) turn[j] = ka_cos_sin(k.pos, p.inv_freq[j]);
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(KA_THREADS) kv_append_kernel(AppendParams p) {
 // Any head dimension, strides and alignment: one wavefront a token, a pair (or an element that does not turn) a lane.
 template <typename T>
 __global__ void __launch_bounds__(64) kv_append_any_kernel(AppendParams p) {
-    const int t = (int)blockIdx.x, lane = threadIdx.x;
+    const int t = (int)pg_block(), lane = threadIdx.x;
     const KaToken k = ka_token(p, t, lane);
     if (!k.live) return;
     const int half = p.rot / 2, D = p.c.D;
@@ -229,14 +229,14 @@ extern "C" int lava_hip_kv_append(const lava_hip_kv_cache* cache, const lava_hip
     const bool f16s = cache->dtype == LAVA_HIP_F16;
     if (!vec) {
         if (f16s)
-            hipLaunchKernelGGL((kv_append_any_kernel<f16>), dim3((unsigned)p.b.T), dim3(64), 0, s, p);
+            hipLaunchKernelGGL((kv_append_any_kernel<f16>), pg_grid(p.b.T), dim3(64), 0, s, p);
         else
-            hipLaunchKernelGGL((kv_append_any_kernel<bf16>), dim3((unsigned)p.b.T), dim3(64), 0, s, p);
+            hipLaunchKernelGGL((kv_append_any_kernel<bf16>), pg_grid(p.b.T), dim3(64), 0, s, p);
         LAVA_LAUNCH_CHECK("kv_append_any_kernel");
         return LAVA_HIP_OK;
     }
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)p.b.T), dim3(KA_THREADS), (size_t)(p.rot / 2) * sizeof(float2), s, p);
+        hipLaunchKernelGGL(kernel, pg_grid(p.b.T), dim3(KA_THREADS), (size_t)(p.rot / 2) * sizeof(float2), s, p);
     };
     f16s ? go(kv_append_kernel<f16>) : go(kv_append_kernel<bf16>);
     LAVA_LAUNCH_CHECK("kv_append_kernel");

@@ -24,6 +24,15 @@ __host__ __device__ __forceinline__ uint32_t div_of(uint32_t n, const FastDiv& f
     return (uint32_t)(((uint64_t)n * f.mul) >> f.shift);
 }
 
+// A launch of n workgroups: HIP takes fewer than 2^32 threads in a dimension, and of more it runs what is left modulo that,
+// without an error.  Up to 2^22 workgroups (of up to 512 threads) lie in x, what is above in y; workgroups
+// from n on, where y rounds up, find nothing to do.
+constexpr uint32_t PG_GRID_X = 1u << 22;
+inline dim3 pg_grid(int64_t n) {
+    return n <= PG_GRID_X ? dim3((unsigned)n) : dim3(PG_GRID_X, (unsigned)((n + PG_GRID_X - 1) / PG_GRID_X));
+}
+__device__ __forceinline__ uint32_t pg_block() { return blockIdx.y * PG_GRID_X + blockIdx.x; }
+
 struct PagedCache {
     void* k;
     void* v;

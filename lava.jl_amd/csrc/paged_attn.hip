@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(64) paged_any_kernel(PaParams p) {
     __shared__ float w[64];
     __shared__ int64_t at[64];
     const int lane = threadIdx.x;
-    const int t = (int)(blockIdx.x / (unsigned)p.Hq), h = (int)(blockIdx.x % (unsigned)p.Hq), D = p.c.D;
+    const int t = (int)(pg_block() / (unsigned)p.Hq), h = (int)(pg_block() % (unsigned)p.Hq), D = p.c.D;
     const int b = paged_find(p.b, t, lane);
     if (b >= p.b.B) return;
     const PagedSeq s = paged_seq(p.b, b);
@@ -362,9 +362,9 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
         });
     }
     if (cache->dtype == LAVA_HIP_F16)
-        hipLaunchKernelGGL((paged_any_kernel<f16>), dim3((unsigned)(p.b.T * p.Hq)), dim3(64), 0, s, p);
+        hipLaunchKernelGGL((paged_any_kernel<f16>), pg_grid((int64_t)p.b.T * p.Hq), dim3(64), 0, s, p);
     else
-        hipLaunchKernelGGL((paged_any_kernel<bf16>), dim3((unsigned)(p.b.T * p.Hq)), dim3(64), 0, s, p);
+        hipLaunchKernelGGL((paged_any_kernel<bf16>), pg_grid((int64_t)p.b.T * p.Hq), dim3(64), 0, s, p);
     LAVA_LAUNCH_CHECK("paged_any_kernel");
     return LAVA_HIP_OK;
 }

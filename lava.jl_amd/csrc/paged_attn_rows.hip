@@ -441,9 +441,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pr
     args.load(lane);
     const PaParams p = args.get();
     constexpr int RPW = 256 / DP;
-    const int per_token = (p.Hq + RPW - 1) / RPW;   // wavefronts a token
-    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const int t = wave / per_token, h0 = (wave - t * per_token) * RPW;
+    const uint32_t per_token = (uint32_t)(p.Hq + RPW - 1) / RPW;   // wavefronts a token
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(pg_block() * 4 + (threadIdx.x >> 6)));
+    const int t = (int)(wave / per_token), h0 = (int)(wave - (uint32_t)t * per_token) * RPW;
     if (t >= p.b.T) return;
     const int h = min(h0 + lane / (DP / 4), p.Hq - 1);
     const int b = paged_find(p.b, t, lane);
@@ -533,9 +533,9 @@ int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream
             return check_launch("paged_join_tiles_kernel");
         }
         const int per_wave = 256 / sh.dp;
-        const unsigned rows = (unsigned)(((int64_t)p.b.T * ((p.Hq + per_wave - 1) / per_wave) + 3) / 4);
+        const dim3 rows = pg_grid(((int64_t)p.b.T * ((p.Hq + per_wave - 1) / per_wave) + 3) / 4);
         auto join = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, p, 16 * sh.nr, 128 * sh.pre_qh);
+            hipLaunchKernelGGL(kernel, rows, dim3(256), 0, s, p, 16 * sh.nr, 128 * sh.pre_qh);
         };
         sh.dp == 64 ? join(paged_join_kernel<T, 64>) : sh.dp == 128 ? join(paged_join_kernel<T, 128>) : join(paged_join_kernel<T, 256>);
         return check_launch("paged_join_kernel");

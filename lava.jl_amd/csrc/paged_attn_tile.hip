@@ -67,14 +67,15 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     int tiles_upto = 0;
     const bool by_tile = !prefix && !plan.falls && pa_by_tile<PRE>(p, plan, BQ, lane, tiles_upto);
     PaOpen open = {};
-    if (by_tile && blockIdx.x < PT_GRID) pa_leave_open(p.ws_open + blockIdx.x, open);
+    const uint32_t block = pg_block();
+    if (by_tile && block < PT_GRID) pa_leave_open(p.ws_open + block, open);
     uint32_t at = 0, stop = 1, per = 1, wg = 0;
     PaSegment sg = {};
     if (by_tile) {
         // key heads innermost, so that an XCD's workgroups share few heads' keys; a sequence's last tiles, which
         // see the most keys, first
-        int idx = (int)(blockIdx.x / (unsigned)p.c.heads);
-        sg.head = (int)blockIdx.x - idx * p.c.heads;
+        int idx = (int)(block / (unsigned)p.c.heads);
+        sg.head = (int)block - idx * p.c.heads;
         sg.b = -1;
         int upto = tiles_upto;
         PagedSeq s = plan.mine;
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
         if (sg.b < 0) return;
         sg.sw = pa_seq<PT_BK, true, PRE>(p, sg.seq, BQ);
     } else {
-        if (blockIdx.x >= PT_GRID) return;
+        if (block >= PT_GRID) return;
         per = pa_per(plan.total, p.by_tiles, PT_LEAST);
         wg = pa_place(PT_GRID);
         at = min(plan.total, wg * per);
@@ -675,8 +676,8 @@ int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStre
     const bool plain = p.cap2 == 0.f && !p.slopes && p.mul > 0.f;
     const int64_t tiles = ((int64_t)p.b.T * p.G / (128 * qh) + p.b.B) * p.c.heads;   // no fewer than there are
     LAVA_REQUIRE(tiles <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "paged attention: problem too large");
-    const unsigned grid = prefix ? PT_GRID : (unsigned)std::max<int64_t>(tiles, PT_GRID);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(grid), dim3(128 * PT_PAIRS), 0, s, p, prefix ? 1 : 0); };
+    const dim3 grid = pg_grid(prefix ? PT_GRID : std::max<int64_t>(tiles, PT_GRID));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(128 * PT_PAIRS), 0, s, p, prefix ? 1 : 0); };
     auto by_d = [&](auto type, auto q, auto any) {
         typedef decltype(type) T;
         constexpr int QH = decltype(q)::value;
