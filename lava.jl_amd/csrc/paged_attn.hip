@@ -116,7 +116,9 @@ __global__ void __launch_bounds__(64) paged_any_kernel(PaParams p) {
                 const T* kr = (const T*)p.c.k + o;
                 float d = 0.f;
                 for (int e = 0; e < D; ++e) d = fmaf(q[e], (float)kr[e], d);
-                x = pa_score(d, p.mul, p.cap2) - slope * fabsf((float)(pos - j));
+                x = d * p.mul;
+                if (p.cap2 != 0.f) x = pa_cap_each(d, pa_cap(x, p.cap2), p.near, p.a);
+                x -= slope * fabsf((float)(pos - j));
             }
         }
         uint64_t live = __builtin_amdgcn_ballot_w64(keep);
@@ -166,7 +168,7 @@ static int pa_prepare(const char* fn, const lava_hip_kv_cache* cache, const lava
         LAVA_ARG(score->window >= 0, "%s: window = %d is negative", fn, score->window);
         LAVA_ARG(aligned(score->slopes, 4) && aligned(score->bidirectional, 4), "%s: slopes or bidirectional misaligned", fn);
         LAVA_ARG(!score->bidirectional || score->causal, "%s: bidirectional keys need a causal call", fn);
-        p->cap2 = score->cap * PA_LOG2E;
+        p->cap2 = std::min(score->cap * PA_LOG2E, 1e38f);   // the exact form's 2 cap2 stays finite
         p->mul = score->cap > 0.f ? (float)(2.0 * score->scale / score->cap * 1.4426950408889634) : (float)(score->scale * 1.4426950408889634);
         LAVA_ARG(std::isfinite(p->mul), "%s: scale / cap overflows", fn);
         if (score->cap > 0.f) {
@@ -174,13 +176,16 @@ static int pa_prepare(const char* fn, const lava_hip_kv_cache* cache, const lava
             const double c[5] = {0.9999999316221511, -0.33332776175690243, 0.13320570647011903, -0.052762128916049526,
                                  0.01673756352440004};
             const double z = (double)score->scale / score->cap;
-            double power = (double)score->cap * 1.4426950408889634 * z;
-            p->near = (float)std::min(0.5 / std::fabs(z), 1e30);
-            for (int i = 0; i < 5; ++i, power *= z * z) p->a[i] = (float)(c[i] * power);
+            double power = (double)score->cap * 1.4426950408889634 * z, reach = 0.5;
+            for (int i = 0; i < 5; ++i, power *= z * z) {
+                p->a[i] = (float)(c[i] * power);
+                // a coefficient that 32 bits do not hold to its last places: only scores that do without its term, below 2^-26 of them
+                if (i > 0 && std::fabs(p->a[i]) < 0x1p-126f) reach = std::min(reach, std::pow(0x1p-26 / std::fabs(c[i]), 0.5 / i));
+            }
+            p->near = (float)std::min(reach / std::fabs(z), 1e15);   // u = s^2 stays in range
             // powers of a large scale / cap leave 32 bits: then the exact form always
             for (int i = 0; i < 5; ++i)
                 if (!std::isfinite(p->a[i])) p->near = -1.f;
-            if (p->near > 1e15f) p->near = 1e15f;   // u = s^2 stays in range
         }
         p->causal = score->causal != 0;
         p->window = score->window;

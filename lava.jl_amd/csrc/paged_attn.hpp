@@ -24,7 +24,7 @@ struct PaParams {
     FastDiv by_g;
     float mul;                    // scores to base 2; with a cap to 2 log2(e) s / cap
     float cap2;                   // cap log2(e), or 0
-    float near, a[5];             // with a cap: |q.k| up to which pa_cap_near holds, and its coefficients
+    float near, a[5];             // with a cap: |q.k| up to which pa_cap_near holds (-1: none), and its coefficients
     int causal, window;
     const float* slopes;
     const int* bidir;
@@ -63,11 +63,10 @@ __device__ __forceinline__ PaRange pa_range(const PaParams& p, int pos, int end,
     return {p.window > 0 ? max(0, pos - p.window + 1) : 0, hi};
 }
 
-// The score in base 2 from the product q.k.
-__device__ __forceinline__ float pa_score(float s, float mul, float cap2) {
-    const float x = s * mul;
-    if (cap2 == 0.f) return x;
-    // cap tanh(z) = cap (1 - 2 / (1 + e^2z)), with x = 2 z log2 e: +-cap where e^2z leaves the range
+// The capped score in base 2: cap tanh(z) = cap (1 - 2 / (1 + e^2z)), with x = 2 z log2 e: +-cap where e^2z leaves the range.
+// Off by up to 2^-21 of the cap, not of the score: 2^-14 at PA_CAP_SMALL, of a size with a score's 32-bit sum; a larger cap's
+// small scores take pa_cap_near.
+__device__ __forceinline__ float pa_cap(float x, float cap2) {
     return fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)), cap2);
 }
 
@@ -77,6 +76,12 @@ __device__ __forceinline__ float pa_score(float s, float mul, float cap2) {
 __device__ __forceinline__ float pa_cap_near(float s, const float (&a)[5]) {
     const float u = s * s;
     return s * fmaf(fmaf(fmaf(fmaf(a[4], u, a[3]), u, a[2]), u, a[1]), u, a[0]);
+}
+// Caps in base 2 up to which the exact form alone serves scores of any size.
+constexpr float PA_CAP_SMALL = 128.f;
+// Scores of any size, each by the form that is right to its own last places.
+__device__ __forceinline__ float pa_cap_each(float s, float exact, float near, const float (&a)[5]) {
+    return fabsf(s) <= near ? pa_cap_near(s, a) : exact;
 }
 
 constexpr float PA_LN2 = 0.69314718055994530942f;

@@ -272,7 +272,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int key = first + 16 * kt + 4 * g + r;
-                        float x = near ? pa_cap_near(st[kt][nr][r], p.a) : pa_score(st[kt][nr][r], p.mul, p.cap2);
+                        const float s = st[kt][nr][r];
+                        float x = s * p.mul;
+                        if (p.cap2 != 0.f) x = near ? pa_cap_near(s, p.a) : pa_cap_each(s, pa_cap(x, p.cap2), p.near, p.a);
                         if (p.slopes) x = fmaf(-slope[nr], fabsf((float)(pos[nr] - key)), x);
                         if (cut) {
                             const bool keep = key >= lo[nr] && key <= last && !((none >> (2 * kt + (g >> 1))) & 1);

@@ -291,8 +291,10 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                         for (int qh = 0; qh < QH; ++qh)
 #pragma unroll
                             for (int r = 0; r < 16; ++r) far = fmaxf(far, fabsf(st[kt][qh][r]));
-                    if (__builtin_amdgcn_ballot_w64(far > p.near) != 0)
-                        each([&](float x, int qh, int) { return pa_score(x, p.mul, p.cap2) - ref[qh]; });
+                    if (__builtin_amdgcn_ballot_w64(far > p.near) != 0 && p.cap2 > PA_CAP_SMALL)
+                        each([&](float x, int qh, int) { return pa_cap_each(x, pa_cap(x * p.mul, p.cap2), p.near, p.a) - ref[qh]; });
+                    else if (__builtin_amdgcn_ballot_w64(far > p.near) != 0)
+                        each([&](float x, int qh, int) { return pa_cap(x * p.mul, p.cap2) - ref[qh]; });
                     else
                         each([&](float x, int qh, int) {
                             const float u = x * x;
