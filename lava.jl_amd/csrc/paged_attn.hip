@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(64) paged_any_kernel(PaParams p) {
     if (b >= p.b.B) return;
     const PagedSeq s = paged_seq(p.b, b);
     if (t < s.first || t >= s.first + s.n) return;
-    const int end = p.P + s.kv, pos = end - s.n + (t - s.first), bid = p.bidir ? p.bidir[b] : 0;
+    const int end = p.P + s.kv, pos = end - s.n + (t - s.first), bid = pa_leading(p, b);
     const PaRange r = pa_range(p, pos, end, bid);
     const float slope = p.slopes ? p.slopes[h] * PA_LOG2E : 0.f;
     const T* qr = (const T*)p.Q + (int64_t)t * p.qst + (int64_t)h * p.qsh;

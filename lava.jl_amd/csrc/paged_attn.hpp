@@ -57,6 +57,8 @@ struct PaOpen {
 struct PaRange {
     int lo, hi;   // positions of the keys a query sees
 };
+// Leading keys that every query of sequence b sees (not less than 0: the last one's position follows from it).
+__device__ __forceinline__ int pa_leading(const PaParams& p, int b) { return p.bidir && b >= 0 ? max(p.bidir[b], 0) : 0; }
 // A query at position pos of a sequence whose last key is at end - 1.
 __device__ __forceinline__ PaRange pa_range(const PaParams& p, int pos, int end, int bid) {
     const int hi = p.causal ? min(max(pos, bid - 1), end - 1) : end - 1;

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
         int pos[NR];
         float slope[NR];
         bool live[NR];
-        const int bid = p.bidir && b >= 0 ? p.bidir[b] : 0;
+        const int bid = pa_leading(p, b);
         const int end = PRE ? p.P + kv : kv, pos0 = end - sg.seq.n;   // of a prefix tile: P
         int lo_max = pa_range(p, pos0 + (int)div_of((uint32_t)min(tile * R + R - 1, rows - 1), p.by_g), end, bid).lo;
         int hi_min = pa_range(p, pos0 + (int)div_of((uint32_t)(tile * R), p.by_g), end, bid).hi;

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
     }
     const int P = PRE ? p.P : 0;
     const int end = P + (b < 0 ? 0 : seq.kv);
-    const int bid = b >= 0 && p.bidir ? p.bidir[b] : 0;
+    const int bid = pa_leading(p, b);
     auto block_of = [&](int pos) { return PRE && pos < P ? pos / PT_BK - p0 : np + (pos - P) / PT_BK - o0; };
     auto first_pos = [&](int blk) { return PRE && blk < np ? (p0 + blk) * PT_BK : P + (o0 + blk - np) * PT_BK; };
     // of rows [r0, r1], in order of their positions, the blocks that some row sees

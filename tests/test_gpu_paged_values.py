@@ -91,3 +91,15 @@ def test_capped_scores_of_all_sizes_in_one_block(gpu, kernel, prefix, cap):
     want, bound = capped(case)
     off = bad(got, want, bound)
     assert not off.any(), (np.argwhere(off)[:4], got[off][:4], want[off][:4], bound[off][:4])
+
+
+# ---- leading keys -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kernel", [0] + list(KERNELS))
+def test_negative_numbers_of_leading_keys(gpu, kernel):
+    """No key lies below them, down to the least integer: the call is a causal one."""
+    announce(f"negative leading keys kernel={kernel}")
+    case = Case(lens=((70, 100), (40, 200), (3, 20), (1, 50)), bidir=[-2 ** 31, -1, -2 ** 31 + 1, -2 ** 31], Hq=4, Hkv=2, D=64, seed=34)
+    got, lse, _ = run(gpu, Device(gpu, case), kernel)
+    want, wlse, bound, lbound = case.reference()
+    assert not bad(got, want, bound).any() and not bad(lse, wlse, lbound).any()
