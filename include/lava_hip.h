@@ -578,8 +578,8 @@ typedef struct lava_hip_kv_cache {
  * tokens at all. */
 typedef struct lava_hip_kv_batch {
     int32_t sequences; /* B */
-    int32_t max_pages; /* entries of a sequence's row of the table */
-    int64_t tokens;    /* T, rows of the (E, H, T) tensors, below 2^31 */
+    int32_t max_pages; /* entries of a sequence's row of the table; max_pages * page_size at most 2^30 */
+    int64_t tokens;    /* T, rows of the (E, H, T) tensors: below 2^31, at most 2^30 for attention */
     int64_t max_q;     /* the most new tokens a sequence has, or 0 if unknown: chooses kernels, never results' validity */
     const int32_t* q_start; /* B + 1 */
     const int32_t* kv_len;  /* B */
@@ -640,7 +640,7 @@ int lava_hip_paged_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch*
 
 /* The same for sequences that all begin with the same prefix_len tokens, held once in the cache, in pages
  * prefix_pages[0 .. ceil(prefix_len / page_size)) (device memory): the batch's kv_len and table are those of each sequence's own tokens,
- * whose positions start at prefix_len.  The prefix is read once for many sequences' queries.
+ * whose positions start at prefix_len, at most 2^30 - 512.  The prefix is read once for many sequences' queries.
  * `bidirectional` is not taken here. */
 int lava_hip_shared_prefix_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
                                 const lava_hip_attn_score* score, const int32_t* prefix_pages, int64_t prefix_len,

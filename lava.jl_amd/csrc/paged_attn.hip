@@ -159,6 +159,9 @@ static int pa_prepare(const char* fn, const lava_hip_kv_cache* cache, const lava
     *done = true;
     int rc = paged_check(fn, cache, batch, &p->c, &p->b);
     if (rc != LAVA_HIP_OK) return rc;
+    // a position is at least its sequence's length less 2^30 then, and itself, less a window (shorter than the table and the
+    // prefix) or a key's position fits 32 bits
+    LAVA_REQUIRE(p->b.T <= 0x40000000, LAVA_HIP_ERR_UNSUPPORTED, "%s: tokens = %d are more than 2^30", fn, p->b.T);
     LAVA_ARG(q_heads >= 0 && q_heads <= 65535, "%s: q_heads = %lld is outside [0, 65535]", fn, (long long)q_heads);
     LAVA_ARG(q_heads % p->c.heads == 0, "%s: %lld query heads are not a multiple of the cache's %d", fn,
              (long long)q_heads, p->c.heads);
