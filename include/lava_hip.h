@@ -618,7 +618,8 @@ int lava_hip_kv_append(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* 
  *   masked (no part of the softmax) unless j <= i (causal) or j < bidirectional[b], and, with window > 0,
  *   only if j > i - window.
  * A query that sees no key gives zeros and a log-sum-exp of -inf.  What masked places of the cache hold, infinities and NaN
- * too, has no part in a result. */
+ * too, has no part in a result.  A value that is not finite at a key that a query sees makes that element of its
+ * result infinite or NaN, however small the key's weight. */
 typedef struct lava_hip_attn_score {
     float scale;
     float cap;                    /* 0: none */

@@ -321,10 +321,21 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
                     pg_split<T>(vread(dt), up, down);
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr) {
-                        pg_add_not_finite(o[dt][nr], TT::mma16(up, pf[nr], f32x4{0.f, 0.f, 0.f, 0.f}), 1.f);
-                        pg_add_not_finite(o[dt][nr], TT::mma16(down, pf[nr], f32x4{0.f, 0.f, 0.f, 0.f}), -1.f);
+                        // 1 for the keys that the row sees, made anew for every dt: kept, they make others spill (D = 256: a quarter of the time)
+                        int from = lo[nr], to = min(hi[nr], end_pos), at = first;
+                        asm volatile("" : "+v"(from), "+v"(to), "+s"(at));
+                        from -= at + 4 * g;
+                        to -= at + 4 * g;
+                        v8 seen;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int key = 16 * (e >> 2) + (e & 3);
+                            seen[e] = key >= from && key <= to ? (T)1.f : (T)0.f;
+                        }
+                        pg_add_not_finite(o[dt][nr], TT::mma16(up, seen, f32x4{0.f, 0.f, 0.f, 0.f}), 1.f);
+                        pg_add_not_finite(o[dt][nr], TT::mma16(down, seen, f32x4{0.f, 0.f, 0.f, 0.f}), -1.f);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
                 pg_drop_not_finite<T, TILE>(lds_v, lane);
             }

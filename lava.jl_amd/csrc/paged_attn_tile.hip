@@ -358,7 +358,9 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 }
             }
             if (lane == 0) fbuf[buf][pr] = rescale ? 1 : 0;
-            auto pstore = [&](auto plain) __attribute__((always_inline)) {
+            // kind 0: scores against an unmoved maximum; 1: a moved one; 2: either, masked keys as -0
+            auto pstore = [&](auto kind) __attribute__((always_inline)) {
+                constexpr int KIND = decltype(kind)::value;
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -370,16 +372,19 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 float x = st[kt][qh][8 * ks + k];
-                                if constexpr (!decltype(plain)::value) x += msub;
-                                u[k] = (T)__builtin_amdgcn_exp2f(x);
+                                if constexpr (KIND > 0) x += msub;
+                                const T q = (T)__builtin_amdgcn_exp2f(x);
+                                u[k] = KIND == 2 && x == -INFINITY ? __builtin_bit_cast(T, (uint16_t)0x8000) : q;
                             }
                             *(lds_v8*)(uintptr_t)paddr(buf, kt, ks, qh) = u;
                         }
             };
-            if (!rescale)
-                pstore(pg_tag<true>{});
+            if (__builtin_expect(careful, 0))
+                pstore(pg_int<2>{});
+            else if (!rescale)
+                pstore(pg_int<0>{});
             else
-                pstore(pg_tag<false>{});
+                pstore(pg_int<1>{});
         };
 
         __syncthreads();   // K_0 .. K_2, V_0 in LDS
@@ -495,10 +500,11 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
                 if constexpr (decltype(slow)::value) {
 #pragma unroll 1
                     for (int kk = 0; kk < 4; ++kk) {
-                        v8 x[QH];
+                        v8 x[QH], seen[QH];
 #pragma unroll
                         for (int qh = 0; qh < QH; ++qh) {
                             x[qh] = pread(kk, qh);
+                            seen[qh] = pg_seen<T>(x[qh]);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) l[qh] = TT::dot2(v2{x[qh][2 * e], x[qh][2 * e + 1]}, l[qh]);
                         }
@@ -509,8 +515,8 @@ __global__ void __launch_bounds__(128 * PT_PAIRS, 1) paged_tile_kernel(PaParams,
 #pragma unroll
                             for (int qh = 0; qh < QH; ++qh) {
                                 o[dt][qh] = TT::mma32(a, x[qh], o[dt][qh]);
-                                pg_add_not_finite(o[dt][qh], TT::mma32(up, x[qh], f32x16{}), 1.f);
-                                pg_add_not_finite(o[dt][qh], TT::mma32(down, x[qh], f32x16{}), -1.f);
+                                pg_add_not_finite(o[dt][qh], TT::mma32(up, seen[qh], f32x16{}), 1.f);
+                                pg_add_not_finite(o[dt][qh], TT::mma32(down, seen[qh], f32x16{}), -1.f);
                                 __builtin_amdgcn_sched_barrier(0);
                             }
                         }

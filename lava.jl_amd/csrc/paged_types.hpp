@@ -47,7 +47,8 @@ struct PgType<bf16> {
 
 // Values that are not finite, at keys that only some rows of a tile see: P V is a matrix product and 0 times infinity is
 // NaN, in rows that do not see the key.  Where a tile of values has any, they enter as zeros, and what they are worth to
-// each row comes from products of P with where they are.
+// each row comes from products of where they are with which keys the row sees -- not with P, whose weight for a key may be below all
+// numbers of the type (f16: a score 17 below the row's largest), where a value that the row sees would vanish.
 
 typedef uint16_t pg_u16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t pg_u16x8 __attribute__((ext_vector_type(8)));
@@ -99,14 +100,23 @@ __device__ __forceinline__ V pg_split(V a, V& up, V& down) {
     return __builtin_bit_cast(V, x);
 }
 
-// What infinities of the sign add to the sums o by `weight`, P's product with where they are: 2^254 times it, which is infinite
-// for every P but 0.
+// 1 for the keys that a row sees, from P with -0 for masked ones.
+template <typename T, typename V>
+__device__ __forceinline__ V pg_seen(V p) {
+    constexpr uint16_t one = __is_same(T, bf16) ? 0x3f80 : 0x3c00;
+    pg_u16x8 x = __builtin_bit_cast(pg_u16x8, p);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = x[e] == 0x8000 ? (uint16_t)0 : one;
+    return __builtin_bit_cast(V, x);
+}
+
+// What infinities of the sign add to the sums o where `count` of them lie at keys that the row sees: infinite for every count but 0.
 template <typename F>
-__device__ __forceinline__ void pg_add_not_finite(F& o, const F& weight, float sign) {
+__device__ __forceinline__ void pg_add_not_finite(F& o, const F& count, float sign) {
 #pragma unroll
     for (int r = 0; r < (int)(sizeof(F) / 4); ++r) {
 #pragma clang fp contract(off)   // a fused product would stay finite, and infinity minus it infinite
-        const float x = weight[r] * 0x1p127f * (sign * 0x1p127f);
+        const float x = count[r] * 0x1p127f * (sign * 0x1p127f);
         o[r] = o[r] + x;
     }
 }

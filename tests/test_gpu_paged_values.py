@@ -93,6 +93,57 @@ def test_capped_scores_of_all_sizes_in_one_block(gpu, kernel, prefix, cap):
     assert not off.any(), (np.argwhere(off)[:4], got[off][:4], want[off][:4], bound[off][:4])
 
 
+# ---- values that are not finite -----------------------------------------------------------------------------------
+
+FAINT = {
+    "decode": dict(lens=((3, 40), (5, 150)), Hq=4, Hkv=2, D=64),
+    "prompt": dict(lens=((90, 200), (64, 70)), Hq=4, Hkv=2, D=128),
+    "window": dict(lens=((90, 200), (5, 150)), Hq=4, Hkv=1, D=128, window=60),
+    "bf16": dict(lens=((90, 200), (5, 150)), Hq=4, Hkv=2, D=64, dtype="bf16"),
+    "d256": dict(lens=((40, 200), (5, 150)), Hq=2, Hkv=1, D=256),
+    "shared": dict(lens=((3, 9), (4, 8), (90, 100)), prefix=150, window=120, Hq=4, Hkv=2, D=64),
+}
+
+
+@pytest.mark.parametrize("name", list(FAINT))
+@pytest.mark.parametrize("kernel", [0] + list(KERNELS))
+def test_values_that_are_not_finite_at_keys_of_little_weight(gpu, kernel, name):
+    """A key whose weight is below the operands' smallest numbers, in a block that only some rows see whole: every row that sees
+    it is not finite in the columns where its values are not, the others do not notice it."""
+    announce(f"not finite values of little weight kernel={kernel} {name}")
+    case = Case(seed=33, **FAINT[name])
+    case.q = to_bits(np.abs(to_f64(case.q, case.dtype)) + 0.5, case.dtype)
+    at = []
+    for b, (n, kv) in enumerate(case.lens):
+        j = kv - 1 - n // 2   # the later half of the new tokens sees it
+        at.append(j)
+        # a score 30 below the others in f16 (weight 2^-43), 110 in bf16 (2^-159)
+        low = -{"f16": 30.0, "bf16": 110.0}[case.dtype] / (1.3 * case.D * case.scale)
+        x = to_f64(case.keys[b], case.dtype) * 0.1
+        x[j] = low
+        case.keys[b] = to_bits(x, case.dtype)
+        case.put(case.k, b, case.keys[b])
+        case.values[b][j, :, 1:4] = 0
+        bits = case.values[b].copy()
+        bits[j, :, 1:4] = to_bits(np.array([np.inf, -np.inf, np.nan]), case.dtype)
+        case.put(case.v, b, bits)
+    got, _, _ = run(gpu, Device(gpu, case), kernel)
+    want, _, bound, _ = case.reference()
+    seen = np.zeros((case.T, 1), bool)
+    for b, (n, kv) in enumerate(case.lens):
+        pos = kv - n + np.arange(n)
+        see = (at[b] <= pos) & ((at[b] > pos - case.window) if case.window else True)
+        assert see.any() and not see.all()
+        seen[case.q_start[b]:case.q_start[b] + n, 0] = see
+    for d in (1, 2, 3):
+        ok = np.where(seen, ~np.isfinite(got[:, :, d]), True)
+        assert ok.all(), (d, np.argwhere(~ok)[:5])
+    rest = np.ones(got.shape, bool)
+    rest[:, :, 1:4] = ~seen[:, :, None]
+    off = bad(got, want, bound) & rest
+    assert not off.any(), (np.argwhere(off)[:5], got[off][:5], want[off][:5])
+
+
 # ---- leading keys -------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kernel", [0] + list(KERNELS))
