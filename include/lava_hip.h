@@ -634,7 +634,8 @@ typedef struct lava_hip_attn_score {
  * h / (q_heads / heads)).  lse (may be NULL) receives the natural logarithm of each row's sum of exp(score),
  * lse[token * q_heads + head].  MFMA kernels take head dimensions that are a multiple of 8, pages of a multiple of 8 tokens, 16-byte
  * aligned Q and cache with strides that are multiples of 8 and O aligned to 8 bytes with strides multiples of 4; a generic kernel
- * the rest.  P is rounded once to the operands' type before the second product; sums are in 32 bits, in a fixed order. */
+ * the rest, and calls of head dimensions above 128 whose row tiles (rows of a key head / 32, or / 16 for at most 16 a sequence,
+ * and one a sequence) times max_pages * page_size / 128 are 2^31 or more.  P is rounded once to the operands' type before the second product; sums are in 32 bits, in a fixed order. */
 int lava_hip_paged_attn(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, const lava_hip_attn_score* score,
                         const void* Q, void* O, int64_t q_heads, const int64_t* q_strides, const int64_t* o_strides,
                         float* lse, void* stream);

@@ -209,9 +209,9 @@ static int64_t pa_max_rows(const PaParams& p, const lava_hip_kv_batch* batch) {
     return q * p.G;
 }
 
-// Whether the cache allows 16-byte reads of 8 keys in one page.
+// Whether the cache allows 16-byte reads of 8 keys in one page (and rows, rounded up to tiles, fit 31 bits).
 static bool pa_vectors(const PaParams& p) {
-    return p.c.D % 8 == 0 && p.c.page % 8 == 0 && p.c.sl % 8 == 0 && p.c.sh % 8 == 0 && p.c.sp % 8 == 0 &&
+    return (int64_t)p.b.T * p.G <= 0x7fffff00 && p.c.D % 8 == 0 && p.c.page % 8 == 0 && p.c.sl % 8 == 0 && p.c.sh % 8 == 0 && p.c.sp % 8 == 0 &&
            aligned(p.c.k, 16) && aligned(p.c.v, 16);
 }
 
@@ -243,6 +243,32 @@ static PaRows pa_rows(const PaParams& p, const PaShape& sh) {
             p.stack ? 2 * (size_t)p.b.T * p.Hq : 0};
 }
 
+// Key heads a pass: the kernels count a launch's blocks of work (row tiles times the keys' blocks, of as many keys as the table
+// has room for) and its workgroups in 31 bits.  Whole tiles need no count of blocks: where even one head has too many, the tile
+// kernel does not split.  0: the row kernel's launch, or the prefix's, does not fit with one head.
+static int pa_heads_a_pass(PaParams* p, const PaShape& sh) {
+    const int64_t most = 0x7fffffff - 1024;   // and what rounding up over the workgroups adds
+    const int64_t rows = (int64_t)p->b.T * p->G, seqs = std::min(p->b.B, p->b.T);   // (those with rows)
+    auto blocks = [](int64_t keys, int64_t size) { return (keys + size - 1) / size; };
+    int64_t work = 1;   // a head's, of the launch that has most
+    if (sh.nr) {
+        const int64_t R = 16 * sh.nr;
+        int64_t tiles = rows / R + seqs;
+        if (p->row_limit < 0x7fffffff) tiles = std::min(tiles, seqs * blocks(p->row_limit, R));
+        int64_t of_keys = tiles * std::max<int64_t>(1, blocks(p->b.kv_max, PR_BK));
+        if (p->stack == 1) of_keys += blocks(rows, R) * blocks(p->P, PR_BK);
+        work = std::max(work, of_keys);
+    }
+    if (sh.pre_qh) work = std::max(work, blocks(rows, 128 * sh.pre_qh) * blocks(p->P, PT_BK));
+    if (sh.qh) {
+        const int64_t tiles = rows / (128 * sh.qh) + seqs;
+        const int64_t of_keys = tiles * std::max<int64_t>(1, blocks(p->b.kv_max, PT_BK) + blocks(p->P, PT_BK));
+        if (of_keys > most) p->whole = 1;
+        work = std::max(work, p->whole ? tiles : of_keys);
+    }
+    return (int)std::min<int64_t>(p->c.heads, most / work);
+}
+
 // What depends on the call's sizes alone: which kernels take which sequences.
 static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
     const int pin = kernel_override(LAVA_HIP_FAMILY_PAGED);
@@ -270,6 +296,14 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
         sh.nr = most <= 16 ? 1 : 2;
         // as many workgroups as fit (LDS: 512 bytes a column of the head)
         sh.row_grid = (unsigned)(PA_CUS * (sh.dp == 64 ? 3 : sh.dp == 128 ? 2 : 1));
+    }
+    sh.heads = pa_heads_a_pass(p, sh);
+    if (sh.heads == 0 && paged_tile_takes(*p) && pin == 0) {   // more rows and wider tables than the row kernel counts: all on tiles
+        sh.qh = 2;
+        sh.nr = sh.pre_qh = 0;
+        sh.row_grid = 0;
+        p->row_limit = p->stack = 0;
+        sh.heads = pa_heads_a_pass(p, sh);
     }
     p->by_rows = fast_div(std::max(1u, sh.row_grid));
     p->by_tiles = fast_div(PT_GRID);
@@ -303,19 +337,23 @@ static void pa_workspace(PaParams* p, const PaShape& sh, void* count, void* rest
     p->row_ml = (float2*)take(n.whole * sizeof(float2));
 }
 
-static int pa_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {
+static int pa_launch(const PaParams& call, const PaShape& sh, int dtype, hipStream_t s) {
     int rc = LAVA_HIP_OK;
-    if (sh.qh) rc = paged_tile_launch(p, sh.qh, false, dtype, s);
-    if (rc == LAVA_HIP_OK && sh.pre_qh) rc = paged_tile_launch(p, sh.pre_qh, true, dtype, s);
-    if (rc == LAVA_HIP_OK && sh.nr) rc = paged_rows_launch(p, sh, dtype, s);
+    for (int h0 = 0; h0 < call.c.heads && rc == LAVA_HIP_OK; h0 += sh.heads) {   // (f16 and bf16: 2 bytes an element)
+        PaParams p = call;
+        const int64_t q0 = (int64_t)h0 * p.G;
+        p.c.heads = std::min(sh.heads, call.c.heads - h0);
+        p.c.k = (uint16_t*)p.c.k + h0 * p.c.sh;
+        p.c.v = (uint16_t*)p.c.v + h0 * p.c.sh;
+        p.Q = (const uint16_t*)p.Q + q0 * p.qsh;
+        p.O = (uint16_t*)p.O + q0 * p.osh;
+        if (p.lse) p.lse += q0;
+        if (p.slopes) p.slopes += q0;
+        if (sh.qh) rc = paged_tile_launch(p, sh.qh, false, dtype, s);
+        if (rc == LAVA_HIP_OK && sh.pre_qh) rc = paged_tile_launch(p, sh.pre_qh, true, dtype, s);
+        if (rc == LAVA_HIP_OK && sh.nr) rc = paged_rows_launch(p, sh, dtype, s);
+    }
     return rc;
-}
-
-// Whether the call's blocks of work can be counted in 31 bits.
-static bool pa_countable(const PaParams& p) {
-    const double tiles = (double)p.b.T * p.G / 16 + 2.0 * p.b.B + 1;
-    const double blocks = ((double)p.b.kv_max + p.P) / PT_BK + 4;
-    return tiles * blocks * p.c.heads < 2147483647.0 && (int64_t)p.b.T * p.G <= 0x7fffff00;
 }
 
 static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch,
@@ -353,10 +391,10 @@ static int pa_attn(const char* fn, const lava_hip_kv_cache* cache, const lava_hi
     p.P = (int)prefix;
     if (p.window >= (int64_t)p.P + p.b.kv_max) p.window = 0;   // hides nothing (and positions less it stay in 32 bits)
     hipStream_t s = as_stream(stream);
-    bool fast = kernel_override(LAVA_HIP_FAMILY_PAGED) != 1 && pa_countable(p) && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
+    bool fast = kernel_override(LAVA_HIP_FAMILY_PAGED) != 1 && pa_vectors(p) && aligned(Q, 16) && aligned(O, 8);
     for (int i = 1; i < 3; ++i) fast = fast && q_strides[i] % 8 == 0 && o_strides[i] % 4 == 0;
-    if (fast) {
-        const PaShape sh = pa_plan_call(&p, pa_max_rows(p, batch));
+    const PaShape sh = fast ? pa_plan_call(&p, pa_max_rows(p, batch)) : PaShape{};
+    if (sh.heads > 0) {
         if (batch->workspace) {
             LAVA_ARG(batch->workspace_bytes >= sh.bytes, "%s: the workspace of %zu bytes is smaller than the %zu this call needs",
                      fn, batch->workspace_bytes, sh.bytes);
@@ -408,12 +446,13 @@ extern "C" int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, co
     *bytes = 0;
     if (done) return LAVA_HIP_OK;
     p.P = (int)std::min<int64_t>(prefix_len, 0x3ffffe00);
-    if (!pa_vectors(p) || !pa_countable(p)) return LAVA_HIP_OK;
+    if (!pa_vectors(p)) return LAVA_HIP_OK;
     // whatever Q's and O's strides are: with those that the tile kernel takes, and without
     for (const int64_t stride : {(int64_t)0, (int64_t)1 << 40}) {
         PaParams q = p;
         q.qst = stride;
-        *bytes = std::max(*bytes, pa_plan_call(&q, pa_max_rows(q, batch)).bytes);
+        const PaShape sh = pa_plan_call(&q, pa_max_rows(q, batch));
+        if (sh.heads > 0) *bytes = std::max(*bytes, sh.bytes);
     }
     return LAVA_HIP_OK;
 }

@@ -19,7 +19,7 @@ struct PaParams {
     void* O;
     float* lse;
     int64_t qsh, qst, osh, ost;   // head and token strides
-    int Hq, G;                    // query heads, those of a key head
+    int Hq, G;                    // query heads of the call (a token's rows of lse, row_o), those of a key head
     int o16;                      // O and its strides allow 16-byte stores
     FastDiv by_g;
     float mul;                    // scores to base 2; with a cap to 2 log2(e) s / cap
@@ -96,6 +96,7 @@ struct PaShape {
     unsigned row_grid;
     int qh;               // tile kernel: 128 qh rows a tile; 0: no launch for sequences
     int pre_qh;           // the stacked prefix's launch of the tile kernel; 0: none
+    int heads;            // key heads a pass over these launches; 0: not even one, the generic kernel
     size_t count_bytes, bytes;   // workspace: arrivals, all of it
 };
 int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s);

@@ -454,11 +454,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pr
     args.load(lane);
     const PaParams p = args.get();
     constexpr int RPW = 256 / DP;
-    const uint32_t per_token = (uint32_t)(p.Hq + RPW - 1) / RPW;   // wavefronts a token
+    const int heads = p.c.heads * p.G;   // of the pass
+    const uint32_t per_token = (uint32_t)(heads + RPW - 1) / RPW;   // wavefronts a token
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(pg_block() * 4 + (threadIdx.x >> 6)));
     const int t = (int)(wave / per_token), h0 = (int)(wave - (uint32_t)t * per_token) * RPW;
     if (t >= p.b.T) return;
-    const int h = min(h0 + lane / (DP / 4), p.Hq - 1);
+    const int h = min(h0 + lane / (DP / 4), heads - 1);
     const int b = paged_find(p.b, t, lane);
     if (b >= p.b.B) return;
     const PagedSeq s = paged_seq(p.b, b);
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(PaParams, int R, int pr
         ml = (first ? pre_ml : own_ml) + at;
         q = (first ? pre_o : own_o) + at * DP;
     }, lane, o, m, l);
-    if (h0 + lane / (DP / 4) < p.Hq) pa_store_row<T, DP>(p, t, h, o, m, l, lane);
+    if (h0 + lane / (DP / 4) < heads) pa_store_row<T, DP>(p, t, h, o, m, l, lane);
 }
 
 int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream_t s) {
@@ -546,7 +547,7 @@ int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream
             return check_launch("paged_join_tiles_kernel");
         }
         const int per_wave = 256 / sh.dp;
-        const dim3 rows = pg_grid(((int64_t)p.b.T * ((p.Hq + per_wave - 1) / per_wave) + 3) / 4);
+        const dim3 rows = pg_grid(((int64_t)p.b.T * ((p.c.heads * p.G + per_wave - 1) / per_wave) + 3) / 4);
         auto join = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, rows, dim3(256), 0, s, p, 16 * sh.nr, 128 * sh.pre_qh);
         };

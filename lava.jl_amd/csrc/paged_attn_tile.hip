@@ -682,8 +682,7 @@ bool paged_tile_takes(const PaParams& p) {
 
 int paged_tile_launch(const PaParams& p, int qh, bool prefix, int dtype, hipStream_t s) {
     const bool plain = p.cap2 == 0.f && !p.slopes && p.mul > 0.f;
-    const int64_t tiles = ((int64_t)p.b.T * p.G / (128 * qh) + p.b.B) * p.c.heads;   // no fewer than there are
-    LAVA_REQUIRE(tiles <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "paged attention: problem too large");
+    const int64_t tiles = ((int64_t)p.b.T * p.G / (128 * qh) + std::min(p.b.B, p.b.T)) * p.c.heads;   // no fewer than there are
     const dim3 grid = pg_grid(prefix ? PT_GRID : std::max<int64_t>(tiles, PT_GRID));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(128 * PT_PAIRS), 0, s, p, prefix ? 1 : 0); };
     auto by_d = [&](auto type, auto q, auto any) {

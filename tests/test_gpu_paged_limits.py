@@ -23,6 +23,56 @@ def pinned_run(lh, dev, kernel):
     return dev.result(), log
 
 
+def widen(lh, dev, page, width):
+    """The same batch with pages of `page` tokens, of which only those in use have memory, and `width` of them a sequence, all
+    but the first none."""
+    c = dev.case
+    assert max(kv for _, kv in c.lens) <= c.page and c.prefix <= c.page
+    table = np.full((c.B, width), -1, np.int32)
+    table[:, 0] = c.table[:, 0]
+    dev.cache = lh.paged_cache_raw(c.dtype, dev.k.ptr, dev.v.ptr, c.D, page, c.Hkv, c.pages, c.cache_strides)
+    dev.table = lh.HIPDeviceArray.from_numpy(table.ravel(), "i32")
+    dev.batch = lh.paged_batch_raw(c.B, c.T, dev.q_start.ptr, dev.kv_len.ptr, dev.table.ptr, width,
+                                   max_q=max(n for n, _ in c.lens))
+
+
+WIDE = {   # (case, kernel pin, kernels that have to run)
+    "rows": (dict(lens=tuple((1, 1 + i % 37) for i in range(70)), Hq=32, Hkv=32, D=64), 0, ["paged_rows_kernel"]),
+    "rows_slopes": (dict(lens=tuple((1 + i % 3, 4 + i % 137) for i in range(70)), Hq=64, Hkv=32, D=64, slopes=True), 2,
+                    ["paged_rows_kernel"]),
+    "tiles": (dict(lens=tuple((40, 40 + i % 137) for i in range(70)), Hq=64, Hkv=32, D=64, dtype="bf16"), 0,
+              ["paged_tile_kernel"]),
+    "tiles_128": (dict(lens=tuple((40, 40 + i % 137) for i in range(70)), Hq=32, Hkv=32, D=64, cap=20.0), 4,
+                  ["paged_tile_kernel", "paged_tile_kernel<32>"]),
+    "shared": (dict(lens=tuple((1, 1 + i % 37) for i in range(70)), prefix=300, Hq=64, Hkv=32, D=64, slopes=True), 0,
+               ["paged_tile_kernel", "paged_rows_kernel", "paged_join_kernel"]),
+    # more blocks of rows than can be counted with one head: all on whole tiles
+    "many_rows": (dict(lens=tuple((1, 1 + i % 37) for i in range(300)), Hq=6, Hkv=3, D=64), 0, ["paged_tile_kernel"]),
+    "many_rows_shared": (dict(lens=tuple((1, 1 + i % 37) for i in range(300)), Hq=6, Hkv=3, D=128, prefix=300, window=200), 0,
+                         ["paged_tile_kernel"]),
+    "shared_rows": (dict(lens=tuple((1, 1 + i % 37) for i in range(70)), prefix=300, Hq=64, Hkv=32, D=64), 2,
+                    ["paged_rows_kernel", "paged_join_kernel"]),
+}
+
+
+@pytest.mark.parametrize("name", list(WIDE))
+def test_tables_as_wide_as_a_sequence_may_be(gpu, name):
+    """2^30 tokens of table a sequence, some hundred in use: the MFMA kernels run, and give the bits of a narrow table."""
+    kw, kernel, names = WIDE[name]
+    announce(f"wide table {name}")
+    case = Case(seed=41, page=512, **kw)
+    dev = Device(gpu, case)
+    (got, lse, raw), log = pinned_run(gpu, dev, kernel)
+    want, wlse, bound, lbound = case.reference()
+    assert not bad(got, want, bound).any() and not bad(lse, wlse, lbound).any()
+    widen(gpu, dev, 1 << 15, 1 << 15)
+    (got, lse, _), log = pinned_run(gpu, dev, kernel)
+    assert "paged_any_kernel" not in log and all(k in log for k in names), log
+    off = bad(got, want, bound)
+    assert not off.any(), (np.argwhere(off)[:5], got[off][:5], want[off][:5])
+    assert not bad(lse, wlse, lbound).any()
+
+
 def test_append_more_tokens_than_a_launch_has_threads(gpu):
     """2^24 + 3 tokens, 256 threads each in the kernel: every query turned, the last keys stored."""
     lh = gpu
