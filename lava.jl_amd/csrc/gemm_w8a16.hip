@@ -26,6 +26,7 @@
 //  * the scale multiply is the fused per-element epilogue, applied to every partial.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <functional>
 #include <map>
 #include <mutex>
@@ -785,7 +786,16 @@ int with_stream_workspace(size_t bytes, void* stream, const std::function<int(vo
         // it and be broken by it)
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
         LAVA_HIP_TRY(hipThreadExchangeStreamCaptureMode(&mode));
-        const hipError_t e = hipMalloc(&buf, bytes);
+        // half as much again as before at least: calls that need a little more each time (a batch that grows by a token a
+        // step) allocate a logarithmic number of times, and the buffers retired are at most twice the one in use
+        const size_t room = std::max(bytes, ws.bytes + ws.bytes / 2);
+        hipError_t e = hipMalloc(&buf, room);
+        if (e == hipSuccess) {
+            bytes = room;
+        } else if (room > bytes) {
+            (void)hipGetLastError();
+            e = hipMalloc(&buf, bytes);
+        }
         (void)hipThreadExchangeStreamCaptureMode(&mode);
         LAVA_HIP_TRY(e);
         // the W8A16 arrival counters start at zero (every call leaves them at zero)

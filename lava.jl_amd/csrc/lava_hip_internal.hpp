@@ -23,7 +23,7 @@ int kernel_override(int family);
 
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-// The library's workspace for `stream` on the current device: grown to at least `bytes` (a
+// The library's workspace for `stream` on the current device: grown to at least `bytes`, and by half of what it was (a
 // grown buffer is retired, not freed), then launch(buffer) runs under the lock that orders its
 // users, so calls from several threads use it one after another in stream order.  The first
 // STREAM_WS_RESERVED bytes hold the W8A16 split-K arrival counters, which every call leaves at

@@ -157,3 +157,27 @@ def test_tile_launches_of_more_workgroups_than_one_dimension_has(gpu):
     (got, lse, _), log = pinned_run(gpu, dev, 4)
     assert log[0] == "paged_tile_kernel", log
     assert not bad(got, want, bound).any() and not bad(lse, wlse, lbound).any()
+
+
+def test_a_growing_batch_allocates_few_workspaces(gpu):
+    """A batch that grows by a token a step: the stream's workspace grows by factors, not with every step (each outgrown buffer
+    is kept for work that is still queued)."""
+    lh = gpu
+    announce("a growing batch behind a shared prefix")
+    n = 64
+    case = Case(lens=tuple((1, 1 + i % 5) for i in range(n)), prefix=40, Hq=32, Hkv=8, D=128, seed=44, tail=0)
+    dev = Device(lh, case)
+    want, _, bound, _ = case.reference()
+    s = lh.Stream()
+    grown = []
+    for b in range(1, n + 1):
+        dev.batch = lh.paged_batch_raw(b, b, dev.q_start.ptr, dev.kv_len.ptr, dev.table.ptr, case.max_pages, max_q=1)
+        lh.kernel_log_clear()
+        dev.launch(stream=s.handle)
+        grown.append(lh.kernel_log().count("fill_bytes_kernel"))   # a new workspace's counters cleared
+    s.synchronize()
+    need = [lh.paged_workspace_bytes(dev.cache, lh.paged_batch_raw(b, b, dev.q_start.ptr, dev.kv_len.ptr, dev.table.ptr,
+                                                                   case.max_pages, max_q=1), case.Hq, case.prefix) for b in (1, n)]
+    assert sum(grown) <= 2 + np.log(need[1] / need[0]) / np.log(1.5), (sum(grown), need)
+    assert not bad(dev.result()[0], want, bound).any()
+    s.close()
