@@ -24,7 +24,6 @@
 
 #include "lds_dma.hpp"
 #include "paged_plan.hpp"
-#include "paged_types.hpp"
 
 namespace lava {
 
@@ -59,6 +58,8 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
     constexpr int IPG = 8 / RPI;                   // of those, per 8 keys
     constexpr int TILE = 32 * RB;
     constexpr int NKS = DP / 32, NDT = DP / 16;
+    // parts are joined in this launch, by paged_join_tiles_kernel, or (behind a stacked prefix) by paged_join_kernel
+    constexpr bool LIVE = NR == 1 && !PRE, LATER = NR == 2 && !PRE;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[4][2][TILE];   // per wavefront: K, V
     __shared__ float2 stat[4][R];
     __shared__ int arrived;
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
     const uint32_t begin = min(plan.total, wg * per), stop = min(plan.total, begin + per);
     PaOpen open = {};
     if (begin >= stop) {
-        if (!(NR == 1 && !PRE)) pa_leave_open(p.ws_open + wg, open);
+        if (LATER) pa_leave_open(p.ws_open + wg, open);
         return;
     }
 
@@ -114,11 +115,6 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
         const int b = sg.b, nb = sg.sw.nb, np = PRE ? sg.sw.np : 0, p0 = sg.sw.p0, o0 = sg.sw.o0;
         const int head = sg.head, tile = sg.tile, blk0 = sg.blk0, kv = sg.seq.kv, rows = sg.seq.n * p.G;
         const int nblk = min(nb - blk0, (int)(stop - at));
-        // rows of a sequence that another launch takes, prefix and all
-        if (PRE && b < 0 && pa_other(p, sg.seq.first + tile * R / p.G, sg.seq.first + min(sg.seq.n - 1, (tile * R + R - 1) / p.G), lane)) {
-            at += (uint32_t)nblk;
-            continue;
-        }
 
         // ---- the rows of this lane; the last position that the first row sees and the first that the last one does
         // bound what needs comparing (rows are in order of their positions)
@@ -381,10 +377,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
             f[nr] = __builtin_amdgcn_exp2f(m[nr] - sub);
         }
         const PaParams e = args.get();
-        const bool whole = nblk == nb, direct = whole && !(PRE && e.stack);
+        const bool whole = nblk == nb, direct = whole && !PRE;
         const PaParts parts = pa_parts(at - (uint32_t)blk0, nb, per);
         constexpr int NH = NR < 2 ? 1 : 2;
-        constexpr bool LIVE = NR == 1 && !PRE;   // parts are read in this launch
         const uint32_t box = lds_addr(&ring[0][0][0]) + 16u * (uint32_t)lane;
 #pragma unroll
         for (int n0 = 0; n0 < NR; n0 += NH) {
@@ -434,15 +429,15 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) paged_rows_kernel(PaPa
                 }
             }
         }
-        if (!whole && !(PRE && e.stack)) {
+        if (!whole) {
             if constexpr (LIVE)
                 pa_arrive<T, DP, 4>(e, parts, R, min(R, rows - tile * R), tile * R, sg.seq.first, head, w, lane, &arrived);
-            else if (blk0 == 0)
+            else if (LATER && blk0 == 0)
                 open = {parts.n, min(R, rows - tile * R), tile * R, sg.seq.first, head};
         }
         at += (uint32_t)nblk;
     }
-    if (!(NR == 1 && !PRE)) pa_leave_open(args.get().ws_open + wg, open);
+    if (LATER) pa_leave_open(args.get().ws_open + wg, open);
 }
 
 // Behind a stacked prefix: a row's parts, the prefix's and its sequence's, each in the order of its keys.  256 / DP rows a
@@ -538,8 +533,8 @@ int paged_rows_launch(const PaParams& p, const PaShape& sh, int dtype, hipStream
         p.P > 0 ? by_shape(pg_tag<true>{}) : by_shape(pg_tag<false>{});
         int rc = check_launch("paged_rows_kernel");
         if (rc != LAVA_HIP_OK) return rc;
-        if (p.stack == 0) {
-            if (sh.nr == 1 && p.P == 0) return rc;   // joined by the last workgroup of a tile to arrive
+        if (p.P == 0) {   // (behind a prefix it is always stacked)
+            if (sh.nr == 1) return rc;   // joined by the last workgroup of a tile to arrive
             auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(sh.row_grid * 4), dim3(256), 0, s, p, 16 * sh.nr, 4); };
             sh.dp == 64    ? join(paged_join_tiles_kernel<T, 64>)
             : sh.dp == 128 ? join(paged_join_tiles_kernel<T, 128>)

@@ -20,7 +20,6 @@
 
 #include "lds_dma.hpp"
 #include "paged_plan.hpp"
-#include "paged_types.hpp"
 
 namespace lava {
 

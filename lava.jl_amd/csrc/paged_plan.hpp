@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "paged_attn.hpp"
+#include "paged_types.hpp"
 
 namespace lava {
 
@@ -62,7 +63,7 @@ struct PaSeq {
 };
 
 // BK: keys of a block.  ABOVE: the launch takes the sequences of more than row_limit rows (and reads the prefix for each of
-// them), else those of at most that many.  PRE: the call has a shared prefix.
+// them), else those of at most that many (whose prefix is stacked).  PRE: the call has a shared prefix.
 template <int BK, bool ABOVE, bool PRE>
 __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, const PagedSeq& s, int R) {
     PaSeq w = {};
@@ -71,7 +72,7 @@ __device__ __forceinline__ PaSeq pa_seq(const PaParams& p, const PagedSeq& s, in
     w.nb = (s.kv + BK - 1) / BK;
     if (p.window > 0 || PRE) {
         const int P = PRE ? p.P : 0, lo = p.window > 0 ? max(0, P + s.kv - s.n - p.window + 1) : 0;   // first position seen
-        if (PRE && (ABOVE || p.stack == 0) && lo < P) {
+        if (PRE && ABOVE && lo < P) {
             w.p0 = lo / BK;
             w.np = (P + BK - 1) / BK - w.p0;
         }
@@ -342,11 +343,6 @@ __device__ __forceinline__ float2 pa_get(const float* p) {
     return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-template <int N>
-struct PaInt {
-    static constexpr int value = N;
-};
-
 // Rows joined by a wavefront, 256 / DP of them at once: DP / 4 lanes a row, 4 columns a lane.  Part j of the lane's row has its
 // (maximum, weight) and sums at part(j, ml, o); n parts (at least one).  Sums are requested beside the weights, one round trip for
 // both: those of a part of no weight are not written, and what is read of them is dropped.  LIVE: the parts come from
@@ -399,9 +395,9 @@ __device__ __forceinline__ void pa_join_rows(int n, F part, int lane, f32x4& o, 
         }
     };
     if (most <= 4) {
-        some_of(0, PaInt<4>{});
+        some_of(0, pg_int<4>{});
     } else {
-        for (int j0 = 0; j0 < most; j0 += 16) some_of(j0, PaInt<16>{});
+        for (int j0 = 0; j0 < most; j0 += 16) some_of(j0, pg_int<16>{});
     }
 }
 
