@@ -17,11 +17,20 @@ from . import _lib
 from .device import DTYPES, HIPDeviceArray
 
 
+def _fits(bits: int, **values: int) -> None:
+    """Refuses what a descriptor's integers would cut off."""
+    for name, x in values.items():
+        if not -2 ** (bits - 1) <= x < 2 ** (bits - 1):
+            raise ValueError(f"{name} = {x} does not fit {bits} bits")
+
+
 def paged_cache_raw(dtype: str, k: int, v: int, head_dim: int, page_size: int, heads: int, pages: int,
                     strides: Sequence[int]) -> _lib.KVCacheDesc:
     """Pages of keys at `k` and of values at `v`, both with element strides of (E, L, H, P)."""
     if dtype not in DTYPES:
         raise ValueError(f"unknown element type {dtype!r}; one of {sorted(DTYPES)}")
+    _fits(32, head_dim=head_dim, page_size=page_size, heads=heads)
+    _fits(64, pages=pages, **{f"strides[{i}]": st for i, st in enumerate(strides)})
     return _lib.KVCacheDesc(k, v, DTYPES[dtype][0], head_dim, page_size, heads, pages, (C.c_int64 * 4)(*strides))
 
 
@@ -29,17 +38,21 @@ def paged_batch_raw(sequences: int, tokens: int, q_start: int, kv_len: int, tabl
                     max_q: int = 0, workspace: int = 0, workspace_bytes: int = 0) -> _lib.KVBatchDesc:
     """A ragged batch by the addresses of its int32 q_start (B + 1), kv_len (B) and page table (B rows of
     max_pages)."""
+    _fits(32, sequences=sequences, max_pages=max_pages)
+    _fits(64, tokens=tokens, max_q=max_q)
     return _lib.KVBatchDesc(sequences, max_pages, tokens, max_q, q_start, kv_len, table, workspace or None,
                             workspace_bytes)
 
 
 def rope_raw(inv_freq: int, rot_dim: int, interleaved: bool = False, positions: int = 0,
              offset: int = 0) -> _lib.RopeDesc:
+    _fits(32, rot_dim=rot_dim, offset=offset)
     return _lib.RopeDesc(inv_freq or None, rot_dim, int(bool(interleaved)), positions or None, offset)
 
 
 def attn_score_raw(scale: float, causal: bool = True, window: int = 0, cap: float = 0.0, slopes: int = 0,
                    bidirectional: int = 0) -> _lib.AttnScoreDesc:
+    _fits(32, window=window)
     return _lib.AttnScoreDesc(scale, cap, int(bool(causal)), window, slopes or None, bidirectional or None)
 
 

@@ -45,3 +45,22 @@ def test_where_the_generic_kernel_takes_over():
     assert needs(241, 241, D=256, **wide) == 0
     assert needs(241, 241, D=128, **wide) > 0
     assert needs(100000, 100000, D=64, **wide) > 0
+
+
+@pytest.mark.parametrize("make", [
+    lambda x: cache(head_dim=x + 64), lambda x: cache(page_size=x + 16), lambda x: cache(heads=x + 2),
+    lambda x: batch(sequences=x + 3), lambda x: batch(max_pages=x + 4), lambda x: lh.rope_raw(1 << 20, x + 64),
+    lambda x: lh.rope_raw(1 << 20, 64, offset=x), lambda x: lh.attn_score_raw(1.0, window=x + 7)])
+def test_integers_that_a_descriptor_would_cut_off_are_refused(make):
+    for x in (2 ** 32, -2 ** 32):
+        with pytest.raises(ValueError, match="32 bits"):
+            make(x)
+    make(0)
+
+
+@pytest.mark.parametrize("make", [lambda x: cache(pages=x), lambda x: cache(strides=(1, 64, x, 2048)), lambda x: batch(tokens=x),
+                                  lambda x: batch(max_q=x)])
+def test_long_integers_that_a_descriptor_would_cut_off_are_refused(make):
+    with pytest.raises(ValueError, match="64 bits"):
+        make(2 ** 64 + 5)
+    make(5)
