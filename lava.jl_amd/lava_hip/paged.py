@@ -152,8 +152,6 @@ def kv_append(cache: PagedCache, batch: PagedBatch, K: HIPDeviceArray, V: HIPDev
         if Q_out.dtype != Q.dtype or Q_out.dims != Q.dims or Q_out.order != "F":
             raise ValueError("Q_out must be like Q")
     rope = None
-    if inv_freq is None and (positions is not None or interleaved or offset):
-        raise ValueError("positions, interleaved and offset are those of a rotation: give inv_freq")
     if inv_freq is not None:
         if inv_freq.dtype != "f32":
             raise ValueError(f"inv_freq must be f32 (got {inv_freq.dtype})")

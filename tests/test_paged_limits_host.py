@@ -1,6 +1,4 @@
 """Limits of the paged cache's entry points that the host checks or plans by: no call here touches a device."""
-from types import SimpleNamespace
-
 import pytest
 
 import lava_hip as lh
@@ -66,10 +64,3 @@ def test_long_integers_that_a_descriptor_would_cut_off_are_refused(make):
     with pytest.raises(ValueError, match="64 bits"):
         make(2 ** 64 + 5)
     make(5)
-
-
-@pytest.mark.parametrize("rotation", [dict(positions=SimpleNamespace(dtype="i32", size=5)), dict(interleaved=True), dict(offset=7)])
-def test_a_rotation_without_frequencies_is_refused(rotation):
-    x = SimpleNamespace(dtype="f16", dims=(64, 2, 5), order="F")
-    with pytest.raises(ValueError, match="inv_freq"):
-        lh.kv_append(SimpleNamespace(dtype="f16", head_dim=64, heads=2), SimpleNamespace(tokens=5), x, x, **rotation)
