@@ -14,7 +14,7 @@ import math
 from typing import Optional, Sequence
 
 from . import _lib
-from .device import DTYPES, HIPDeviceArray
+from .device import DTYPES, HIPDeviceArray, synchronize
 
 
 def _fits(bits: int, **values: int) -> None:
@@ -123,7 +123,18 @@ class PagedBatch:
             raise ValueError(f"shape mismatch: q_start {q_start.dims}, kv_len {kv_len.dims}, table {table.dims}")
         self.q_start, self.kv_len, self.table = q_start, kv_len, table
         self.tokens = tokens
+        self.workspace: Optional[HIPDeviceArray] = None
         self.desc = paged_batch_raw(B, tokens, q_start.ptr, kv_len.ptr, table.ptr, table.dims[0], max_q)
+
+    def own_workspace(self, cache: PagedCache, q_heads: int, prefix_len: int = 0) -> "PagedBatch":
+        """Gives the batch's attention calls a workspace of its own in place of the stream's (allocated here, so before a
+        capture): for calls that may run at once with others of their stream's, such as replayed graphs."""
+        ws = HIPDeviceArray("u8", (paged_workspace_bytes(cache.desc, self.desc, q_heads, prefix_len),))
+        ws.fill_bytes(0)
+        synchronize()   # whatever stream the calls are on
+        self.workspace = ws
+        self.desc.workspace, self.desc.workspace_bytes = ws.ptr or None, ws.nbytes
+        return self
 
 
 def _check_tokens(name: str, a: HIPDeviceArray, cache: PagedCache, batch: PagedBatch) -> None:

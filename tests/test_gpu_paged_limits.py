@@ -181,3 +181,42 @@ def test_a_growing_batch_allocates_few_workspaces(gpu):
     assert sum(grown) <= 2 + np.log(need[1] / need[0]) / np.log(1.5), (sum(grown), need)
     assert not bad(dev.result()[0], want, bound).any()
     s.close()
+
+
+def test_a_captured_step_of_a_batch_with_its_own_workspace(gpu):
+    """A decode step captured on a fresh stream, which has no workspace yet: replayed beside eager calls on that stream."""
+    lh = gpu
+    announce("a captured step with its own workspace")
+    D, page, Hkv, Hq, B = 64, 16, 2, 8, 3
+    rng = np.random.default_rng(45)
+    lens = np.array([200, 17, 90], np.int32)
+    cache = lh.PagedCache("f16", D, page, Hkv, 30)
+    for a in (cache.k, cache.v):
+        a.copy_from(rng.standard_normal(a.dims).astype(np.float16))
+    table = np.full((14, B), -1, np.int32, order="F")
+    table[:, 0] = rng.permutation(14)
+    table[:6, 1:] = 14 + rng.permutation(12).reshape(6, 2)
+    i32 = lambda a: lh.HIPDeviceArray.from_numpy(np.asarray(a, np.int32), "i32")
+    batch = lh.PagedBatch(B, i32(np.arange(B + 1)), i32(lens), lh.HIPDeviceArray.from_numpy(table, "i32"), max_q=1)
+    Q = lh.HIPDeviceArray.from_numpy(np.asfortranarray(rng.standard_normal((D, Hq, B)).astype(np.float16)), "f16")
+    O, P = (lh.HIPDeviceArray("f16", (D, Hq, B)) for _ in range(2))
+    lh.paged_attn(P, cache, batch, Q)
+    lh.synchronize()
+    want = P.to_numpy()
+    s = lh.Stream()
+    g = lh.Graph(s)
+    assert batch.own_workspace(cache, Hq) is batch
+    with g.capture():
+        lh.paged_attn(O, cache, batch, Q, stream=s.handle)
+    for _ in range(4):
+        O.fill_bytes(0x5a)
+        lh.synchronize()
+        g.launch()
+        s.synchronize()
+        assert (O.to_numpy().view(np.uint16) == want.view(np.uint16)).all()
+        lh.paged_attn(P, cache, batch, Q, stream=s.handle)
+        s.synchronize()
+        assert (P.to_numpy().view(np.uint16) == want.view(np.uint16)).all()
+    g.close()
+    s.close()
+    cache.close()
