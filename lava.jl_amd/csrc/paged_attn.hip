@@ -219,8 +219,14 @@ static bool pa_vectors(const PaParams& p) {
 // kernel.  (us, row / tile kernel: 16 x 17 tokens of 4 heads over 2000 keys, 68 rows 75 / 44; 8 x 32 over 3000, 128 rows 69 / 48; one of
 // 16 over 2000, 64 rows 30 / 33.)
 constexpr int PA_TILE_ROWS = 32;
-// Behind a shared prefix those of more rows, which fill a tile by themselves, read it by themselves.
+// Behind a shared prefix those of more rows, which fill a tile by themselves, read it by themselves.  (us, together / by
+// themselves; 8 sequences, 4 heads a key head, up to 300 keys behind 1024 and behind 8192: 260 rows each 64 / 31 and 129 / 132, 384 78 / 32
+// and 164 / 140; 128 rows 56 / 31 and 79 / 81, 252 64 / 32 and 116 / 110: behind a short prefix fewer would do.)
 constexpr int PA_SHARE_ROWS = 256;
+// Rows of a stacked prefix up to which its tiles have 128 rows: two of 256 would leave CUs without a part and cost more each.  (us
+// behind 1024 and 8192, 256 / 128 rows a tile: 40 rows 35 / 29 and 40 / 35, 256 40 / 34 and 51 / 40, 320 48 / 42 and 56 / 58, 384
+// 48 / 42 and 56 / 59, 640 59 / 53 and 82 / 80, 1024 73 / 66 and 93 / 99.)
+constexpr int PA_PREFIX_ROWS = 320;
 constexpr size_t PA_ALIGN = 256;
 
 // Rows a tile of the tile kernel: 128 take 0.6 of the time of 256 (a fragment read feeds one product, not two), so they pay
@@ -282,7 +288,10 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
         // where the sequences' mean is above the limit the tile kernel takes the short ones too (it reads their keys as
         // fast) rather than a launch for them
         p->row_limit = pin >= 3 || rows > limit * (int64_t)p->b.B ? 0 : limit;
-        // tiles enough for the CUs over few keys, or keys fewer than a split costs: never split, so no launch to join parts
+        // tiles enough for the CUs over few keys, or keys fewer than a split costs: never split, so no launch to join parts, 2 to
+        // 4 us.  (us, never / as the device finds; prompts of 32 heads on 8: 8 of 1344 tokens 153 / 158, one of 1792 51.5 / 54.0, 4 of
+        // 2048 158 / 160; past 32 blocks one of 2176 62.7 / 64.7, 8 352 / 358, 4 of 2560 236 / 238, but over few long keys whole
+        // tiles leave CUs idle: 64 tokens behind 8000.)
         const int64_t blocks = ((int64_t)p->b.kv_max + p->P + PT_BK - 1) / PT_BK;
         p->whole = blocks <= PT_SPLIT || (blocks <= 32 && rows / (128 * sh.qh) * p->c.heads >= 128);
     }
@@ -290,7 +299,7 @@ static PaShape pa_plan_call(PaParams* p, int64_t max_rows) {
         if (p->P > 0) {   // the prefix once for all: beside the sequences, or on the tile kernel for many rows
             const bool many = rows > PA_TILE_ROWS && paged_tile_takes(*p) && pin != 2;
             p->stack = many ? 2 : 1;
-            sh.pre_qh = many ? (rows <= 320 ? 1 : 2) : 0;
+            sh.pre_qh = many ? (rows <= PA_PREFIX_ROWS ? 1 : 2) : 0;
         }
         const int64_t most = p->stack == 1 ? rows : std::min<int64_t>(max_rows, p->row_limit);
         sh.nr = most <= 16 ? 1 : 2;
