@@ -632,7 +632,7 @@ typedef struct lava_hip_attn_score {
 /* O = softmax(scores of Q with the cached keys) times the cached values, for the new tokens of every sequence:
  * Q and O are (E, H, T) tensors of q_heads heads, a multiple of the cache's (query head h reads key head
  * h / (q_heads / heads)).  lse (may be NULL) receives the natural logarithm of each row's sum of exp(score),
- * lse[token * q_heads + head].  MFMA kernels take head dimensions that are a multiple of 8, pages of a multiple of 8 tokens, 16-byte
+ * lse[token * q_heads + head].  O and lse overlap each other, Q and the cache nowhere.  MFMA kernels take head dimensions that are a multiple of 8, pages of a multiple of 8 tokens, 16-byte
  * aligned Q and cache with strides that are multiples of 8 and O aligned to 8 bytes with strides multiples of 4; a generic kernel
  * the rest, and calls of head dimensions above 128 whose row tiles (rows of a key head / 32, or / 16 for at most 16 a sequence,
  * and one a sequence) times max_pages * page_size / 128 are 2^31 or more.  P is rounded once to the operands' type before the second product; sums are in 32 bits, in a fixed order. */

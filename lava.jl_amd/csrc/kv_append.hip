@@ -8,8 +8,8 @@
 // token's cosines and sines are computed once into LDS for all heads, and every thread moves two 16-byte
 // chunks, those of a pair where halves turn.  The angle in turns, pos * inv_freq / 2 pi, is reduced in 64 bits
 // (at position 2^20 32 bits would be off by 0.06 of a radian); sine and cosine of the rest are in 32.
-// Measured (32 + 2 x 8 heads, D = 128): 64 decoded tokens 4.3 us, of which the launch and its lookups are all but 0.3; 16 prompts
-// of 333 to 4096 tokens 123 us, 5.5 TB/s of what is read and written.
+// Measured (32 + 2 x 8 heads, D = 128): 64 decoded tokens 4.6 us, of which the launch and its lookups are all but 0.3; 16 prompts
+// of 333 to 4096 tokens 122 us, 5.5 TB/s of what is read and written.
 
 #include "paged.hpp"
 

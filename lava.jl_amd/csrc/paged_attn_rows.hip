@@ -16,9 +16,9 @@
 //    timing: those of tiles of 16 rows by the last workgroup of a tile to arrive, others by a second small kernel.
 // K and V pages are found 8 keys at a time (page sizes are multiples of 8); a page number that is none reads as zeros
 // and is masked, as are rows at and past the sequence's end.
-// Measured (back to back): 64 decoded tokens, 32 heads on 8, D = 128, 100 to 8192 keys each 222 us, 5.4 TB/s of the cache read; one
-// of 777 keys 9.8 us, a chain of five dependent reads; 3 of 30000 to 131071 keys on 2 key heads, capped, 55; 32 sequences of 1
-// to 4 drafted tokens, 12 heads of D = 64, windows of 1024 and slopes, 26.
+// Measured (calls in a row): 64 decoded tokens, 32 heads on 8, D = 128, 100 to 8192 keys each 217 us, 5.5 TB/s of the cache read; one
+// of 777 keys 9.6 us, a chain of five dependent reads; 3 of 30000 to 131071 keys on 2 key heads, capped, 55 (60 over changing inputs,
+// which no cache holds); 32 sequences of 1 to 4 drafted tokens, 12 heads of D = 64, windows of 1024 and slopes, 24.
 
 #include <algorithm>
 

@@ -10,11 +10,12 @@
 //    compare, blocks that none sees are skipped, and a pair whose rows see nothing yet has no maximum (unset, -inf);
 //  * the scale and the maximum are one fma a score, P = exp2(fma(S, c, -m)); ANY: caps (a polynomial where a block's scores
 //    are small, pa_cap_near), slopes, a scale that is not positive.  Folding the scale into Q and the maximum into the
-//    product, as flash_fwd5_kernel does for f16, is 3.5 % faster on f16 prompts (4 of 4096 tokens: 655 against 679 us)
+//    product, as flash_fwd5_kernel does for f16, is 3.5 % faster on f16 prompts (4 of 4096 tokens, early calls: 655 against 679 us)
 //    and rounds each q once more: 3.8e-4 off against 2.9e-4, of which the results' own rounding is 2.1e-4.
 
-// Measured (back to back): 4 prompts of 4096 tokens, 32 heads on 8, D = 128, 675 us, 815 TFLOP/s; 12 sequences' chunks and decode
-// steps behind 777 to 6000 keys, capped, 343; 8 prompts of 301 to 1537 tokens, 12 heads of D = 64, 52; a prompt of 64 tokens 9.
+// Measured (calls in a row; the first 40 after a pause, until the clock has settled, in brackets): 4 prompts of 4096 tokens, 32 heads on
+// 8, D = 128, 565 us (720), 970 TFLOP/s; 12 sequences' chunks and decode steps behind 777 to 6000 keys, capped, 300 (366); 8 prompts of
+// 301 to 1537 tokens, 12 heads of D = 64, 49; a prompt of 64 tokens 9.
 
 #include <algorithm>
 
