@@ -18,6 +18,9 @@ int hip_fail(hipError_t e, const char* what);
 // that succeeded is appended to the thread's kernel log (lava_hip_kernel_log), which keeps the pointer: a
 // string literal, a kernel's separate form as "kernel+form".
 int check_launch(const char* kernel);
+// Whether HIP can launch the grid: fewer than 2^32 threads in each dimension (of more it runs what is left modulo 2^32, without an
+// error).  If not, the thread's next launch check says so.
+bool launch_fits(const dim3& grid, const dim3& block);
 // The kernel choice pinned for a family (LAVA_HIP_FAMILY_*) by lava_hip_set_kernel_override; 0 = automatic.
 int kernel_override(int family);
 
@@ -71,4 +74,12 @@ inline bool whole_lines(const void* p, int64_t ld_bytes) { return aligned(p, 128
     do {                                           \
         int _lava_rc = ::lava::check_launch(name); \
         if (_lava_rc != LAVA_HIP_OK) return _lava_rc; \
+    } while (0)
+
+// Every launch of the library goes through launch_fits.
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)                                              \
+    do {                                                                                                       \
+        const dim3 lava_grid_ = (grid), lava_block_ = (block);                                                 \
+        if (::lava::launch_fits(lava_grid_, lava_block_)) kernel<<<lava_grid_, lava_block_, lds, stream>>>(__VA_ARGS__); \
     } while (0)

@@ -65,7 +65,21 @@ static const char* klog_text() {
     return g_klog + at;
 }
 
+static thread_local bool g_launch_too_large = false;
+
+bool launch_fits(const dim3& grid, const dim3& block) {
+    const uint64_t most = 0xffffffffu;
+    const bool fits = (uint64_t)grid.x * block.x <= most && (uint64_t)grid.y * block.y <= most && (uint64_t)grid.z * block.z <= most;
+    if (!fits) g_launch_too_large = true;
+    return fits;
+}
+
 int check_launch(const char* kernel) {
+    if (g_launch_too_large) {
+        g_launch_too_large = false;
+        set_error("%s would need 2^32 threads or more in one dimension of a launch", kernel);
+        return LAVA_HIP_ERR_UNSUPPORTED;
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) {
         set_error("launch of %s failed: %s (%d)", kernel, hipGetErrorString(e), (int)e);
