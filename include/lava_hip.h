@@ -150,7 +150,8 @@ void lava_hip_kernel_log_clear(void);
  *                        (f16 / bf16 / int8 / unsigned bytes, any operand layout; the fused
  *                        epilogue for f16 / bf16), not its K-split form;
  *  LAVA_HIP_FAMILY_PAGED: attention over the paged cache: 1 the generic kernel, 2 the row kernel,
- *                        3 the tile kernel (D <= 128) with 256 rows a tile, 4 with 128.
+ *                        3 the tile kernel (D <= 128) with 256 rows a tile, 4 with 128;
+ *  LAVA_HIP_FAMILY_W8A8: layers with 8-bit tokens: 1 the generic kernel.
  * Unknown families or choices return LAVA_HIP_ERR_INVALID_ARG. */
 /* Reads [src, src + bytes) once with 16-byte nontemporal loads, `unroll` (4, 8 or 16) in flight
  * per thread, `blocks` workgroups of 256 threads, and writes the XOR of what each thread read to
@@ -181,6 +182,7 @@ int lava_hip_mfma_loop(int op, const void* a, const void* b, size_t bytes, int b
 #define LAVA_HIP_FAMILY_ATTN 1
 #define LAVA_HIP_FAMILY_GEMM 2
 #define LAVA_HIP_FAMILY_PAGED 3
+#define LAVA_HIP_FAMILY_W8A8 4
 int lava_hip_set_kernel_override(int family, int choice);
 
 /* ========================================================================= */
@@ -652,6 +654,118 @@ int lava_hip_shared_prefix_attn(const lava_hip_kv_cache* cache, const lava_hip_k
 /* The workspace that a call with these descriptors (prefix_len 0: lava_hip_paged_attn) needs, 0 included. */
 int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, const lava_hip_kv_batch* batch, int64_t q_heads,
                                    int64_t prefix_len, size_t* bytes);
+
+/* ========================================================================= */
+/* Feed-forward layers with 8-bit weights and tokens, and their experts.      */
+/* No counterpart in the reference, whose 8-bit products are the int8 GEMM    */
+/* and the per-element dequantising callback (src/compiler/spirv/coopmat.jl:  */
+/* 115-151, src/device/coopmat_intrinsics.jl:535-628): both at once, for      */
+/* programs that generate tokens.                                             */
+/* ========================================================================= */
+
+/* Quantises `tokens` rows of k values (F16, BF16 or F32; row t at X + t * ldx elements) to 8 bits, a scale a row:
+ *   scale[t] = max |x| / 127, Q[t][j] = the integer nearest to 127 x / max |x| (ties to even; of the real quotient, so no
+ * rounding of a quotient or of the scale moves it), row t of Q at Q + t * ldq.  A row of zeros gives zeros and a scale of 0; a
+ * row that holds an infinity or NaN gives zeros and a scale of NaN, so that what is computed from it shows.  Q and scale
+ * do not overlap X.  Columns of Q from k on are left as they are. */
+int lava_hip_quantize_i8(int x_dtype, const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens, int64_t ldx,
+                         int64_t ldq, void* stream);
+
+/* x / (1 + exp(-x)); lava_hip_w8_layer takes it beside LAVA_HIP_ACT_NONE to LAVA_HIP_ACT_GELU_ERF. */
+#define LAVA_HIP_ACT_SILU 4
+
+/* A linear layer with 8-bit weights, or one for each of several experts: weight j of channel n of expert e is
+ * w[e * expert_stride + n * ldw + j] (K contiguous, a column-major (K, N, experts) array), its scale scale[e * n_channels + n],
+ * its bias bias[e * n_channels + n].  A gated layer's first n / 2 channels are the gate's. */
+typedef struct lava_hip_w8_layer {
+    const int8_t* w;
+    const float* scale;
+    const float* bias;     /* or NULL */
+    int64_t n;             /* channels; of a gated layer an even number */
+    int64_t k;             /* at most 131071: the 32-bit sums of any bytes are exact */
+    int64_t ldw;           /* >= k */
+    int64_t expert_stride; /* >= n * ldw where experts > 1 */
+    int32_t experts;
+    int32_t act;           /* LAVA_HIP_ACT_* */
+    int32_t gated;
+} lava_hip_w8_layer;
+
+/* The layer (experts 1) on rows of 8-bit tokens, K contiguous at X + t * ldx, each with its scale:
+ *   y[t][n] = (sum_j X[t][j] w[n][j]) * x_scale[t] * scale[n] + bias[n]
+ *   Y[t][n] = act(y[t][n]), or of a gated layer act(y[t][n]) * y[t][n + N / 2] for n < N / 2,
+ * rounded once to y_dtype (F16, BF16 or F32), row t at Y + t * ldy.  The sums are exact in 32-bit integers, the rest is in
+ * 32-bit floating point in the order written, whichever kernel runs: its choice changes no bit of Y.  MFMA kernels that load 16 bytes
+ * at a time take k, ldx and ldw that are multiples of 16 and 16-byte aligned X and w; any other layout runs on a
+ * generic one.  One launch, no workspace.  Y overlaps no other operand. */
+int lava_hip_gemm_w8a8(const lava_hip_w8_layer* layer, const int8_t* X, const float* x_scale, int64_t tokens, int64_t ldx,
+                       int y_dtype, void* Y, int64_t ldy, void* stream);
+
+#define LAVA_HIP_SCORE_SOFTMAX 0
+#define LAVA_HIP_SCORE_SIGMOID 1
+
+/* How tokens are routed to experts by their logits x:
+ *   p = softmax(x) over the experts, or sigmoid(x);  c = p + bias;
+ *   with top_groups < groups: the experts fall into `groups` runs of equal length, a run counts the sum of its group_best (1 or 2)
+ *   highest c, and only the top_groups highest runs stay;
+ *   the top_k highest c are chosen, highest first; weight = p of the chosen, divided by the chosen ones' sum
+ *   if renormalize, times scale.
+ * Equal c or counts go to the lower number; c is compared in 64 bits where 32 do not tell two apart.  A logit of -inf, or a bias of
+ * -inf, masks its expert: where fewer than top_k are left, the rest of a token's experts are -1 with a weight of 0 (a run counts
+ * its masked experts as -inf).  A token with a NaN or +inf among its logits or c has no experts (-1) and weights of NaN. */
+typedef struct lava_hip_moe_router {
+    int32_t experts;     /* 1 .. 1024 */
+    int32_t top_k;       /* 1 .. min(experts, 32) */
+    int32_t score;       /* LAVA_HIP_SCORE_* */
+    int32_t groups;      /* 1 .. 64, a divisor of experts */
+    int32_t top_groups;  /* 1 .. groups */
+    int32_t group_best;  /* 1 or 2, at most experts / groups */
+    int32_t renormalize;
+    float scale;
+    const float* bias;   /* device, experts, or NULL */
+} lava_hip_moe_router;
+
+/* The tokens of each expert: of the tokens * top_k assignments a = token * top_k + rank, those of expert e are
+ * order[offsets[e] .. offsets[e + 1]), in ascending order.  Assignments to no expert (-1, or any number outside [0, experts))
+ * are in no run; order holds -1 behind the last run.  lava_hip_moe_route and lava_hip_moe_sort write a plan, lava_hip_experts_w8a8
+ * reads one; there nothing that offsets and order hold makes a kernel read or write outside the buffers: offsets are cut to
+ * [0, tokens * top_k], and a row whose entry of order is outside [0, tokens * top_k) is left out. */
+typedef struct lava_hip_moe_plan {
+    int64_t tokens;      /* tokens * top_k below 2^31 */
+    int32_t experts;     /* 1 .. 1024 */
+    int32_t top_k;       /* 1 .. 32 */
+    int32_t* offsets;    /* device, experts + 1 */
+    int32_t* order;      /* device, tokens * top_k */
+    void* workspace;     /* device, 4-byte aligned, lava_hip_moe_plan_workspace_bytes; what only reads a plan needs none.  Calls that may run
+                          * at once, two replayed graphs' too, need one each */
+    size_t workspace_bytes;
+} lava_hip_moe_plan;
+
+/* The workspace that writing a plan of these sizes needs, 0 included; nothing has to be in it. */
+int lava_hip_moe_plan_workspace_bytes(int64_t tokens, int32_t experts, int32_t top_k, size_t* bytes);
+
+/* Routes tokens by their logits (F16, BF16 or F32; row t at logits + t * ldl): ids and weights are (top_k, tokens) arrays, the
+ * rank fastest.  plan (or NULL) is written beside them, for the same tokens, experts and top_k. */
+int lava_hip_moe_route(const lava_hip_moe_router* router, int dtype, const void* logits, int64_t ldl, int64_t tokens,
+                       int32_t* ids, float* weights, const lava_hip_moe_plan* plan, void* stream);
+
+/* Writes the plan of given ids, (top_k, tokens). */
+int lava_hip_moe_sort(const int32_t* ids, const lava_hip_moe_plan* plan, void* stream);
+
+/* The experts' layers on the rows of a plan.  Row i of a run is token order[i] / top_k of X, or with LAVA_HIP_X_SORTED row i of
+ * X itself (x_scale likewise); its result is row order[i] of Y, or with LAVA_HIP_Y_SORTED row i.  X has tokens rows, or with
+ * LAVA_HIP_X_SORTED tokens * top_k, Y has tokens * top_k.  Rows of Y that belong to no run are left as they are.  No two
+ * places of order within the runs are alike.  Otherwise as lava_hip_gemm_w8a8; one launch, no workspace. */
+#define LAVA_HIP_X_SORTED 1u
+#define LAVA_HIP_Y_SORTED 2u
+int lava_hip_experts_w8a8(const lava_hip_moe_plan* plan, const lava_hip_w8_layer* layer, const int8_t* X,
+                          const float* x_scale, int64_t ldx, int y_dtype, void* Y, int64_t ldy, uint32_t flags,
+                          void* stream);
+
+/* out[t] = base[t] + sum over j of weights[t * top_k + j] * Y[t * top_k + j], rows of n values of one type (F16, BF16 or F32), in
+ * 32 bits in the order of j, rounded once.  base may be NULL, or out itself with the same stride; Y overlaps out nowhere.  A
+ * negative id's row of Y is not read (its weight counts times 0: a weight of NaN shows); ids NULL: every row is read. */
+int lava_hip_moe_combine(int dtype, const void* Y, int64_t ldy, const int32_t* ids, const float* weights, int64_t tokens,
+                         int32_t top_k, int64_t n, const void* base, int64_t ldb, void* out, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,648 @@
+// moe.hip -- tokens routed to experts, sorted by them, and the experts' results summed.
+//
+// Routing: L lanes of a wavefront hold a token's logits, V each, and take the highest one top_k times by a reduction over
+// the lanes.  Without a bias the order of p is that of the logits, which are compared as they are.  With one, and for
+// groups counted by two, c = p + bias is taken in 32 bits first; where two that the choice tells apart lie nearer to each
+// other than c's rounding may move them, the wavefront's tokens are done again in 64.
+//
+// Sorting: workgroup b has tokens [b * span, (b + 1) * span), counts its assignments per expert, and in a second launch
+// (in the same one where a workgroup has all tokens) adds the counts of the lower workgroups and places its own in
+// order: a stable counting sort without global atomics, the same in every run.
+#include <hip/hip_runtime.h>
+
+#include "gemm_common.hpp"
+#include "lava_hip_internal.hpp"
+#include "w8a8.hpp"
+
+namespace lava {
+
+namespace {
+
+constexpr int MOE_THREADS = 1024, MOE_WAVES = MOE_THREADS / 64;
+constexpr int MOE_EXPERTS = 1024, MOE_TOP_K = 32;
+constexpr int MOE_BLOCKS = 256;    // workgroups that share a sort, at most
+constexpr int MOE_SPAN = 64;       // tokens a workgroup, at least
+
+struct Plan {   // what a kernel needs of a plan
+    int32_t* offsets;   // null: none is written
+    int32_t* order;
+    int32_t* counts;    // [workgroup][expert]
+    int tokens, experts, top_k, span;
+};
+
+// tokens a workgroup has
+int span_of(int64_t tokens) {
+    const int64_t per = (tokens + MOE_BLOCKS - 1) / MOE_BLOCKS;
+    return (int)((per + MOE_SPAN - 1) / MOE_SPAN * MOE_SPAN);
+}
+int blocks_of(int64_t tokens) {
+    if (tokens == 0) return 1;
+    const int span = span_of(tokens);
+    return (int)((tokens + span - 1) / span);
+}
+
+struct Router {
+    const float* bias;
+    int experts, top_k, softmax, groups, top_groups, group_best, renormalize;
+    float scale;
+};
+
+template <typename Real>
+__device__ __forceinline__ Real exp_of(Real x) {
+    if constexpr (sizeof(Real) == 8) return exp(x);
+    else return expf(x);
+}
+
+template <typename Real>
+__device__ __forceinline__ Real neg_inf() {
+    return -(Real)__builtin_inff();
+}
+
+// The highest of c over the L lanes of a token and its place e = v * L + lane, the lowest of equal ones.
+template <int L, int V, typename Real>
+__device__ __forceinline__ void highest(const Real (&c)[V], int lane, Real& top, int& at) {
+    top = c[0];
+    at = lane;
+#pragma unroll
+    for (int v = 1; v < V; ++v)
+        if (c[v] > top) {
+            top = c[v];
+            at = v * L + lane;
+        }
+#pragma unroll
+    for (int d = 1; d < L; d <<= 1) {
+        const Real o = __shfl_xor(top, d, 64);
+        const int oa = __shfl_xor(at, d, 64);
+        if (o > top || (o == top && oa < at)) {
+            top = o;
+            at = oa;
+        }
+    }
+}
+
+template <int L, int V, typename Real>
+__device__ __forceinline__ void take_out(Real (&c)[V], int lane, int at) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+        if (at == v * L + lane) c[v] = neg_inf<Real>();
+}
+
+// The experts of the token that these L lanes hold, in sel (rank r in lane r % L, sel[r / L]): true unless 32 bits do not
+// settle the order.
+template <int L, int V, typename Real>
+__device__ bool choose(const Router& r, const float (&x)[V], int lane, int (&sel)[32 / L + (L > 32)]) {
+    constexpr bool SINGLE = sizeof(Real) == 4;
+    // Without a bias the logits' own order is the one asked for, of single experts and of groups counted by their best.
+    const bool by_logit = r.bias == nullptr && (r.top_groups == r.groups || r.group_best == 1);
+    Real c[V];
+    Real near = 0;   // how near two c may be that 32 bits cannot tell apart, without the part that grows with c
+    if (by_logit) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = (Real)x[v];
+    } else {
+        Real top = 0, norm = 1;
+        if (r.softmax) {
+            float m = x[0];
+#pragma unroll
+            for (int v = 1; v < V; ++v) m = fmaxf(m, x[v]);
+#pragma unroll
+            for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+            top = m == neg_inf<float>() ? (Real)0 : (Real)m;
+            Real sum = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum += exp_of<Real>((Real)x[v] - top);
+#pragma unroll
+            for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, 64);
+            norm = sum > 0 ? 1 / sum : (Real)0;
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = v * L + lane;
+            Real p = r.softmax ? exp_of<Real>((Real)x[v] - top) * norm : 1 / (1 + exp_of<Real>(-(Real)x[v]));
+            if (e < r.experts && r.bias) p += (Real)r.bias[e];
+            c[v] = x[v] == neg_inf<float>() ? neg_inf<Real>() : p;
+        }
+        // of p: exp, sum (V + 6 additions, V at most 64) and quotient, at most 2^-17 of the largest; a sigmoid's at most 2^-21
+        if (SINGLE) near = r.softmax ? norm * (Real)0x1p-16f : (Real)0x1p-20f;
+    }
+    auto apart = [&](Real hi, Real lo, int terms) {
+        if (!SINGLE || by_logit || lo == neg_inf<Real>()) return true;
+        return hi - lo > terms * (near + (Real)0x1p-22f * fmax((Real)fabs(hi), (Real)fabs(lo)));
+    };
+    bool sure = true;
+    if (r.top_groups < r.groups) {
+        const int size = r.experts / r.groups;
+        constexpr int GV = 64 / L;
+        Real count[GV];   // group g in lane g % L
+#pragma unroll
+        for (int i = 0; i < GV; ++i) count[i] = neg_inf<Real>();
+        for (int g = 0; g < r.groups; ++g) {
+            Real b1 = neg_inf<Real>(), b2 = neg_inf<Real>();   // its best two
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if ((unsigned)(v * L + lane - g * size) < (unsigned)size) {
+                    b2 = fmax(b2, fmin(b1, c[v]));
+                    b1 = fmax(b1, c[v]);
+                }
+#pragma unroll
+            for (int d = 1; d < L; d <<= 1) {
+                const Real o1 = __shfl_xor(b1, d, 64), o2 = __shfl_xor(b2, d, 64);
+                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+                b1 = fmax(b1, o1);
+            }
+            const Real sum = r.group_best == 2 ? b1 + b2 : b1;
+#pragma unroll
+            for (int i = 0; i < GV; ++i)
+                if (g == i * L + lane) count[i] = sum;
+        }
+        uint64_t kept = 0;
+        Real last = 0;
+        for (int i = 0; i <= r.top_groups; ++i) {
+            Real top;
+            int g;
+            highest<L, GV, Real>(count, lane, top, g);
+            if (i == r.top_groups) {
+                sure = sure && apart(last, top, r.group_best);
+                break;
+            }
+            last = top;
+            if (top == neg_inf<Real>()) break;   // groups of masked experts only: none of them is open anyway
+            kept |= 1ull << g;
+            take_out<L, GV, Real>(count, lane, g);
+        }
+        // groups that count -inf though one of their experts is left (the second best is masked): by their number
+        if (last == neg_inf<Real>()) {
+            int more = r.top_groups - __popcll(kept);
+            for (int g = 0; g < r.groups && more > 0; ++g)
+                if (!(kept >> g & 1)) {
+                    kept |= 1ull << g;
+                    --more;
+                }
+        }
+        const float inv = 1.f / (float)size;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int g = (int)(((float)(v * L + lane) + 0.5f) * inv);
+            if (!(kept >> (g & 63) & 1)) c[v] = neg_inf<Real>();
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 32 / L + (L > 32); ++i) sel[i] = -1;
+    Real last = 0;
+    for (int i = 0; i <= r.top_k; ++i) {
+        Real top;
+        int at;
+        highest<L, V, Real>(c, lane, top, at);
+        if (i > 0) sure = sure && apart(last, top, 1);
+        if (i == r.top_k || top == neg_inf<Real>()) break;   // the same in all lanes of a token, but not of a wavefront
+        last = top;
+#pragma unroll
+        for (int j = 0; j < 32 / L + (L > 32); ++j)
+            if (i == j * L + lane) sel[j] = at;
+        take_out<L, V, Real>(c, lane, at);
+    }
+    return sure;
+}
+
+// Adds the tokens' assignments to counts (LDS) or places them: base[e] is the next free place of expert e's run.
+// Stable: 1024 assignments at a time, a thread each; its place is base + those of lower wavefronts + those of lower lanes.
+__device__ void place(const Plan& p, const int32_t* ids, int first, int last, int32_t* base, uint16_t* below) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E = p.experts;
+    const int bits = 32 - __clz(E - 1 > 0 ? E - 1 : 1);
+    for (int i0 = first; i0 < last; i0 += MOE_THREADS) {
+        for (int i = threadIdx.x; i < MOE_WAVES * E; i += MOE_THREADS) below[i] = 0;
+        __syncthreads();
+        const int i = i0 + threadIdx.x;
+        const int e = i < last ? ids[i] : -1;
+        const bool ok = e >= 0 && e < E;
+        uint64_t same = __ballot(ok);   // lanes of the same expert
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot(ok && (e >> b & 1));
+            same &= (e >> b & 1) ? set : ~set;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (ok && rank == 0) below[w * E + e] = (uint16_t)__popcll(same);
+        __syncthreads();
+        if (ok) {
+            int at = base[e] + rank;
+            for (int v = 0; v < w; ++v) at += below[v * E + e];
+            p.order[at] = i;
+        }
+        __syncthreads();
+        for (int j = threadIdx.x; j < E; j += MOE_THREADS) {
+            int sum = 0;
+            for (int v = 0; v < MOE_WAVES; ++v) sum += below[v * E + j];
+            base[j] += sum;
+        }
+        __syncthreads();
+    }
+}
+
+// Exclusive scan of v over the workgroup's threads; total: of all.
+__device__ __forceinline__ int scan(int v, int32_t* tmp, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(sum, d, 64);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 63) tmp[w] = sum;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < MOE_WAVES; ++i) {
+        if (i < w) before += tmp[i];
+        total += tmp[i];
+    }
+    __syncthreads();
+    return before + sum - v;
+}
+
+// Of workgroup b, whose own and the others' counts are known: writes its part of the plan.
+__device__ void finish_plan(const Plan& p, const int32_t* ids, int b, int blocks, int before, int all, int32_t* base,
+                            uint16_t* below, int32_t* tmp) {
+    int total;
+    const int start = scan(all, tmp, total);   // of expert threadIdx.x
+    if (threadIdx.x < (unsigned)p.experts) {
+        base[threadIdx.x] = start + before;
+        if (b == 0) p.offsets[threadIdx.x] = start;
+    }
+    if (b == 0 && threadIdx.x == 0) p.offsets[p.experts] = total;
+    const int rows = p.tokens * p.top_k;
+    for (int64_t i = (int64_t)total + b * MOE_THREADS + threadIdx.x; i < rows; i += (int64_t)blocks * MOE_THREADS) p.order[i] = -1;
+    __syncthreads();
+    const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens);
+    place(p, ids, b * p.span * p.top_k, (int)(last * p.top_k), base, below);
+}
+
+struct SortShared {
+    int32_t base[MOE_EXPERTS];
+    int32_t tmp[MOE_WAVES];
+};
+
+}  // namespace
+
+// COUNT: routes nothing, counts given ids.
+template <typename T, int L, int V>
+__global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const T* __restrict__ logits, int64_t ldl,
+                                                                int32_t* ids, float* weights, Plan p) {
+    extern __shared__ uint16_t below[];   // MOE_WAVES * experts where one workgroup has all tokens and writes the plan
+    __shared__ SortShared sh;
+    constexpr int PER = MOE_WAVES * (64 / L), S = 32 / L + (L > 32);
+    const int lane = threadIdx.x & (L - 1), b = blockIdx.x;
+    if (p.offsets) {
+        if (threadIdx.x < MOE_EXPERTS) sh.base[threadIdx.x] = 0;
+        __syncthreads();
+    }
+    const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens);
+    for (int64_t t0 = (int64_t)b * p.span; t0 < last; t0 += PER) {
+        const int64_t t = t0 + threadIdx.x / L;
+        const bool live = t < last;
+        const T* row = logits + (live ? t : 0) * ldl;
+        float x[V];
+        bool bad = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int e = v * L + lane;
+            x[v] = neg_inf<float>();
+            if (live && e < r.experts) {
+                x[v] = (float)row[e];
+                bad |= !(x[v] < __builtin_inff());
+                if (r.bias) bad |= !(r.bias[e] < __builtin_inff());
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) bad |= __shfl_xor((int)bad, d, 64) != 0;
+        if (bad) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = neg_inf<float>();
+        }
+        int sel[S];
+        const bool sure = choose<L, V, float>(r, x, lane, sel);
+        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, lane, sel);
+
+        // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
+        // so that p of far masked or shut out experts, below the least float, does not make 0 / 0
+        float xs[S], top = neg_inf<float>(), m = neg_inf<float>(), all = 0.f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : neg_inf<float>();
+            top = fmaxf(top, xs[i]);
+        }
+        if (r.softmax && !r.renormalize) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) m = fmaxf(m, x[v]);
+        }
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) {
+            top = fmaxf(top, __shfl_xor(top, d, 64));
+            m = fmaxf(m, __shfl_xor(m, d, 64));
+        }
+        if (!r.renormalize) top = r.softmax ? m : 0.f;
+        else if (!r.softmax) top = fminf(top, 0.f);
+        if (top == neg_inf<float>()) top = 0.f;
+        float w[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            // softmax: exp(x - top); sigmoid: exp(-top) / (1 + exp(-x)), where top is 0 unless every x is below it
+            w[i] = sel[i] < 0    ? 0.f
+                   : r.softmax   ? expf(xs[i] - top)
+                   : xs[i] > 0.f ? 1.f / (1.f + expf(-xs[i]))
+                                 : expf(xs[i] - top) / (1.f + expf(xs[i]));
+            if (r.renormalize) all += w[i];
+        }
+        if (r.softmax && !r.renormalize) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) all += expf(x[v] - top);
+        }
+#pragma unroll
+        for (int d = 1; d < L; d <<= 1) all += __shfl_xor(all, d, 64);
+        if (!r.renormalize && !r.softmax) all = 1.f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int rank = i * L + lane;
+            if (!live || rank >= r.top_k) continue;
+            float o = w[i] / all * r.scale;
+            if (sel[i] < 0) o = bad ? __builtin_nanf("") : 0.f;
+            ids[t * r.top_k + rank] = sel[i];
+            weights[t * r.top_k + rank] = o;
+            if (p.offsets && sel[i] >= 0) atomicAdd(&sh.base[sel[i]], 1);
+        }
+    }
+    if (!p.offsets) return;
+    __syncthreads();   // the counts, and this workgroup's ids in memory
+    if (gridDim.x > 1) {
+        if (threadIdx.x < (unsigned)p.experts) p.counts[b * p.experts + threadIdx.x] = sh.base[threadIdx.x];
+        return;
+    }
+    const int all = threadIdx.x < (unsigned)p.experts ? sh.base[threadIdx.x] : 0;
+    __syncthreads();
+    finish_plan(p, ids, 0, 1, 0, all, sh.base, below, sh.tmp);
+}
+
+// Counts given ids; a workgroup that has all tokens places them too.
+__global__ void __launch_bounds__(MOE_THREADS) moe_count_kernel(const int32_t* __restrict__ ids, Plan p) {
+    extern __shared__ uint16_t below[];
+    __shared__ SortShared sh;
+    const int b = blockIdx.x;
+    if (threadIdx.x < MOE_EXPERTS) sh.base[threadIdx.x] = 0;
+    __syncthreads();
+    const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens) * p.top_k;
+    for (int64_t i = (int64_t)b * p.span * p.top_k + threadIdx.x; i < last; i += MOE_THREADS) {
+        const int e = ids[i];
+        if (e >= 0 && e < p.experts) atomicAdd(&sh.base[e], 1);
+    }
+    __syncthreads();
+    const int all = threadIdx.x < (unsigned)p.experts ? sh.base[threadIdx.x] : 0;
+    if (gridDim.x > 1) {
+        if (threadIdx.x < (unsigned)p.experts) p.counts[b * p.experts + threadIdx.x] = all;
+        return;
+    }
+    __syncthreads();
+    finish_plan(p, ids, 0, 1, 0, all, sh.base, below, sh.tmp);
+}
+
+__global__ void __launch_bounds__(MOE_THREADS) moe_place_kernel(const int32_t* __restrict__ ids, Plan p) {
+    extern __shared__ uint16_t below[];
+    __shared__ SortShared sh;
+    int before = 0, all = 0;
+    if (threadIdx.x < (unsigned)p.experts)
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+            const int c = p.counts[b * p.experts + threadIdx.x];
+            all += c;
+            if (b < (int)blockIdx.x) before += c;
+        }
+    finish_plan(p, ids, blockIdx.x, gridDim.x, before, all, sh.base, below, sh.tmp);
+}
+
+// A thread 4 columns of a token; the plain form of any alignment one column.
+template <typename T, int C>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const T* __restrict__ Y, int64_t ldy, const int32_t* __restrict__ ids,
+                                                          const float* __restrict__ weights, int top_k, int64_t n,
+                                                          const T* base, int64_t ldb, T* out, int64_t ldo, int per_row) {
+    const int64_t t = blockIdx.x / per_row;
+    const int64_t col = ((int64_t)(blockIdx.x % per_row) * 256 + threadIdx.x) * C;
+    if (col >= n) return;
+    typedef T Tv __attribute__((ext_vector_type(C)));
+    float sum[C];
+    if (base) {
+        const Tv v = *reinterpret_cast<const Tv*>(base + t * ldb + col);
+#pragma unroll
+        for (int i = 0; i < C; ++i) sum[i] = (float)v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) sum[i] = 0.f;
+    }
+    for (int j = 0; j < top_k; ++j) {
+        const int64_t a = t * top_k + j;
+        const float w = weights[a];
+        if (ids && ids[a] < 0) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) sum[i] += w * 0.f;
+            continue;
+        }
+        const Tv v = *reinterpret_cast<const Tv*>(Y + a * ldy + col);
+#pragma unroll
+        for (int i = 0; i < C; ++i) sum[i] = __builtin_fmaf(w, (float)v[i], sum[i]);
+    }
+    Tv o;
+#pragma unroll
+    for (int i = 0; i < C; ++i) o[i] = narrow<T>(sum[i]);
+    *reinterpret_cast<Tv*>(out + t * ldo + col) = o;
+}
+
+namespace {
+
+int check_router(const lava_hip_moe_router* r) {
+    LAVA_ARG(r != nullptr, "moe_route: null router");
+    LAVA_ARG(r->experts >= 1 && r->top_k >= 1, "moe_route: %d of %d experts", r->top_k, r->experts);
+    LAVA_REQUIRE(r->experts <= MOE_EXPERTS && r->top_k <= MOE_TOP_K, LAVA_HIP_ERR_UNSUPPORTED,
+                 "moe_route: %d of %d experts (at most %d of %d)", r->top_k, r->experts, MOE_TOP_K, MOE_EXPERTS);
+    LAVA_ARG(r->top_k <= r->experts, "moe_route: top_k = %d of %d experts", r->top_k, r->experts);
+    LAVA_ARG(r->score == LAVA_HIP_SCORE_SOFTMAX || r->score == LAVA_HIP_SCORE_SIGMOID, "moe_route: unknown score %d", r->score);
+    LAVA_ARG(r->groups >= 1 && r->experts % r->groups == 0, "moe_route: %d experts in %d groups", r->experts, r->groups);
+    LAVA_REQUIRE(r->groups <= 64, LAVA_HIP_ERR_UNSUPPORTED, "moe_route: %d groups (at most 64)", r->groups);
+    LAVA_ARG(r->top_groups >= 1 && r->top_groups <= r->groups, "moe_route: top_groups = %d of %d", r->top_groups, r->groups);
+    LAVA_ARG((r->group_best == 1 || r->group_best == 2) && r->group_best <= r->experts / r->groups,
+             "moe_route: group_best = %d of groups of %d", r->group_best, r->experts / r->groups);
+    LAVA_ARG(r->scale - r->scale == 0.f, "moe_route: scale is not finite");
+    LAVA_ARG(aligned(r->bias, 4), "moe_route: misaligned bias");
+    return LAVA_HIP_OK;
+}
+
+size_t plan_bytes(int64_t tokens, int experts) {
+    const int blocks = blocks_of(tokens);
+    return blocks > 1 ? (size_t)blocks * experts * sizeof(int32_t) : 0;
+}
+
+int check_sizes(const char* name, int64_t tokens, int experts, int top_k) {
+    LAVA_ARG(tokens >= 0, "%s: negative tokens (%lld)", name, (long long)tokens);
+    LAVA_ARG(experts >= 1 && top_k >= 1, "%s: a plan of %d of %d experts", name, top_k, experts);
+    LAVA_REQUIRE(experts <= MOE_EXPERTS && top_k <= MOE_TOP_K, LAVA_HIP_ERR_UNSUPPORTED,
+                 "%s: a plan of %d of %d experts (at most %d of %d)", name, top_k, experts, MOE_TOP_K, MOE_EXPERTS);
+    LAVA_REQUIRE(tokens <= 0x7fffffff / top_k, LAVA_HIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d experts are too many", name,
+                 (long long)tokens, top_k);
+    return LAVA_HIP_OK;
+}
+
+Plan plan_of(const lava_hip_moe_plan* plan) {
+    Plan p = {};
+    p.offsets = plan->offsets;
+    p.order = plan->order;
+    p.counts = static_cast<int32_t*>(plan->workspace);
+    p.tokens = (int)plan->tokens;
+    p.experts = plan->experts;
+    p.top_k = plan->top_k;
+    p.span = plan->tokens ? span_of(plan->tokens) : MOE_SPAN;
+    return p;
+}
+
+size_t below_bytes(int experts) { return (size_t)MOE_WAVES * experts * sizeof(uint16_t); }
+
+int launch_place(const int32_t* ids, const Plan& p, int blocks, hipStream_t s) {
+    hipLaunchKernelGGL(moe_place_kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), below_bytes(p.experts), s, ids, p);
+    LAVA_LAUNCH_CHECK("moe_place_kernel");
+    return LAVA_HIP_OK;
+}
+
+template <typename T>
+int launch_route(const Router& r, const void* logits, int64_t ldl, int32_t* ids, float* weights, const Plan& p, int blocks,
+                 hipStream_t s) {
+    const size_t lds = p.offsets && blocks == 1 ? below_bytes(p.experts) : 0;
+    const T* x = static_cast<const T*>(logits);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), lds, s, r, x, ldl, ids, weights, p);
+    };
+    if (r.experts <= 64) go(moe_route_kernel<T, 16, 4>);
+    else if (r.experts <= 128) go(moe_route_kernel<T, 16, 8>);
+    else if (r.experts <= 256) go(moe_route_kernel<T, 16, 16>);
+    else go(moe_route_kernel<T, 64, 16>);
+    LAVA_LAUNCH_CHECK("moe_route_kernel");
+    return p.offsets && blocks > 1 ? launch_place(ids, p, blocks, s) : LAVA_HIP_OK;
+}
+
+template <typename T>
+int launch_combine(const void* Y, int64_t ldy, const int32_t* ids, const float* weights, int64_t tokens, int top_k, int64_t n,
+                   const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t s) {
+    const bool vec = n % 4 == 0 && ldy % 4 == 0 && ldo % 4 == 0 && (base == nullptr || ldb % 4 == 0) &&
+                     aligned(Y, 4 * sizeof(T)) && aligned(out, 4 * sizeof(T)) && aligned(base, 4 * sizeof(T));
+    const int64_t per_row = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+    LAVA_REQUIRE(per_row <= 0x7fffffff && tokens <= 0xffffff / per_row, LAVA_HIP_ERR_UNSUPPORTED,
+                 "moe_combine: %lld tokens of %lld values are too many", (long long)tokens, (long long)n);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, s, static_cast<const T*>(Y), ldy, ids, weights,
+                           top_k, n, static_cast<const T*>(base), ldb, static_cast<T*>(out), ldo, (int)per_row);
+    };
+    if (vec) go(moe_combine_kernel<T, 4>);
+    else go(moe_combine_kernel<T, 1>);
+    LAVA_LAUNCH_CHECK("moe_combine_kernel");
+    return LAVA_HIP_OK;
+}
+
+bool float_type(int dtype) { return dtype == LAVA_HIP_F32 || dtype == LAVA_HIP_F16 || dtype == LAVA_HIP_BF16; }
+
+}  // namespace
+
+int check_plan(const char* name, const lava_hip_moe_plan* plan, bool write) {
+    LAVA_ARG(plan != nullptr, "%s: null plan", name);
+    const int rc = check_sizes(name, plan->tokens, plan->experts, plan->top_k);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_ARG((plan->offsets != nullptr && plan->order != nullptr) || (plan->tokens == 0 && !(write && !plan->offsets)),
+             "%s: null offsets or order", name);
+    LAVA_ARG(aligned(plan->offsets, 4) && aligned(plan->order, 4) && aligned(plan->workspace, 4), "%s: misaligned plan", name);
+    if (write) {
+        const size_t need = plan_bytes(plan->tokens, plan->experts);
+        LAVA_ARG(need == 0 || (plan->workspace != nullptr && plan->workspace_bytes >= need),
+                 "%s: the plan's workspace of %zu bytes is smaller than %zu", name, plan->workspace_bytes, need);
+    }
+    return LAVA_HIP_OK;
+}
+
+}  // namespace lava
+
+using namespace lava;
+
+extern "C" {
+
+int lava_hip_moe_plan_workspace_bytes(int64_t tokens, int32_t experts, int32_t top_k, size_t* bytes) {
+    LAVA_ARG(bytes != nullptr, "moe_plan_workspace_bytes: null output pointer");
+    const int rc = check_sizes("moe_plan_workspace_bytes", tokens, experts, top_k);
+    if (rc != LAVA_HIP_OK) return rc;
+    *bytes = plan_bytes(tokens, experts);
+    return LAVA_HIP_OK;
+}
+
+int lava_hip_moe_route(const lava_hip_moe_router* router, int dtype, const void* logits, int64_t ldl, int64_t tokens,
+                       int32_t* ids, float* weights, const lava_hip_moe_plan* plan, void* stream) {
+    int rc = check_router(router);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_ARG(float_type(dtype), "moe_route: dtype %d is not f32, f16 or bf16", dtype);
+    rc = check_sizes("moe_route", tokens, router->experts, router->top_k);
+    if (rc != LAVA_HIP_OK) return rc;
+    if (plan != nullptr) {
+        rc = check_plan("moe_route", plan, true);
+        if (rc != LAVA_HIP_OK) return rc;
+        LAVA_ARG(plan->tokens == tokens && plan->experts == router->experts && plan->top_k == router->top_k,
+                 "moe_route: a plan of %lld tokens and %d of %d experts", (long long)plan->tokens, plan->top_k, plan->experts);
+    }
+    if (tokens == 0 && plan == nullptr) return LAVA_HIP_OK;
+    LAVA_ARG(tokens == 0 || (logits != nullptr && ids != nullptr && weights != nullptr), "moe_route: null pointer");
+    LAVA_ARG(ldl >= router->experts, "moe_route: ldl = %lld is smaller than the experts", (long long)ldl);
+    LAVA_ARG(aligned(logits, dtype == LAVA_HIP_F32 ? 4 : 2) && aligned(ids, 4) && aligned(weights, 4),
+             "moe_route: operands not aligned to their element size");
+    rc = lava_hip_init();
+    if (rc != LAVA_HIP_OK) return rc;
+    Router r = {router->bias, router->experts, router->top_k, router->score == LAVA_HIP_SCORE_SOFTMAX, router->groups,
+                router->top_groups, router->group_best, router->renormalize, router->scale};
+    Plan p = {};
+    if (plan != nullptr) p = plan_of(plan);
+    p.tokens = (int)tokens;
+    p.span = tokens ? span_of(tokens) : MOE_SPAN;
+    const int blocks = blocks_of(tokens);
+    hipStream_t s = as_stream(stream);
+    if (dtype == LAVA_HIP_F32) return launch_route<float>(r, logits, ldl, ids, weights, p, blocks, s);
+    if (dtype == LAVA_HIP_F16) return launch_route<f16>(r, logits, ldl, ids, weights, p, blocks, s);
+    return launch_route<bf16>(r, logits, ldl, ids, weights, p, blocks, s);
+}
+
+int lava_hip_moe_sort(const int32_t* ids, const lava_hip_moe_plan* plan, void* stream) {
+    int rc = check_plan("moe_sort", plan, true);
+    if (rc != LAVA_HIP_OK) return rc;
+    LAVA_ARG(plan->tokens == 0 || ids != nullptr, "moe_sort: null ids");
+    LAVA_ARG(aligned(ids, 4), "moe_sort: misaligned ids");
+    rc = lava_hip_init();
+    if (rc != LAVA_HIP_OK) return rc;
+    const Plan p = plan_of(plan);
+    const int blocks = blocks_of(plan->tokens);
+    hipStream_t s = as_stream(stream);
+    hipLaunchKernelGGL(moe_count_kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), blocks > 1 ? 0 : below_bytes(p.experts), s,
+                       ids, p);
+    LAVA_LAUNCH_CHECK("moe_count_kernel");
+    return blocks > 1 ? launch_place(ids, p, blocks, s) : LAVA_HIP_OK;
+}
+
+int lava_hip_moe_combine(int dtype, const void* Y, int64_t ldy, const int32_t* ids, const float* weights, int64_t tokens,
+                         int32_t top_k, int64_t n, const void* base, int64_t ldb, void* out, int64_t ldo, void* stream) {
+    LAVA_ARG(float_type(dtype), "moe_combine: dtype %d is not f32, f16 or bf16", dtype);
+    LAVA_ARG(tokens >= 0 && n >= 0 && top_k >= 0, "moe_combine: negative extent (tokens=%lld top_k=%d n=%lld)",
+             (long long)tokens, top_k, (long long)n);
+    if (tokens == 0 || n == 0) return LAVA_HIP_OK;
+    LAVA_ARG(out != nullptr && (top_k == 0 || (Y != nullptr && weights != nullptr)), "moe_combine: null pointer");
+    LAVA_ARG((top_k == 0 || ldy >= n) && ldo >= n && (base == nullptr || ldb >= n),
+             "moe_combine: a stride (%lld, %lld, %lld) is smaller than n", (long long)ldy, (long long)ldb, (long long)ldo);
+    const size_t sz = dtype == LAVA_HIP_F32 ? 4 : 2;
+    LAVA_ARG(aligned(Y, sz) && aligned(base, sz) && aligned(out, sz) && aligned(ids, 4) && aligned(weights, 4),
+             "moe_combine: operands not aligned to their element size");
+    LAVA_ARG(base != out || ldb == ldo, "moe_combine: base in place of out with another stride");
+    const int rc = lava_hip_init();
+    if (rc != LAVA_HIP_OK) return rc;
+    hipStream_t s = as_stream(stream);
+    if (dtype == LAVA_HIP_F32)
+        return launch_combine<float>(Y, ldy, ids, weights, tokens, top_k, n, base, ldb, out, ldo, s);
+    if (dtype == LAVA_HIP_F16)
+        return launch_combine<f16>(Y, ldy, ids, weights, tokens, top_k, n, base, ldb, out, ldo, s);
+    return launch_combine<bf16>(Y, ldy, ids, weights, tokens, top_k, n, base, ldb, out, ldo, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,99 @@
+// quantize.hip -- rows of values to 8 bits with a scale a row.
+//
+// q is the integer nearest to the real number 127 x / max |x|.  In 32 bits t = x * (127 / max) is off by at most 2 half
+// ulps, 127 * 2 * 2^-24 < 2e-5, so t rounds to the right integer unless it lies that near to a border between two; there
+// 254 |x| against (2 n + 1) max, products that are exact in 64 bits, decides (ties to even).
+#include <hip/hip_runtime.h>
+
+#include "gemm_common.hpp"
+#include "lava_hip_internal.hpp"
+
+namespace lava {
+
+namespace {
+
+// |x| as bits that compare like |x|; infinities and NaN are at least 0x7f800000
+__device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __noinline__ float nearest_exact(float x, float top) {
+    const double a = 254.0 * (double)fabsf(x), lo = floor(a / (2.0 * (double)top));
+    const double border = (2.0 * lo + 1.0) * (double)top;
+    // a / (2 top) may round up to the next integer: then a < 2 lo top, below the border all the same
+    const double n = a > border || (a == border && fmod(lo, 2.0) == 1.0) ? lo + 1.0 : lo;
+    return copysignf((float)n, x);
+}
+
+struct Scale {
+    float top;     // max |x|
+    float up, r;   // t = (x * up) * r: up lifts rows so small that 127 / top overflows
+    bool ok;       // finite
+};
+
+__device__ __forceinline__ Scale make_scale(uint32_t bits) {
+    Scale s;
+    s.ok = bits < 0x7f800000u;
+    s.top = __uint_as_float(bits);
+    s.up = s.top < 0x1p-100f ? 0x1p100f : 1.f;
+    s.r = s.top > 0.f && s.ok ? 127.f / (s.top * s.up) : 0.f;
+    return s;
+}
+
+__device__ __forceinline__ float nearest(float x, const Scale& s) {
+    const float t = (x * s.up) * s.r, q = rintf(t);
+    if (__builtin_expect(fabsf(t - q) > 0.4999f, 0)) return nearest_exact(x, s.top);
+    return q;
+}
+
+}  // namespace
+
+// A workgroup a row, any alignment.
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ X, int8_t* __restrict__ Q,
+                                                       float* __restrict__ scale, int64_t k, int64_t ldx, int64_t ldq) {
+    __shared__ uint32_t part[4];
+    const T* x = X + blockIdx.x * ldx;
+    int8_t* q = Q + blockIdx.x * ldq;
+    uint32_t top = 0;
+    for (int64_t j = threadIdx.x; j < k; j += 256) top = max(top, mag((float)x[j]));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = max(max(part[0], part[1]), max(part[2], part[3]));
+    const Scale s = make_scale(top);
+    if (threadIdx.x == 0) scale[blockIdx.x] = s.ok ? s.top / 127.f : __builtin_nanf("");
+    for (int64_t j = threadIdx.x; j < k; j += 256) q[j] = s.ok ? (int8_t)(int)nearest((float)x[j], s) : (int8_t)0;
+}
+
+template <typename T>
+static int launch_quantize(const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens, int64_t ldx, int64_t ldq,
+                           hipStream_t s) {
+    hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, s, static_cast<const T*>(X), Q, scale, k,
+                       ldx, ldq);
+    LAVA_LAUNCH_CHECK("quantize_kernel");
+    return LAVA_HIP_OK;
+}
+
+}  // namespace lava
+
+using namespace lava;
+
+extern "C" int lava_hip_quantize_i8(int x_dtype, const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens,
+                                    int64_t ldx, int64_t ldq, void* stream) {
+    LAVA_ARG(x_dtype == LAVA_HIP_F32 || x_dtype == LAVA_HIP_F16 || x_dtype == LAVA_HIP_BF16,
+             "quantize_i8: dtype %d is not f32, f16 or bf16", x_dtype);
+    LAVA_ARG(k >= 0 && tokens >= 0, "quantize_i8: negative extent (k=%lld tokens=%lld)", (long long)k, (long long)tokens);
+    if (tokens == 0) return LAVA_HIP_OK;
+    LAVA_ARG(scale != nullptr && (k == 0 || (X != nullptr && Q != nullptr)), "quantize_i8: null pointer");
+    LAVA_ARG(ldx >= k, "quantize_i8: ldx = %lld is smaller than k", (long long)ldx);
+    LAVA_ARG(ldq >= k, "quantize_i8: ldq = %lld is smaller than k", (long long)ldq);
+    LAVA_ARG(aligned(X, x_dtype == LAVA_HIP_F32 ? 4 : 2) && aligned(scale, 4),
+             "quantize_i8: operands not aligned to their element size");
+    LAVA_REQUIRE(tokens <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "quantize_i8: %lld tokens are too many", (long long)tokens);
+    const int rc = lava_hip_init();
+    if (rc != LAVA_HIP_OK) return rc;
+    hipStream_t s = as_stream(stream);
+    if (x_dtype == LAVA_HIP_F32) return launch_quantize<float>(X, Q, scale, k, tokens, ldx, ldq, s);
+    if (x_dtype == LAVA_HIP_F16) return launch_quantize<f16>(X, Q, scale, k, tokens, ldx, ldq, s);
+    return launch_quantize<bf16>(X, Q, scale, k, tokens, ldx, ldq, s);
+}

@@ -90,10 +90,10 @@ int check_launch(const char* kernel) {
 }
 
 // Kernel choices pinned by lava_hip_set_kernel_override, per family (0 = automatic).
-static std::atomic<int> g_override[4];
+static std::atomic<int> g_override[5];
 
 int kernel_override(int family) {
-    return family > 0 && family < 4 ? g_override[family].load(std::memory_order_relaxed) : 0;
+    return family > 0 && family < 5 ? g_override[family].load(std::memory_order_relaxed) : 0;
 }
 
 __global__ void fill_bytes_kernel(uint8_t* __restrict__ dst, uint8_t value, size_t n) {
@@ -241,7 +241,8 @@ void lava_hip_kernel_log_clear(void) { g_klaunched = 0; }
 int lava_hip_set_kernel_override(int family, int choice) {
     const bool ok = (family == LAVA_HIP_FAMILY_ATTN && (choice == 0 || choice == 3 || choice == 5)) ||
                     (family == LAVA_HIP_FAMILY_GEMM && choice >= 0 && choice <= 4) ||
-                    (family == LAVA_HIP_FAMILY_PAGED && choice >= 0 && choice <= 4);
+                    (family == LAVA_HIP_FAMILY_PAGED && choice >= 0 && choice <= 4) ||
+                    (family == LAVA_HIP_FAMILY_W8A8 && choice >= 0 && choice <= 4);
     LAVA_ARG(ok, "set_kernel_override: unknown family %d or choice %d", family, choice);
     g_override[family].store(choice, std::memory_order_relaxed);
     return LAVA_HIP_OK;

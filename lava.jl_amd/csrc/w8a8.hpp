@@ -1,0 +1,153 @@
+// w8a8.hpp -- what the kernels of layers with 8-bit weights and tokens share (internal): their arguments, the rows of a
+// tile, and the finish of a sum.
+//
+// A tile is BM rows of one expert's run (of a plain layer: of the tokens) times BN channels.  A kernel's grid holds an
+// upper bound of the row tiles -- the runs' lengths are device memory: rows / BM whole ones and one begun per expert --
+// and a workgroup finds its own by a scan of the offsets (w8_find); those behind the last end at once.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "gemm_common.hpp"
+#include "lava_hip_internal.hpp"
+
+namespace lava {
+
+struct W8Args {
+    const int8_t* x;
+    const float* xs;
+    const int8_t* w;
+    const float* ws;
+    const float* bias;
+    void* y;
+    int64_t ldx, ldw, expert_stride, ldy;
+    const int32_t* offsets;   // of a plan; null: a plain layer on rows 0 .. rows - 1
+    const int32_t* order;
+    int n;                    // channels
+    int n_out;                // columns of Y
+    int k;
+    int rows;                 // tokens, or a plan's tokens * top_k
+    int top_k, experts;
+    int act, gated, y_dtype;
+    int x_sorted, y_sorted;
+    int yvec;                 // Y takes 4 columns a store
+};
+
+struct W8Tile {
+    int expert;
+    int first;   // its first row, of the tokens or in the plan's order
+    int rows;    // 1 .. BM
+};
+
+// Row tile t of BM rows; false behind the last.  Every lane of the wavefront takes part and gets the same answer.
+__device__ __forceinline__ bool w8_find(const W8Args& a, int BM, int t, W8Tile& out) {
+    if (a.offsets == nullptr) {
+        out.expert = 0;
+        out.first = t * BM;
+        out.rows = min(BM, a.rows - out.first);
+        return out.rows > 0;
+    }
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < a.experts; e0 += 64) {
+        const int e = e0 + lane;
+        int lo = 0, hi = 0;
+        if (e < a.experts) {
+            lo = min(max(a.offsets[e], 0), a.rows);
+            hi = min(max(a.offsets[e + 1], lo), a.rows);
+        }
+        int tiles = (hi - lo + BM - 1) / BM;
+        int sum = tiles;   // of this lane's and the lower ones
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int below = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += below;
+        }
+        const uint64_t past = __ballot(sum > t);
+        if (past != 0) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            const int at = t - (__shfl(sum, l, 64) - __shfl(tiles, l, 64));   // which of the expert's tiles
+            const int s = __shfl(lo, l, 64), n = __shfl(hi, l, 64) - s;
+            out.expert = __builtin_amdgcn_readfirstlane(e0 + l);
+            out.first = __builtin_amdgcn_readfirstlane(s + at * BM);
+            out.rows = __builtin_amdgcn_readfirstlane(min(BM, n - at * BM));
+            return true;
+        }
+        t -= __shfl(sum, 63, 64);
+    }
+    return false;
+}
+
+// The rows of X and Y of row i of a tile: -1 where the plan's entry is none.
+__device__ __forceinline__ void w8_rows(const W8Args& a, const W8Tile& tile, int i, int& xr, int& yr) {
+    const int at = tile.first + i;
+    xr = yr = at;
+    if (a.offsets == nullptr) return;
+    const int slot = a.order[at];
+    const bool ok = slot >= 0 && slot < a.rows;
+    xr = !ok ? -1 : a.x_sorted ? at : slot / a.top_k;
+    yr = !ok ? -1 : a.y_sorted ? at : slot;
+}
+
+// y of a finished sum: the same operations in every kernel, so that the choice of one moves no bit.
+__device__ __forceinline__ float w8_value(int32_t sum, float xs, float ws, float bias) {
+    return __builtin_fmaf((float)sum * xs, ws, bias);
+}
+
+// The activations, each as a product of x with something between 0 and 1, without the cancellation of 1 - 1 at negative x.
+// v_exp_f32 and v_rcp_f32 are off by 1 ulp; the exponent's rounding adds |x| 2^-24.
+__device__ __forceinline__ float w8_act(int act, float x) {
+    switch (act) {
+    case LAVA_HIP_ACT_RELU: return x < 0.f ? 0.f : x;   // NaN stays
+    case LAVA_HIP_ACT_SILU: return x * __builtin_amdgcn_rcpf(1.f + epi_exp(-x));
+    case LAVA_HIP_ACT_GELU_TANH:   // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
+        return x * __builtin_amdgcn_rcpf(1.f + epi_exp(-1.5957691216057308f * __builtin_fmaf(0.044715f * x * x, x, x)));
+    case LAVA_HIP_ACT_GELU_ERF: return 0.5f * x * erfcf(x * -0.7071067811865476f);
+    default: return x;
+    }
+}
+
+// Columns col .. col + 3 of a row of Y (element offset `at` of column col), those below n_out.
+__device__ __forceinline__ void w8_store(const W8Args& a, int64_t at, int col, const float* v) {
+    const int n = min(4, a.n_out - col);
+    if (a.y_dtype == LAVA_HIP_F32) {
+        float* p = static_cast<float*>(a.y) + at;
+        if (a.yvec && n == 4) {
+            *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < n) p[r] = v[r];
+        }
+    } else if (a.y_dtype == LAVA_HIP_F16) {
+        f16* p = static_cast<f16*>(a.y) + at;
+        if (a.yvec && n == 4) {
+            *reinterpret_cast<f16x4*>(p) = f16x4{narrow<f16>(v[0]), narrow<f16>(v[1]), narrow<f16>(v[2]), narrow<f16>(v[3])};
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < n) p[r] = narrow<f16>(v[r]);
+        }
+    } else {
+        bf16* p = static_cast<bf16*>(a.y) + at;
+        if (a.yvec && n == 4) {
+            *reinterpret_cast<bf16x4*>(p) =
+                bf16x4{narrow<bf16>(v[0]), narrow<bf16>(v[1]), narrow<bf16>(v[2]), narrow<bf16>(v[3])};
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < n) p[r] = narrow<bf16>(v[r]);
+        }
+    }
+}
+
+// Row tiles of BM rows that a grid has to hold.
+inline int64_t w8_row_tiles(const W8Args& a, int BM) {
+    if (a.offsets == nullptr) return ((int64_t)a.rows + BM - 1) / BM;
+    return (int64_t)a.rows / BM + (a.experts < a.rows ? a.experts : a.rows);
+}
+
+int launch_w8_generic(const W8Args& a, hipStream_t s);
+
+// The checks of a plan (moe.hip); write: one that a call writes.
+int check_plan(const char* name, const lava_hip_moe_plan* plan, bool write);
+
+}  // namespace lava

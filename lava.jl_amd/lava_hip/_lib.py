@@ -19,7 +19,7 @@ ERR_NO_DEVICE = -4
 
 # element type codes
 F16, BF16, F32, I8, U8, I32, U32, F64 = 0, 1, 2, 3, 4, 5, 6, 7
-ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF = 0, 1, 2, 3
+ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF, ACT_SILU = 0, 1, 2, 3, 4
 
 A_ROWMAJOR, B_ROWMAJOR, C_ROWMAJOR = 1, 2, 4
 
@@ -79,6 +79,25 @@ class AttnScoreDesc(C.Structure):
     """lava_hip_attn_score."""
     _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int32), ("window", C.c_int32), ("slopes", vp),
                 ("bidirectional", vp)]
+
+
+class W8LayerDesc(C.Structure):
+    """lava_hip_w8_layer."""
+    _fields_ = [("w", vp), ("scale", vp), ("bias", vp), ("n", i64), ("k", i64), ("ldw", i64), ("expert_stride", i64),
+                ("experts", C.c_int32), ("act", C.c_int32), ("gated", C.c_int32)]
+
+
+class MoeRouterDesc(C.Structure):
+    """lava_hip_moe_router."""
+    _fields_ = [("experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32), ("groups", C.c_int32),
+                ("top_groups", C.c_int32), ("group_best", C.c_int32), ("renormalize", C.c_int32), ("scale", C.c_float),
+                ("bias", vp)]
+
+
+class MoePlanDesc(C.Structure):
+    """lava_hip_moe_plan."""
+    _fields_ = [("tokens", i64), ("experts", C.c_int32), ("top_k", C.c_int32), ("offsets", vp), ("order", vp),
+                ("workspace", vp), ("workspace_bytes", C.c_size_t)]
 
 
 # name -> (restype, argtypes)
@@ -145,6 +164,13 @@ PROTOTYPES: dict[str, tuple] = {
                                          i64, vp, vp, i64, C.POINTER(i64), C.POINTER(i64), vp, vp]),
     "lava_hip_paged_workspace_bytes": (ci, [C.POINTER(KVCacheDesc), C.POINTER(KVBatchDesc), i64, i64,
                                             C.POINTER(C.c_size_t)]),
+    "lava_hip_quantize_i8": (ci, [ci, vp, vp, vp, i64, i64, i64, i64, vp]),
+    "lava_hip_gemm_w8a8": (ci, [C.POINTER(W8LayerDesc), vp, vp, i64, i64, ci, vp, i64, vp]),
+    "lava_hip_moe_plan_workspace_bytes": (ci, [i64, C.c_int32, C.c_int32, C.POINTER(C.c_size_t)]),
+    "lava_hip_moe_route": (ci, [C.POINTER(MoeRouterDesc), ci, vp, i64, i64, vp, vp, C.POINTER(MoePlanDesc), vp]),
+    "lava_hip_moe_sort": (ci, [vp, C.POINTER(MoePlanDesc), vp]),
+    "lava_hip_experts_w8a8": (ci, [C.POINTER(MoePlanDesc), C.POINTER(W8LayerDesc), vp, vp, i64, ci, vp, i64, u32, vp]),
+    "lava_hip_moe_combine": (ci, [ci, vp, i64, vp, vp, i64, C.c_int32, i64, vp, i64, vp, i64, vp]),
     "lava_hip_release_workspaces": (ci, []),
     "lava_hip_read_stream": (ci, [vp, C.c_size_t, vp, ci, ci, vp]),
     "lava_hip_mfma_loop": (ci, [ci, vp, vp, C.c_size_t, ci, ci, ci, vp, vp]),
@@ -158,7 +184,10 @@ PROTOTYPES: dict[str, tuple] = {
 }
 
 # kernel families of lava_hip_set_kernel_override
-FAMILY_ATTN, FAMILY_GEMM, FAMILY_PAGED = 1, 2, 3
+FAMILY_ATTN, FAMILY_GEMM, FAMILY_PAGED, FAMILY_W8A8 = 1, 2, 3, 4
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+X_SORTED, Y_SORTED = 1, 2
 
 _lib: C.CDLL | None = None
 
