@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) w8a8_generic_kernel(W8Args a, int tiles_n
             v[i] = w8_act(a.act, value(j, i));
             if (a.gated) v[i] *= value(j | 1, i);
         }
-        w8_store(a, (int64_t)yr * a.ldy + cc, cc, v);
+        w8_store(a, (int64_t)yr * a.ldy + cc, a.n_out - cc, v);
     }
 }
 
@@ -139,14 +139,28 @@ int check_layer(const char* name, const lava_hip_w8_layer* l, const int8_t* X, c
     a.act = l->act;
     a.gated = l->gated != 0;
     a.y_dtype = y_dtype;
-    a.yvec = aligned(Y, 4 * ysz) && ldy % 4 == 0;
+    a.yvec = aligned(Y, 16) && ldy * (int64_t)ysz % 16 == 0;
     return LAVA_HIP_OK;
 }
 
 int run(const W8Args& a, void* stream) {
     const int rc = lava_hip_init();
     if (rc != LAVA_HIP_OK) return rc;
-    return launch_w8_generic(a, as_stream(stream));
+    hipStream_t s = as_stream(stream);
+    const int pin = kernel_override(LAVA_HIP_FAMILY_W8A8);
+    // rows of a plain layer, or on average of an expert's run
+    const int64_t rows = a.offsets ? ((int64_t)a.rows + a.experts - 1) / a.experts : a.rows;
+    if (pin == 1) return launch_w8_generic(a, s);
+    const bool stream_fits = w8_stream_fits(a), small = w8_tile_fits(a, 128), large = w8_tile_fits(a, 256);
+    if (stream_fits && (pin == 2 || (pin == 0 && rows <= 64))) return launch_w8_stream(a, (int)(rows < 64 ? rows : 64), s);
+    if (small && pin == 3) return launch_w8_tile(a, 128, s);
+    if (large && pin == 4) return launch_w8_tile(a, 256, s);
+    if (small) {
+        const int64_t cols = a.gated ? 2 * (int64_t)a.n_out : a.n_out;
+        const int64_t big = ((rows + 255) / 256) * ((cols + 255) / 256) * a.experts;
+        return launch_w8_tile(a, large && big >= 144 ? 256 : 128, s);
+    }
+    return launch_w8_generic(a, s);
 }
 
 }  // namespace

@@ -29,7 +29,7 @@ struct W8Args {
     int top_k, experts;
     int act, gated, y_dtype;
     int x_sorted, y_sorted;
-    int yvec;                 // Y takes 4 columns a store
+    int yvec;                 // Y takes 16 bytes a store
 };
 
 struct W8Tile {
@@ -105,38 +105,42 @@ __device__ __forceinline__ float w8_act(int act, float x) {
     }
 }
 
-// Columns col .. col + 3 of a row of Y (element offset `at` of column col), those below n_out.
-__device__ __forceinline__ void w8_store(const W8Args& a, int64_t at, int col, const float* v) {
-    const int n = min(4, a.n_out - col);
-    if (a.y_dtype == LAVA_HIP_F32) {
-        float* p = static_cast<float*>(a.y) + at;
-        if (a.yvec && n == 4) {
-            *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (r < n) p[r] = v[r];
-        }
-    } else if (a.y_dtype == LAVA_HIP_F16) {
-        f16* p = static_cast<f16*>(a.y) + at;
-        if (a.yvec && n == 4) {
-            *reinterpret_cast<f16x4*>(p) = f16x4{narrow<f16>(v[0]), narrow<f16>(v[1]), narrow<f16>(v[2]), narrow<f16>(v[3])};
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (r < n) p[r] = narrow<f16>(v[r]);
-        }
-    } else {
-        bf16* p = static_cast<bf16*>(a.y) + at;
-        if (a.yvec && n == 4) {
-            *reinterpret_cast<bf16x4*>(p) =
-                bf16x4{narrow<bf16>(v[0]), narrow<bf16>(v[1]), narrow<bf16>(v[2]), narrow<bf16>(v[3])};
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (r < n) p[r] = narrow<bf16>(v[r]);
-        }
+__device__ __forceinline__ void w8_act4(int act, float (&v)[4]) {
+    switch (act) {   // uniform: one branch for the four
+    case LAVA_HIP_ACT_NONE: return;
+#define LAVA_W8_ACT(A)                                            \
+    case A:                                                       \
+        _Pragma("unroll") for (int r = 0; r < 4; ++r) v[r] = w8_act(A, v[r]); \
+        return;
+        LAVA_W8_ACT(LAVA_HIP_ACT_RELU)
+        LAVA_W8_ACT(LAVA_HIP_ACT_SILU)
+        LAVA_W8_ACT(LAVA_HIP_ACT_GELU_TANH)
+        LAVA_W8_ACT(LAVA_HIP_ACT_GELU_ERF)
+#undef LAVA_W8_ACT
     }
+}
+
+// `left` columns of a row of Y, at most C (4 or 8), from element offset `at` on.
+template <typename T, int C>
+__device__ __forceinline__ void w8_put(const W8Args& a, int64_t at, int left, const float (&v)[C]) {
+    typedef T Tv __attribute__((ext_vector_type(C)));
+    T* p = static_cast<T*>(a.y) + at;
+    if (a.yvec && left >= C) {
+        Tv o;
+#pragma unroll
+        for (int r = 0; r < C; ++r) o[r] = narrow<T>(v[r]);
+        __builtin_nontemporal_store(o, reinterpret_cast<Tv*>(p));
+    } else {
+#pragma unroll
+        for (int r = 0; r < C; ++r)
+            if (r < left) p[r] = narrow<T>(v[r]);
+    }
+}
+template <int C>
+__device__ __forceinline__ void w8_store(const W8Args& a, int64_t at, int left, const float (&v)[C]) {
+    if (a.y_dtype == LAVA_HIP_F32) w8_put<float, C>(a, at, left, v);
+    else if (a.y_dtype == LAVA_HIP_F16) w8_put<f16, C>(a, at, left, v);
+    else w8_put<bf16, C>(a, at, left, v);
 }
 
 // Row tiles of BM rows that a grid has to hold.
@@ -145,7 +149,19 @@ inline int64_t w8_row_tiles(const W8Args& a, int BM) {
     return (int64_t)a.rows / BM + (a.experts < a.rows ? a.experts : a.rows);
 }
 
+// Whether X and w can be read 16 bytes at a time.
+inline bool w8_chunks_fit(const W8Args& a) {
+    return a.k % 16 == 0 && a.ldx % 16 == 0 && a.ldw % 16 == 0 && (a.experts == 1 || a.expert_stride % 16 == 0) && aligned(a.x, 16) &&
+           aligned(a.w, 16);
+}
+
 int launch_w8_generic(const W8Args& a, hipStream_t s);
+// Few rows (w8a8_stream.hip): `rows` that a tile should hold, at most 64.
+bool w8_stream_fits(const W8Args& a);
+int launch_w8_stream(const W8Args& a, int rows, hipStream_t s);
+// Tiles of BM x BM, 128 or 256 (w8a8_tile.hip).
+bool w8_tile_fits(const W8Args& a, int BM);
+int launch_w8_tile(const W8Args& a, int BM, hipStream_t s);
 
 // The checks of a plan (moe.hip); write: one that a call writes.
 int check_plan(const char* name, const lava_hip_moe_plan* plan, bool write);
