@@ -5,6 +5,8 @@
 // 254 |x| against (2 n + 1) max, products that are exact in 64 bits, decides (ties to even).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "gemm_common.hpp"
 #include "lava_hip_internal.hpp"
 
@@ -46,7 +48,84 @@ __device__ __forceinline__ float nearest(float x, const Scale& s) {
 
 }  // namespace
 
-// A workgroup a row, any alignment.
+// Rows held in registers, THREADS lanes a row, CH chunks of 8 values a lane; chunks aligned to 16 bytes (of Q to 8).
+template <typename T, int THREADS, int CH>
+__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
+    quantize_rows_kernel(const T* __restrict__ X, int8_t* __restrict__ Q, float* __restrict__ scale, int k, int tokens, int64_t ldx,
+                         int64_t ldq) {
+    constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, WAVES = THREADS / 64;
+    __shared__ uint32_t part[WAVES];
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    const int64_t row = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
+    if (row >= tokens) return;   // whole wavefronts: THREADS is a multiple of 64
+    const int t = threadIdx.x % THREADS;
+    const T* x = X + row * ldx;
+    int8_t* q = Q + row * ldq;
+    T8 v[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int at = 8 * (c * THREADS + t);
+        if (at + 8 <= k) {
+            v[c] = __builtin_nontemporal_load(reinterpret_cast<const T8*>(x + at));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] = at + i < k ? x[at + i] : (T)0.f;
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, mag((float)v[c][i]));
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) top = max(top, part[i]);
+    }
+    const Scale s = make_scale(top);
+    if (t == 0) scale[row] = s.ok ? s.top / 127.f : __builtin_nanf("");
+    const bool plain = s.up == 1.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int at = 8 * (c * THREADS + t);
+        if (at >= k) break;
+        // t + 1.5 * 2^23 has the integer nearest to t in its low bits
+        float y[8], off = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float z = (float)v[c][i] * s.r;
+            y[i] = z + 12582912.f;
+            off = fmaxf(off, fabsf(z - (y[i] - 12582912.f)));
+        }
+        if (__builtin_expect(!(plain && off <= 0.4999f), 0)) {
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+                const float n = s.ok ? nearest((float)v[c][i], s) : 0.f;
+                if (at + i < k) q[at + i] = (int8_t)(int)n;
+            }
+            continue;
+        }
+        uint32_t word[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[4 * h + 1]), __float_as_uint(y[4 * h]), 0x0c0c0400u);
+            const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(y[4 * h + 3]), __float_as_uint(y[4 * h + 2]), 0x0c0c0400u);
+            word[h] = lo | hi << 16;
+        }
+        if (at + 8 <= k) {
+            *reinterpret_cast<uint2*>(q + at) = uint2{word[0], word[1]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (at + i < k) q[at + i] = (int8_t)(word[i >> 2] >> 8 * (i & 3));
+        }
+    }
+}
+
+// A workgroup a row, any alignment and length; the row is read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ X, int8_t* __restrict__ Q,
                                                        float* __restrict__ scale, int64_t k, int64_t ldx, int64_t ldq) {
@@ -68,9 +147,34 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ X, 
 template <typename T>
 static int launch_quantize(const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens, int64_t ldx, int64_t ldq,
                            hipStream_t s) {
-    hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, s, static_cast<const T*>(X), Q, scale, k,
-                       ldx, ldq);
-    LAVA_LAUNCH_CHECK("quantize_kernel");
+    const T* x = static_cast<const T*>(X);
+    const bool chunks = aligned(X, 16) && ldx * (int64_t)sizeof(T) % 16 == 0 && aligned(Q, 8) && ldq % 8 == 0;
+    if (!chunks || k == 0 || k > 65536) {
+        hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, s, x, Q, scale, k, ldx, ldq);
+        LAVA_LAUNCH_CHECK("quantize_kernel");
+        return LAVA_HIP_OK;
+    }
+    auto go = [&](auto kernel, int threads) {
+        const int per = threads < 256 ? 256 / threads : 1;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + per - 1) / per)), dim3(threads < 256 ? 256 : threads), 0, s, x, Q, scale,
+                           (int)k, (int)tokens, ldx, ldq);
+    };
+    // a wavefront a row where there are rows for all CUs, else more lanes, fewer values each
+    const int threads = k <= 512 || (k <= 4096 && tokens >= 1024) ? 64 : k <= 16384 ? 256 : 1024;
+    const int ch = (int)((k + 8 * threads - 1) / (8 * threads));
+    auto by_ch = [&](auto ttag) {
+        constexpr int N = decltype(ttag)::value;
+        if (ch <= 1) go(quantize_rows_kernel<T, N, 1>, N);
+        else if (ch <= 2) go(quantize_rows_kernel<T, N, 2>, N);
+        else if (ch <= 3) go(quantize_rows_kernel<T, N, 3>, N);
+        else if (ch <= 4) go(quantize_rows_kernel<T, N, 4>, N);
+        else if (ch <= 6) go(quantize_rows_kernel<T, N, 6>, N);
+        else go(quantize_rows_kernel<T, N, 8>, N);
+    };
+    if (threads == 64) by_ch(std::integral_constant<int, 64>{});
+    else if (threads == 256) by_ch(std::integral_constant<int, 256>{});
+    else by_ch(std::integral_constant<int, 1024>{});
+    LAVA_LAUNCH_CHECK("quantize_rows_kernel");
     return LAVA_HIP_OK;
 }
 

@@ -43,9 +43,12 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
     struct Chunk {
         i32x4 x[4][MB], v[4][NB];
     };
+    // Rows of a power-of-two length lie on the same memory channels byte for byte: each workgroup begins at another chunk.
     const int chunks = (a.k + CHUNK - 1) / CHUNK;
+    const int turn = (tn + (tn >> 3)) % chunks;
     // 16 bytes are wholly inside K or outside (k is a multiple of 16); outside the first ones of the row are read, and X's count as zero
     auto load = [&](Chunk& c, int n) __attribute__((always_inline)) {
+        n = n + turn < chunks ? n + turn : n + turn - chunks;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const int k = n * CHUNK + 64 * s;
@@ -57,6 +60,7 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
         }
     };
     auto multiply = [&](Chunk& c, int n) __attribute__((always_inline)) {
+        n = n + turn < chunks ? n + turn : n + turn - chunks;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const bool in = n * CHUNK + 64 * s + kofs < a.k;

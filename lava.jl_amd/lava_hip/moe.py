@@ -12,7 +12,7 @@ from typing import Optional
 from . import _lib
 from .device import HIPDeviceArray
 from .kernels import _DCODE
-from .w8a8 import W8Layer, _code, _fits, _matrix, _scales
+from .w8a8 import W8Layer, _code, _cut, _fits, _matrix, _scales
 
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
 
@@ -44,7 +44,8 @@ def moe_plan_workspace_bytes(tokens: int, experts: int, top_k: int) -> int:
 
 def moe_route_raw(router: _lib.MoeRouterDesc, dtype: str, logits: int, ldl: int, tokens: int, ids: int, weights: int,
                   plan: Optional[_lib.MoePlanDesc] = None, stream: Optional[int] = None) -> None:
-    _fits(64, ldl=ldl, tokens=tokens)
+    if _cut(ldl, tokens):
+        _fits(64, ldl=ldl, tokens=tokens)
     _lib.call("lava_hip_moe_route", C.byref(router), _code(dtype), logits or None, ldl, tokens, ids or None, weights or None,
               C.byref(plan) if plan is not None else None, stream)
 
@@ -55,7 +56,8 @@ def moe_sort_raw(ids: int, plan: _lib.MoePlanDesc, stream: Optional[int] = None)
 
 def experts_w8a8_raw(plan: _lib.MoePlanDesc, layer: _lib.W8LayerDesc, X: int, x_scale: int, ldx: int, y_dtype: str, Y: int,
                      ldy: int, x_sorted: bool = False, y_sorted: bool = False, stream: Optional[int] = None) -> None:
-    _fits(64, ldx=ldx, ldy=ldy)
+    if _cut(ldx, ldy):
+        _fits(64, ldx=ldx, ldy=ldy)
     flags = (_lib.X_SORTED if x_sorted else 0) | (_lib.Y_SORTED if y_sorted else 0)
     _lib.call("lava_hip_experts_w8a8", C.byref(plan), C.byref(layer), X or None, x_scale or None, ldx, _code(y_dtype),
               Y or None, ldy, flags, stream)
@@ -63,8 +65,9 @@ def experts_w8a8_raw(plan: _lib.MoePlanDesc, layer: _lib.W8LayerDesc, X: int, x_
 
 def moe_combine_raw(dtype: str, Y: int, ldy: int, ids: int, weights: int, tokens: int, top_k: int, n: int, out: int,
                     ldo: int, base: int = 0, ldb: int = 0, stream: Optional[int] = None) -> None:
-    _fits(64, ldy=ldy, tokens=tokens, n=n, ldo=ldo, ldb=ldb)
-    _fits(32, top_k=top_k)
+    if _cut(ldy, tokens, n, ldo, ldb, top_k << 32):
+        _fits(64, ldy=ldy, tokens=tokens, n=n, ldo=ldo, ldb=ldb)
+        _fits(32, top_k=top_k)
     _lib.call("lava_hip_moe_combine", _code(dtype), Y or None, ldy, ids or None, weights or None, tokens, top_k, n,
               base or None, ldb, out or None, ldo, stream)
 

@@ -24,6 +24,15 @@ def _fits(bits: int, **values: int) -> None:
             raise ValueError(f"{name} = {x} does not fit {bits} bits")
 
 
+def _cut(*values: int) -> bool:
+    """Whether a 64-bit argument would be cut off: their bits together leave the range where one does, unless a negative one
+    hides it, which the library refuses."""
+    together = 0
+    for x in values:
+        together |= x
+    return not -2 ** 63 <= together < 2 ** 63
+
+
 def _code(dtype: str) -> int:
     if dtype not in _DCODE:
         raise _lib.Unsupported(_lib.ERR_UNSUPPORTED, f"{dtype!r} is not f32, f16 or bf16")
@@ -32,7 +41,8 @@ def _code(dtype: str) -> int:
 
 def quantize_i8_raw(dtype: str, X: int, Q: int, scale: int, k: int, tokens: int, ldx: int, ldq: int,
                     stream: Optional[int] = None) -> None:
-    _fits(64, k=k, tokens=tokens, ldx=ldx, ldq=ldq)
+    if _cut(k, tokens, ldx, ldq):
+        _fits(64, k=k, tokens=tokens, ldx=ldx, ldq=ldq)
     _lib.call("lava_hip_quantize_i8", _code(dtype), X or None, Q or None, scale or None, k, tokens, ldx, ldq, stream)
 
 
@@ -49,7 +59,8 @@ def w8_layer_raw(w: int, scale: int, n: int, k: int, ldw: int, bias: int = 0, ac
 
 def w8a8_raw(layer: _lib.W8LayerDesc, X: int, x_scale: int, tokens: int, ldx: int, y_dtype: str, Y: int, ldy: int,
              stream: Optional[int] = None) -> None:
-    _fits(64, tokens=tokens, ldx=ldx, ldy=ldy)
+    if _cut(tokens, ldx, ldy):
+        _fits(64, tokens=tokens, ldx=ldx, ldy=ldy)
     _lib.call("lava_hip_gemm_w8a8", C.byref(layer), X or None, x_scale or None, tokens, ldx, _code(y_dtype), Y or None, ldy,
               stream)
 
