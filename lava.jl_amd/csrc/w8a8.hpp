@@ -155,6 +155,14 @@ inline bool w8_chunks_fit(const W8Args& a) {
            aligned(a.w, 16);
 }
 
+// Offsets from the buffers' bases are 32-bit: the rows of a tile, or all tokens where they are gathered, and the channels of
+// a tile have to span less than 2 GiB.
+inline bool w8_spans_fit(const W8Args& a, int rows, int channels) {
+    const bool gather = a.offsets != nullptr && !a.x_sorted;
+    const int64_t lim = (int64_t)1 << 31, xrows = gather ? a.rows / a.top_k : rows;
+    return a.ldx < lim && a.ldw < lim && xrows * a.ldx < lim && channels * a.ldw < lim;
+}
+
 int launch_w8_generic(const W8Args& a, hipStream_t s);
 // Few rows (w8a8_stream.hip): `rows` that a tile should hold, at most 64.
 bool w8_stream_fits(const W8Args& a);

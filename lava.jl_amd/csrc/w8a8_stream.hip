@@ -3,16 +3,33 @@
 // A workgroup has 16 MB rows and 16 NB channels over all of K.  Its wavefronts take 256 bytes of K in turn, each lane 16 bytes
 // of a channel (and of a row of X, from L2) a load, in the MFMA operand's own layout: no LDS, no barrier until the end, and as
 // many loads in flight as registers hold.  The wavefronts' sums are added in LDS, in whole numbers, so in any order.
+#include <type_traits>
+
+#include "lds_dma.hpp"
 #include "w8a8.hpp"
 
 namespace lava {
+
+namespace {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w8_buffer(const int8_t* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p), 0, (int)bytes, 0x00020000);
+}
+// 16 bytes at voff + soff; STREAM: with the nontemporal hint, for what is read once
+template <bool STREAM>
+__device__ __forceinline__ i32x4 w8_load(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, STREAM ? 2 : 0));
+}
+}  // namespace
 
 template <int MB, int NB, int WAVES, bool GATED>
 __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int tiles_n) {
     static_assert(!GATED || NB == 2, "a gated tile is 16 channels of the gate and their 16 factors");
     constexpr int DEPTH = 16 / (MB + NB) > 4 ? 4 : 16 / (MB + NB) < 2 ? 2 : 16 / (MB + NB);   // chunks in flight
     constexpr int CHUNK = 256;
+    static_assert(WAVES >= 3, "three wavefronts fetch what the finish needs");
     __shared__ i32x4 part[WAVES][MB * NB][64];
+    __shared__ float s_ws[32], s_bias[32], s_xs[16 * MB];
+    __shared__ int s_yr[16 * MB];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tn = blockIdx.x % tiles_n;
     W8Tile tile;
@@ -21,18 +38,37 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
     const int r16 = lane & 15, kofs = 16 * (lane >> 4);
     const int col0 = tn * (GATED ? 16 : 16 * NB);
 
-    // Rows and channels that are none read the tile's first ones: their sums are not stored.
-    const int8_t *xp[MB], *wp[NB];
+    // Rows, channels and bytes of K that are none get an offset outside the buffer and read zero.
+    const bool gather = a.offsets != nullptr && !a.x_sorted;
+    const int xfirst = gather ? 0 : tile.first, xrows = gather ? a.rows / a.top_k : tile.rows;
+    const auto rx = w8_buffer(a.x + (int64_t)xfirst * a.ldx, (int64_t)(xrows - 1) * a.ldx + a.k);
+    const int cols_in = min(GATED ? 16 : 16 * NB, a.n_out - col0);
+    const int8_t* wbase = a.w + (int64_t)tile.expert * a.expert_stride + (int64_t)col0 * a.ldw;
+    const int64_t wbytes = (int64_t)(cols_in - 1) * a.ldw + a.k;
+    const auto rw = w8_buffer(wbase, wbytes), ru = w8_buffer(GATED ? wbase + (int64_t)half * a.ldw : wbase, wbytes);
+    // What the finish needs, requested first: channel row l's scale (lanes 0 ..) and bias (32 ..), row l's scale, row l of Y.
+    float held = 0.f;
+    if (w == 0) {
+        const int c = (lane & 31) < 16 * NB ? (GATED ? lane & 15 : lane & 31) : 0;
+        const int64_t ch = (int64_t)tile.expert * a.n + col0 + min(c, cols_in - 1) + (GATED && (lane & 16) ? half : 0);
+        const float* p = lane < 32 ? a.ws : a.bias;
+        if (p) held = p[ch];
+    } else if (w <= 2 && lane < tile.rows) {
+        int xr, yr;
+        w8_rows(a, tile, lane, xr, yr);
+        held = w == 2 ? __int_as_float(yr) : xr < 0 ? 0.f : a.xs[xr];
+    }
+    uint32_t xoff[MB], woff[NB];
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
-        int xr, yr;
-        w8_rows(a, tile, min(16 * i + r16, tile.rows - 1), xr, yr);
-        xp[i] = a.x + (int64_t)max(xr, 0) * a.ldx + kofs;
+        int xr = -1, yr;
+        if (16 * i + r16 < tile.rows) w8_rows(a, tile, 16 * i + r16, xr, yr);
+        xoff[i] = xr < 0 ? OOB_OFS : (uint32_t)((int64_t)(xr - xfirst) * a.ldx + kofs);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int c = min(col0 + (GATED ? 0 : 16 * j) + r16, a.n_out - 1) + (GATED && j ? half : 0);
-        wp[j] = a.w + (int64_t)tile.expert * a.expert_stride + (int64_t)c * a.ldw + kofs;
+        const int c = (GATED ? 0 : 16 * j) + r16;
+        woff[j] = c < cols_in ? (uint32_t)(c * a.ldw + kofs) : OOB_OFS;
     }
     i32x4 acc[MB][NB];
 #pragma unroll
@@ -46,87 +82,84 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
     // Rows of a power-of-two length lie on the same memory channels byte for byte: each workgroup begins at another chunk.
     const int chunks = (a.k + CHUNK - 1) / CHUNK;
     const int turn = (tn + (tn >> 3)) % chunks;
-    // 16 bytes are wholly inside K or outside (k is a multiple of 16); outside the first ones of the row are read, and X's count as zero
+    // the wavefront's chunk n; from `chunks` on none
     auto load = [&](Chunk& c, int n) __attribute__((always_inline)) {
-        n = n + turn < chunks ? n + turn : n + turn - chunks;
+        const int at = n >= chunks ? a.k : (n + turn < chunks ? n + turn : n + turn - chunks) * CHUNK;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const int k = n * CHUNK + 64 * s;
-            const int at = k + kofs < a.k ? k : -kofs;
+            const bool in = at + 64 * s + kofs < a.k;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) c.v[s][j] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp[j] + at));
+            for (int j = 0; j < NB; ++j) c.v[s][j] = w8_load<true>(GATED && j ? ru : rw, in ? woff[j] : OOB_OFS, at + 64 * s);
 #pragma unroll
-            for (int i = 0; i < MB; ++i) c.x[s][i] = *reinterpret_cast<const i32x4*>(xp[i] + at);
+            for (int i = 0; i < MB; ++i) c.x[s][i] = w8_load<false>(rx, in ? xoff[i] : OOB_OFS, at + 64 * s);
         }
     };
-    auto multiply = [&](Chunk& c, int n) __attribute__((always_inline)) {
-        n = n + turn < chunks ? n + turn : n + turn - chunks;
+    auto multiply = [&](Chunk& c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const bool in = n * CHUNK + 64 * s + kofs < a.k;
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int i = 0; i < MB; ++i) {
-                const i32x4 x = in ? c.x[s][i] : i32x4{0, 0, 0, 0};
+            for (int i = 0; i < MB; ++i)
 #pragma unroll
                 for (int j = 0; j < NB; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.v[s][j], x, acc[i][j], 0, 0, 0);
-            }
-        }
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.v[s][j], c.x[s][i], acc[i][j], 0, 0, 0);
     };
+    // No branch around a load: the compiler would wait for all that are in flight where it joins.
     Chunk ring[DEPTH];
+    const int turns = (chunks + WAVES - 1) / WAVES;   // of every wavefront
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-        if (w + d * WAVES < chunks) load(ring[d], w + d * WAVES);
-    for (int n = w; n < chunks; n += DEPTH * WAVES) {
+    for (int d = 0; d < DEPTH; ++d) load(ring[d], w + d * WAVES);
+    int n = 0;
+    for (; n + DEPTH < turns; n += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            const int at = n + d * WAVES;
-            if (at < chunks) {
-                multiply(ring[d], at);
-                if (at + DEPTH * WAVES < chunks) load(ring[d], at + DEPTH * WAVES);
-            }
+            multiply(ring[d]);
+            __builtin_amdgcn_sched_barrier(0);
+            load(ring[d], w + (n + d + DEPTH) * WAVES);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) multiply(ring[d]);
 #pragma unroll
     for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) part[w][i * NB + j][lane] = acc[i][j];
+    if (w == 0) (lane < 32 ? s_ws : s_bias)[lane & 31] = held;
+    else if (w == 1 && lane < 16 * MB) s_xs[lane] = held;
+    else if (w == 2 && lane < 16 * MB) s_yr[lane] = __float_as_int(held);
     __syncthreads();
 
     // Block b of the results (16 rows, 16 columns of Y) is finished by wavefront b % WAVES; a lane has row lane % 16, columns
     // 4 (lane / 16) and the next three.
     constexpr int OB = GATED ? MB : MB * NB;
-    const int64_t sbase = (int64_t)tile.expert * a.n;
     for (int b = w; b < OB; b += WAVES) {
         const int i = GATED ? b : b / NB, j = GATED ? 0 : b % NB;
-        const int m = 16 * i + r16, col = col0 + 16 * j + 4 * (lane >> 4);
-        if (m >= tile.rows || col >= a.n_out) continue;
-        int xr, yr;
-        w8_rows(a, tile, m, xr, yr);
-        if (yr < 0) continue;
-        const float xs = a.xs[xr];
-        auto values = [&](int blk, int64_t ch, float (&v)[4]) {
-            i32x4 s = part[0][blk][lane];
+        const int m = 16 * i + r16, c = 16 * j + 4 * (lane >> 4);
+        const int yr = m < tile.rows ? s_yr[m] : -1;
+        if (yr < 0 || c >= cols_in) continue;
+        const float xs = s_xs[m];
+        auto values = [&](int jj, float (&v)[4]) {
+            const int at = GATED ? 16 * jj + 4 * (lane >> 4) : c;
+            i32x4 s = part[0][i * NB + jj][lane];
 #pragma unroll
-            for (int z = 1; z < WAVES; ++z) s += part[z][blk][lane];
+            for (int z = 1; z < WAVES; ++z) s += part[z][i * NB + jj][lane];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (col + r < a.n_out) v[r] = w8_value(s[r], xs, a.ws[ch + r], a.bias ? a.bias[ch + r] : 0.f);
+            for (int r = 0; r < 4; ++r) v[r] = w8_value(s[r], xs, s_ws[at + r], s_bias[at + r]);
         };
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        values(i * NB + j, sbase + col, v);
+        float v[4];
+        values(j, v);
         w8_act4(a.act, v);
         if constexpr (GATED) {
-            float u[4] = {0.f, 0.f, 0.f, 0.f};
-            values(i * NB + 1, sbase + half + col, u);
+            float u[4];
+            values(1, u);
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] *= u[r];
         }
-        w8_store(a, (int64_t)yr * a.ldy + col, a.n_out - col, v);
+        w8_store(a, (int64_t)yr * a.ldy + col0 + c, cols_in - c, v);
     }
 }
 
-bool w8_stream_fits(const W8Args& a) { return a.k > 0 && w8_chunks_fit(a); }
+bool w8_stream_fits(const W8Args& a) { return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, 64, 32); }
 
 int launch_w8_stream(const W8Args& a, int rows, hipStream_t s) {
     const int MB = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;

@@ -224,13 +224,7 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
     }
 }
 
-// Offsets from the buffers' bases are 32-bit: the rows of a tile, or all tokens where they are gathered, and the channels of a
-// tile span less than 2 GiB.
-bool w8_tile_fits(const W8Args& a, int BM) {
-    const bool gather = a.offsets != nullptr && !a.x_sorted;
-    const int64_t lim = (int64_t)1 << 31, xrows = gather ? a.rows / a.top_k : BM;
-    return a.k > 0 && w8_chunks_fit(a) && xrows * a.ldx < lim && BM * a.ldw < lim;
-}
+bool w8_tile_fits(const W8Args& a, int BM) { return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, BM, BM); }
 
 int launch_w8_tile(const W8Args& a, int BM, hipStream_t s) {
     const int cols = a.gated ? BM / 2 : BM;
