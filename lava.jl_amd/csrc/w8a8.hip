@@ -153,6 +153,7 @@ int run(const W8Args& a, void* stream) {
     if (pin == 1) return launch_w8_generic(a, s);
     const bool stream_fits = w8_stream_fits(a), small = w8_tile_fits(a, 128), large = w8_tile_fits(a, 256);
     if (stream_fits && (pin == 2 || (pin == 0 && rows <= 64))) return launch_w8_stream(a, (int)(rows < 64 ? rows : 64), s);
+    if (pin >= 16 && w8_mid_fits(a)) return launch_w8_mid(a, pin / 16, pin % 16, s);
     if (small && pin == 3) return launch_w8_tile(a, 128, s);
     if (large && pin == 4) return launch_w8_tile(a, 256, s);
     if (small) {

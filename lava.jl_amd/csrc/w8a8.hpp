@@ -143,6 +143,46 @@ __device__ __forceinline__ void w8_store(const W8Args& a, int64_t at, int left, 
     else w8_put<bf16, C>(a, at, left, v);
 }
 
+// 8 columns of a row of Y from their sums (of a gated layer the gates' and, 16 places on, the factors').
+template <bool GATED>
+__device__ __forceinline__ void w8_finish8(int act, const i32x4* sums, float xs, const f32x4* ws, const f32x4* bs, float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const i32x4 g = sums[h];
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = w8_value(g[r], xs, ws[h][r], bs[h][r]);
+        w8_act4(act, o);
+        if constexpr (GATED) {
+            const i32x4 u = sums[4 + h];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] *= w8_value(u[r], xs, ws[2 + h][r], bs[2 + h][r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[4 * h + r] = o[r];
+    }
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w8_buffer(const int8_t* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p), 0, (int)bytes, 0x00020000);
+}
+// 16 bytes at voff + soff; STREAM: with the nontemporal hint, for what is read once
+template <bool STREAM>
+__device__ __forceinline__ i32x4 w8_load(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
+    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, STREAM ? 2 : 0));
+}
+
+// lo and hi: whole 128-byte lines of K of 8 channels each, lane l channel l % 8, bytes 16 (l / 8).  An MFMA's lane l has
+// channel l % 16 and 16 bytes of K, whichever they are, as X's lanes have the same: here those at 32 (l / 16) in v0 and the next
+// 16 in v1, for which lanes 8 .. 15 of each 16 of lo change places with 0 .. 7 of hi.
+__device__ __forceinline__ void w8_whole_lines(const i32x4& lo, const i32x4& hi, i32x4& v0, i32x4& v1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        v0[r] = __builtin_amdgcn_update_dpp(lo[r], hi[r], 0x128, 0xf, 0xc, false);   // row_ror:8 into lanes 8 .. 15
+        v1[r] = __builtin_amdgcn_update_dpp(hi[r], lo[r], 0x128, 0xf, 0x3, false);
+    }
+}
+
 // Row tiles of BM rows that a grid has to hold.
 inline int64_t w8_row_tiles(const W8Args& a, int BM) {
     if (a.offsets == nullptr) return ((int64_t)a.rows + BM - 1) / BM;
@@ -167,6 +207,9 @@ int launch_w8_generic(const W8Args& a, hipStream_t s);
 // Few rows (w8a8_stream.hip): `rows` that a tile should hold, at most 64.
 bool w8_stream_fits(const W8Args& a);
 int launch_w8_stream(const W8Args& a, int rows, hipStream_t s);
+// 16 MB rows (MB 2, 4 or 8) x 64 NB channels (NB 1, 2 or 4; w8a8_mid.hip).
+bool w8_mid_fits(const W8Args& a);
+int launch_w8_mid(const W8Args& a, int MB, int NB, hipStream_t s);
 // Tiles of BM x BM, 128 or 256 (w8a8_tile.hip).
 bool w8_tile_fits(const W8Args& a, int BM);
 int launch_w8_tile(const W8Args& a, int BM, hipStream_t s);

@@ -1,7 +1,7 @@
 // w8a8_stream.hip -- layers with 8-bit weights on few tokens: bound by reading the weights once.
 //
-// A workgroup has 16 MB rows and 16 NB channels over all of K.  Its wavefronts take 256 bytes of K in turn, each lane 16 bytes
-// of a channel (and of a row of X, from L2) a load, in the MFMA operand's own layout: no LDS, no barrier until the end, and as
+// A workgroup has 16 MB rows and 16 NB channels over all of K.  Its wavefronts take 256 bytes of K in turn, whole lines of 8
+// channels a load (and rows of X, from L2), straight to the MFMA operand's registers: no LDS, no barrier until the end, and as
 // many loads in flight as registers hold.  The wavefronts' sums are added in LDS, in whole numbers, so in any order.
 #include <type_traits>
 
@@ -9,17 +9,6 @@
 #include "w8a8.hpp"
 
 namespace lava {
-
-namespace {
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t w8_buffer(const int8_t* p, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t*>(p), 0, (int)bytes, 0x00020000);
-}
-// 16 bytes at voff + soff; STREAM: with the nontemporal hint, for what is read once
-template <bool STREAM>
-__device__ __forceinline__ i32x4 w8_load(__amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
-    return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, STREAM ? 2 : 0));
-}
-}  // namespace
 
 template <int MB, int NB, int WAVES, bool GATED>
 __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int tiles_n) {
@@ -35,7 +24,7 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
     W8Tile tile;
     if (!w8_find(a, 16 * MB, blockIdx.x / tiles_n, tile)) return;
     const int half = a.n >> 1;
-    const int r16 = lane & 15, kofs = 16 * (lane >> 4);
+    const int r16 = lane & 15;
     const int col0 = tn * (GATED ? 16 : 16 * NB);
 
     // Rows, channels and bytes of K that are none get an offset outside the buffer and read zero.
@@ -58,17 +47,20 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
         w8_rows(a, tile, lane, xr, yr);
         held = w == 2 ? __int_as_float(yr) : xr < 0 ? 0.f : a.xs[xr];
     }
-    uint32_t xoff[MB], woff[NB];
+    uint32_t xoff[MB], woff[NB][2];
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
         int xr = -1, yr;
         if (16 * i + r16 < tile.rows) w8_rows(a, tile, 16 * i + r16, xr, yr);
-        xoff[i] = xr < 0 ? OOB_OFS : (uint32_t)((int64_t)(xr - xfirst) * a.ldx + kofs);
+        xoff[i] = xr < 0 ? OOB_OFS : (uint32_t)((int64_t)(xr - xfirst) * a.ldx + 32 * (lane >> 4));
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int c = (GATED ? 0 : 16 * j) + r16;
-        woff[j] = c < cols_in ? (uint32_t)(c * a.ldw + kofs) : OOB_OFS;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int c = (GATED ? 0 : 16 * j) + 8 * h + (lane & 7);
+            woff[j][h] = c < cols_in ? (uint32_t)(c * a.ldw + 16 * (lane >> 3)) : OOB_OFS;
+        }
     }
     i32x4 acc[MB][NB];
 #pragma unroll
@@ -76,8 +68,10 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
 #pragma unroll
         for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
 
+    // Two pieces of 128 bytes of K: of a block of channels, v[p][j][0] is the first 8 channels' whole lines, lane l channel l % 8,
+    // bytes 16 (l / 8); v[p][j][1] the other 8's.
     struct Chunk {
-        i32x4 x[4][MB], v[4][NB];
+        i32x4 x[2][MB][2], v[2][NB][2];
     };
     // Rows of a power-of-two length lie on the same memory channels byte for byte: each workgroup begins at another chunk.
     const int chunks = (a.k + CHUNK - 1) / CHUNK;
@@ -86,22 +80,34 @@ __global__ void __launch_bounds__(64 * WAVES) w8a8_stream_kernel(W8Args a, int t
     auto load = [&](Chunk& c, int n) __attribute__((always_inline)) {
         const int at = n >= chunks ? a.k : (n + turn < chunks ? n + turn : n + turn - chunks) * CHUNK;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const bool in = at + 64 * s + kofs < a.k;
+        for (int p = 0; p < 2; ++p) {
+            const int k = at + 128 * p;
+            const bool in = k + 16 * (lane >> 3) < a.k;
 #pragma unroll
-            for (int j = 0; j < NB; ++j) c.v[s][j] = w8_load<true>(GATED && j ? ru : rw, in ? woff[j] : OOB_OFS, at + 64 * s);
+            for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int i = 0; i < MB; ++i) c.x[s][i] = w8_load<false>(rx, in ? xoff[i] : OOB_OFS, at + 64 * s);
+                for (int h = 0; h < 2; ++h) c.v[p][j][h] = w8_load<true>(GATED && j ? ru : rw, in ? woff[j][h] : OOB_OFS, k);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool xin = k + 32 * (lane >> 4) + 16 * h < a.k;
+#pragma unroll
+                for (int i = 0; i < MB; ++i) c.x[p][i][h] = w8_load<false>(rx, xin ? xoff[i] : OOB_OFS, k + 16 * h);
+            }
         }
     };
     auto multiply = [&](Chunk& c) __attribute__((always_inline)) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
-            for (int i = 0; i < MB; ++i)
+            for (int j = 0; j < NB; ++j) {
+                i32x4 v0, v1;
+                w8_whole_lines(c.v[p][j][0], c.v[p][j][1], v0, v1);
 #pragma unroll
-                for (int j = 0; j < NB; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(c.v[s][j], c.x[s][i], acc[i][j], 0, 0, 0);
+                for (int i = 0; i < MB; ++i) {
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v0, c.x[p][i][0], acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v1, c.x[p][i][1], acc[i][j], 0, 0, 0);
+                }
+            }
     };
     // No branch around a load: the compiler would wait for all that are in flight where it joins.
     Chunk ring[DEPTH];

@@ -15,11 +15,11 @@
 
 namespace lava {
 
-template <int WM, int WN, bool GATED>
-__global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
+template <int WM, int WN, int ST, bool GATED>
+__global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
     constexpr int BM = 32 * WM, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
     constexpr int Q = WM * WN, R = WM + WN;   // MFMAs of half a stage, and fragments read (and requests made) beside them
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * STAGE];
     __shared__ float s_xs[BM], s_ws[BN], s_bias[BN];
     __shared__ int s_xr[BM], s_yr[BM];
 
@@ -119,13 +119,13 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
         }
     };
 
-    if (ktiles == 1) cut_k();
 #pragma unroll
-    for (int q = 0; q < R; ++q) dma(q, 0, 0);
-    if (ktiles == 2) cut_k();
+    for (int t = 0; t < ST; ++t) {
+        if (t + 1 == ktiles) cut_k();
 #pragma unroll
-    for (int q = 0; q < R; ++q) dma(q, 1, ktiles > 1 ? (uint32_t)TN_KB : 0u);
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(R) : "memory");
+        for (int q = 0; q < R; ++q) dma(q, t, (uint32_t)min(t, ktiles - 1) * TN_KB);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * R) : "memory");
     __syncthreads();
     Frag fa, fb;
 #pragma unroll
@@ -133,11 +133,12 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
         read(fa, smem, 0, t);
         __builtin_amdgcn_sched_barrier(0);
     }
+    int st = 0;
     for (int kt = 0; kt < ktiles; ++kt) {
-        const int st = kt & 1;
-        const uint8_t *base = smem + st * STAGE, *next = smem + (st ^ 1) * STAGE;
-        const uint32_t kofs2 = (uint32_t)min(kt + 2, ktiles - 1) * TN_KB;
-        if (kt + 3 == ktiles) cut_k();
+        const int st1 = ST == 2 ? st ^ 1 : st + 1 == ST ? 0 : st + 1;
+        const uint8_t *base = smem + st * STAGE, *next = smem + st1 * STAGE;
+        const uint32_t kofs2 = (uint32_t)min(kt + ST, ktiles - 1) * TN_KB;
+        if (kt + ST + 1 == ktiles) cut_k();
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             acc[q / WN][q % WN] = Mfma16<int8_t>::run(fa.v[q % WN], fa.x[q / WN], acc[q / WN][q % WN]);
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
             for (int t = q * R / Q; t < (q + 1) * R / Q; ++t) read(fb, base, 1, t);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's part of the next stage landed
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * R) : "memory");   // this wavefront's part of the next stage landed
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -158,6 +159,7 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        st = st1;
     }
 
     // ---- finish: acc[i][j][r] is row 16 WM wm + 16 i + lane % 16, channel row 16 WN wn + 16 j + 4 (lane / 16) + r.  A wavefront
@@ -167,7 +169,7 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
     __syncthreads();
     constexpr int COLS = GATED ? 8 * WN : 16 * WN;         // of Y, a wavefront's
     constexpr int PITCH = 16 * WN * 4 + 16;                // padded: the 16 rows of a store start on distinct banks
-    static_assert(4 * 32 * PITCH <= 2 * STAGE, "four wavefronts' rows in the stages' LDS");
+    static_assert(4 * 32 * PITCH <= ST * STAGE, "four wavefronts' rows in the stages' LDS");
     constexpr int LANES = COLS / 8, ROWS = 64 / LANES;     // lanes a row, rows a pass
     uint8_t* ep = smem + w * 32 * PITCH;
     const int cc = (lane % LANES) * 8;                     // this lane's first column of the wavefront's
@@ -194,23 +196,8 @@ __global__ void __launch_bounds__(256, WM * WN > 16 ? 1 : 2) w8a8_tile_kernel(W8
             const int row = t * ROWS + lane / LANES, at = wm * 16 * WM + 16 * i0 + row;
             const float xs = s_xs[at];
             const int yr = s_yr[at];
-            const i32x4* sums = reinterpret_cast<const i32x4*>(ep + row * PITCH + cr * 4);
             float v[8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const i32x4 g = sums[h];
-                float o[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[r] = w8_value(g[r], xs, ws[h][r], bs[h][r]);
-                w8_act4(a.act, o);
-                if constexpr (GATED) {
-                    const i32x4 u = sums[4 + h];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] *= w8_value(u[r], xs, ws[2 + h][r], bs[2 + h][r]);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[4 * h + r] = o[r];
-            }
+            w8_finish8<GATED>(a.act, reinterpret_cast<const i32x4*>(ep + row * PITCH + cr * 4), xs, ws, bs, v);
             if (yr >= 0 && left > 0) w8_store(a, (int64_t)yr * a.ldy + col0 + wn * COLS + cc, left, v);
         }
         __builtin_amdgcn_s_waitcnt(0xc07f);   // read before the next rows overwrite them
@@ -233,10 +220,10 @@ int launch_w8_tile(const W8Args& a, int BM, hipStream_t s) {
     const dim3 grid((unsigned)(tm * tn));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, (int)tm, (int)tn); };
     if (BM == 256) {
-        a.gated ? go(w8a8_tile_kernel<8, 8, true>) : go(w8a8_tile_kernel<8, 8, false>);
+        a.gated ? go(w8a8_tile_kernel<8, 8, 2, true>) : go(w8a8_tile_kernel<8, 8, 2, false>);
         LAVA_LAUNCH_CHECK("w8a8_tile_kernel<256>");
     } else {
-        a.gated ? go(w8a8_tile_kernel<4, 4, true>) : go(w8a8_tile_kernel<4, 4, false>);
+        a.gated ? go(w8a8_tile_kernel<4, 4, 4, true>) : go(w8a8_tile_kernel<4, 4, 4, false>);
         LAVA_LAUNCH_CHECK("w8a8_tile_kernel<128>");
     }
     return LAVA_HIP_OK;
