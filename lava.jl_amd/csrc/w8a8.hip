@@ -148,20 +148,10 @@ int run(const W8Args& a, void* stream) {
     if (rc != LAVA_HIP_OK) return rc;
     hipStream_t s = as_stream(stream);
     const int pin = kernel_override(LAVA_HIP_FAMILY_W8A8);
-    // rows of a plain layer, or on average of an expert's run
-    const int64_t rows = a.offsets ? ((int64_t)a.rows + a.experts - 1) / a.experts : a.rows;
     if (pin == 1) return launch_w8_generic(a, s);
-    const bool stream_fits = w8_stream_fits(a), small = w8_tile_fits(a, 128), large = w8_tile_fits(a, 256);
-    if (stream_fits && (pin == 2 || (pin == 0 && rows <= 64))) return launch_w8_stream(a, (int)(rows < 64 ? rows : 64), s);
-    if (pin >= 16 && w8_mid_fits(a)) return launch_w8_mid(a, pin / 16, pin % 16, s);
-    if (small && pin == 3) return launch_w8_tile(a, 128, s);
-    if (large && pin == 4) return launch_w8_tile(a, 256, s);
-    if (small) {
-        const int64_t cols = a.gated ? 2 * (int64_t)a.n_out : a.n_out;
-        const int64_t big = ((rows + 255) / 256) * ((cols + 255) / 256) * a.experts;
-        return launch_w8_tile(a, large && big >= 144 ? 256 : 128, s);
-    }
-    return launch_w8_generic(a, s);
+    if (w8_stream_fits(a) && (pin == 2 || (pin == 0 && w8_stream_preferred(a)))) return launch_w8_stream(a, s);
+    const int tile = pin >= 3 && w8_tile_fits(a, pin - 3) ? pin - 3 : w8_tile_choice(a);
+    return tile >= 0 ? launch_w8_tile(a, tile, s) : launch_w8_generic(a, s);
 }
 
 }  // namespace

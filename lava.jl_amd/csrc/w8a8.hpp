@@ -38,6 +38,17 @@ struct W8Tile {
     int rows;    // 1 .. BM
 };
 
+// Of lane l: the sum of v over lanes 0 .. l.
+__device__ __forceinline__ int wave_sums(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1, 2, 4, 8: within 16 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15: lane 15's to 16 .. 31, 47's to 48 .. 63
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31: lane 31's to 32 .. 63
+    return v;
+}
+
 // Row tile t of BM rows; false behind the last.  Every lane of the wavefront takes part and gets the same answer.
 __device__ __forceinline__ bool w8_find(const W8Args& a, int BM, int t, W8Tile& out) {
     if (a.offsets == nullptr) {
@@ -48,30 +59,20 @@ __device__ __forceinline__ bool w8_find(const W8Args& a, int BM, int t, W8Tile& 
     }
     const int lane = threadIdx.x & 63;
     for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int e = e0 + lane;
-        int lo = 0, hi = 0;
-        if (e < a.experts) {
-            lo = min(max(a.offsets[e], 0), a.rows);
-            hi = min(max(a.offsets[e + 1], lo), a.rows);
-        }
-        int tiles = (hi - lo + BM - 1) / BM;
-        int sum = tiles;   // of this lane's and the lower ones
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int below = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += below;
-        }
+        const int e = min(e0 + lane, a.experts);
+        const int lo = min(max(a.offsets[e], 0), a.rows), hi = min(max(a.offsets[min(e + 1, a.experts)], lo), a.rows);
+        const int tiles = (hi - lo + BM - 1) / BM, sum = wave_sums(tiles);
         const uint64_t past = __ballot(sum > t);
         if (past != 0) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            const int at = t - (__shfl(sum, l, 64) - __shfl(tiles, l, 64));   // which of the expert's tiles
-            const int s = __shfl(lo, l, 64), n = __shfl(hi, l, 64) - s;
-            out.expert = __builtin_amdgcn_readfirstlane(e0 + l);
-            out.first = __builtin_amdgcn_readfirstlane(s + at * BM);
-            out.rows = __builtin_amdgcn_readfirstlane(min(BM, n - at * BM));
+            const int at = t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(tiles, l));   // which of the expert's tiles
+            const int s = __builtin_amdgcn_readlane(lo, l), n = __builtin_amdgcn_readlane(hi, l) - s;
+            out.expert = e0 + l;
+            out.first = s + at * BM;
+            out.rows = min(BM, n - at * BM);
             return true;
         }
-        t -= __shfl(sum, 63, 64);
+        t -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
 }
@@ -204,15 +205,17 @@ inline bool w8_spans_fit(const W8Args& a, int rows, int channels) {
 }
 
 int launch_w8_generic(const W8Args& a, hipStream_t s);
-// Few rows (w8a8_stream.hip): `rows` that a tile should hold, at most 64.
+// Few rows (w8a8_stream.hip).
 bool w8_stream_fits(const W8Args& a);
-int launch_w8_stream(const W8Args& a, int rows, hipStream_t s);
-// 16 MB rows (MB 2, 4 or 8) x 64 NB channels (NB 1, 2 or 4; w8a8_mid.hip).
-bool w8_mid_fits(const W8Args& a);
-int launch_w8_mid(const W8Args& a, int MB, int NB, hipStream_t s);
-// Tiles of BM x BM, 128 or 256 (w8a8_tile.hip).
-bool w8_tile_fits(const W8Args& a, int BM);
-int launch_w8_tile(const W8Args& a, int BM, hipStream_t s);
+bool w8_stream_preferred(const W8Args& a);
+int launch_w8_stream(const W8Args& a, hipStream_t s);
+// Tiles (w8a8_tile.hip): 0 to 3 for 64 x 64, 64 x 128, 128 x 128 and 256 x 256 rows and channels; the one to take, -1 if none fits;
+// how many a call has (of a plan: is likely to have); the experts that are likely to have rows (w8_met).
+bool w8_tile_fits(const W8Args& a, int tile);
+int w8_tile_choice(const W8Args& a);
+double w8_tile_count(const W8Args& a, int bm, int bn);
+double w8_met(const W8Args& a);
+int launch_w8_tile(const W8Args& a, int tile, hipStream_t s);
 
 // The checks of a plan (moe.hip); write: one that a call writes.
 int check_plan(const char* name, const lava_hip_moe_plan* plan, bool write);

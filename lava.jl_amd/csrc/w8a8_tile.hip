@@ -1,27 +1,32 @@
-// w8a8_tile.hip -- layers with 8-bit weights and tokens on 256 x 256 or 128 x 128 tiles (rows x channels).
+// w8a8_tile.hip -- layers with 8-bit weights and tokens on tiles of 64 x 64 to 256 x 256 (rows x channels).
 //
 // The loop is the tile GEMM's (gemm_tn_kernel.hpp): 4 wavefronts, each 16 WM rows x 16 WN channels in 16x16x64 MFMAs; K 128
 // bytes at a time, both operands' slices straight to LDS (buffer_load ... lds, 16-byte chunk c of row r at slot c ^ r % 8, so
-// that a fragment's 16 rows lie on all banks), two stages, one barrier in the middle of a stage: the MFMAs of its first half
-// run while the second half's fragments are read, those of the second half while the next stage's are read and the stage
-// after it is requested.  What differs:
+// that a fragment's 16 rows lie on all banks), ST stages, one barrier in the middle of a stage: the MFMAs of its first half
+// run while the second half's fragments are read, those of the second half while the next stage's are read and the one ST
+// further on is requested.  What differs:
 //  * a row of X is found by the plan, so a lane keeps one offset for each of its requests (rows and channels that are none,
 //    and chunks past K, get an offset outside the buffer and read zero);
 //  * a gated layer's tile has 16 channels of the gate and their 16 factors in turn, so that a lane has both of a column in its
 //    accumulators;
 //  * the sums go through LDS to lanes that have 8 columns of a row, which they finish, round to Y's type and store.
+#include <math.h>
+
 #include "gemm_tn_kernel.hpp"
 #include "w8a8.hpp"
 
 namespace lava {
 
 template <int WM, int WN, int ST, bool GATED>
-__global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
     constexpr int BM = 32 * WM, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
-    constexpr int Q = WM * WN, R = WM + WN;   // MFMAs of half a stage, and fragments read (and requests made) beside them
+    constexpr int Q = WM * WN, R = WM + WN;               // of a wavefront: MFMAs of half a stage, fragments read beside them
+    constexpr int XD = WM, D = R;                         // and its requests of a stage, those for X first
+    static_assert(WM % 2 == 0 && (!GATED || WN % 2 == 0), "rows are finished 32 at a time, gates and factors are blocks of 16");
+    static_assert(WN == 2 || WN == 4 || WN == 8, "a power of two of lanes finishes a row");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * STAGE];
     __shared__ float s_xs[BM], s_ws[BN], s_bias[BN];
-    __shared__ int s_xr[BM], s_yr[BM];
+    __shared__ int s_yr[BM];
 
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int tm, tn;
@@ -32,20 +37,24 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
     const int half = a.n >> 1;
     const int col0 = tn * (GATED ? BN / 2 : BN);   // first column of Y
 
-    for (int i = threadIdx.x; i < BM; i += 256) {
-        int xr = -1, yr = -1;
-        if (i < tile.rows) w8_rows(a, tile, i, xr, yr);
-        s_xr[i] = xr;
-        s_yr[i] = yr;
-        s_xs[i] = xr < 0 ? 0.f : a.xs[xr];
+    // What the finish needs, requested first and held until then: of row threadIdx.x its scale and row of Y, of channel row
+    // threadIdx.x its scale and bias.
+    static_assert(BM <= 256 && BN <= 256, "a row and a channel a thread");
+    float held_xs = 0.f, held_ws = 0.f, held_bias = 0.f;
+    int held_yr = -1;
+    if (threadIdx.x < (unsigned)tile.rows) {
+        int xr;
+        w8_rows(a, tile, threadIdx.x, xr, held_yr);
+        if (xr >= 0) held_xs = a.xs[xr];
     }
-    for (int i = threadIdx.x; i < BN; i += 256) {
-        const int c = col0 + (GATED ? (i >> 5) * 16 + (i & 15) : i);
+    if (threadIdx.x < BN) {
+        const int i = threadIdx.x, c = col0 + (GATED ? (i >> 5) * 16 + (i & 15) : i);
         const int64_t ch = (int64_t)tile.expert * a.n + (GATED && (i & 16) ? half + c : c);
-        s_ws[i] = c < a.n_out ? a.ws[ch] : 0.f;
-        s_bias[i] = c < a.n_out && a.bias ? a.bias[ch] : 0.f;
+        if (c < a.n_out) {
+            held_ws = a.ws[ch];
+            if (a.bias) held_bias = a.bias[ch];
+        }
     }
-    __syncthreads();
 
     // X: rows of the tokens by offsets from the first of all, or rows of the tile by offsets from its own first
     const bool gather = a.offsets != nullptr && !a.x_sorted;
@@ -59,40 +68,42 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
     const v4i ru = make_rsrc(GATED ? wbase + (int64_t)half * a.ldw : wbase, wbytes);
     // a request covers 8 rows: lane l row l / 8, slot l % 8, which holds chunk slot ^ row % 8
     const int lr = lane >> 3, chunk = 16 * ((lane & 7) ^ lr);
-    uint32_t xoff[WM], woff[WN], wsoff[WN];
+    uint32_t xoff[XD], woff[D - XD], wsoff[D - XD];
 #pragma unroll
-    for (int i = 0; i < WM; ++i) {
-        const int xr = s_xr[8 * WM * w + 8 * i + lr];
+    for (int i = 0; i < XD; ++i) {
+        const int r = 8 * XD * w + 8 * i + lr;
+        int xr = -1, yr;
+        if (r < tile.rows) w8_rows(a, tile, r, xr, yr);
         xoff[i] = xr < 0 ? OOB_OFS : (uint32_t)((int64_t)(xr - xfirst) * a.ldx + chunk);
     }
 #pragma unroll
-    for (int i = 0; i < WN; ++i) {
-        const int r = 8 * WN * w + 8 * i;
+    for (int i = 0; i < D - XD; ++i) {
+        const int r = 8 * (D - XD) * w + 8 * i;
         const int c = GATED ? (r >> 5) * 16 + (r & 8) : r;
         wsoff[i] = (uint32_t)(c * a.ldw);
         woff[i] = c + lr < cols_in ? (uint32_t)(lr * a.ldw + chunk) : OOB_OFS;
     }
-    const uint32_t lds_x = lds_addr(smem) + w * 8 * WM * TN_KB, lds_w = lds_addr(smem) + XS + w * 8 * WN * TN_KB;
+    const uint32_t lds_x = lds_addr(smem) + w * XD * 1024, lds_w = lds_addr(smem) + XS + w * (D - XD) * 1024;
 
-    // request q (of WM for X and WN for W) of the stage at byte kofs of K
+    // request q of the stage at byte kofs of K
     auto dma = [&](int q, int stage, uint32_t kofs) __attribute__((always_inline)) {
-        if (q < WM) {
+        if (q < XD) {
             dma16(rx, xoff[q], kofs, lds_x + stage * STAGE + q * 1024);
         } else {
-            const int i = q - WM;
-            const bool up = GATED && ((i >> 1) & 1);   // 8 WN w + 8 i is in a block of factors (WN a multiple of 4)
+            const int i = q - XD;
+            const bool up = GATED && ((8 * (D - XD) * w + 8 * i) & 16);   // a block of factors; uniform
             dma16(up ? ru : rw, woff[i], wsoff[i] + kofs, lds_w + stage * STAGE + i * 1024);
         }
     };
-    // Before the last stage's requests: chunks past K get an offset that reads zero (once, in the kept offsets: a choice at
-    // every request costs the compiler the accumulators' places, 1185 against 9xx us for 8192 gated rows).
+    // Before the last stage's requests: chunks past K get an offset that reads zero (once, in the kept offsets: a
+    // choice at every request costs the compiler the accumulators' places, 8192 gated rows 1183 us against 780).
     const int ktiles = (a.k + TN_KB - 1) / TN_KB;
     auto cut_k = [&]() __attribute__((always_inline)) {
         const bool in = (ktiles - 1) * TN_KB + chunk < a.k;
 #pragma unroll
-        for (int i = 0; i < WM; ++i) xoff[i] = in ? xoff[i] : OOB_OFS;
+        for (int i = 0; i < XD; ++i) xoff[i] = in ? xoff[i] : OOB_OFS;
 #pragma unroll
-        for (int i = 0; i < WN; ++i) woff[i] = in ? woff[i] : OOB_OFS;
+        for (int i = 0; i < D - XD; ++i) woff[i] = in ? woff[i] : OOB_OFS;
     };
 
     i32x4 acc[WM][WN];
@@ -123,9 +134,9 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
     for (int t = 0; t < ST; ++t) {
         if (t + 1 == ktiles) cut_k();
 #pragma unroll
-        for (int q = 0; q < R; ++q) dma(q, t, (uint32_t)min(t, ktiles - 1) * TN_KB);
+        for (int q = 0; q < D; ++q) dma(q, t, (uint32_t)min(t, ktiles - 1) * TN_KB);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * R) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 1) * D) : "memory");
     __syncthreads();
     Frag fa, fb;
 #pragma unroll
@@ -146,17 +157,16 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
             for (int t = q * R / Q; t < (q + 1) * R / Q; ++t) read(fb, base, 1, t);
             __builtin_amdgcn_sched_barrier(0);
         }
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * R) : "memory");   // this wavefront's part of the next stage landed
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((ST - 2) * D) : "memory");   // this wavefront's part of the next stage landed
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < Q; ++q) {
             acc[q / WN][q % WN] = Mfma16<int8_t>::run(fb.v[q % WN], fb.x[q / WN], acc[q / WN][q % WN]);
 #pragma unroll
-            for (int t = q * R / Q; t < (q + 1) * R / Q; ++t) {
-                read(fa, next, 0, t);
-                dma(t, st, kofs2);
-            }
+            for (int t = q * R / Q; t < (q + 1) * R / Q; ++t) read(fa, next, 0, t);
+#pragma unroll
+            for (int t = q * D / Q; t < (q + 1) * D / Q; ++t) dma(t, st, kofs2);
             __builtin_amdgcn_sched_barrier(0);
         }
         st = st1;
@@ -166,6 +176,14 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
     // stages the sums of 32 rows at a time in LDS of its own and reads them back by rows, a lane 8 columns of Y (of a gated layer
     // their 8 gates and 8 factors), which it finishes and stores.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (threadIdx.x < BM) {
+        s_xs[threadIdx.x] = held_xs;
+        s_yr[threadIdx.x] = held_yr;
+    }
+    if (threadIdx.x < BN) {
+        s_ws[threadIdx.x] = held_ws;
+        s_bias[threadIdx.x] = held_bias;
+    }
     __syncthreads();
     constexpr int COLS = GATED ? 8 * WN : 16 * WN;         // of Y, a wavefront's
     constexpr int PITCH = 16 * WN * 4 + 16;                // padded: the 16 rows of a store start on distinct banks
@@ -191,7 +209,7 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
                 *reinterpret_cast<i32x4*>(ep + (16 * ii + (lane & 15)) * PITCH + (16 * j + 4 * (lane >> 4)) * 4) = acc[i0 + ii][j];
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the wavefront's sums are in LDS
         __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
+#pragma unroll 2
         for (int t = 0; t < 32 / ROWS; ++t) {
             const int row = t * ROWS + lane / LANES, at = wm * 16 * WM + 16 * i0 + row;
             const float xs = s_xs[at];
@@ -204,29 +222,74 @@ __global__ void __launch_bounds__(256, 1) w8a8_tile_kernel(W8Args a, int tiles_m
         __builtin_amdgcn_wave_barrier();
     };
     rows32(std::integral_constant<int, 0>{});
-    rows32(std::integral_constant<int, 2>{});
-    if constexpr (WM > 4) {
-        rows32(std::integral_constant<int, 4 % WM>{});
-        rows32(std::integral_constant<int, 6 % WM>{});
-    }
+    if constexpr (WM > 2) rows32(std::integral_constant<int, 2>{});
+    if constexpr (WM > 4) rows32(std::integral_constant<int, 4>{});
+    if constexpr (WM > 6) rows32(std::integral_constant<int, 6>{});
 }
 
-bool w8_tile_fits(const W8Args& a, int BM) { return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, BM, BM); }
-
-int launch_w8_tile(const W8Args& a, int BM, hipStream_t s) {
-    const int cols = a.gated ? BM / 2 : BM;
-    const int64_t tm = w8_row_tiles(a, BM), tn = ((int64_t)a.n_out + cols - 1) / cols;
-    LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "w8a8_tile_kernel would need %lld workgroups", (long long)(tm * tn));
+template <int WM, int WN, int ST>
+int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
+    const int cols = (a.gated ? 16 : 32) * WN;
+    const int64_t tm = w8_row_tiles(a, 32 * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;
+    LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s would need %lld workgroups", name, (long long)(tm * tn));
     const dim3 grid((unsigned)(tm * tn));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, (int)tm, (int)tn); };
-    if (BM == 256) {
-        a.gated ? go(w8a8_tile_kernel<8, 8, 2, true>) : go(w8a8_tile_kernel<8, 8, 2, false>);
-        LAVA_LAUNCH_CHECK("w8a8_tile_kernel<256>");
-    } else {
-        a.gated ? go(w8a8_tile_kernel<4, 4, 4, true>) : go(w8a8_tile_kernel<4, 4, 4, false>);
-        LAVA_LAUNCH_CHECK("w8a8_tile_kernel<128>");
-    }
+    a.gated ? go(w8a8_tile_kernel<WM, WN, ST, true>) : go(w8a8_tile_kernel<WM, WN, ST, false>);
+    LAVA_LAUNCH_CHECK(name);
     return LAVA_HIP_OK;
+}
+
+// What a tile of 64 x 64, 64 x 128, 128 x 128 or 256 x 256 costs a CU that has others to run beside it (the largest has none): us
+// before and behind the loop, and us each 128 bytes of K.  Measured at 4096 x 4096 with K from 128 to 5632.
+constexpr struct {
+    int bm, bn;
+    float fixed, stage;
+} W8_TILES[4] = {{64, 64, 0.85f, 0.215f}, {64, 128, 1.7f, 0.356f}, {128, 128, 3.5f, 0.61f}, {256, 256, 16.f, 1.75f}};
+
+bool w8_tile_fits(const W8Args& a, int tile) {
+    return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, W8_TILES[tile].bm, W8_TILES[tile].bn);
+}
+
+double w8_met(const W8Args& a) { return a.offsets ? a.experts * -expm1(-(double)a.rows / a.experts) : 1; }
+
+double w8_tile_count(const W8Args& a, int bm, int bn) {
+    const double tn = (a.n_out + (a.gated ? bn / 2 : bn) - 1) / (a.gated ? bn / 2 : bn);
+    if (a.offsets == nullptr) return ((a.rows + bm - 1) / bm) * tn;
+    // of a plan: each expert that has rows has half a tile more than whole ones
+    const double met = w8_met(a), whole = (double)a.rows / bm + 0.5 * met;
+    return (met > whole ? met : whole) * tn;
+}
+
+// The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and a third of one for the end.
+// us, this rule's / the others of {64 x 64, 64 x 128, 128 x 128, 256 x 256}: 64 rows x 14336 x 4096 12.3 / 14.9, 25.8, 48; 128 rows
+// 15.2 / 16.2, 27, 50; 333 rows 30.6 / 42.6, 32.7, 52.7; 1024 x 4096 x 4096 21.1 / 28.5, 24.9, 51; 4096 x 4096 x 4096 62 / 94 (128 x 128); 5003
+// tokens, 4 of 60 experts of 2048 x 1408, 105.8 / 137, 111.7, 153; 1000 tokens, 8 of 64, 61.7 / 70.6, 65.4, 92.
+int w8_tile_choice(const W8Args& a) {
+    const double stages = (a.k + TN_KB - 1) / TN_KB;
+    int best = -1;
+    double least = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (!w8_tile_fits(a, i)) continue;
+        const double per_cu = w8_tile_count(a, W8_TILES[i].bm, W8_TILES[i].bn) / 256;
+        const double cost = (per_cu <= 1 ? 1 : per_cu + 0.35) * (W8_TILES[i].fixed + W8_TILES[i].stage * stages);
+        if (best < 0 || cost < least) {
+            best = i;
+            least = cost;
+        }
+    }
+    return best;
+}
+
+int launch_w8_tile(const W8Args& a, int tile, hipStream_t s) {
+    // Where a CU has one tile at most, a stage more in flight; else more tiles a CU (128 x 128, us with 2 stages / 3: 1024 x 4096 x
+    // 4096, 256 tiles, 26.8 / 21.1; 2048 rows 36 / 41.6).
+    const bool lone = w8_tile_count(a, W8_TILES[tile].bm, W8_TILES[tile].bn) <= 256;
+    switch (tile) {
+    case 0: return lone ? launch_tile<2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
+    case 1: return lone ? launch_tile<2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
+    case 2: return lone ? launch_tile<4, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
+    default: return launch_tile<8, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
+    }
 }
 
 }  // namespace lava
