@@ -1,14 +1,18 @@
 // moe.hip -- tokens routed to experts, sorted by them, and the experts' results summed.
 //
-// Routing: L lanes of a wavefront hold a token's logits, V each, and take the highest one top_k times by a reduction over
-// the lanes.  Without a bias the order of p is that of the logits, which are compared as they are.  With one, and for
-// groups counted by two, c = p + bias is taken in 32 bits first; where two that the choice tells apart lie nearer to each
-// other than c's rounding may move them, the wavefront's tokens are done again in 64.
+// Routing: L lanes of a wavefront (16; 64 above 256 experts) have a token, lane l the logits of experts V l .. V l + V - 1, and
+// take the highest one top_k times: a maximum over the lanes by rotations within 16 lanes, then the lowest expert that has
+// it.  (A token a wavefront costs more: of 64 lanes' reductions each is half as long again and serves one token instead of
+// four; 16384 tokens of 256 experts, 8 groups, 32 us against NN.)  Without a bias the order of p is that of the logits, which are
+// compared as they are.  With one, and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the
+// choice tells apart lie nearer to each other than c's rounding may move them, the wavefront's tokens are done again in 64.
 //
 // Sorting: workgroup b has tokens [b * span, (b + 1) * span), counts its assignments per expert, and in a second launch
 // (in the same one where a workgroup has all tokens) adds the counts of the lower workgroups and places its own in
 // order: a stable counting sort without global atomics, the same in every run.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "gemm_common.hpp"
 #include "lava_hip_internal.hpp"
@@ -47,51 +51,77 @@ struct Router {
     float scale;
 };
 
-template <typename Real>
-__device__ __forceinline__ Real exp_of(Real x) {
-    if constexpr (sizeof(Real) == 8) return exp(x);
-    else return expf(x);
-}
+constexpr float NONE = -__builtin_inff();
 
-template <typename Real>
-__device__ __forceinline__ Real neg_inf() {
-    return -(Real)__builtin_inff();
+// ---- over the L lanes of a token, the result the same in all of them, bit for bit (each step is symmetric) ----
+// Two wait states lie between a result and its use by another lane.
+#define LAVA_ROW_ALL(OP)                                                       \
+    "s_nop 1\n\t" OP " %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0xf\n\t"   \
+    "s_nop 1\n\t" OP " %0, %0, %0 row_ror:4 row_mask:0xf bank_mask:0xf\n\t"   \
+    "s_nop 1\n\t" OP " %0, %0, %0 row_ror:2 row_mask:0xf bank_mask:0xf\n\t"   \
+    "s_nop 1\n\t" OP " %0, %0, %0 row_ror:1 row_mask:0xf bank_mask:0xf"
+// f(x, the other's x) of lane l and lane l ^ 16, or l ^ 32: v_permlane16_swap exchanges one copy's odd rows of 16 lanes with the
+// other's even ones.
+template <int D, typename F>
+__device__ __forceinline__ uint32_t across(uint32_t x, F f) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 both;
+    if constexpr (D == 16) both = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(x, x, false, false));
+    else both = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(x, x, false, false));
+    return f(both[0], both[1]);
 }
-
-// The highest of c over the L lanes of a token and its place e = v * L + lane, the lowest of equal ones.
-template <int L, int V, typename Real>
-__device__ __forceinline__ void highest(const Real (&c)[V], int lane, Real& top, int& at) {
-    top = c[0];
-    at = lane;
+template <int L, typename F>
+__device__ __forceinline__ uint32_t rows(uint32_t x, F f) {
+    if constexpr (L > 16) x = across<16>(x, f);
+    if constexpr (L > 32) x = across<32>(x, f);
+    return x;
+}
+template <int L>
+__device__ __forceinline__ float all_max(float x) {
+    asm(LAVA_ROW_ALL("v_max_f32_dpp") : "+v"(x));
+    return __uint_as_float(rows<L>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }));
+}
+template <int L>
+__device__ __forceinline__ float all_sum(float x) {
+    asm(LAVA_ROW_ALL("v_add_f32_dpp") : "+v"(x));
+    return __uint_as_float(rows<L>(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+template <int L>
+__device__ __forceinline__ int all_min(int x) {
+    asm(LAVA_ROW_ALL("v_min_i32_dpp") : "+v"(x));
+    return (int)rows<L>((uint32_t)x, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
+}
+#undef LAVA_ROW_ALL
+template <int L>
+__device__ __forceinline__ double all_max(double x) {
 #pragma unroll
-    for (int v = 1; v < V; ++v)
-        if (c[v] > top) {
-            top = c[v];
-            at = v * L + lane;
-        }
+    for (int d = 1; d < L; d <<= 1) x = fmax(x, __shfl_xor(x, d, 64));
+    return x;
+}
+template <int L>
+__device__ __forceinline__ double all_sum(double x) {
 #pragma unroll
-    for (int d = 1; d < L; d <<= 1) {
-        const Real o = __shfl_xor(top, d, 64);
-        const int oa = __shfl_xor(at, d, 64);
-        if (o > top || (o == top && oa < at)) {
-            top = o;
-            at = oa;
-        }
-    }
+    for (int d = 1; d < L; d <<= 1) x += __shfl_xor(x, d, 64);
+    return x;
 }
 
-template <int L, int V, typename Real>
-__device__ __forceinline__ void take_out(Real (&c)[V], int lane, int at) {
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-        if (at == v * L + lane) c[v] = neg_inf<Real>();
-}
+// p of a logit: in 32 bits by v_exp_f32 and v_rcp_f32 (1 ulp each; the exponent's rounding is below |x| 2^-24, of p (1 - p) |x| <
+// 0.3 in all), enough to choose by where `apart` says so
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+__device__ __forceinline__ float quotient(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ double quotient(double x) { return 1.0 / x; }
 
-// The experts of the token that these L lanes hold, in sel (rank r in lane r % L, sel[r / L]): true unless 32 bits do not
+// The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L]; true unless 32 bits do not
 // settle the order.
 template <int L, int V, typename Real>
-__device__ bool choose(const Router& r, const float (&x)[V], int lane, int (&sel)[32 / L + (L > 32)]) {
+__device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], int lane, int (&sel)[2]) {
     constexpr bool SINGLE = sizeof(Real) == 4;
+    constexpr Real LEAST = (Real)NONE;
     // Without a bias the logits' own order is the one asked for, of single experts and of groups counted by their best.
     const bool by_logit = r.bias == nullptr && (r.top_groups == r.groups || r.group_best == 1);
     Real c[V];
@@ -105,101 +135,114 @@ __device__ bool choose(const Router& r, const float (&x)[V], int lane, int (&sel
             float m = x[0];
 #pragma unroll
             for (int v = 1; v < V; ++v) m = fmaxf(m, x[v]);
-#pragma unroll
-            for (int d = 1; d < L; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-            top = m == neg_inf<float>() ? (Real)0 : (Real)m;
+            m = all_max<L>(m);
+            top = m == NONE ? (Real)0 : (Real)m;
             Real sum = 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) sum += exp_of<Real>((Real)x[v] - top);
-#pragma unroll
-            for (int d = 1; d < L; d <<= 1) sum += __shfl_xor(sum, d, 64);
+            for (int v = 0; v < V; ++v) sum += exp_of((Real)x[v] - top);
+            sum = all_sum<L>(sum);
             norm = sum > 0 ? 1 / sum : (Real)0;
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int e = v * L + lane;
-            Real p = r.softmax ? exp_of<Real>((Real)x[v] - top) * norm : 1 / (1 + exp_of<Real>(-(Real)x[v]));
-            if (e < r.experts && r.bias) p += (Real)r.bias[e];
-            c[v] = x[v] == neg_inf<float>() ? neg_inf<Real>() : p;
+            const Real p = r.softmax ? exp_of((Real)x[v] - top) * norm : quotient(1 + exp_of(-(Real)x[v]));
+            c[v] = x[v] == NONE ? LEAST : p + (Real)bias[v];
         }
-        // of p: exp, sum (V + 6 additions, V at most 64) and quotient, at most 2^-17 of the largest; a sigmoid's at most 2^-21
-        if (SINGLE) near = r.softmax ? norm * (Real)0x1p-16f : (Real)0x1p-20f;
+        // of p: the exponent's rounding, exp, a sum of V + 6 additions (V at most 16) and the quotient: below 2^-18 of the largest p; a
+        // sigmoid's below 2^-21
+        if (SINGLE) near = r.softmax ? norm * (Real)0x1p-16f : (Real)0x1p-19f;
     }
     auto apart = [&](Real hi, Real lo, int terms) {
-        if (!SINGLE || by_logit || lo == neg_inf<Real>()) return true;
+        if (!SINGLE || by_logit || lo == LEAST) return true;
         return hi - lo > terms * (near + (Real)0x1p-22f * fmax((Real)fabs(hi), (Real)fabs(lo)));
     };
     bool sure = true;
     if (r.top_groups < r.groups) {
-        const int size = r.experts / r.groups;
+        // a group's best two: of a lane's experts, then over the lanes
+        const int size = r.experts / r.groups, base = (threadIdx.x & 63) - lane;
+        auto best_two = [&](Real& b1, Real& b2, int lo, int hi) __attribute__((always_inline)) {
+            b1 = b2 = LEAST;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const Real o = lane * V + v >= lo && lane * V + v < hi ? c[v] : LEAST;
+                b2 = fmax(b2, fmin(b1, o));
+                b1 = fmax(b1, o);
+            }
+        };
+        auto join = [&](Real& b1, Real& b2, int d) __attribute__((always_inline)) {
+            const Real o1 = __shfl_xor(b1, d, 64), o2 = __shfl_xor(b2, d, 64);
+            b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+            b1 = fmax(b1, o1);
+        };
         constexpr int GV = 64 / L;
-        Real count[GV];   // group g in lane g % L
+        Real count[GV], b1, b2;   // group g's in lane g % L's count[g / L]
 #pragma unroll
-        for (int i = 0; i < GV; ++i) count[i] = neg_inf<Real>();
+        for (int i = 0; i < GV; ++i) count[i] = LEAST;
+        const int span = size / V;
+        if (size % V == 0 && (span & (span - 1)) == 0) {   // whole lanes, a power of two of them: all groups at once
+            best_two(b1, b2, 0, r.experts);
+            for (int d = 1; d < span; d <<= 1) join(b1, b2, d);
+            // at most L / span groups, so one a lane
+            const Real o = __shfl(r.group_best == 2 ? b1 + b2 : b1, base + min(lane * span, L - 1), 64);
+            count[0] = lane < r.groups ? o : LEAST;
+        } else {
+            for (int g = 0; g < r.groups; ++g) {
+                best_two(b1, b2, g * size, (g + 1) * size);
+#pragma unroll
+                for (int d = 1; d < L; d <<= 1) join(b1, b2, d);
+                const Real o = r.group_best == 2 ? b1 + b2 : b1;
+#pragma unroll
+                for (int i = 0; i < GV; ++i) count[i] = g == i * L + lane ? o : count[i];
+            }
+        }
+        int rank[GV];   // the groups in front of this one
+#pragma unroll
+        for (int i = 0; i < GV; ++i) rank[i] = 0;
         for (int g = 0; g < r.groups; ++g) {
-            Real b1 = neg_inf<Real>(), b2 = neg_inf<Real>();   // its best two
+            Real mine = count[0];
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if ((unsigned)(v * L + lane - g * size) < (unsigned)size) {
-                    b2 = fmax(b2, fmin(b1, c[v]));
-                    b1 = fmax(b1, c[v]);
-                }
+            for (int i = 1; i < GV; ++i) mine = g / L == i ? count[i] : mine;
+            const Real o = __shfl(mine, base + g % L, 64);
 #pragma unroll
-            for (int d = 1; d < L; d <<= 1) {
-                const Real o1 = __shfl_xor(b1, d, 64), o2 = __shfl_xor(b2, d, 64);
-                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
-                b1 = fmax(b1, o1);
-            }
-            const Real sum = r.group_best == 2 ? b1 + b2 : b1;
-#pragma unroll
-            for (int i = 0; i < GV; ++i)
-                if (g == i * L + lane) count[i] = sum;
+            for (int i = 0; i < GV; ++i) rank[i] += o > count[i] || (o == count[i] && g < i * L + lane);
         }
+        Real worst = LEAST, next = LEAST;   // -(the least that stays), the highest that does not
         uint64_t kept = 0;
-        Real last = 0;
-        for (int i = 0; i <= r.top_groups; ++i) {
-            Real top;
-            int g;
-            highest<L, GV, Real>(count, lane, top, g);
-            if (i == r.top_groups) {
-                sure = sure && apart(last, top, r.group_best);
-                break;
-            }
-            last = top;
-            if (top == neg_inf<Real>()) break;   // groups of masked experts only: none of them is open anyway
-            kept |= 1ull << g;
-            take_out<L, GV, Real>(count, lane, g);
+#pragma unroll
+        for (int i = 0; i < GV; ++i) {
+            const bool in = i * L + lane < r.groups, stays = in && rank[i] < r.top_groups;
+            worst = fmax(worst, stays ? -count[i] : LEAST);
+            next = fmax(next, in && !stays ? count[i] : LEAST);
+            const uint64_t all = __ballot(stays) >> base;   // the token's lanes on
+            kept |= (L == 64 ? all : all & ((1ull << (L & 63)) - 1)) << (i * (L & 63));
         }
-        // groups that count -inf though one of their experts is left (the second best is masked): by their number
-        if (last == neg_inf<Real>()) {
-            int more = r.top_groups - __popcll(kept);
-            for (int g = 0; g < r.groups && more > 0; ++g)
-                if (!(kept >> g & 1)) {
-                    kept |= 1ull << g;
-                    --more;
-                }
-        }
+        sure = apart(-all_max<L>(worst), all_max<L>(next), r.group_best);
         const float inv = 1.f / (float)size;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int g = (int)(((float)(v * L + lane) + 0.5f) * inv);
-            if (!(kept >> (g & 63) & 1)) c[v] = neg_inf<Real>();
+            const int g = (int)(((float)(lane * V + v) + 0.5f) * inv);
+            if (!(kept >> (g & 63) & 1)) c[v] = LEAST;
         }
     }
-#pragma unroll
-    for (int i = 0; i < 32 / L + (L > 32); ++i) sel[i] = -1;
+    sel[0] = sel[1] = -1;
     Real last = 0;
-    for (int i = 0; i <= r.top_k; ++i) {
-        Real top;
-        int at;
-        highest<L, V, Real>(c, lane, top, at);
-        if (i > 0) sure = sure && apart(last, top, 1);
-        if (i == r.top_k || top == neg_inf<Real>()) break;   // the same in all lanes of a token, but not of a wavefront
-        last = top;
+    for (int i = 0; i < r.top_k + (SINGLE && !by_logit); ++i) {
+        Real top = c[0];
 #pragma unroll
-        for (int j = 0; j < 32 / L + (L > 32); ++j)
-            if (i == j * L + lane) sel[j] = at;
-        take_out<L, V, Real>(c, lane, at);
+        for (int v = 1; v < V; ++v) top = fmax(top, c[v]);
+        top = all_max<L>(top);
+        if (i > 0) sure = sure && apart(last, top, 1);
+        last = top;
+        if (i == r.top_k) break;
+        int at = L * V;   // the lowest expert that has it
+#pragma unroll
+        for (int v = V - 1; v >= 0; --v) at = c[v] == top ? lane * V + v : at;
+        at = all_min<L>(at);
+#pragma unroll
+        for (int v = 0; v < V; ++v) c[v] = lane * V + v == at ? LEAST : c[v];
+        at = top == LEAST ? -1 : at;   // none left
+        sel[0] = i == lane ? at : sel[0];
+        if (L < 32) sel[1] = i == L + lane ? at : sel[1];
     }
     return sure;
 }
@@ -279,21 +322,30 @@ __device__ void finish_plan(const Plan& p, const int32_t* ids, int b, int blocks
 struct SortShared {
     int32_t base[MOE_EXPERTS];
     int32_t tmp[MOE_WAVES];
+    int32_t part[2][MOE_THREADS];   // moe_place_kernel
 };
+static_assert(MOE_THREADS == MOE_EXPERTS, "a thread an expert");
 
 }  // namespace
 
-// COUNT: routes nothing, counts given ids.
-template <typename T, int L, int V>
+// VEC: rows of logits aligned to V of them (or 16 bytes), experts a multiple of V.
+template <typename T, int L, int V, bool VEC>
 __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const T* __restrict__ logits, int64_t ldl,
                                                                 int32_t* ids, float* weights, Plan p) {
     extern __shared__ uint16_t below[];   // MOE_WAVES * experts where one workgroup has all tokens and writes the plan
     __shared__ SortShared sh;
-    constexpr int PER = MOE_WAVES * (64 / L), S = 32 / L + (L > 32);
+    constexpr int PER = MOE_THREADS / L, S = L < 32 ? 2 : 1;   // tokens at once; ranks a lane
     const int lane = threadIdx.x & (L - 1), b = blockIdx.x;
     if (p.offsets) {
-        if (threadIdx.x < MOE_EXPERTS) sh.base[threadIdx.x] = 0;
+        sh.base[threadIdx.x] = 0;
         __syncthreads();
+    }
+    float bias[V];
+    bool bad_bias = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = r.bias && lane * V + v < r.experts ? r.bias[lane * V + v] : 0.f;
+        bad_bias |= !(bias[v] < __builtin_inff());
     }
     const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens);
     for (int64_t t0 = (int64_t)b * p.span; t0 < last; t0 += PER) {
@@ -301,69 +353,67 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
         const bool live = t < last;
         const T* row = logits + (live ? t : 0) * ldl;
         float x[V];
-        bool bad = false;
+        if constexpr (VEC) {
+            constexpr int C = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
+            typedef T Tv __attribute__((ext_vector_type(C)));
+            const bool in = live && lane * V < r.experts;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int e = v * L + lane;
-            x[v] = neg_inf<float>();
-            if (live && e < r.experts) {
-                x[v] = (float)row[e];
-                bad |= !(x[v] < __builtin_inff());
-                if (r.bias) bad |= !(r.bias[e] < __builtin_inff());
+            for (int v = 0; v < V; v += C) {
+                const Tv q = *reinterpret_cast<const Tv*>(row + (in ? lane * V + v : 0));
+#pragma unroll
+                for (int i = 0; i < C; ++i) x[v + i] = in ? (float)q[i] : NONE;
             }
-        }
+        } else {
 #pragma unroll
-        for (int d = 1; d < L; d <<= 1) bad |= __shfl_xor((int)bad, d, 64) != 0;
-        if (bad) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) x[v] = neg_inf<float>();
+            for (int v = 0; v < V; ++v) x[v] = live && lane * V + v < r.experts ? (float)row[lane * V + v] : NONE;
         }
-        int sel[S];
-        const bool sure = choose<L, V, float>(r, x, lane, sel);
-        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, lane, sel);
+        bool bad = bad_bias;
+#pragma unroll
+        for (int v = 0; v < V; ++v) bad |= !(x[v] < __builtin_inff());
+        bad = all_min<L>(bad ? 0 : 1) == 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[v] = bad ? NONE : x[v];
+        int sel[2];
+        const bool sure = choose<L, V, float>(r, x, bias, lane, sel);
+        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, lane, sel);
 
         // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
         // so that p of far masked or shut out experts, below the least float, does not make 0 / 0
-        float xs[S], top = neg_inf<float>(), m = neg_inf<float>(), all = 0.f;
+        float xs[S], weight[S], top = NONE, all = 0.f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-            xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : neg_inf<float>();
+            xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : NONE;
             top = fmaxf(top, xs[i]);
         }
         if (r.softmax && !r.renormalize) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) m = fmaxf(m, x[v]);
+            for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
         }
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) {
-            top = fmaxf(top, __shfl_xor(top, d, 64));
-            m = fmaxf(m, __shfl_xor(m, d, 64));
-        }
-        if (!r.renormalize) top = r.softmax ? m : 0.f;
-        else if (!r.softmax) top = fminf(top, 0.f);
-        if (top == neg_inf<float>()) top = 0.f;
-        float w[S];
+        top = all_max<L>(top);
+        if (!r.softmax) top = r.renormalize ? fminf(top, 0.f) : 0.f;
+        if (top == NONE) top = 0.f;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             // softmax: exp(x - top); sigmoid: exp(-top) / (1 + exp(-x)), where top is 0 unless every x is below it
-            w[i] = sel[i] < 0    ? 0.f
-                   : r.softmax   ? expf(xs[i] - top)
-                   : xs[i] > 0.f ? 1.f / (1.f + expf(-xs[i]))
-                                 : expf(xs[i] - top) / (1.f + expf(xs[i]));
-            if (r.renormalize) all += w[i];
+            weight[i] = sel[i] < 0    ? 0.f
+                        : r.softmax   ? expf(xs[i] - top)
+                        : xs[i] > 0.f ? 1.f / (1.f + expf(-xs[i]))
+                                      : expf(xs[i] - top) / (1.f + expf(xs[i]));
+            all += weight[i];
         }
-        if (r.softmax && !r.renormalize) {
+        if (!r.renormalize) {
+            all = r.softmax ? 0.f : lane == 0 ? 1.f : 0.f;
+            if (r.softmax) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) all += expf(x[v] - top);
+                for (int v = 0; v < V; ++v) all += expf(x[v] - top);
+            }
         }
-#pragma unroll
-        for (int d = 1; d < L; d <<= 1) all += __shfl_xor(all, d, 64);
-        if (!r.renormalize && !r.softmax) all = 1.f;
+        all = all_sum<L>(all);
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             const int rank = i * L + lane;
             if (!live || rank >= r.top_k) continue;
-            float o = w[i] / all * r.scale;
+            float o = weight[i] / all * r.scale;
             if (sel[i] < 0) o = bad ? __builtin_nanf("") : 0.f;
             ids[t * r.top_k + rank] = sel[i];
             weights[t * r.top_k + rank] = o;
@@ -372,11 +422,11 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
     }
     if (!p.offsets) return;
     __syncthreads();   // the counts, and this workgroup's ids in memory
+    const int all = threadIdx.x < (unsigned)p.experts ? sh.base[threadIdx.x] : 0;
     if (gridDim.x > 1) {
-        if (threadIdx.x < (unsigned)p.experts) p.counts[b * p.experts + threadIdx.x] = sh.base[threadIdx.x];
+        if (threadIdx.x < (unsigned)p.experts) p.counts[b * p.experts + threadIdx.x] = all;
         return;
     }
-    const int all = threadIdx.x < (unsigned)p.experts ? sh.base[threadIdx.x] : 0;
     __syncthreads();
     finish_plan(p, ids, 0, 1, 0, all, sh.base, below, sh.tmp);
 }
@@ -386,7 +436,7 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_count_kernel(const int32_t* _
     extern __shared__ uint16_t below[];
     __shared__ SortShared sh;
     const int b = blockIdx.x;
-    if (threadIdx.x < MOE_EXPERTS) sh.base[threadIdx.x] = 0;
+    sh.base[threadIdx.x] = 0;
     __syncthreads();
     const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens) * p.top_k;
     for (int64_t i = (int64_t)b * p.span * p.top_k + threadIdx.x; i < last; i += MOE_THREADS) {
@@ -406,13 +456,35 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_count_kernel(const int32_t* _
 __global__ void __launch_bounds__(MOE_THREADS) moe_place_kernel(const int32_t* __restrict__ ids, Plan p) {
     extern __shared__ uint16_t below[];
     __shared__ SortShared sh;
+    // the counts of expert threadIdx.x % width, of every parts-th workgroup, 16 in flight
+    int width = 64;
+    while (width < p.experts) width <<= 1;
+    const int parts = MOE_THREADS / width, e = threadIdx.x & (width - 1), part = threadIdx.x / width;
     int before = 0, all = 0;
-    if (threadIdx.x < (unsigned)p.experts)
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-            const int c = p.counts[b * p.experts + threadIdx.x];
-            all += c;
-            if (b < (int)blockIdx.x) before += c;
+    if (e < p.experts) {
+        const int32_t* c = p.counts + e;
+        for (int b0 = part; b0 < (int)gridDim.x; b0 += 16 * parts) {
+            int n[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) n[i] = b0 + i * parts < (int)gridDim.x ? c[(b0 + i * parts) * p.experts] : 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                all += n[i];
+                if (b0 + i * parts < (int)blockIdx.x) before += n[i];
+            }
         }
+    }
+    sh.part[0][threadIdx.x] = before;
+    sh.part[1][threadIdx.x] = all;
+    __syncthreads();
+    if (threadIdx.x < (unsigned)p.experts)
+        for (int i = 1; i < parts; ++i) {
+            before += sh.part[0][threadIdx.x + i * width];
+            all += sh.part[1][threadIdx.x + i * width];
+        }
+    else
+        before = all = 0;   // the other parts' are in theirs
+    __syncthreads();
     finish_plan(p, ids, blockIdx.x, gridDim.x, before, all, sh.base, below, sh.tmp);
 }
 
@@ -511,13 +583,22 @@ int launch_route(const Router& r, const void* logits, int64_t ldl, int32_t* ids,
                  hipStream_t s) {
     const size_t lds = p.offsets && blocks == 1 ? below_bytes(p.experts) : 0;
     const T* x = static_cast<const T*>(logits);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), lds, s, r, x, ldl, ids, weights, p);
+    auto by_v = [&](auto ltag, auto vtag) {
+        constexpr int V = decltype(vtag)::value;
+        constexpr int L = decltype(ltag)::value;
+        constexpr size_t al = V * sizeof(T) < 16 ? V * sizeof(T) : 16;
+        const bool vec = r.experts % V == 0 && ldl * (int64_t)sizeof(T) % al == 0 && aligned(logits, al);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), lds, s, r, x, ldl, ids, weights, p);
+        };
+        vec ? go(moe_route_kernel<T, L, V, true>) : go(moe_route_kernel<T, L, V, false>);
     };
-    if (r.experts <= 64) go(moe_route_kernel<T, 16, 4>);
-    else if (r.experts <= 128) go(moe_route_kernel<T, 16, 8>);
-    else if (r.experts <= 256) go(moe_route_kernel<T, 16, 16>);
-    else go(moe_route_kernel<T, 64, 16>);
+    std::integral_constant<int, 16> few;
+    if (r.experts <= 64) by_v(few, std::integral_constant<int, 4>{});
+    else if (r.experts <= 128) by_v(few, std::integral_constant<int, 8>{});
+    else if (r.experts <= 256) by_v(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
+    else if (r.experts <= 512) by_v(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+    else by_v(std::integral_constant<int, 64>{}, std::integral_constant<int, 16>{});
     LAVA_LAUNCH_CHECK("moe_route_kernel");
     return p.offsets && blocks > 1 ? launch_place(ids, p, blocks, s) : LAVA_HIP_OK;
 }
