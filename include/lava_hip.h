@@ -696,9 +696,10 @@ typedef struct lava_hip_w8_layer {
  *   y[t][n] = (sum_j X[t][j] w[n][j]) * x_scale[t] * scale[n] + bias[n]
  *   Y[t][n] = act(y[t][n]), or of a gated layer act(y[t][n]) * y[t][n + N / 2] for n < N / 2,
  * rounded once to y_dtype (F16, BF16 or F32), row t at Y + t * ldy.  The sums are exact in 32-bit integers, the rest is in
- * 32-bit floating point in the order written, whichever kernel runs: its choice changes no bit of Y.  MFMA kernels that load 16 bytes
- * at a time take k, ldx and ldw that are multiples of 16 and 16-byte aligned X and w; any other layout runs on a
- * generic one.  One launch, no workspace.  Y overlaps no other operand. */
+ * 32-bit floating point in the order written, whichever kernel runs: its choice changes no bit of Y.  The fast kernels take
+ * k, ldx and ldw (and an expert_stride) that are multiples of 16 and 16-byte aligned X and w whose rows of a tile span less than
+ * 2 GiB (all tokens, where a plan gathers them); any other layout runs on a generic one, also on matrix instructions.  One
+ * launch, no workspace.  Y overlaps no other operand. */
 int lava_hip_gemm_w8a8(const lava_hip_w8_layer* layer, const int8_t* X, const float* x_scale, int64_t tokens, int64_t ldx,
                        int y_dtype, void* Y, int64_t ldy, void* stream);
 

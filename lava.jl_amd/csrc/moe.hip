@@ -1,11 +1,13 @@
 // moe.hip -- tokens routed to experts, sorted by them, and the experts' results summed.
 //
-// Routing: L lanes of a wavefront (16; 64 above 256 experts) have a token, lane l the logits of experts V l .. V l + V - 1, and
-// take the highest one top_k times: a maximum over the lanes by rotations within 16 lanes, then the lowest expert that has
-// it.  (A token a wavefront costs more: of 64 lanes' reductions each is half as long again and serves one token instead of
-// four; 16384 tokens of 256 experts, 8 groups, 32 us against NN.)  Without a bias the order of p is that of the logits, which are
+// Routing: L lanes of a wavefront (16 up to 128 experts, 32 up to 256, then 64) have a token, lane l the logits of experts
+// V l .. V l + V - 1, and take the highest one top_k times: a maximum over the lanes by rotations within 16 lanes, then the
+// lowest expert that has it.  (A token a wavefront costs more: of 64 lanes' reductions each is half as long again and serves one token instead of
+// four: 16384 tokens of 64 experts 20.0 us against 13.7.)  Without a bias the order of p is that of the logits, which are
 // compared as they are.  With one, and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the
 // choice tells apart lie nearer to each other than c's rounding may move them, the wavefront's tokens are done again in 64.
+// Bound by issue: 8 ranks of 256 experts in 8 groups with a bias take 28 us for 16384 tokens (0.3 TB/s of logits), of which
+// the few that are done again are the last 8; one token 6.
 //
 // Sorting: workgroup b has tokens [b * span, (b + 1) * span), counts its assignments per expert, and in a second launch
 // (in the same one where a workgroup has all tokens) adds the counts of the lower workgroups and places its own in
@@ -48,6 +50,7 @@ int blocks_of(int64_t tokens) {
 struct Router {
     const float* bias;
     int experts, top_k, softmax, groups, top_groups, group_best, renormalize;
+    int by_logit;   // without a bias the logits' own order is the one asked for, of single experts and of groups counted by their best
     float scale;
 };
 
@@ -95,12 +98,20 @@ __device__ __forceinline__ int all_min(int x) {
     asm(LAVA_ROW_ALL("v_min_i32_dpp") : "+v"(x));
     return (int)rows<L>((uint32_t)x, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
 }
+template <int L>
+__device__ __forceinline__ uint32_t all_max(uint32_t x) {
+    asm(LAVA_ROW_ALL("v_max_u32_dpp") : "+v"(x));
+    return rows<L>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
 #undef LAVA_ROW_ALL
+// The upper halves of bits that order as the numbers do, then the lower ones of those that have the highest.
 template <int L>
 __device__ __forceinline__ double all_max(double x) {
-#pragma unroll
-    for (int d = 1; d < L; d <<= 1) x = fmax(x, __shfl_xor(x, d, 64));
-    return x;
+    const uint64_t b = __builtin_bit_cast(uint64_t, x), sign = 1ull << 63;
+    const uint64_t key = b & sign ? ~b : b | sign;
+    const uint32_t hi = (uint32_t)(key >> 32), top = all_max<L>(hi);
+    const uint64_t best = (uint64_t)top << 32 | all_max<L>(hi == top ? (uint32_t)key : 0u);
+    return __builtin_bit_cast(double, best & sign ? best ^ sign : ~best);
 }
 template <int L>
 __device__ __forceinline__ double all_sum(double x) {
@@ -116,14 +127,14 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float quotient(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ double quotient(double x) { return 1.0 / x; }
 
-// The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L]; true unless 32 bits do not
-// settle the order.
+// The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L] (and, where they are chosen
+// by their logits, those in xs); true unless 32 bits do not settle the order.
 template <int L, int V, typename Real>
-__device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], int lane, int (&sel)[2]) {
+__device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], int lane, int (&sel)[2],
+                                       float (&xs)[2]) {
     constexpr bool SINGLE = sizeof(Real) == 4;
     constexpr Real LEAST = (Real)NONE;
-    // Without a bias the logits' own order is the one asked for, of single experts and of groups counted by their best.
-    const bool by_logit = r.bias == nullptr && (r.top_groups == r.groups || r.group_best == 1);
+    const bool by_logit = r.by_logit;
     Real c[V];
     Real near = 0;   // how near two c may be that 32 bits cannot tell apart, without the part that grows with c
     if (by_logit) {
@@ -148,9 +159,10 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
             const Real p = r.softmax ? exp_of((Real)x[v] - top) * norm : quotient(1 + exp_of(-(Real)x[v]));
             c[v] = x[v] == NONE ? LEAST : p + (Real)bias[v];
         }
-        // of p: the exponent's rounding, exp, a sum of V + 6 additions (V at most 16) and the quotient: below 2^-18 of the largest p; a
-        // sigmoid's below 2^-21
-        if (SINGLE) near = r.softmax ? norm * (Real)0x1p-16f : (Real)0x1p-19f;
+        // Each p is off by, in units of 2^-24: a sigmoid p (1 - p) (|x| + 2 of exp) < 0.8, the sum 1, the quotient 2, below 4;
+        // a softmax, of the largest p, the exponent 0.4, exp 2, the sum V + 6 <= 22 additions of terms off by ln 1024 + 2 on
+        // average, the quotient and the product 2, below 36.
+        if (SINGLE) near = r.softmax ? norm * (Real)0x1p-17f : (Real)0x1p-21f;
     }
     auto apart = [&](Real hi, Real lo, int terms) {
         if (!SINGLE || by_logit || lo == LEAST) return true;
@@ -225,6 +237,7 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
         }
     }
     sel[0] = sel[1] = -1;
+    xs[0] = xs[1] = NONE;
     Real last = 0;
     for (int i = 0; i < r.top_k + (SINGLE && !by_logit); ++i) {
         Real top = c[0];
@@ -242,20 +255,24 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
         for (int v = 0; v < V; ++v) c[v] = lane * V + v == at ? LEAST : c[v];
         at = top == LEAST ? -1 : at;   // none left
         sel[0] = i == lane ? at : sel[0];
-        if (L < 32) sel[1] = i == L + lane ? at : sel[1];
+        xs[0] = i == lane ? (float)top : xs[0];
+        if (L < 32) {
+            sel[1] = i == L + lane ? at : sel[1];
+            xs[1] = i == L + lane ? (float)top : xs[1];
+        }
     }
     return sure;
 }
 
 // Adds the tokens' assignments to counts (LDS) or places them: base[e] is the next free place of expert e's run.
 // Stable: 1024 assignments at a time, a thread each; its place is base + those of lower wavefronts + those of lower lanes.
-__device__ void place(const Plan& p, const int32_t* ids, int first, int last, int32_t* base, uint16_t* below) {
+__device__ void place(const Plan& p, const int32_t* ids, int64_t first, int64_t last, int32_t* base, uint16_t* below) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E = p.experts;
     const int bits = 32 - __clz(E - 1 > 0 ? E - 1 : 1);
-    for (int i0 = first; i0 < last; i0 += MOE_THREADS) {
+    for (int64_t i0 = first; i0 < last; i0 += MOE_THREADS) {
         for (int i = threadIdx.x; i < MOE_WAVES * E; i += MOE_THREADS) below[i] = 0;
         __syncthreads();
-        const int i = i0 + threadIdx.x;
+        const int64_t i = i0 + threadIdx.x;
         const int e = i < last ? ids[i] : -1;
         const bool ok = e >= 0 && e < E;
         uint64_t same = __ballot(ok);   // lanes of the same expert
@@ -269,7 +286,7 @@ __device__ void place(const Plan& p, const int32_t* ids, int first, int last, in
         if (ok) {
             int at = base[e] + rank;
             for (int v = 0; v < w; ++v) at += below[v * E + e];
-            p.order[at] = i;
+            p.order[at] = (int32_t)i;
         }
         __syncthreads();
         for (int j = threadIdx.x; j < E; j += MOE_THREADS) {
@@ -316,7 +333,7 @@ __device__ void finish_plan(const Plan& p, const int32_t* ids, int b, int blocks
     for (int64_t i = (int64_t)total + b * MOE_THREADS + threadIdx.x; i < rows; i += (int64_t)blocks * MOE_THREADS) p.order[i] = -1;
     __syncthreads();
     const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens);
-    place(p, ids, b * p.span * p.top_k, (int)(last * p.top_k), base, below);
+    place(p, ids, (int64_t)b * p.span * p.top_k, last * p.top_k, base, below);
 }
 
 struct SortShared {
@@ -374,17 +391,19 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
 #pragma unroll
         for (int v = 0; v < V; ++v) x[v] = bad ? NONE : x[v];
         int sel[2];
-        const bool sure = choose<L, V, float>(r, x, bias, lane, sel);
-        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, lane, sel);
+        float xs[2];
+        const bool sure = choose<L, V, float>(r, x, bias, lane, sel, xs);
+        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, lane, sel, xs);
 
         // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
         // so that p of far masked or shut out experts, below the least float, does not make 0 / 0
-        float xs[S], weight[S], top = NONE, all = 0.f;
+        float weight[S], top = NONE, all = 0.f;
+        if (!r.by_logit) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-            xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : NONE;
-            top = fmaxf(top, xs[i]);
+            for (int i = 0; i < S; ++i) xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : NONE;
         }
+#pragma unroll
+        for (int i = 0; i < S; ++i) top = fmaxf(top, xs[i]);
         if (r.softmax && !r.renormalize) {
 #pragma unroll
             for (int v = 0; v < V; ++v) top = fmaxf(top, x[v]);
@@ -675,7 +694,8 @@ int lava_hip_moe_route(const lava_hip_moe_router* router, int dtype, const void*
     rc = lava_hip_init();
     if (rc != LAVA_HIP_OK) return rc;
     Router r = {router->bias, router->experts, router->top_k, router->score == LAVA_HIP_SCORE_SOFTMAX, router->groups,
-                router->top_groups, router->group_best, router->renormalize, router->scale};
+                router->top_groups, router->group_best, router->renormalize,
+                router->bias == nullptr && (router->top_groups == router->groups || router->group_best == 1), router->scale};
     Plan p = {};
     if (plan != nullptr) p = plan_of(plan);
     p.tokens = (int)tokens;

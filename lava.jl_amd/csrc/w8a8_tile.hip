@@ -25,7 +25,8 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
     static_assert(WM % 2 == 0 && (!GATED || WN % 2 == 0), "rows are finished 32 at a time, gates and factors are blocks of 16");
     static_assert(WN == 2 || WN == 4 || WN == 8, "a power of two of lanes finishes a row");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * STAGE];
-    __shared__ float s_xs[BM], s_ws[BN], s_bias[BN];
+    __shared__ __attribute__((aligned(16))) float s_ws[BN], s_bias[BN];
+    __shared__ float s_xs[BM];
     __shared__ int s_yr[BM];
 
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
