@@ -128,10 +128,10 @@ __device__ __forceinline__ float quotient(float x) { return __builtin_amdgcn_rcp
 __device__ __forceinline__ double quotient(double x) { return 1.0 / x; }
 
 // The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L] (and, where they are chosen
-// by their logits, those in xs); true unless 32 bits do not settle the order.
+// by their logits, those in xs); true unless 32 bits do not settle the order.  most: the largest finite |bias|.
 template <int L, int V, typename Real>
-__device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], int lane, int (&sel)[2],
-                                       float (&xs)[2]) {
+__device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], float most, int lane,
+                                       int (&sel)[2], float (&xs)[2]) {
     constexpr bool SINGLE = sizeof(Real) == 4;
     constexpr Real LEAST = (Real)NONE;
     const bool by_logit = r.by_logit;
@@ -159,14 +159,16 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
             const Real p = r.softmax ? exp_of((Real)x[v] - top) * norm : quotient(1 + exp_of(-(Real)x[v]));
             c[v] = x[v] == NONE ? LEAST : p + (Real)bias[v];
         }
-        // Each p is off by, in units of 2^-24: a sigmoid p (1 - p) (|x| + 2 of exp) < 0.8, the sum 1, the quotient 2, below 4;
-        // a softmax, of the largest p, the exponent 0.4, exp 2, the sum V + 6 <= 22 additions of terms off by ln 1024 + 2 on
-        // average, the quotient and the product 2, below 36.
+        // Each p is off by, in units of 2^-24: a sigmoid 2 p (1 - p) |x| < 0.5 of the exponent and log2 e, 2 p (1 - p) <= 0.5 of
+        // exp, the sum 1, the quotient 2, below 4; a softmax, of the largest p, the exponent 1.1, exp 2, the sum V + 6 <= 22
+        // additions of terms off by 3 ln 1024 + 2 on average, the quotient and the product 2, below 52.
         if (SINGLE) near = r.softmax ? norm * (Real)0x1p-17f : (Real)0x1p-21f;
     }
     auto apart = [&](Real hi, Real lo, int terms) {
         if (!SINGLE || by_logit || lo == LEAST) return true;
-        return hi - lo > terms * (near + (Real)0x1p-22f * fmax((Real)fabs(hi), (Real)fabs(lo)));
+        // the sum of two c may be far below them: their own roundings
+        const Real more = terms == 2 ? (Real)0x1p-21f * (1 + (Real)most) : (Real)0;
+        return hi - lo > terms * (near + (Real)0x1p-22f * fmax((Real)fabs(hi), (Real)fabs(lo))) + more;
     };
     bool sure = true;
     if (r.top_groups < r.groups) {
@@ -357,13 +359,15 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
         sh.base[threadIdx.x] = 0;
         __syncthreads();
     }
-    float bias[V];
+    float bias[V], most = 0.f;
     bool bad_bias = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         bias[v] = r.bias && lane * V + v < r.experts ? r.bias[lane * V + v] : 0.f;
         bad_bias |= !(bias[v] < __builtin_inff());
+        most = fmaxf(most, bias[v] == NONE ? 0.f : fabsf(bias[v]));
     }
+    if (r.group_best == 2) most = all_max<L>(most);   // only those counts need it
     const int64_t last = min((int64_t)(b + 1) * p.span, (int64_t)p.tokens);
     for (int64_t t0 = (int64_t)b * p.span; t0 < last; t0 += PER) {
         const int64_t t = t0 + threadIdx.x / L;
@@ -392,8 +396,8 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
         for (int v = 0; v < V; ++v) x[v] = bad ? NONE : x[v];
         int sel[2];
         float xs[2];
-        const bool sure = choose<L, V, float>(r, x, bias, lane, sel, xs);
-        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, lane, sel, xs);
+        const bool sure = choose<L, V, float>(r, x, bias, most, lane, sel, xs);
+        if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, most, lane, sel, xs);
 
         // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
         // so that p of far masked or shut out experts, below the least float, does not make 0 / 0

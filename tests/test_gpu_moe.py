@@ -92,6 +92,29 @@ def test_route_of_equal_and_nearly_equal_scores(gpu, score, biased, groups, top,
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(8, 4), (24, 12), (400, 50)])
+@pytest.mark.parametrize("most", [0.5, 64.0, 2.0 ** 20])
+def test_route_of_groups_whose_biases_cancel(gpu, score, E, groups, most):
+    """Runs that count their two highest, one far above and one far below zero: 32 bits round each by more than the counts differ,
+    2^-18 of a logit a step, which is far more than 64 bits lose."""
+    lh = gpu
+    announce(f"route groups with biases of {most} and {-most}, {score} {groups} runs")
+    rng = np.random.default_rng(21)
+    T, size = 120, E // groups
+    x = np.full((T, groups, size), -3.0)
+    x[:, :, :2] = 0.3
+    steps = rng.integers(0, 64, (T, groups))
+    x[:, :, 0] += steps * 2.0 ** -18
+    x[:, :, 1] += (np.argsort(rng.random((T, groups)), axis=1) + 64 - steps) * 2.0 ** -18
+    x = x.reshape(T, E).astype(np.float32)
+    bias = np.full((groups, size), -2 * most, np.float32)
+    bias[:, 0], bias[:, 1] = most, -most
+    bias = bias.ravel()
+    r = lh.MoeRouter(E, 2, score, up(lh, bias), groups, 2, 2)
+    check_route(route(lh, x, "f32", r), x, "f32", 2, score=score, bias=bias, groups=groups, top_groups=2, group_best=2)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("dtype,E,k,groups,top", [("f32", 40, 8, 1, 1), ("bf16", 40, 8, 5, 2), ("f16", 300, 9, 1, 1)])
 @pytest.mark.parametrize("renorm", [False, True])
 def test_route_of_masked_and_bad_logits(gpu, score, dtype, E, k, groups, top, renorm):
