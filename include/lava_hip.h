@@ -683,7 +683,7 @@ typedef struct lava_hip_w8_layer {
     const int8_t* w;
     const float* scale;
     const float* bias;     /* or NULL */
-    int64_t n;             /* channels; of a gated layer an even number */
+    int64_t n;             /* channels, at most 2^31 - 256; of a gated layer an even number */
     int64_t k;             /* at most 131071: the 32-bit sums of any bytes are exact */
     int64_t ldw;           /* >= k */
     int64_t expert_stride; /* >= n * ldw where experts > 1 */
@@ -733,7 +733,7 @@ typedef struct lava_hip_moe_router {
  * reads one; there nothing that offsets and order hold makes a kernel read or write outside the buffers: offsets are cut to
  * [0, tokens * top_k], and a row whose entry of order is outside [0, tokens * top_k) is left out. */
 typedef struct lava_hip_moe_plan {
-    int64_t tokens;      /* tokens * top_k below 2^31 */
+    int64_t tokens;      /* tokens * top_k at most 2^31 - 256 */
     int32_t experts;     /* 1 .. 1024 */
     int32_t top_k;       /* 1 .. 32 */
     int32_t* offsets;    /* device, experts + 1 */

@@ -576,7 +576,7 @@ int check_sizes(const char* name, int64_t tokens, int experts, int top_k) {
     LAVA_ARG(experts >= 1 && top_k >= 1, "%s: a plan of %d of %d experts", name, top_k, experts);
     LAVA_REQUIRE(experts <= MOE_EXPERTS && top_k <= MOE_TOP_K, LAVA_HIP_ERR_UNSUPPORTED,
                  "%s: a plan of %d of %d experts (at most %d of %d)", name, top_k, experts, MOE_TOP_K, MOE_EXPERTS);
-    LAVA_REQUIRE(tokens <= 0x7fffffff / top_k, LAVA_HIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d experts are too many", name,
+    LAVA_REQUIRE(tokens <= W8_MOST / top_k, LAVA_HIP_ERR_UNSUPPORTED, "%s: %lld tokens of %d experts are too many", name,
                  (long long)tokens, top_k);
     return LAVA_HIP_OK;
 }

@@ -106,7 +106,7 @@ int check_layer(const char* name, const lava_hip_w8_layer* l, const int8_t* X, c
                 int y_dtype, void* Y, int64_t ldy, bool nothing, W8Args& a) {
     LAVA_ARG(l != nullptr, "%s: null layer", name);
     LAVA_ARG(l->n >= 0 && l->k >= 0, "%s: negative extent (n=%lld k=%lld)", name, (long long)l->n, (long long)l->k);
-    LAVA_REQUIRE(l->n <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s: n = %lld is too large", name, (long long)l->n);
+    LAVA_REQUIRE(l->n <= W8_MOST, LAVA_HIP_ERR_UNSUPPORTED, "%s: n = %lld is too large", name, (long long)l->n);
     LAVA_REQUIRE(l->k <= 131071, LAVA_HIP_ERR_UNSUPPORTED, "%s: the sums of k = %lld products of bytes may leave 32 bits (at most 131071)",
                  name, (long long)l->k);
     LAVA_ARG(l->act >= LAVA_HIP_ACT_NONE && l->act <= LAVA_HIP_ACT_SILU, "%s: unknown activation %d", name, l->act);
@@ -166,7 +166,7 @@ int lava_hip_gemm_w8a8(const lava_hip_w8_layer* layer, const int8_t* X, const fl
                        int y_dtype, void* Y, int64_t ldy, void* stream) {
     W8Args a = {};
     LAVA_ARG(tokens >= 0, "gemm_w8a8: negative tokens (%lld)", (long long)tokens);
-    LAVA_REQUIRE(tokens <= 0x7fffffff, LAVA_HIP_ERR_UNSUPPORTED, "gemm_w8a8: %lld tokens are too many", (long long)tokens);
+    LAVA_REQUIRE(tokens <= W8_MOST, LAVA_HIP_ERR_UNSUPPORTED, "gemm_w8a8: %lld tokens are too many", (long long)tokens);
     const int rc = check_layer("gemm_w8a8", layer, X, x_scale, ldx, y_dtype, Y, ldy, tokens == 0, a);
     if (rc != LAVA_HIP_OK) return rc;
     LAVA_ARG(layer->experts == 1, "gemm_w8a8: a layer of %d experts", layer->experts);

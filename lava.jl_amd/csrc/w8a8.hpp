@@ -12,6 +12,9 @@
 
 namespace lava {
 
+// Channels and rows at most: the last tile's, up to 255 behind them, are counted in 32 bits too.
+constexpr int64_t W8_MOST = 0x7fffff00;
+
 struct W8Args {
     const int8_t* x;
     const float* xs;

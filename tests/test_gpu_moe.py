@@ -447,3 +447,83 @@ def test_a_captured_layer_of_experts(gpu, T):
         assert (np.abs(ref.to_float(got.T, "bf16") - out) <= slack).all()
     g.close()
     st.close()
+
+
+def test_two_layers_of_experts_at_once(gpu):
+    """On two streams, each with a plan of its own: the bits of one behind the other."""
+    lh = gpu
+    announce("two layers of experts at once")
+    rng = np.random.default_rng(31)
+    blocks = [Block(lh, rng, T, 16, 4, 256, 128) for T in (300, 170)]
+    streams = [lh.Stream() for _ in blocks]
+    for b in blocks:
+        T, E, _, D, _ = b.shape
+        b.set(rng.standard_normal((T, D)), rng.standard_normal((T, E)).astype(np.float32))
+    want = []
+    for b in blocks:
+        b.run()
+        lh.synchronize()
+        want.append(b.out.to_numpy())
+        b.out.fill_bytes(FILL)
+    lh.synchronize()
+    for _ in range(10):
+        for b, st in zip(blocks, streams):
+            b.run(st.handle)
+    for b, st, w in zip(blocks, streams, want):
+        st.synchronize()
+        np.testing.assert_array_equal(b.out.to_numpy(), w)
+        st.close()
+
+
+@pytest.mark.parametrize("T,E,k", [(16500, 16, 4), (33000, 130, 2)])
+def test_route_of_more_tokens_than_a_workgroup_has_at_once(gpu, T, E, k):
+    """Workgroups of 128 and 192 tokens."""
+    lh = gpu
+    announce(f"route {T} tokens, {k} of {E}")
+    x = np.random.default_rng(32).standard_normal((T, E)).astype(np.float32)
+    check_route(route(lh, x, "f32", lh.MoeRouter(E, k, "sigmoid")), x, "f32", k, score="sigmoid")
+
+
+# ---- sizes past 32 bits ------------------------------------------------------------------------
+
+def put(lh, a, at, b):
+    b = np.ascontiguousarray(b)
+    lh._lib.call("lava_hip_memcpy_h2d", a.ptr + at, b.ctypes.data, b.nbytes)
+
+
+@pytest.mark.parametrize("x_sorted", [False, True])
+def test_experts_whose_tokens_and_weights_pass_32_bits(gpu, choice, x_sorted):  # noqa: F811
+    """Rows 65536 bytes apart: the last token and the second expert lie 2 GiB behind the first."""
+    lh = gpu
+    announce(f"experts past 2 GiB, x_sorted={x_sorted}, choice {choice}")
+    T, N, K, ld, stride = 32790, 40, 128, 65536, 2 ** 31 + 65536
+    rng = np.random.default_rng(33)
+    seen = [0, 1, 70, T - 2, T - 1]
+    x, w = rng.integers(-127, 128, (len(seen), K)).astype(np.int8), rng.integers(-127, 128, (2, N, K)).astype(np.int8)
+    X, W = lh.HIPDeviceArray("i8", (ld * T,)), lh.HIPDeviceArray("i8", (stride + N * ld,))
+    Y = blank(lh, "f32", T, N)
+    ids = np.full((T, 1), -1, np.int32)
+    ids[seen, 0] = [0, 1, 1, 0, 1]
+    offsets, order = ref.plan(ids, 2)
+    at = [int(np.flatnonzero(order == t)[0]) if x_sorted else t for t in seen]
+    if x_sorted:      # the plan's rows moved to the end, so that they lie far from X
+        order = np.concatenate((np.full(T - 5, -1), order[:5])).astype(np.int32)
+        offsets = np.array([T - 5, T - 3, T], np.int32)
+        at = [T - 5 + a for a in at]
+    for a, row in zip(at, x):
+        put(lh, X, a * ld, row)
+    for e in range(2):
+        for n in range(N):
+            put(lh, W, e * stride + n * ld, w[e, n])
+    XS, WS, O, R = up(lh, np.ones(T, np.float32)), up(lh, np.ones((2, N), np.float32)), up(lh, offsets), up(lh, order)
+    layer = lh.w8_layer_raw(W.ptr, WS.ptr, N, K, ld, experts=2, expert_stride=stride)
+    try:
+        lh.experts_w8a8_raw(lh.moe_plan_raw(T, 2, 1, O.ptr, R.ptr), layer, X.ptr, XS.ptr, ld, "f32", Y.ptr, N, x_sorted=x_sorted)
+        lh.synchronize()
+        got = Y.to_numpy().T
+    finally:
+        for a in (X, W, Y):
+            a.close()
+    for i, t in enumerate(seen):
+        np.testing.assert_array_equal(got[t], w[ids[t, 0]].astype(np.float64) @ x[i].astype(np.float64))
+    assert untouched(np.delete(got, seen, 0))

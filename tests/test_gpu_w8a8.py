@@ -269,3 +269,56 @@ def test_quantised_tokens_through_a_layer(gpu, rng):
         lh.w8a8(Y, layer, X, S)
     with pytest.raises(ValueError):
         lh.quantize_i8(Q, WS, X)
+
+
+def test_a_layer_whose_tokens_and_channels_pass_32_bits(gpu, choice):
+    """Rows 65536 bytes apart: the last token and the last channel lie 2 GiB behind the first."""
+    lh = gpu
+    announce(f"linear past 2 GiB, choice {choice}")
+    K, ld, far = 128, 65536, 32800
+    rng = np.random.default_rng(12)
+    a = lh.HIPDeviceArray("i8", (ld * far,))
+    few, one = rng.integers(-127, 128, (40, K)).astype(np.int8), rng.integers(-127, 128, (3, K)).astype(np.int8)
+    seen = [0, 32768, far - 1]
+    a.fill_bytes(0)
+    for n, row in zip(seen, one):
+        lh._lib.call("lava_hip_memcpy_h2d", a.ptr + n * ld, row.ctypes.data, K)
+    F, ones = up(lh, few), up(lh, np.ones(far, np.float32))
+    try:
+        for far_tokens in (False, True):
+            T, N = (far, 40) if far_tokens else (40, far)
+            Y = blank(lh, "f32", T, N)
+            X, W = (a, F) if far_tokens else (F, a)
+            layer = lh.w8_layer_raw(W.ptr, ones.ptr, N, K, K if far_tokens else ld)
+            lh.w8a8_raw(layer, X.ptr, ones.ptr, T, ld if far_tokens else K, "f32", Y.ptr, N)
+            lh.synchronize()
+            got = Y.to_numpy() if far_tokens else Y.to_numpy().T      # (40, far)
+            Y.close()
+            want = np.zeros((40, far))
+            want[:, seen] = few.astype(np.float64) @ one.T.astype(np.float64)
+            np.testing.assert_array_equal(got, want)
+    finally:
+        a.close()
+
+
+def test_quantize_around_2_32_threads(gpu):
+    """Launches of 2^32 threads in one dimension, which HIP runs modulo 2^32, are refused by name."""
+    lh = gpu
+    T = 2 ** 24
+    announce(f"quantize {T} rows of 1")
+    X, Q, S = lh.HIPDeviceArray("f16", (T,)), lh.HIPDeviceArray("i8", (T,)), lh.HIPDeviceArray("f32", (T,))
+    try:
+        X.fill_bytes(0x3c)
+        Q.fill_bytes(FILL)
+        lh.synchronize()
+        with pytest.raises(lh.Unsupported, match="quantize_kernel"):
+            lh.quantize_i8_raw("f16", X.ptr, Q.ptr, S.ptr, 1, T, 1, 1)
+        lh.synchronize()
+        assert untouched(Q.to_numpy())
+        lh.quantize_i8_raw("f16", X.ptr, Q.ptr, S.ptr, 1, T - 1, 1, 1)
+        lh.synchronize()
+        q = Q.to_numpy()
+        assert (q[:-1] == 127).all() and q[-1] == FILL
+    finally:
+        for a in (X, Q, S):
+            a.close()

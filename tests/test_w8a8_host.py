@@ -238,3 +238,15 @@ def test_the_reference_routes_as_written():
     assert ids.tolist() == [[0, 1]]
     ids, w = ref.route(np.full((1, 4), -np.inf), 2, "softmax")
     assert ids.tolist() == [[-1, -1]] and not w.any()
+
+
+def test_the_last_tiles_rows_and_channels_are_counted_in_32_bits():
+    """A tile begun at 2^31 - 256 or behind ends past 2^31."""
+    top = 2 ** 31 - 256
+    with pytest.raises(lh.Unsupported, match="too large"):
+        linear(layer(n=top + 1), ldy=top + 1)
+    with pytest.raises(lh.Unsupported, match="too many"):
+        linear(tokens=top + 1)
+    with pytest.raises(lh.Unsupported, match="too many"):
+        lh.moe_plan_workspace_bytes(top // 8 + 1, 64, 8)
+    assert lh.moe_plan_workspace_bytes(top // 8, 64, 8) == 256 * 64 * 4
