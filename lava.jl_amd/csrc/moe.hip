@@ -28,6 +28,7 @@ constexpr int MOE_THREADS = 1024, MOE_WAVES = MOE_THREADS / 64;
 constexpr int MOE_EXPERTS = 1024, MOE_TOP_K = 32;
 constexpr int MOE_BLOCKS = 256;    // workgroups that share a sort, at most
 constexpr int MOE_SPAN = 64;       // tokens a workgroup, at least
+constexpr int MOE_COLUMNS = 8;     // of a row that a thread sums
 
 struct Plan {   // what a kernel needs of a plan
     int32_t* offsets;   // null: none is written
@@ -511,23 +512,33 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_place_kernel(const int32_t* _
     finish_plan(p, ids, blockIdx.x, gridDim.x, before, all, sh.base, below, sh.tmp);
 }
 
-// A thread 4 columns of a token; the plain form of any alignment one column.
-template <typename T, int C>
+// A thread 8 columns of a token, of any alignment.  Bound by the bytes: 8 rows of 2048 bf16 for 8192 tokens 48.2 us, 6.3 TB/s (with 4
+// columns a thread 57.6, with 2 94.5); rows of 2047 54.2.
+template <typename T>
 __global__ void __launch_bounds__(256) moe_combine_kernel(const T* __restrict__ Y, int64_t ldy, const int32_t* __restrict__ ids,
                                                           const float* __restrict__ weights, int top_k, int64_t n,
                                                           const T* base, int64_t ldb, T* out, int64_t ldo, int per_row) {
+    constexpr int C = MOE_COLUMNS;
+    typedef T Tv __attribute__((ext_vector_type(C)));
+    typedef Tv Tvu __attribute__((aligned(sizeof(T))));
     const int64_t t = blockIdx.x / per_row;
     const int64_t col = ((int64_t)(blockIdx.x % per_row) * 256 + threadIdx.x) * C;
     if (col >= n) return;
-    typedef T Tv __attribute__((ext_vector_type(C)));
+    const bool whole = col + C <= n;
+    auto load = [&](const T* p) __attribute__((always_inline)) {
+        if (whole) return (Tv)*reinterpret_cast<const Tvu*>(p);
+        Tv v;
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[i] = col + i < n ? p[i] : (T)0.f;
+        return v;
+    };
     float sum[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) sum[i] = 0.f;
     if (base) {
-        const Tv v = *reinterpret_cast<const Tv*>(base + t * ldb + col);
+        const Tv v = load(base + t * ldb + col);
 #pragma unroll
         for (int i = 0; i < C; ++i) sum[i] = (float)v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < C; ++i) sum[i] = 0.f;
     }
     for (int j = 0; j < top_k; ++j) {
         const int64_t a = t * top_k + j;
@@ -537,14 +548,21 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const T* __restrict__ 
             for (int i = 0; i < C; ++i) sum[i] += w * 0.f;
             continue;
         }
-        const Tv v = *reinterpret_cast<const Tv*>(Y + a * ldy + col);
+        const Tv v = load(Y + a * ldy + col);
 #pragma unroll
         for (int i = 0; i < C; ++i) sum[i] = __builtin_fmaf(w, (float)v[i], sum[i]);
     }
-    Tv o;
+    T* o = out + t * ldo + col;
+    Tv r;
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = narrow<T>(sum[i]);
-    *reinterpret_cast<Tv*>(out + t * ldo + col) = o;
+    for (int i = 0; i < C; ++i) r[i] = narrow<T>(sum[i]);
+    if (whole) {
+        *reinterpret_cast<Tvu*>(o) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (col + i < n) o[i] = r[i];
+    }
 }
 
 namespace {
@@ -629,17 +647,11 @@ int launch_route(const Router& r, const void* logits, int64_t ldl, int32_t* ids,
 template <typename T>
 int launch_combine(const void* Y, int64_t ldy, const int32_t* ids, const float* weights, int64_t tokens, int top_k, int64_t n,
                    const void* base, int64_t ldb, void* out, int64_t ldo, hipStream_t s) {
-    const bool vec = n % 4 == 0 && ldy % 4 == 0 && ldo % 4 == 0 && (base == nullptr || ldb % 4 == 0) &&
-                     aligned(Y, 4 * sizeof(T)) && aligned(out, 4 * sizeof(T)) && aligned(base, 4 * sizeof(T));
-    const int64_t per_row = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+    const int64_t per_row = (n + 256 * MOE_COLUMNS - 1) / (256 * MOE_COLUMNS);
     LAVA_REQUIRE(per_row <= 0x7fffffff && tokens <= 0xffffff / per_row, LAVA_HIP_ERR_UNSUPPORTED,
                  "moe_combine: %lld tokens of %lld values are too many", (long long)tokens, (long long)n);
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(tokens * per_row)), dim3(256), 0, s, static_cast<const T*>(Y), ldy, ids, weights,
-                           top_k, n, static_cast<const T*>(base), ldb, static_cast<T*>(out), ldo, (int)per_row);
-    };
-    if (vec) go(moe_combine_kernel<T, 4>);
-    else go(moe_combine_kernel<T, 1>);
+    hipLaunchKernelGGL(moe_combine_kernel<T>, dim3((unsigned)(tokens * per_row)), dim3(256), 0, s, static_cast<const T*>(Y), ldy, ids,
+                       weights, top_k, n, static_cast<const T*>(base), ldb, static_cast<T*>(out), ldo, (int)per_row);
     LAVA_LAUNCH_CHECK("moe_combine_kernel");
     return LAVA_HIP_OK;
 }

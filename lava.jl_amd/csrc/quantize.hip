@@ -1,7 +1,7 @@
 // quantize.hip -- rows of values to 8 bits with a scale a row.
 //
 // q is the integer nearest to the real number 127 x / max |x|.  In 32 bits t = x * (127 / max) is off by at most 2 half
-// ulps, 127 * 2 * 2^-24 < 2e-5, so t rounds to the right integer unless it lies that near to a border between two; there
+// ulps, 127 * 2 * 2^-24 < 1.6e-5, so t rounds to the right integer unless it lies that near to a border between two; there
 // 254 |x| against (2 n + 1) max, products that are exact in 64 bits, decides (ties to even).
 #include <hip/hip_runtime.h>
 
@@ -16,14 +16,6 @@ namespace {
 
 // |x| as bits that compare like |x|; infinities and NaN are at least 0x7f800000
 __device__ __forceinline__ uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-__device__ __noinline__ float nearest_exact(float x, float top) {
-    const double a = 254.0 * (double)fabsf(x), lo = floor(a / (2.0 * (double)top));
-    const double border = (2.0 * lo + 1.0) * (double)top;
-    // a / (2 top) may round up to the next integer: then a < 2 lo top, below the border all the same
-    const double n = a > border || (a == border && fmod(lo, 2.0) == 1.0) ? lo + 1.0 : lo;
-    return copysignf((float)n, x);
-}
 
 struct Scale {
     float top;     // max |x|
@@ -40,15 +32,25 @@ __device__ __forceinline__ Scale make_scale(uint32_t bits) {
     return s;
 }
 
+constexpr float NEAR_BORDER = 0.49998f;
+
+// The integer for an x whose t lies near a border.
+__device__ __forceinline__ float by_border(float x, float t, float top) {
+    const float n = floorf(fabsf(t));
+    const double a = 254.0 * (double)fabsf(x), border = (2.0 * (double)n + 1.0) * (double)top;
+    return copysignf(a > border || (a == border && ((int)n & 1)) ? n + 1.f : n, x);
+}
+
 __device__ __forceinline__ float nearest(float x, const Scale& s) {
     const float t = (x * s.up) * s.r, q = rintf(t);
-    if (__builtin_expect(fabsf(t - q) > 0.4999f, 0)) return nearest_exact(x, s.top);
+    if (__builtin_expect(fabsf(t - q) > NEAR_BORDER, 0)) return by_border(x, t, s.top);
     return q;
 }
 
 }  // namespace
 
-// Rows held in registers, THREADS lanes a row, CH chunks of 8 values a lane; chunks aligned to 16 bytes (of Q to 8).
+// Rows held in registers, THREADS lanes a row, CH chunks of 8 values a lane, of any alignment.  Bound by the bytes: 40961 rows of
+// 1408 bf16 30.8 us, 5.6 TB/s; a single row by its launch and a chain of reads, 2 to 3 us.
 template <typename T, int THREADS, int CH>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
     quantize_rows_kernel(const T* __restrict__ X, int8_t* __restrict__ Q, float* __restrict__ scale, int k, int tokens, int64_t ldx,
@@ -56,6 +58,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
     constexpr int BLOCK = THREADS < 256 ? 256 : THREADS, WAVES = THREADS / 64;
     __shared__ uint32_t part[WAVES];
     typedef T T8 __attribute__((ext_vector_type(8)));
+    typedef T8 T8u __attribute__((aligned(sizeof(T))));
+    typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(1)));
     const int64_t row = (int64_t)blockIdx.x * (BLOCK / THREADS) + threadIdx.x / THREADS;
     if (row >= tokens) return;   // whole wavefronts: THREADS is a multiple of 64
     const int t = threadIdx.x % THREADS;
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
     for (int c = 0; c < CH; ++c) {
         const int at = 8 * (c * THREADS + t);
         if (at + 8 <= k) {
-            v[c] = __builtin_nontemporal_load(reinterpret_cast<const T8*>(x + at));
+            v[c] = __builtin_nontemporal_load(reinterpret_cast<const T8u*>(x + at));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] = at + i < k ? x[at + i] : (T)0.f;
@@ -100,13 +104,20 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
             y[i] = z + 12582912.f;
             off = fmaxf(off, fabsf(z - (y[i] - 12582912.f)));
         }
-        if (__builtin_expect(!(plain && off <= 0.4999f), 0)) {
+        if (__builtin_expect(!plain || !s.ok, 0)) {
 #pragma unroll 1
             for (int i = 0; i < 8; ++i) {
                 const float n = s.ok ? nearest((float)v[c][i], s) : 0.f;
                 if (at + i < k) q[at + i] = (int8_t)(int)n;
             }
             continue;
+        }
+        if (__builtin_expect(off > NEAR_BORDER, 0)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float z = (float)v[c][i] * s.r;
+                if (fabsf(z - (y[i] - 12582912.f)) > NEAR_BORDER) y[i] = 12582912.f + by_border((float)v[c][i], z, s.top);
+            }
         }
         uint32_t word[2];
 #pragma unroll
@@ -116,7 +127,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
             word[h] = lo | hi << 16;
         }
         if (at + 8 <= k) {
-            *reinterpret_cast<uint2*>(q + at) = uint2{word[0], word[1]};
+            *reinterpret_cast<u32x2u*>(q + at) = u32x2u{word[0], word[1]};
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -125,7 +136,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS)
     }
 }
 
-// A workgroup a row, any alignment and length; the row is read twice.
+// A workgroup a row, of any length; the row is read twice.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ X, int8_t* __restrict__ Q,
                                                        float* __restrict__ scale, int64_t k, int64_t ldx, int64_t ldq) {
@@ -148,8 +159,7 @@ template <typename T>
 static int launch_quantize(const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens, int64_t ldx, int64_t ldq,
                            hipStream_t s) {
     const T* x = static_cast<const T*>(X);
-    const bool chunks = aligned(X, 16) && ldx * (int64_t)sizeof(T) % 16 == 0 && aligned(Q, 8) && ldq % 8 == 0;
-    if (!chunks || k == 0 || k > 65536) {
+    if (k == 0 || k > 65536) {
         hipLaunchKernelGGL(quantize_kernel<T>, dim3((unsigned)tokens), dim3(256), 0, s, x, Q, scale, k, ldx, ldq);
         LAVA_LAUNCH_CHECK("quantize_kernel");
         return LAVA_HIP_OK;
@@ -159,8 +169,11 @@ static int launch_quantize(const void* X, int8_t* Q, float* scale, int64_t k, in
         hipLaunchKernelGGL(kernel, dim3((unsigned)((tokens + per - 1) / per)), dim3(threads < 256 ? 256 : threads), 0, s, x, Q, scale,
                            (int)k, (int)tokens, ldx, ldq);
     };
-    // a wavefront a row where there are rows for all CUs, else more lanes, fewer values each
-    const int threads = k <= 512 || (k <= 4096 && tokens >= 1024) ? 64 : k <= 16384 ? 256 : 1024;
+    // A wavefront a row where a lane has few values or there are rows for all CUs many times over, a workgroup of 256 for longer
+    // rows, of 1024 for few long ones.  us with 64 / 256 / 1024 lanes a row of bf16: 40961 x 1408 30.8 / 48.9 / 161, 16384 x 2048
+    // 20.8 / 23.3 / 66, 8192 x 4096 24.9 / 20.0 / 38.6, 1024 x 2048 6.7 / 4.5 / 6.2, 8192 x 8192 - / 34.8 / 47.6, 1024 x 14336 - /
+    // 16.8 / 13.3, 1 x 14336 - / 5.9 / 4.0.
+    const int threads = k <= 1024 || (k <= 2048 && tokens >= 8192) ? 64 : k > 16384 || (k > 4096 && tokens <= 1024) ? 1024 : 256;
     const int ch = (int)((k + 8 * threads - 1) / (8 * threads));
     auto by_ch = [&](auto ttag) {
         constexpr int N = decltype(ttag)::value;

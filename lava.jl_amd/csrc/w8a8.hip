@@ -139,7 +139,6 @@ int check_layer(const char* name, const lava_hip_w8_layer* l, const int8_t* X, c
     a.act = l->act;
     a.gated = l->gated != 0;
     a.y_dtype = y_dtype;
-    a.yvec = aligned(Y, 16) && ldy * (int64_t)ysz % 16 == 0;
     return LAVA_HIP_OK;
 }
 

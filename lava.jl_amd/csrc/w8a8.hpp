@@ -32,7 +32,6 @@ struct W8Args {
     int top_k, experts;
     int act, gated, y_dtype;
     int x_sorted, y_sorted;
-    int yvec;                 // Y takes 16 bytes a store
 };
 
 struct W8Tile {
@@ -124,16 +123,17 @@ __device__ __forceinline__ void w8_act4(int act, float (&v)[4]) {
     }
 }
 
-// `left` columns of a row of Y, at most C (4 or 8), from element offset `at` on.
+// `left` columns of a row of Y, at most C (4 or 8), from element offset `at` on, of any alignment.
 template <typename T, int C>
 __device__ __forceinline__ void w8_put(const W8Args& a, int64_t at, int left, const float (&v)[C]) {
     typedef T Tv __attribute__((ext_vector_type(C)));
+    typedef Tv Tvu __attribute__((aligned(sizeof(T))));
     T* p = static_cast<T*>(a.y) + at;
-    if (a.yvec && left >= C) {
+    if (left >= C) {
         Tv o;
 #pragma unroll
         for (int r = 0; r < C; ++r) o[r] = narrow<T>(v[r]);
-        __builtin_nontemporal_store(o, reinterpret_cast<Tv*>(p));
+        __builtin_nontemporal_store((Tvu)o, reinterpret_cast<Tvu*>(p));
     } else {
 #pragma unroll
         for (int r = 0; r < C; ++r)
