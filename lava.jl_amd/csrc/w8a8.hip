@@ -26,7 +26,8 @@ __device__ __forceinline__ uint4 load16(const int8_t* row, int k, int end) {
 
 // Any layout: 64 rows x 64 channels a workgroup of 4 wavefronts, K 64 at a time through registers and LDS, one 16x16x64
 // MFMA a wavefront and block of 16 channels.  Of a gated layer's 64 channels each second block of 16 is the other half's, so that a
-// lane holds a column's gate and its factor.
+// lane holds a column's gate and its factor.  Bound by the latency of one chunk of K in flight: 333 rows x 14336 x 4096 72 us (540 TOP/s),
+// with rows of 4095 bytes 100; one row x 4096 x 4096 28 us.
 __global__ void __launch_bounds__(256) w8a8_generic_kernel(W8Args a, int tiles_n) {
     __shared__ __attribute__((aligned(16))) int8_t sx[WG_TILE * WG_PITCH], sw[WG_TILE * WG_PITCH];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;

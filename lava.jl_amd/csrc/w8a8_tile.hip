@@ -1,15 +1,20 @@
 // w8a8_tile.hip -- layers with 8-bit weights and tokens on tiles of 64 x 64 to 256 x 256 (rows x channels).
 //
-// The loop is the tile GEMM's (gemm_tn_kernel.hpp): 4 wavefronts, each 16 WM rows x 16 WN channels in 16x16x64 MFMAs; K 128
-// bytes at a time, both operands' slices straight to LDS (buffer_load ... lds, 16-byte chunk c of row r at slot c ^ r % 8, so
-// that a fragment's 16 rows lie on all banks), ST stages, one barrier in the middle of a stage: the MFMAs of its first half
-// run while the second half's fragments are read, those of the second half while the next stage's are read and the one ST
+// The loop is the tile GEMM's (gemm_tn_kernel.hpp): 4 wavefronts, of the largest tile 8, each 16 WM rows x 16 WN channels in
+// 16x16x64 MFMAs; K 128 bytes at a time, both operands' slices straight to LDS (buffer_load ... lds, 16-byte chunk c of row r at slot
+// c ^ r % 8, so that a fragment's 16 rows lie on all banks), ST stages, one barrier in the middle of a stage: the MFMAs of its first
+// half run while the second half's fragments are read, those of the second half while the next stage's are read and the one ST
 // further on is requested.  What differs:
 //  * a row of X is found by the plan, so a lane keeps one offset for each of its requests (rows and channels that are none,
 //    and chunks past K, get an offset outside the buffer and read zero);
 //  * a gated layer's tile has 16 channels of the gate and their 16 factors in turn, so that a lane has both of a column in its
 //    accumulators;
 //  * the sums go through LDS to lanes that have 8 columns of a row, which they finish, round to Y's type and store.
+// Measured: 8192 rows x 28672 gated channels x 4096 730 to 790 us (2440 to 2640 TOP/s) on 256 x 256 tiles, whose matrix cores are 0.66
+// busy at a clock that falls to 1.8 GHz under them (with 4 wavefronts of 128 x 128 0.57 and 1.9, 760 to 780 us; 16384 rows x 8192 x 1024
+// 181 us against 230); 16 rows x 14336 x 4096 11.6 us, 5.1 TB/s of weights; 64 tokens' 8 of 64 experts, gate and up of 2816 x 2048,
+// 64 us, 5.7 TB/s.  Between those, latency: of a tile's first requests and of its finish where K is short, of requests that miss
+// L2 (two or three stages in flight a workgroup).
 #include <math.h>
 
 #include "gemm_tn_kernel.hpp"
@@ -17,11 +22,12 @@
 
 namespace lava {
 
-template <int WM, int WN, int ST, bool GATED>
-__global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
-    constexpr int BM = 32 * WM, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
+template <int MW, int WM, int WN, int ST, bool GATED>
+__global__ void __launch_bounds__(128 * MW, MW == 2 && ST * (WM + WN) <= 19 ? 2 : 1)
+    w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
+    constexpr int WAVES = 2 * MW, BM = 16 * WM * MW, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
     constexpr int Q = WM * WN, R = WM + WN;               // of a wavefront: MFMAs of half a stage, fragments read beside them
-    constexpr int XD = WM, D = R;                         // and its requests of a stage, those for X first
+    constexpr int XD = WM, D = WM + 2 * WN / MW;          // and its requests of a stage, those for X first
     static_assert(WM % 2 == 0 && (!GATED || WN % 2 == 0), "rows are finished 32 at a time, gates and factors are blocks of 16");
     static_assert(WN == 2 || WN == 4 || WN == 8, "a power of two of lanes finishes a row");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * STAGE];
@@ -40,7 +46,7 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
 
     // What the finish needs, requested first and held until then: of row threadIdx.x its scale and row of Y, of channel row
     // threadIdx.x its scale and bias.
-    static_assert(BM <= 256 && BN <= 256, "a row and a channel a thread");
+    static_assert(BM <= 128 * MW && BN <= 128 * MW, "a row and a channel a thread");
     float held_xs = 0.f, held_ws = 0.f, held_bias = 0.f;
     int held_yr = -1;
     if (threadIdx.x < (unsigned)tile.rows) {
@@ -97,7 +103,7 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
         }
     };
     // Before the last stage's requests: chunks past K get an offset that reads zero (once, in the kept offsets: a
-    // choice at every request costs the compiler the accumulators' places, 8192 gated rows 1183 us against 780).
+    // choice at every request costs the compiler the accumulators' places, 8192 gated rows 1183 us against 780, with 4 wavefronts).
     const int ktiles = (a.k + TN_KB - 1) / TN_KB;
     auto cut_k = [&]() __attribute__((always_inline)) {
         const bool in = (ktiles - 1) * TN_KB + chunk < a.k;
@@ -188,9 +194,10 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
     __syncthreads();
     constexpr int COLS = GATED ? 8 * WN : 16 * WN;         // of Y, a wavefront's
     constexpr int PITCH = 16 * WN * 4 + 16;                // padded: the 16 rows of a store start on distinct banks
-    static_assert(4 * 32 * PITCH <= ST * STAGE, "four wavefronts' rows in the stages' LDS");
+    constexpr int EI = WAVES * 32 * PITCH <= ST * STAGE ? 2 : 1;   // blocks of 16 rows at a time
+    static_assert(WAVES * EI * 16 * PITCH <= ST * STAGE, "the wavefronts' rows in the stages' LDS");
     constexpr int LANES = COLS / 8, ROWS = 64 / LANES;     // lanes a row, rows a pass
-    uint8_t* ep = smem + w * 32 * PITCH;
+    uint8_t* ep = smem + w * EI * 16 * PITCH;
     const int cc = (lane % LANES) * 8;                     // this lane's first column of the wavefront's
     const int cr = GATED ? (cc >> 4) * 32 + (cc & 15) : cc;   // and channel row
     const int left = a.n_out - (col0 + wn * COLS + cc);    // columns of Y from there on
@@ -201,17 +208,17 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
         ws[h] = *reinterpret_cast<const f32x4*>(s_ws + c);
         bs[h] = *reinterpret_cast<const f32x4*>(s_bias + c);
     }
-    auto rows32 = [&](auto itag) __attribute__((always_inline)) {
+    auto finish = [&](auto itag) __attribute__((always_inline)) {
         constexpr int i0 = decltype(itag)::value;
 #pragma unroll
-        for (int ii = 0; ii < 2; ++ii)
+        for (int ii = 0; ii < EI; ++ii)
 #pragma unroll
             for (int j = 0; j < WN; ++j)
                 *reinterpret_cast<i32x4*>(ep + (16 * ii + (lane & 15)) * PITCH + (16 * j + 4 * (lane >> 4)) * 4) = acc[i0 + ii][j];
         __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the wavefront's sums are in LDS
         __builtin_amdgcn_wave_barrier();
 #pragma unroll 2
-        for (int t = 0; t < 32 / ROWS; ++t) {
+        for (int t = 0; t < 16 * EI / ROWS; ++t) {
             const int row = t * ROWS + lane / LANES, at = wm * 16 * WM + 16 * i0 + row;
             const float xs = s_xs[at];
             const int yr = s_yr[at];
@@ -222,30 +229,32 @@ __global__ void __launch_bounds__(256, ST * (WM + WN) > 19 ? 1 : 2) w8a8_tile_ke
         __builtin_amdgcn_s_waitcnt(0xc07f);   // read before the next rows overwrite them
         __builtin_amdgcn_wave_barrier();
     };
-    rows32(std::integral_constant<int, 0>{});
-    if constexpr (WM > 2) rows32(std::integral_constant<int, 2>{});
-    if constexpr (WM > 4) rows32(std::integral_constant<int, 4>{});
-    if constexpr (WM > 6) rows32(std::integral_constant<int, 6>{});
+    finish(std::integral_constant<int, 0>{});
+    if constexpr (WM > EI) finish(std::integral_constant<int, EI>{});
+    if constexpr (WM > 2 * EI) finish(std::integral_constant<int, 2 * EI>{});
+    if constexpr (WM > 3 * EI) finish(std::integral_constant<int, 3 * EI>{});
+    static_assert(WM <= 4 * EI, "four times");
 }
 
-template <int WM, int WN, int ST>
+template <int MW, int WM, int WN, int ST>
 int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
     const int cols = (a.gated ? 16 : 32) * WN;
-    const int64_t tm = w8_row_tiles(a, 32 * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;
+    const int64_t tm = w8_row_tiles(a, 16 * MW * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;
     LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s would need %lld workgroups", name, (long long)(tm * tn));
     const dim3 grid((unsigned)(tm * tn));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a, (int)tm, (int)tn); };
-    a.gated ? go(w8a8_tile_kernel<WM, WN, ST, true>) : go(w8a8_tile_kernel<WM, WN, ST, false>);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(128 * MW), 0, s, a, (int)tm, (int)tn); };
+    a.gated ? go(w8a8_tile_kernel<MW, WM, WN, ST, true>) : go(w8a8_tile_kernel<MW, WM, WN, ST, false>);
     LAVA_LAUNCH_CHECK(name);
     return LAVA_HIP_OK;
 }
 
-// What a tile of 64 x 64, 64 x 128, 128 x 128 or 256 x 256 costs a CU that has others to run beside it (the largest has none): us
-// before and behind the loop, and us each 128 bytes of K.  Measured at 4096 x 4096 with K from 128 to 5632.
+// What a tile of 64 x 64, 64 x 128, 128 x 128 or 256 x 256 costs a CU: us before and behind the loop, and us each 128 bytes of K.
+// Fitted to the times of all four at 700 shapes of 40 to 8192 rows, 1024 to 20480 channels and K of 128 to 7168.
 constexpr struct {
     int bm, bn;
     float fixed, stage;
-} W8_TILES[4] = {{64, 64, 0.85f, 0.215f}, {64, 128, 1.7f, 0.356f}, {128, 128, 3.5f, 0.61f}, {256, 256, 16.f, 1.75f}};
+} W8_TILES[4] = {{64, 64, 0.9f, 0.25f}, {64, 128, 1.7f, 0.44f}, {128, 128, 5.f, 0.49f}, {256, 256, 15.f, 1.12f}};
+constexpr float W8_END = 0.31f;
 
 bool w8_tile_fits(const W8Args& a, int tile) {
     return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, W8_TILES[tile].bm, W8_TILES[tile].bn);
@@ -261,10 +270,11 @@ double w8_tile_count(const W8Args& a, int bm, int bn) {
     return (met > whole ? met : whole) * tn;
 }
 
-// The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and a third of one for the end.
-// us, this rule's / the others of {64 x 64, 64 x 128, 128 x 128, 256 x 256}: 64 rows x 14336 x 4096 12.3 / 14.9, 25.8, 48; 128 rows
-// 15.2 / 16.2, 27, 50; 333 rows 30.6 / 42.6, 32.7, 52.7; 1024 x 4096 x 4096 21.1 / 28.5, 24.9, 51; 4096 x 4096 x 4096 62 / 94 (128 x 128); 5003
-// tokens, 4 of 60 experts of 2048 x 1408, 105.8 / 137, 111.7, 153; 1000 tokens, 8 of 64, 61.7 / 70.6, 65.4, 92.
+// The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and a third of one for the end.  Over those
+// shapes 1.4 % behind the best of the four (at worst a fifth, at K of 256 and below), over 200 plans of 8 to 256 experts 3 %.
+// us of {64 x 64, 64 x 128, 128 x 128, 256 x 256}, the rule's in brackets: 64 rows x 14336 x 4096 {[17.1], 22.4, 24.6, 54}, 333 rows
+// {47.7, 42.1, [38.6], 56}, 2048 x 4096 x 4096 {53.6, 51.3, [36.7], 49.6}, 4096 x 4096 x 4096 {103, 91, 70, [58.8]}, 5003 tokens and 4 of
+// 60 experts of 2048 x 1408 {168, 128, 130, [131]}, of 2816 x 2048 {304, 236, 228, [212]}.
 int w8_tile_choice(const W8Args& a) {
     const double stages = (a.k + TN_KB - 1) / TN_KB;
     int best = -1;
@@ -272,7 +282,7 @@ int w8_tile_choice(const W8Args& a) {
     for (int i = 0; i < 4; ++i) {
         if (!w8_tile_fits(a, i)) continue;
         const double per_cu = w8_tile_count(a, W8_TILES[i].bm, W8_TILES[i].bn) / 256;
-        const double cost = (per_cu <= 1 ? 1 : per_cu + 0.35) * (W8_TILES[i].fixed + W8_TILES[i].stage * stages);
+        const double cost = (per_cu <= 1 ? 1 : per_cu + W8_END) * (W8_TILES[i].fixed + W8_TILES[i].stage * stages);
         if (best < 0 || cost < least) {
             best = i;
             least = cost;
@@ -286,10 +296,10 @@ int launch_w8_tile(const W8Args& a, int tile, hipStream_t s) {
     // 4096, 256 tiles, 26.8 / 21.1; 2048 rows 36 / 41.6).
     const bool lone = w8_tile_count(a, W8_TILES[tile].bm, W8_TILES[tile].bn) <= 256;
     switch (tile) {
-    case 0: return lone ? launch_tile<2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
-    case 1: return lone ? launch_tile<2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
-    case 2: return lone ? launch_tile<4, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
-    default: return launch_tile<8, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
+    case 0: return lone ? launch_tile<2, 2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
+    case 1: return lone ? launch_tile<2, 2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
+    case 2: return lone ? launch_tile<2, 4, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<2, 4, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
+    default: return launch_tile<4, 4, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
     }
 }
 
