@@ -153,7 +153,7 @@ void lava_hip_kernel_log_clear(void);
  *                        3 the tile kernel (D <= 128) with 256 rows a tile, 4 with 128;
  *  LAVA_HIP_FAMILY_W8A8: layers with 8-bit tokens: 1 the generic kernel, 2 the streaming kernel of few
  *                        rows, 3 the tile kernel with 64 x 64 rows and channels a tile, 4 with 64 x 128, 5 with
- *                        128 x 128, 6 with 256 x 256.
+ *                        128 x 128, 6 with 128 x 256, 7 with 256 x 256.
  * Unknown families or choices return LAVA_HIP_ERR_INVALID_ARG. */
 /* Reads [src, src + bytes) once with 16-byte nontemporal loads, `unroll` (4, 8 or 16) in flight
  * per thread, `blocks` workgroups of 256 threads, and writes the XOR of what each thread read to

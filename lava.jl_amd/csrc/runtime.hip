@@ -242,7 +242,7 @@ int lava_hip_set_kernel_override(int family, int choice) {
     const bool ok = (family == LAVA_HIP_FAMILY_ATTN && (choice == 0 || choice == 3 || choice == 5)) ||
                     (family == LAVA_HIP_FAMILY_GEMM && choice >= 0 && choice <= 4) ||
                     (family == LAVA_HIP_FAMILY_PAGED && choice >= 0 && choice <= 4) ||
-                    (family == LAVA_HIP_FAMILY_W8A8 && choice >= 0 && choice <= 6);
+                    (family == LAVA_HIP_FAMILY_W8A8 && choice >= 0 && choice <= 7);
     LAVA_ARG(ok, "set_kernel_override: unknown family %d or choice %d", family, choice);
     g_override[family].store(choice, std::memory_order_relaxed);
     return LAVA_HIP_OK;

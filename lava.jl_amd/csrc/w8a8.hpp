@@ -212,8 +212,9 @@ int launch_w8_generic(const W8Args& a, hipStream_t s);
 bool w8_stream_fits(const W8Args& a);
 bool w8_stream_preferred(const W8Args& a);
 int launch_w8_stream(const W8Args& a, hipStream_t s);
-// Tiles (w8a8_tile.hip): 0 to 3 for 64 x 64, 64 x 128, 128 x 128 and 256 x 256 rows and channels; the one to take, -1 if none fits;
+// Tiles (w8a8_tile.hip): 64 x 64, 64 x 128, 128 x 128, 128 x 256 and 256 x 256 rows and channels; the one to take, -1 if none fits;
 // how many a call has (of a plan: is likely to have); the experts that are likely to have rows (w8_met).
+constexpr int W8_TILE_KINDS = 5;
 bool w8_tile_fits(const W8Args& a, int tile);
 int w8_tile_choice(const W8Args& a);
 double w8_tile_count(const W8Args& a, int bm, int bn);

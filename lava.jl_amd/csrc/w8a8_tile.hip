@@ -1,6 +1,6 @@
 // w8a8_tile.hip -- layers with 8-bit weights and tokens on tiles of 64 x 64 to 256 x 256 (rows x channels).
 //
-// The loop is the tile GEMM's (gemm_tn_kernel.hpp): 4 wavefronts, of the largest tile 8, each 16 WM rows x 16 WN channels in
+// The loop is the tile GEMM's (gemm_tn_kernel.hpp): 4 wavefronts, of tiles above 64 rows 8, each 16 WM rows x 16 WN channels in
 // 16x16x64 MFMAs; K 128 bytes at a time, both operands' slices straight to LDS (buffer_load ... lds, 16-byte chunk c of row r at slot
 // c ^ r % 8, so that a fragment's 16 rows lie on all banks), ST stages, one barrier in the middle of a stage: the MFMAs of its first
 // half run while the second half's fragments are read, those of the second half while the next stage's are read and the one ST
@@ -22,8 +22,9 @@
 
 namespace lava {
 
+// MW wavefronts along the rows, two along the channels.
 template <int MW, int WM, int WN, int ST, bool GATED>
-__global__ void __launch_bounds__(128 * MW, MW == 2 && ST * (WM + WN) <= 19 ? 2 : 1)
+__global__ void __launch_bounds__(128 * MW, MW == 2 || ST * (16 * WM * MW + 32 * WN) * TN_KB <= 80 * 1024 ? MW : 2)
     w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
     constexpr int WAVES = 2 * MW, BM = 16 * WM * MW, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
     constexpr int Q = WM * WN, R = WM + WN;               // of a wavefront: MFMAs of half a stage, fragments read beside them
@@ -248,13 +249,17 @@ int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
     return LAVA_HIP_OK;
 }
 
-// What a tile of 64 x 64, 64 x 128, 128 x 128 or 256 x 256 costs a CU: us before and behind the loop, and us each 128 bytes of K.
-// Fitted to the times of all four at 700 shapes of 40 to 8192 rows, 1024 to 20480 channels and K of 128 to 7168.
+// What a tile costs a CU: us before and behind the loop, us each 128 bytes of K, and, where a CU has several, the share of one at the
+// end in which CUs wait for others (a CU runs several of the small ones at once, one of the two largest).  Fitted to the times of
+// all five at 730 shapes of 40 to 8192 rows, 1024 to 20480 channels and K of 128 to 7168 and at 240 plans of 8 to 256 experts.
 constexpr struct {
     int bm, bn;
-    float fixed, stage;
-} W8_TILES[4] = {{64, 64, 0.9f, 0.25f}, {64, 128, 1.7f, 0.44f}, {128, 128, 5.f, 0.49f}, {256, 256, 15.f, 1.12f}};
-constexpr float W8_END = 0.31f;
+    float fixed, stage, end;
+} W8_TILES[W8_TILE_KINDS] = {{64, 64, 0.74f, 0.40f, 0.3f},
+                             {64, 128, 2.8f, 0.39f, 0.3f},
+                             {128, 128, 2.7f, 0.62f, 0.3f},
+                             {128, 256, 10.2f, 0.80f, 0.53f},
+                             {256, 256, 14.6f, 1.47f, 0.53f}};
 
 bool w8_tile_fits(const W8Args& a, int tile) {
     return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, W8_TILES[tile].bm, W8_TILES[tile].bn);
@@ -270,19 +275,19 @@ double w8_tile_count(const W8Args& a, int bm, int bn) {
     return (met > whole ? met : whole) * tn;
 }
 
-// The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and a third of one for the end.  Over those
-// shapes 1.4 % behind the best of the four (at worst a fifth, at K of 256 and below), over 200 plans of 8 to 256 experts 3 %.
-// us of {64 x 64, 64 x 128, 128 x 128, 256 x 256}, the rule's in brackets: 64 rows x 14336 x 4096 {[17.1], 22.4, 24.6, 54}, 333 rows
-// {47.7, 42.1, [38.6], 56}, 2048 x 4096 x 4096 {53.6, 51.3, [36.7], 49.6}, 4096 x 4096 x 4096 {103, 91, 70, [58.8]}, 5003 tokens and 4 of
-// 60 experts of 2048 x 1408 {168, 128, 130, [131]}, of 2816 x 2048 {304, 236, 228, [212]}.
+// The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and the end.  Over those shapes 0.5 % behind
+// the best of the five, over the plans 3.4 % (at worst half, at few tiles).  us of {64 x 64, 64 x 128, 128 x 128, 128 x 256, 256 x 256},
+// the rule's in brackets: 64 rows x 14336 x 4096 {[16.8], 22.4, 23.2, 32.8, 54}, 333 rows {47, 41.3, 38.6, [34.4], 55}, 2048 x 4096 x
+// 4096 {54, 51.9, 37.6, [35.9], 47}, 1024 rows {29.8, 26.1, [22.2], 29.4, 45.8}, 4096 rows {103, 86, 71, 68, [59.1]}; 5003 tokens and 4
+// of 60 experts of 2048 x 1408 {168, 129, [123], 116, 132}, of 2816 x 2048 {298, 235, 220, [207], 208}.
 int w8_tile_choice(const W8Args& a) {
     const double stages = (a.k + TN_KB - 1) / TN_KB;
     int best = -1;
     double least = 0;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W8_TILE_KINDS; ++i) {
         if (!w8_tile_fits(a, i)) continue;
         const double per_cu = w8_tile_count(a, W8_TILES[i].bm, W8_TILES[i].bn) / 256;
-        const double cost = (per_cu <= 1 ? 1 : per_cu + W8_END) * (W8_TILES[i].fixed + W8_TILES[i].stage * stages);
+        const double cost = (per_cu <= 1 ? 1 : per_cu + W8_TILES[i].end) * (W8_TILES[i].fixed + W8_TILES[i].stage * stages);
         if (best < 0 || cost < least) {
             best = i;
             least = cost;
@@ -293,12 +298,13 @@ int w8_tile_choice(const W8Args& a) {
 
 int launch_w8_tile(const W8Args& a, int tile, hipStream_t s) {
     // Where a CU has one tile at most, a stage more in flight; else more tiles a CU (128 x 128, us with 2 stages / 3: 1024 x 4096 x
-    // 4096, 256 tiles, 26.8 / 21.1; 2048 rows 36 / 41.6).
+    // 4096, 256 tiles, 26.7 / 22.1; 2048 rows 36.7 / 41.5).
     const bool lone = w8_tile_count(a, W8_TILES[tile].bm, W8_TILES[tile].bn) <= 256;
     switch (tile) {
     case 0: return lone ? launch_tile<2, 2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
     case 1: return lone ? launch_tile<2, 2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
-    case 2: return lone ? launch_tile<2, 4, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<2, 4, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
+    case 2: return lone ? launch_tile<4, 2, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 2, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
+    case 3: return launch_tile<4, 2, 8, 3>(a, s, "w8a8_tile_kernel<128,256>");
     default: return launch_tile<4, 4, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
     }
 }

@@ -32,7 +32,7 @@ def untouched(a):
     return (np.ascontiguousarray(a).view(np.uint8) == FILL).all()
 
 
-@pytest.fixture(params=range(7))
+@pytest.fixture(params=range(8))
 def choice(gpu, request):
     """Every kernel of the family: one that cannot take a call leaves it to the automatic choice."""
     gpu.set_kernel_override(gpu.FAMILY_W8A8, request.param)
@@ -235,7 +235,7 @@ def test_every_kernel_gives_the_same_bits(gpu, T, N, K, act, gated):
     lh = gpu
     x, xs, w, ws, bias = make(np.random.default_rng(11), T, N, K)
     got = {}
-    for c in range(7):
+    for c in range(8):
         announce(f"linear {T} x {N} x {K} {act}, choice {c}")
         lh.set_kernel_override(lh.FAMILY_W8A8, c)
         try:
