@@ -11,7 +11,7 @@
 //    accumulators;
 //  * the sums go through LDS to lanes that have 8 columns of a row, which they finish, round to Y's type and store.
 // Measured: 8192 rows x 28672 gated channels x 4096 730 to 790 us (2440 to 2640 TOP/s) on 256 x 256 tiles, whose matrix cores are 0.66
-// busy at a clock that falls to 1.8 GHz under them (with 4 wavefronts of 128 x 128 0.57 and 1.9, 760 to 780 us; 16384 rows x 8192 x 1024
+// busy at a clock that falls to 1.8 GHz under them (with 4 wavefronts of 128 x 128 each 0.57 and 1.9, 760 to 780 us; 16384 rows x 8192 x 1024
 // 181 us against 230); 16 rows x 14336 x 4096 11.6 us, 5.1 TB/s of weights; 64 tokens' 8 of 64 experts, gate and up of 2816 x 2048,
 // 64 us, 5.7 TB/s.  Between those, latency: of a tile's first requests and of its finish where K is short, of requests that miss
 // L2 (two or three stages in flight a workgroup).
@@ -22,13 +22,13 @@
 
 namespace lava {
 
-// MW wavefronts along the rows, two along the channels.
-template <int MW, int WM, int WN, int ST, bool GATED>
-__global__ void __launch_bounds__(128 * MW, MW == 2 || ST * (16 * WM * MW + 32 * WN) * TN_KB <= 80 * 1024 ? MW : 2)
+// MW wavefronts along the rows, NW along the channels.
+template <int MW, int NW, int WM, int WN, int ST, bool GATED>
+__global__ void __launch_bounds__(64 * MW * NW, MW * NW == 4 || ST * 16 * (WM * MW + WN * NW) * TN_KB > 80 * 1024 ? 2 : 4)
     w8a8_tile_kernel(W8Args a, int tiles_m, int tiles_n) {
-    constexpr int WAVES = 2 * MW, BM = 16 * WM * MW, BN = 32 * WN, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
+    constexpr int WAVES = MW * NW, BM = 16 * WM * MW, BN = 16 * WN * NW, XS = BM * TN_KB, STAGE = (BM + BN) * TN_KB;
     constexpr int Q = WM * WN, R = WM + WN;               // of a wavefront: MFMAs of half a stage, fragments read beside them
-    constexpr int XD = WM, D = WM + 2 * WN / MW;          // and its requests of a stage, those for X first
+    constexpr int XD = 2 * WM / NW, D = XD + 2 * WN / MW;         // and its requests of a stage, those for X first
     static_assert(WM % 2 == 0 && (!GATED || WN % 2 == 0), "rows are finished 32 at a time, gates and factors are blocks of 16");
     static_assert(WN == 2 || WN == 4 || WN == 8, "a power of two of lanes finishes a row");
     __shared__ __attribute__((aligned(1024))) uint8_t smem[ST * STAGE];
@@ -41,13 +41,13 @@ __global__ void __launch_bounds__(128 * MW, MW == 2 || ST * (16 * WM * MW + 32 *
     xcd_tile(blockIdx.x, tiles_m, tiles_n, 4, tm, tn);
     W8Tile tile;
     if (!w8_find(a, BM, tm, tile)) return;
-    const int wm = w >> 1, wn = w & 1;
+    const int wm = w / NW, wn = w % NW;
     const int half = a.n >> 1;
     const int col0 = tn * (GATED ? BN / 2 : BN);   // first column of Y
 
     // What the finish needs, requested first and held until then: of row threadIdx.x its scale and row of Y, of channel row
     // threadIdx.x its scale and bias.
-    static_assert(BM <= 128 * MW && BN <= 128 * MW, "a row and a channel a thread");
+    static_assert(BM <= 64 * WAVES && BN <= 64 * WAVES, "a row and a channel a thread");
     float held_xs = 0.f, held_ws = 0.f, held_bias = 0.f;
     int held_yr = -1;
     if (threadIdx.x < (unsigned)tile.rows) {
@@ -237,14 +237,14 @@ __global__ void __launch_bounds__(128 * MW, MW == 2 || ST * (16 * WM * MW + 32 *
     static_assert(WM <= 4 * EI, "four times");
 }
 
-template <int MW, int WM, int WN, int ST>
+template <int MW, int NW, int WM, int WN, int ST>
 int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
-    const int cols = (a.gated ? 16 : 32) * WN;
+    const int cols = (a.gated ? 8 : 16) * WN * NW;
     const int64_t tm = w8_row_tiles(a, 16 * MW * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;
     LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s would need %lld workgroups", name, (long long)(tm * tn));
     const dim3 grid((unsigned)(tm * tn));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(128 * MW), 0, s, a, (int)tm, (int)tn); };
-    a.gated ? go(w8a8_tile_kernel<MW, WM, WN, ST, true>) : go(w8a8_tile_kernel<MW, WM, WN, ST, false>);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * MW * NW), 0, s, a, (int)tm, (int)tn); };
+    a.gated ? go(w8a8_tile_kernel<MW, NW, WM, WN, ST, true>) : go(w8a8_tile_kernel<MW, NW, WM, WN, ST, false>);
     LAVA_LAUNCH_CHECK(name);
     return LAVA_HIP_OK;
 }
@@ -278,7 +278,7 @@ double w8_tile_count(const W8Args& a, int bm, int bn) {
 // The least estimate: up to 256 tiles in the time of one, more in that of their share of a CU and the end.  Over those shapes 0.5 % behind
 // the best of the five, over the plans 3.4 % (at worst half, at few tiles).  us of {64 x 64, 64 x 128, 128 x 128, 128 x 256, 256 x 256},
 // the rule's in brackets: 64 rows x 14336 x 4096 {[16.8], 22.4, 23.2, 32.8, 54}, 333 rows {47, 41.3, 38.6, [34.4], 55}, 2048 x 4096 x
-// 4096 {54, 51.9, 37.6, [35.9], 47}, 1024 rows {29.8, 26.1, [22.2], 29.4, 45.8}, 4096 rows {103, 86, 71, 68, [59.1]}; 5003 tokens and 4
+// 4096 {54, 51.9, 37.6, [35.9], 47}, 1024 rows {29.8, 26.1, [22.2], 29.4, 45.8}, 4096 rows {103, 86, 71, 64, [58]}; 5003 tokens and 4
 // of 60 experts of 2048 x 1408 {168, 129, [123], 116, 132}, of 2816 x 2048 {298, 235, 220, [207], 208}.
 int w8_tile_choice(const W8Args& a) {
     const double stages = (a.k + TN_KB - 1) / TN_KB;
@@ -301,11 +301,11 @@ int launch_w8_tile(const W8Args& a, int tile, hipStream_t s) {
     // 4096, 256 tiles, 26.7 / 22.1; 2048 rows 36.7 / 41.5).
     const bool lone = w8_tile_count(a, W8_TILES[tile].bm, W8_TILES[tile].bn) <= 256;
     switch (tile) {
-    case 0: return lone ? launch_tile<2, 2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
-    case 1: return lone ? launch_tile<2, 2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
-    case 2: return lone ? launch_tile<4, 2, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 2, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
-    case 3: return launch_tile<4, 2, 8, 3>(a, s, "w8a8_tile_kernel<128,256>");
-    default: return launch_tile<4, 4, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
+    case 0: return lone ? launch_tile<2, 2, 2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
+    case 1: return lone ? launch_tile<2, 2, 2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 2, 2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
+    case 2: return lone ? launch_tile<4, 2, 2, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 2, 2, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
+    case 3: return launch_tile<2, 4, 4, 4, 3>(a, s, "w8a8_tile_kernel<128,256>");
+    default: return launch_tile<4, 2, 4, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
     }
 }
 
