@@ -6,98 +6,162 @@
 namespace lava {
 
 namespace {
-constexpr int WG_TILE = 64, WG_K = 64, WG_PITCH = WG_K + 16;   // padded: the 16 rows of a fragment on distinct banks
-
-// 16 bytes of a row from byte k on, zeros from `end` on; any alignment.
-__device__ __forceinline__ uint4 load16(const int8_t* row, int k, int end) {
-    uint4 v = {0, 0, 0, 0};
-    if (k + 16 <= end) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else if (k < end) {
-        uint32_t word[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (k + i < end) word[i >> 2] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
-        v = uint4{word[0], word[1], word[2], word[3]};
-    }
+// 16 bytes of a row from byte at on, any alignment.
+__device__ __forceinline__ uint4 load16(const int8_t* row, int at) {
+    uint4 v;
+    __builtin_memcpy(&v, row + at, 16);
     return v;
+}
+// The same, zeros from byte k on.
+__device__ __forceinline__ uint4 load16(const int8_t* row, int at, int k) {
+    if (at + 16 <= k) return load16(row, at);
+    if (at >= k) return uint4{0, 0, 0, 0};
+    unsigned __int128 v = 0;
+    if (k >= 16) {   // the row's last 16 bytes, the first of them cut off
+        __builtin_memcpy(&v, row + k - 16, 16);
+        v >>= 8 * (at + 16 - k);
+    } else {
+        for (int i = k - 1; i >= at; --i) v = v << 8 | (uint8_t)row[i];
+    }
+    return __builtin_bit_cast(uint4, v);
 }
 }  // namespace
 
-// Any layout: 64 rows x 64 channels a workgroup of 4 wavefronts, K 64 at a time through registers and LDS, one 16x16x64
-// MFMA a wavefront and block of 16 channels.  Of a gated layer's 64 channels each second block of 16 is the other half's, so that a
-// lane holds a column's gate and its factor.  Bound by the latency of one chunk of K in flight: 333 rows x 14336 x 4096 72 us (540 TOP/s),
-// with rows of 4095 bytes 100; one row x 4096 x 4096 28 us.
+// Any layout: TILE rows x TILE channels a workgroup of 2 x 2 wavefronts, K bytes of K at a time through registers, which hold the next
+// ones during the MFMAs, and LDS.  Of a gated layer's channels each second block of 16 is the other half's, so that a lane holds a
+// column's gate and its factor.  Bound by the latency of one chunk of K in flight a workgroup and by rows that begin inside a
+// 16-byte word: 4096 x 4096 x 4095 150 us (917 TOP/s; of 4096 on the tiles 58), 16 rows x 14336 x 4095 22.8, one row x 4096 x 4095 18.
+template <int TILE, int K>
 __global__ void __launch_bounds__(256) w8a8_generic_kernel(W8Args a, int tiles_n) {
-    __shared__ __attribute__((aligned(16))) int8_t sx[WG_TILE * WG_PITCH], sw[WG_TILE * WG_PITCH];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    constexpr int PITCH = K + 16, F = TILE / 32;   // padded: the 16 rows of a fragment on distinct banks; fragments a wavefront
+    __shared__ __attribute__((aligned(16))) int8_t sx[TILE * PITCH], sw[TILE * PITCH];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w >> 1, wn = w & 1;
     const int tn = blockIdx.x % tiles_n;
     W8Tile tile;
-    if (!w8_find(a, WG_TILE, blockIdx.x / tiles_n, tile)) return;
+    if (!w8_find(a, TILE, blockIdx.x / tiles_n, tile)) return;
     const int half = a.n >> 1;
     // channel of row r of the weights' tile, and the column of Y it goes to
-    auto column = [&](int r) { return a.gated ? tn * 32 + (r >> 5) * 16 + (r & 15) : tn * WG_TILE + r; };
+    auto column = [&](int r) { return a.gated ? tn * (TILE / 2) + (r >> 5) * 16 + (r & 15) : tn * TILE + r; };
     const int8_t* wbase = a.w + (int64_t)tile.expert * a.expert_stride;
 
-    const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;   // what this thread stages: a row, 16 bytes of it
-    int xr = -1, yr;
-    if (r < tile.rows) w8_rows(a, tile, r, xr, yr);
-    const int8_t* xrow = a.x + (int64_t)(xr < 0 ? 0 : xr) * a.ldx;
-    const int col = column(r);
-    const bool wok = col < a.n_out;
-    const int8_t* wrow = wbase + (int64_t)(!wok ? 0 : a.gated && (r & 16) ? half + col : col) * a.ldw;
-
-    i32x4 acc[4];
+    // What this thread stages: 16 bytes of 4 rows of each; rows that are none are the first one, and not stored.
+    constexpr int ROWS = TILE * K / 16 / 256;
+    const int first = threadIdx.x / (K / 16), c = threadIdx.x % (K / 16) * 16;
+    const int8_t *xrow[ROWS], *wrow[ROWS];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = i32x4{0, 0, 0, 0};
-    for (int k0 = 0; k0 < a.k; k0 += WG_K) {
-        const uint4 vx = load16(xrow, k0 + c, xr < 0 ? 0 : a.k), vw = load16(wrow, k0 + c, wok ? a.k : 0);
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = first + i * (TILE / ROWS), col = column(r);
+        int xr = -1, yr;
+        if (r < tile.rows) w8_rows(a, tile, r, xr, yr);
+        xrow[i] = a.x + (int64_t)(xr < 0 ? 0 : xr) * a.ldx;
+        wrow[i] = wbase + (int64_t)(col >= a.n_out ? 0 : a.gated && (r & 16) ? half + col : col) * a.ldw;
+    }
+    uint4 vx[ROWS], vw[ROWS];
+    auto stage = [&]() __attribute__((always_inline)) {
         __syncthreads();
-        *reinterpret_cast<uint4*>(sx + r * WG_PITCH + c) = vx;
-        *reinterpret_cast<uint4*>(sw + r * WG_PITCH + c) = vw;
-        __syncthreads();
-        const int at = (lane & 15) * WG_PITCH + (lane >> 4) * 16;
-        const uint4 fx = *reinterpret_cast<const uint4*>(sx + 16 * w * WG_PITCH + at);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            acc[j] = Mfma16<int8_t>::run(*reinterpret_cast<const uint4*>(sw + 16 * j * WG_PITCH + at), fx, acc[j]);
+        for (int i = 0; i < ROWS; ++i) {
+            const int at = (first + i * (TILE / ROWS)) * PITCH + c;
+            *reinterpret_cast<uint4*>(sx + at) = vx[i];
+            *reinterpret_cast<uint4*>(sw + at) = vw[i];
+        }
+        __syncthreads();
+    };
+    i32x4 acc[F][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i)
+#pragma unroll
+        for (int j = 0; j < F; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    auto multiply = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < K / 64; ++u) {
+            const int at = (lane & 15) * PITCH + u * 64 + (lane >> 4) * 16;
+            uint4 fx[F], fw[F];
+#pragma unroll
+            for (int i = 0; i < F; ++i) {
+                fx[i] = *reinterpret_cast<const uint4*>(sx + (TILE / 2 * wm + 16 * i) * PITCH + at);
+                fw[i] = *reinterpret_cast<const uint4*>(sw + (TILE / 2 * wn + 16 * i) * PITCH + at);
+            }
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = Mfma16<int8_t>::run(fw[j], fx[i], acc[i][j]);
+        }
+    };
+    const int whole = a.k / K;
+    if (whole > 0) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            vx[i] = load16(xrow[i], c);
+            vw[i] = load16(wrow[i], c);
+        }
+    }
+    for (int n = 1; n <= whole; ++n) {
+        stage();
+        const int at = min(n, whole - 1) * K + c;   // no branch around the loads: the compiler would wait where it joins
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            vx[i] = load16(xrow[i], at);
+            vw[i] = load16(wrow[i], at);
+        }
+        multiply();
+    }
+    if (whole * K < a.k) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            vx[i] = load16(xrow[i], whole * K + c, a.k);
+            vw[i] = load16(wrow[i], whole * K + c, a.k);
+        }
+        stage();
+        multiply();
     }
 
-    // acc[j][i]: row 16 w + lane % 16, channel row 16 j + 4 (lane / 16) + i
-    const int m = 16 * w + (lane & 15);
-    if (m >= tile.rows) return;
-    w8_rows(a, tile, m, xr, yr);
-    if (yr < 0) return;
-    const float xs = a.xs[xr];
+    // acc[i][j][r]: row TILE / 2 wm + 16 i + lane % 16, channel row TILE / 2 wn + 16 j + 4 (lane / 16) + r
     const int64_t sbase = (int64_t)tile.expert * a.n;
-    auto value = [&](int j, int i) {
-        const int row = 16 * j + 4 * (lane >> 4) + i, cc = column(row);
-        const int64_t ch = sbase + (a.gated && (row & 16) ? half + cc : cc);
-        return cc < a.n_out ? w8_value(acc[j][i], xs, a.ws[ch], a.bias ? a.bias[ch] : 0.f) : 0.f;
-    };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (a.gated && (j & 1)) continue;
-        const int cc = column(16 * j + 4 * (lane >> 4));
-        if (cc >= a.n_out) continue;
-        float v[4];
+    for (int i = 0; i < F; ++i) {
+        const int m = TILE / 2 * wm + 16 * i + (lane & 15);
+        if (m >= tile.rows) continue;
+        int xr, yr;
+        w8_rows(a, tile, m, xr, yr);
+        if (yr < 0) continue;
+        const float xs = a.xs[xr];
+        auto value = [&](int j, int r) {
+            const int row = TILE / 2 * wn + 16 * j + 4 * (lane >> 4) + r, cc = column(row);
+            const int64_t ch = sbase + (a.gated && (row & 16) ? half + cc : cc);
+            return cc < a.n_out ? w8_value(acc[i][j][r], xs, a.ws[ch], a.bias ? a.bias[ch] : 0.f) : 0.f;
+        };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = w8_act(a.act, value(j, i));
-            if (a.gated) v[i] *= value(j | 1, i);
+        for (int j = 0; j < F; ++j) {
+            if (a.gated && (j & 1)) continue;
+            const int cc = column(TILE / 2 * wn + 16 * j + 4 * (lane >> 4));
+            if (cc >= a.n_out) continue;
+            float v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[r] = w8_act(a.act, value(j, r));
+                if (a.gated) v[r] *= value(j | 1, r);
+            }
+            w8_store(a, (int64_t)yr * a.ldy + cc, a.n_out - cc, v);
         }
-        w8_store(a, (int64_t)yr * a.ldy + cc, a.n_out - cc, v);
     }
 }
 
-int launch_w8_generic(const W8Args& a, hipStream_t s) {
-    const int64_t tiles_n = ((int64_t)a.n_out + (a.gated ? 31 : 63)) / (a.gated ? 32 : 64);
-    const int64_t blocks = w8_row_tiles(a, WG_TILE) * tiles_n;
+template <int TILE, int K>
+static int launch_generic(const W8Args& a, hipStream_t s) {
+    const int cols = a.gated ? TILE / 2 : TILE;
+    const int64_t tiles_n = ((int64_t)a.n_out + cols - 1) / cols, blocks = w8_row_tiles(a, TILE) * tiles_n;
     LAVA_REQUIRE(blocks <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "w8a8_generic_kernel would need %lld workgroups",
                  (long long)blocks);
-    hipLaunchKernelGGL(w8a8_generic_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a, (int)tiles_n);
+    hipLaunchKernelGGL((w8a8_generic_kernel<TILE, K>), dim3((unsigned)blocks), dim3(256), 0, s, a, (int)tiles_n);
     LAVA_LAUNCH_CHECK("w8a8_generic_kernel");
     return LAVA_HIP_OK;
+}
+
+// The large tile where every CU has one.  us of 64 x 64 / 128 x 128: 1024 x 4096 x 4095, 256 large tiles, 61 / 68; 333 x 14336 x 4095, 336,
+// 86 / 69; 2048 x 4096 x 1111 48 / 41; 200 x 14336 x 777, 224, 21 / 28.
+int launch_w8_generic(const W8Args& a, hipStream_t s) {
+    return w8_tile_count(a, 128, 128) > 256 ? launch_generic<128, 128>(a, s) : launch_generic<64, 256>(a, s);
 }
 
 namespace {
