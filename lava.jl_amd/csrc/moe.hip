@@ -7,12 +7,12 @@
 // compared as they are.  With one, and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the
 // choice tells apart lie nearer to each other than c's rounding may move them, the wavefront's tokens are done again in 64.
 // Bound by issue: 8 ranks of 256 experts in 8 groups with a bias take 28 us for 16384 tokens (0.3 TB/s of logits), of which
-// the few that are done again are the last 8; one token 6.
+// the few that are done again are the last 7; one token 6.
 //
 // Sorting: workgroup b has tokens [b * span, (b + 1) * span), counts its assignments per expert, and in a second launch
 // (in the same one where a workgroup has all tokens) adds the counts of the lower workgroups and places its own in
-// order: a stable counting sort without global atomics, the same in every run.  16384 tokens, 8 of 256: the second launch 10 us,
-// about half of it each workgroup's look at all 256 workgroups' counts (64 MB from L2 in all).
+// order: a stable counting sort without global atomics, the same in every run.  Every workgroup looks at all the others' counts, which
+// are bytes where they fit: 16384 tokens, 8 of 256, the second launch 6.8 us, with counts of 32 bits 10.2.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -34,8 +34,9 @@ constexpr int MOE_COLUMNS = 8;     // of a row that a thread sums
 struct Plan {   // what a kernel needs of a plan
     int32_t* offsets;   // null: none is written
     int32_t* order;
-    int32_t* counts;    // [workgroup][expert]
+    int32_t* counts;    // [workgroup][expert], or bytes, rows of whole words
     int tokens, experts, top_k, span;
+    int bytes;          // no count is above 255
 };
 
 // tokens a workgroup has
@@ -176,15 +177,6 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
     if (r.top_groups < r.groups) {
         // a group's best two: of a lane's experts, then over the lanes
         const int size = r.experts / r.groups, base = (threadIdx.x & 63) - lane;
-        auto best_two = [&](Real& b1, Real& b2, int lo, int hi) __attribute__((always_inline)) {
-            b1 = b2 = LEAST;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const Real o = lane * V + v >= lo && lane * V + v < hi ? c[v] : LEAST;
-                b2 = fmax(b2, fmin(b1, o));
-                b1 = fmax(b1, o);
-            }
-        };
         auto join = [&](Real& b1, Real& b2, int d) __attribute__((always_inline)) {
             const Real o1 = __shfl_xor(b1, d, 64), o2 = __shfl_xor(b2, d, 64);
             b2 = fmax(fmin(b1, o1), fmax(b2, o2));
@@ -196,17 +188,38 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
         for (int i = 0; i < GV; ++i) count[i] = LEAST;
         const int span = size / V;
         if (size % V == 0 && (span & (span - 1)) == 0) {   // whole lanes, a power of two of them: all groups at once
-            best_two(b1, b2, 0, r.experts);
+            b1 = b2 = LEAST;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {   // beyond the experts c is the least
+                b2 = fmax(b2, fmin(b1, c[v]));
+                b1 = fmax(b1, c[v]);
+            }
             for (int d = 1; d < span; d <<= 1) join(b1, b2, d);
             // at most L / span groups, so one a lane
             const Real o = __shfl(r.group_best == 2 ? b1 + b2 : b1, base + min(lane * span, L - 1), 64);
             count[0] = lane < r.groups ? o : LEAST;
-        } else {
+        } else {   // one group after another: its highest, then its highest without that one
             for (int g = 0; g < r.groups; ++g) {
-                best_two(b1, b2, g * size, (g + 1) * size);
+                const int lo = g * size, hi = lo + size;
+                auto highest = [&](int but) __attribute__((always_inline)) {
+                    Real m = LEAST;
 #pragma unroll
-                for (int d = 1; d < L; d <<= 1) join(b1, b2, d);
-                const Real o = r.group_best == 2 ? b1 + b2 : b1;
+                    for (int v = 0; v < V; ++v) {
+                        const int e = lane * V + v;
+                        m = fmax(m, e >= lo && e < hi && e != but ? c[v] : LEAST);
+                    }
+                    return all_max<L>(m);
+                };
+                Real o = highest(-1);
+                if (r.group_best == 2) {
+                    int at = L * V;
+#pragma unroll
+                    for (int v = V - 1; v >= 0; --v) {
+                        const int e = lane * V + v;
+                        at = e >= lo && e < hi && c[v] == o ? e : at;
+                    }
+                    o += highest(all_min<L>(at));
+                }
 #pragma unroll
                 for (int i = 0; i < GV; ++i) count[i] = g == i * L + lane ? o : count[i];
             }
@@ -343,9 +356,10 @@ __device__ void finish_plan(const Plan& p, const int32_t* ids, int b, int blocks
 struct SortShared {
     int32_t base[MOE_EXPERTS];
     int32_t tmp[MOE_WAVES];
-    int32_t part[2][MOE_THREADS];   // moe_place_kernel
 };
 static_assert(MOE_THREADS == MOE_EXPERTS, "a thread an expert");
+
+__host__ __device__ constexpr int byte_row(int experts) { return (experts + 3) & ~3; }
 
 }  // namespace
 
@@ -449,7 +463,12 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
     __syncthreads();   // the counts, and this workgroup's ids in memory
     const int all = threadIdx.x < (unsigned)p.experts ? sh.base[threadIdx.x] : 0;
     if (gridDim.x > 1) {
-        if (threadIdx.x < (unsigned)p.experts) p.counts[b * p.experts + threadIdx.x] = all;
+        if (p.bytes) {
+            if (threadIdx.x < (unsigned)byte_row(p.experts))
+                reinterpret_cast<uint8_t*>(p.counts)[b * byte_row(p.experts) + threadIdx.x] = (uint8_t)all;
+        } else if (threadIdx.x < (unsigned)p.experts) {
+            p.counts[b * p.experts + threadIdx.x] = all;
+        }
         return;
     }
     __syncthreads();
@@ -478,39 +497,59 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_count_kernel(const int32_t* _
     finish_plan(p, ids, 0, 1, 0, all, sh.base, below, sh.tmp);
 }
 
+// Adds the workgroups' counts, in front of this one's and all.  BYTES: four experts a load, both sums in one word (at most 256 * 255).
+template <bool BYTES>
 __global__ void __launch_bounds__(MOE_THREADS) moe_place_kernel(const int32_t* __restrict__ ids, Plan p) {
     extern __shared__ uint16_t below[];
     __shared__ SortShared sh;
-    // the counts of expert threadIdx.x % width, of every parts-th workgroup, 16 in flight
-    int width = 64;
-    while (width < p.experts) width <<= 1;
-    const int parts = MOE_THREADS / width, e = threadIdx.x & (width - 1), part = threadIdx.x / width;
-    int before = 0, all = 0;
-    if (e < p.experts) {
-        const int32_t* c = p.counts + e;
-        for (int b0 = part; b0 < (int)gridDim.x; b0 += 16 * parts) {
-            int n[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) n[i] = b0 + i * parts < (int)gridDim.x ? c[(b0 + i * parts) * p.experts] : 0;
+    constexpr int C = BYTES ? 4 : 1, MOST = 16;   // experts a thread; parts of the workgroups' rows that are read side by side
+    __shared__ uint32_t part[BYTES ? 1 : 2][C * MOE_THREADS];
+    const int mine = blockIdx.x, blocks = gridDim.x, words = BYTES ? byte_row(p.experts) / 4 : p.experts;
+    int width = 64 / C;
+    while (width < words) width <<= 1;
+    const int parts = min(MOST, MOE_THREADS / width), at = threadIdx.x & (width - 1), row = threadIdx.x / width;
+    uint32_t before[C] = {}, all[C] = {};
+    if (at < words && row < parts) {
+        for (int b0 = row; b0 < blocks; b0 += 16 * parts) {
+            uint32_t n[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                all += n[i];
-                if (b0 + i * parts < (int)blockIdx.x) before += n[i];
+                const int b = b0 + i * parts;
+                n[i] = b < blocks ? reinterpret_cast<const uint32_t*>(p.counts)[b * words + at] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool lower = b0 + i * parts < mine;
+                if constexpr (BYTES) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) all[c] += (n[i] >> 8 * c & 255u) * (lower ? 0x10001u : 0x10000u);
+                } else {
+                    all[0] += n[i];
+                    before[0] += lower ? n[i] : 0u;
+                }
             }
         }
     }
-    sh.part[0][threadIdx.x] = before;
-    sh.part[1][threadIdx.x] = all;
-    __syncthreads();
-    if (threadIdx.x < (unsigned)p.experts)
-        for (int i = 1; i < parts; ++i) {
-            before += sh.part[0][threadIdx.x + i * width];
-            all += sh.part[1][threadIdx.x + i * width];
+    if (row < parts) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            part[0][C * (row * width + at) + c] = all[c];
+            if constexpr (!BYTES) part[1][row * width + at] = before[c];
         }
-    else
-        before = all = 0;   // the other parts' are in theirs
+    }
     __syncthreads();
-    finish_plan(p, ids, blockIdx.x, gridDim.x, before, all, sh.base, below, sh.tmp);
+    uint32_t sum = 0, lower = 0;
+    if (threadIdx.x < (unsigned)p.experts) {
+        for (int i = 0; i < parts; ++i) {
+            sum += part[0][i * C * width + threadIdx.x];
+            if constexpr (!BYTES) lower += part[1][i * width + threadIdx.x];
+        }
+        if constexpr (BYTES) {
+            lower = sum & 0xffffu;
+            sum >>= 16;
+        }
+    }
+    finish_plan(p, ids, mine, blocks, (int)lower, (int)sum, sh.base, below, sh.tmp);
 }
 
 // A thread 8 columns of a token, of any alignment.  Bound by the bytes: 8 rows of 2048 bf16 for 8192 tokens 48.2 us, 6.3 TB/s (with 4
@@ -615,7 +654,10 @@ Plan plan_of(const lava_hip_moe_plan* plan) {
 size_t below_bytes(int experts) { return (size_t)MOE_WAVES * experts * sizeof(uint16_t); }
 
 int launch_place(const int32_t* ids, const Plan& p, int blocks, hipStream_t s) {
-    hipLaunchKernelGGL(moe_place_kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), below_bytes(p.experts), s, ids, p);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(MOE_THREADS), below_bytes(p.experts), s, ids, p);
+    };
+    p.bytes ? go(moe_place_kernel<true>) : go(moe_place_kernel<false>);
     LAVA_LAUNCH_CHECK("moe_place_kernel");
     return LAVA_HIP_OK;
 }
@@ -717,6 +759,7 @@ int lava_hip_moe_route(const lava_hip_moe_router* router, int dtype, const void*
     if (plan != nullptr) p = plan_of(plan);
     p.tokens = (int)tokens;
     p.span = tokens ? span_of(tokens) : MOE_SPAN;
+    p.bytes = p.span <= 255;   // a token has an expert once
     const int blocks = blocks_of(tokens);
     hipStream_t s = as_stream(stream);
     if (dtype == LAVA_HIP_F32) return launch_route<float>(r, logits, ldl, ids, weights, p, blocks, s);
