@@ -254,6 +254,24 @@ def test_experts(gpu, choice, i, sorted_):  # noqa: F811
     check_experts(run_experts(lh, *args), *args)
 
 
+@pytest.mark.parametrize("K", [65, 80])
+@pytest.mark.parametrize("sorted_", [(False, True), (True, False)])
+def test_experts_of_many_tiles(gpu, K, sorted_):
+    lh = gpu
+    announce(f"experts of many tiles, K = {K}, sorted={sorted_}")
+    ids, x, xs, w, ws, bias = experts_case(np.random.default_rng(20), 2000, 4, 2, 1100, K)
+    if not sorted_[0]:
+        x, xs = x[:2000], xs[:2000]
+    args = (ids, x, xs, w, ws, bias, "silu", True, "bf16", *sorted_)
+    for c in (0, 1):
+        lh.set_kernel_override(lh.FAMILY_W8A8, c)
+        try:
+            got = run_experts(lh, *args)
+        finally:
+            lh.set_kernel_override(lh.FAMILY_W8A8, 0)
+        check_experts(got, *args)
+
+
 @pytest.mark.parametrize("pad", [(16, 32, 4), (1, 0, 1), (0, 3, 0)])
 def test_experts_strides(gpu, choice, pad):  # noqa: F811
     lh = gpu
@@ -475,9 +493,9 @@ def test_two_layers_of_experts_at_once(gpu):
         st.close()
 
 
-@pytest.mark.parametrize("T,E,k", [(16500, 16, 4), (33000, 130, 2)])
+@pytest.mark.parametrize("T,E,k", [(16500, 16, 4), (33000, 130, 2), (66000, 7, 2)])
 def test_route_of_more_tokens_than_a_workgroup_has_at_once(gpu, T, E, k):
-    """Workgroups of 128 and 192 tokens."""
+    """Workgroups of 128, 192 and 320 tokens."""
     lh = gpu
     announce(f"route {T} tokens, {k} of {E}")
     x = np.random.default_rng(32).standard_normal((T, E)).astype(np.float32)

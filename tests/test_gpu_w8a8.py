@@ -229,6 +229,25 @@ def test_linear_shows_scales_that_are_not_finite(gpu, choice):
         np.testing.assert_array_equal(got[keep], good[keep])
 
 
+@pytest.mark.parametrize("T,N,K", [(2100, 2180, 97), (2180, 2100, 272), (40, 33000, 131), (2050, 2306, 15)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_linear_of_many_tiles(gpu, T, N, K, gated):
+    """More tiles than CUs, on the kernel the library chooses and on the generic one."""
+    lh = gpu
+    x, xs, w, ws, bias = make(np.random.default_rng(13), T, N, K)
+    want = ref.layer(x, xs, w, ws, bias, "relu", gated, "f16")
+    got = {}
+    for c in (0, 1):
+        announce(f"linear {T} x {N} x {K} gated={gated}, choice {c}")
+        lh.set_kernel_override(lh.FAMILY_W8A8, c)
+        try:
+            got[c] = run(lh, x, xs, w, ws, bias, "relu", gated, "f16", (K % 2, K % 3, 1))
+        finally:
+            lh.set_kernel_override(lh.FAMILY_W8A8, 0)
+        check(got[c], want, "f16")
+    np.testing.assert_array_equal(got[0].view(np.uint16), got[1].view(np.uint16))
+
+
 @pytest.mark.parametrize("T,N,K,act,gated", [(1, 128, 512, "silu", True), (16, 256, 256, "none", False), (40, 96, 128, "gelu_erf", False),
                                              (200, 384, 640, "gelu_tanh", True), (600, 512, 256, "silu", False)])
 def test_every_kernel_gives_the_same_bits(gpu, T, N, K, act, gated):
