@@ -95,7 +95,7 @@ __device__ __forceinline__ float w8_value(int32_t sum, float xs, float ws, float
     return __builtin_fmaf((float)sum * xs, ws, bias);
 }
 
-// The activations, each as a product of x with something between 0 and 1, without the cancellation of 1 - 1 at negative x.
+// The activations, without the cancellation of 1 - 1 at negative x.
 // v_exp_f32 and v_rcp_f32 are off by 1 ulp; the exponent's rounding adds |x| 2^-24.
 __device__ __forceinline__ float w8_act(int act, float x) {
     switch (act) {
@@ -103,7 +103,23 @@ __device__ __forceinline__ float w8_act(int act, float x) {
     case LAVA_HIP_ACT_SILU: return x * __builtin_amdgcn_rcpf(1.f + epi_exp(-x));
     case LAVA_HIP_ACT_GELU_TANH:   // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
         return x * __builtin_amdgcn_rcpf(1.f + epi_exp(-1.5957691216057308f * __builtin_fmaf(0.044715f * x * x, x, x)));
-    case LAVA_HIP_ACT_GELU_ERF: return 0.5f * x * erfcf(x * -0.7071067811865476f);
+    case LAVA_HIP_ACT_GELU_ERF: {
+        // max(x, 0) - |x| / 2 erfc(z), z = |x| / sqrt 2, which is t P(t) exp(-z^2), t = 1 / (1 + 0.4 z): P fitted by least squares to
+        // exp(z^2) erfc(z) / t for z up to 11.4, behind which the term is below the least float; 7.2e-8 of it off, with the roundings
+        // of 32 bits at |x| < 3 the result 5.5e-7.  (erfcf: a layer of 19350 rows x 2048 x 128 98 us against 68.)
+        const float a = fabsf(x) > 16.f ? 16.f : fabsf(x);   // NaN stays
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.28284271f, 1.f));
+        float p = 0.043427813f;
+        p = __builtin_fmaf(p, t, -0.15090661f);
+        p = __builtin_fmaf(p, t, 0.10587774f);
+        p = __builtin_fmaf(p, t, 0.062928755f);
+        p = __builtin_fmaf(p, t, 0.097026626f);
+        p = __builtin_fmaf(p, t, 0.1860581f);
+        p = __builtin_fmaf(p, t, 0.20375505f);
+        p = __builtin_fmaf(p, t, 0.22618327f);
+        p = __builtin_fmaf(p, t, 0.22564933f);
+        return fmaxf(x, 0.f) - 0.5f * a * (t * p) * __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+    }
     default: return x;
     }
 }
