@@ -712,7 +712,9 @@ int lava_hip_gemm_w8a8(const lava_hip_w8_layer* layer, const int8_t* X, const fl
  *   highest c, and only the top_groups highest runs stay;
  *   the top_k highest c are chosen, highest first; weight = p of the chosen, divided by the chosen ones' sum
  *   if renormalize, times scale.
- * Equal c or counts go to the lower number; c is compared in 64 bits where 32 do not tell two apart.  A logit of -inf, or a bias of
+ * Equal c or counts go to the lower number; c is compared in 64 bits where 32 do not tell two apart.  Without a bias experts, and
+ * runs that count their best one, are compared by x itself, which orders them as p does and tells apart p that are equal in 64 bits
+ * (a sigmoid's above 37); runs that count two are compared by the sum of p in any case.  A logit of -inf, or a bias of
  * -inf, masks its expert: where fewer than top_k are left, the rest of a token's experts are -1 with a weight of 0 (a run counts
  * its masked experts as -inf).  A token with a NaN or +inf among its logits or c has no experts (-1) and weights of NaN. */
 typedef struct lava_hip_moe_router {

@@ -3,9 +3,10 @@
 // Routing: L lanes of a wavefront (16 up to 128 experts, 32 up to 256, then 64) have a token, lane l the logits of experts
 // V l .. V l + V - 1, and take the highest one top_k times: a maximum over the lanes by rotations within 16 lanes, then the
 // lowest expert that has it.  (A token a wavefront costs more: of 64 lanes' reductions each is half as long again and serves one token instead of
-// four: 16384 tokens of 64 experts 20.0 us against 13.7.)  Without a bias the order of p is that of the logits, which are
-// compared as they are.  With one, and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the
-// choice tells apart lie nearer to each other than c's rounding may move them, the wavefront's tokens are done again in 64.
+// four: 16384 tokens of 64 experts 20.0 us against 13.7.)  Without a bias the order of p is that of the logits, by which
+// experts, and groups counted by their best, are then compared: p of two may be equal in 64 bits (sigmoids of 38 and 39).  With one,
+// and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the choice tells apart lie nearer to each
+// other than c's rounding may move them, the wavefront's tokens are done again in 64.
 // Bound by issue: 8 ranks of 256 experts in 8 groups with a bias take 28 us for 16384 tokens (0.3 TB/s of logits), of which
 // the few that are done again are the last 7; one token 6.
 //
@@ -53,7 +54,7 @@ int blocks_of(int64_t tokens) {
 struct Router {
     const float* bias;
     int experts, top_k, softmax, groups, top_groups, group_best, renormalize;
-    int by_logit;   // without a bias the logits' own order is the one asked for, of single experts and of groups counted by their best
+    int by_logit;   // nothing is compared by p: there is no bias, and groups are counted by their best or all stay
     float scale;
 };
 
@@ -130,14 +131,14 @@ __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 __device__ __forceinline__ float quotient(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ double quotient(double x) { return 1.0 / x; }
 
-// The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L] (and, where they are chosen
-// by their logits, those in xs); true unless 32 bits do not settle the order.  most: the largest finite |bias|.
+// The experts of the token that these L lanes have, highest first, rank r in lane r % L's sel[r / L] (and, where there is no bias,
+// their logits in xs); true unless 32 bits do not settle the order.  most: the largest finite |bias|.
 template <int L, int V, typename Real>
 __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], const float (&bias)[V], float most, int lane,
                                        int (&sel)[2], float (&xs)[2]) {
     constexpr bool SINGLE = sizeof(Real) == 4;
     constexpr Real LEAST = (Real)NONE;
-    const bool by_logit = r.by_logit;
+    bool by_logit = r.by_logit;
     Real c[V];
     Real near = 0;   // how near two c may be that 32 bits cannot tell apart, without the part that grows with c
     if (by_logit) {
@@ -251,7 +252,9 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
         for (int v = 0; v < V; ++v) {
             const int g = (int)(((float)(lane * V + v) + 0.5f) * inv);
             if (!(kept >> (g & 63) & 1)) c[v] = LEAST;
+            else if (r.bias == nullptr) c[v] = (Real)x[v];
         }
+        by_logit = r.bias == nullptr;   // from here on: single experts
     }
     sel[0] = sel[1] = -1;
     xs[0] = xs[1] = NONE;
@@ -281,7 +284,7 @@ __device__ __forceinline__ bool choose(const Router& r, const float (&x)[V], con
     return sure;
 }
 
-// Adds the tokens' assignments to counts (LDS) or places them: base[e] is the next free place of expert e's run.
+// Places the tokens' assignments: base[e] is the next free place of expert e's run.
 // Stable: 1024 assignments at a time, a thread each; its place is base + those of lower wavefronts + those of lower lanes.
 __device__ void place(const Plan& p, const int32_t* ids, int64_t first, int64_t last, int32_t* base, uint16_t* below) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, E = p.experts;
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
         // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
         // so that p of far masked or shut out experts, below the least float, does not make 0 / 0
         float weight[S], top = NONE, all = 0.f;
-        if (!r.by_logit) {
+        if (r.bias) {
 #pragma unroll
             for (int i = 0; i < S; ++i) xs[i] = sel[i] >= 0 ? (float)row[sel[i]] : NONE;
         }
