@@ -136,7 +136,8 @@ int lava_hip_release_workspaces(void);
  * K-split form), gemm_small_kernel<any> behind gemm_small_kernel and gemm_small_kernel<u8,any> behind
  * gemm_small_kernel<u8> (operands of any alignment), flash_fwd5_kernel<32> and flash_fwd6_kernel<32>
  * behind the name without <32> (32 queries a wavefront pair or group instead of 64), paged_tile_kernel<32>
- * behind paged_tile_kernel (32 rows a wavefront pair, 128 a tile). */
+ * behind paged_tile_kernel (32 rows a wavefront pair, 128 a tile), w8a8_tile_kernel<64,64,4> behind
+ * w8a8_tile_kernel<64,64> (4 stages in its ring) and the other tiles' likewise. */
 const char* lava_hip_kernel_log(void);
 void lava_hip_kernel_log_clear(void);
 

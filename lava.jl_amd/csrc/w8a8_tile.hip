@@ -300,13 +300,17 @@ int launch_w8_tile(const W8Args& a, int tile, hipStream_t s) {
     // Where a CU has one tile at most, a stage more in flight; else more tiles a CU (128 x 128, us with 2 stages / 3: 1024 x 4096 x
     // 4096, 256 tiles, 26.7 / 22.1; 2048 rows 36.7 / 41.5).
     const bool lone = w8_tile_count(a, W8_TILES[tile].bm, W8_TILES[tile].bn) <= 256;
+    // the log names a tile and its form with that many stages
+#define LAVA_W8_TILE(MW, NW, WM, WN, ST, TILE) \
+    launch_tile<MW, NW, WM, WN, ST>(a, s, "w8a8_tile_kernel<" TILE ">+w8a8_tile_kernel<" TILE "," #ST ">")
     switch (tile) {
-    case 0: return lone ? launch_tile<2, 2, 2, 2, 4>(a, s, "w8a8_tile_kernel<64,64>") : launch_tile<2, 2, 2, 2, 3>(a, s, "w8a8_tile_kernel<64,64>");
-    case 1: return lone ? launch_tile<2, 2, 2, 4, 3>(a, s, "w8a8_tile_kernel<64,128>") : launch_tile<2, 2, 2, 4, 2>(a, s, "w8a8_tile_kernel<64,128>");
-    case 2: return lone ? launch_tile<4, 2, 2, 4, 3>(a, s, "w8a8_tile_kernel<128,128>") : launch_tile<4, 2, 2, 4, 2>(a, s, "w8a8_tile_kernel<128,128>");
-    case 3: return launch_tile<2, 4, 4, 4, 3>(a, s, "w8a8_tile_kernel<128,256>");
-    default: return launch_tile<4, 2, 4, 8, 2>(a, s, "w8a8_tile_kernel<256,256>");
+    case 0: return lone ? LAVA_W8_TILE(2, 2, 2, 2, 4, "64,64") : LAVA_W8_TILE(2, 2, 2, 2, 3, "64,64");
+    case 1: return lone ? LAVA_W8_TILE(2, 2, 2, 4, 3, "64,128") : LAVA_W8_TILE(2, 2, 2, 4, 2, "64,128");
+    case 2: return lone ? LAVA_W8_TILE(4, 2, 2, 4, 3, "128,128") : LAVA_W8_TILE(4, 2, 2, 4, 2, "128,128");
+    case 3: return LAVA_W8_TILE(2, 4, 4, 4, 3, "128,256");
+    default: return LAVA_W8_TILE(4, 2, 4, 8, 2, "256,256");
     }
+#undef LAVA_W8_TILE
 }
 
 }  // namespace lava
