@@ -213,8 +213,10 @@ int run(const W8Args& a, void* stream) {
     hipStream_t s = as_stream(stream);
     const int pin = kernel_override(LAVA_HIP_FAMILY_W8A8);
     if (pin == 1) return launch_w8_generic(a, s);
-    if (w8_stream_fits(a) && (pin == 2 || (pin == 0 && w8_stream_preferred(a)))) return launch_w8_stream(a, s);
-    const int tile = pin >= 3 && w8_tile_fits(a, pin - 3) ? pin - 3 : w8_tile_choice(a);
+    if (pin >= 3 && w8_tile_fits(a, pin - 3)) return launch_w8_tile(a, pin - 3, s);
+    // a pinned tile that cannot take the call leaves it to the choice without a pin
+    if (w8_stream_fits(a) && (pin == 2 || w8_stream_preferred(a))) return launch_w8_stream(a, s);
+    const int tile = w8_tile_choice(a);
     return tile >= 0 ? launch_w8_tile(a, tile, s) : launch_w8_generic(a, s);
 }
 

@@ -122,6 +122,26 @@ def test_layouts_of_the_generic_kernel(gpu, pin, K, pad, offset):
     check(got, ref.layer(x, xs, w, ws, bias, "none", False, "f32"), "f32")
 
 
+@pytest.mark.parametrize("T,pin,ld,want", [(5, 7, 2 ** 23 - 16, 7), (5, 7, 2 ** 23, 2), (40, 7, 2 ** 23, 3), (40, 2, 2 ** 25, 2), (40, 2, 2 ** 27, 1),
+                                             (5, 3, 2 ** 25, 2), (40, 3, 2 ** 25, 1), (40, 6, 2 ** 25, 1)])
+def test_channels_that_a_kernel_cannot_span(gpu, T, pin, ld, want):
+    """Channels so far apart that a tile's would span 2 GiB: the pinned kernel is passed over for the one that runs without a pin."""
+    lh = gpu
+    announce(f"rows of weights {ld} bytes apart, {T} tokens, pin {pin}")
+    rng = np.random.default_rng(53)
+    x, w = rng.integers(-127, 128, (T, 128)).astype(np.int8), rng.integers(-127, 128, (2, 128)).astype(np.int8)
+    W, X, one, Y = lh.HIPDeviceArray("i8", (ld + 128,)), up(lh, x), up(lh, np.ones(T, np.float32)), blank(lh, "f32", T, 2)
+    for n in range(2):
+        lh._lib.call("lava_hip_memcpy_h2d", W.ptr + n * ld, w[n].ctypes.data, 128)
+    try:
+        _, log = ran(lh, pin, lambda: lh.w8a8_raw(lh.w8_layer_raw(W.ptr, one.ptr, 2, 128, ld), X.ptr, one.ptr, T, 128, "f32", Y.ptr, 2))
+        lh.synchronize()
+        assert log == names(want, False)
+        np.testing.assert_array_equal(Y.to_numpy().T, x.astype(np.float64) @ w.T.astype(np.float64))
+    finally:
+        W.close()
+
+
 # rows, channels, K and the pin whose kernel the library takes by itself, more tiles than CUs or not
 CHOSEN = [(1, 4096, 4096, 2, False), (16, 7168, 512, 2, False), (16, 7169, 512, 3, False), (17, 64, 512, 3, False),
           (16, 14336, 4096, 3, False), (40, 33000, 256, 3, True), (64, 28672, 4096, 4, False), (512, 4096, 2048, 4, False),
