@@ -151,7 +151,7 @@ template <int TILE, int K>
 static int launch_generic(const W8Args& a, hipStream_t s) {
     const int cols = a.gated ? TILE / 2 : TILE;
     const int64_t tiles_n = ((int64_t)a.n_out + cols - 1) / cols, blocks = w8_row_tiles(a, TILE) * tiles_n;
-    LAVA_REQUIRE(blocks <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "w8a8_generic_kernel would need %lld workgroups",
+    LAVA_REQUIRE(w8_launch_fits(a, TILE, cols, 256), LAVA_HIP_ERR_UNSUPPORTED, "w8a8_generic_kernel would need %lld workgroups",
                  (long long)blocks);
     hipLaunchKernelGGL((w8a8_generic_kernel<TILE, K>), dim3((unsigned)blocks), dim3(256), 0, s, a, (int)tiles_n);
     LAVA_LAUNCH_CHECK("w8a8_generic_kernel");

@@ -224,6 +224,11 @@ inline bool w8_spans_fit(const W8Args& a, int rows, int channels) {
     return a.ldx < lim && a.ldw < lim && xrows * a.ldx < lim && channels * a.ldw < lim;
 }
 
+// Whether a launch holds the tiles of bm rows and bn columns of Y: fewer than 2^32 threads.
+inline bool w8_launch_fits(const W8Args& a, int bm, int bn, int threads) {
+    return w8_row_tiles(a, bm) <= 0xffffffffll / threads / (((int64_t)a.n_out + bn - 1) / bn);
+}
+
 int launch_w8_generic(const W8Args& a, hipStream_t s);
 // Few rows (w8a8_stream.hip).
 bool w8_stream_fits(const W8Args& a);

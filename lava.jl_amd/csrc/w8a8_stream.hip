@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) w8a8_stream_kernel(W8Args a, int tiles_n)
     w8_store(a, (int64_t)s_yr[m] * a.ldy + col0 + c, cols_in - c, v);
 }
 
-bool w8_stream_fits(const W8Args& a) { return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, 16, 16); }
+bool w8_stream_fits(const W8Args& a) { return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, 16, 16) && w8_launch_fits(a, 16, 16, 256); }
 
 // Up to 16 rows (of a plan: on average of an expert's that has any) on fewer tiles of 64 x 64 than half the CUs: those take as long
 // as all CUs' would, as a CU reads HBM at some 25 bytes a ns at most.  us, here / on tiles: 16 rows x 4096 x 4096 7.2 / 9.2, x 4096 x
@@ -148,7 +148,6 @@ bool w8_stream_preferred(const W8Args& a) { return a.rows <= 16 * w8_met(a) && w
 
 int launch_w8_stream(const W8Args& a, hipStream_t s) {
     const int64_t tm = w8_row_tiles(a, 16), tn = ((int64_t)a.n_out + 15) / 16;
-    LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "w8a8_stream_kernel would need %lld workgroups", (long long)(tm * tn));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(256), 0, s, a, (int)tn); };
     a.gated ? go(w8a8_stream_kernel<true>) : go(w8a8_stream_kernel<false>);
     LAVA_LAUNCH_CHECK("w8a8_stream_kernel");

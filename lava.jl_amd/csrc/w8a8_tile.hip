@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(64 * MW * NW, MW * NW == 4 || ST * 16 * (WM * 
 template <int MW, int NW, int WM, int WN, int ST>
 int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
     const int cols = (a.gated ? 8 : 16) * WN * NW;
-    const int64_t tm = w8_row_tiles(a, 16 * MW * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;
-    LAVA_REQUIRE(tm * tn <= 0xffffff, LAVA_HIP_ERR_UNSUPPORTED, "%s would need %lld workgroups", name, (long long)(tm * tn));
+    const int64_t tm = w8_row_tiles(a, 16 * MW * WM), tn = ((int64_t)a.n_out + cols - 1) / cols;   // w8_tile_fits: of them few enough
     const dim3 grid((unsigned)(tm * tn));
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * MW * NW), 0, s, a, (int)tm, (int)tn); };
     a.gated ? go(w8a8_tile_kernel<MW, NW, WM, WN, ST, true>) : go(w8a8_tile_kernel<MW, NW, WM, WN, ST, false>);
@@ -253,16 +252,17 @@ int launch_tile(const W8Args& a, hipStream_t s, const char* name) {
 // end in which CUs wait for others (a CU runs several of the small ones at once, one of the two largest).  Fitted to the times of
 // all five at 730 shapes of 40 to 8192 rows, 1024 to 20480 channels and K of 128 to 7168 and at 240 plans of 8 to 256 experts.
 constexpr struct {
-    int bm, bn;
+    int bm, bn, threads;
     float fixed, stage, end;
-} W8_TILES[W8_TILE_KINDS] = {{64, 64, 0.74f, 0.40f, 0.3f},
-                             {64, 128, 2.8f, 0.39f, 0.3f},
-                             {128, 128, 2.7f, 0.62f, 0.3f},
-                             {128, 256, 10.2f, 0.80f, 0.53f},
-                             {256, 256, 14.6f, 1.47f, 0.53f}};
+} W8_TILES[W8_TILE_KINDS] = {{64, 64, 256, 0.74f, 0.40f, 0.3f},
+                             {64, 128, 256, 2.8f, 0.39f, 0.3f},
+                             {128, 128, 512, 2.7f, 0.62f, 0.3f},
+                             {128, 256, 512, 10.2f, 0.80f, 0.53f},
+                             {256, 256, 512, 14.6f, 1.47f, 0.53f}};
 
 bool w8_tile_fits(const W8Args& a, int tile) {
-    return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, W8_TILES[tile].bm, W8_TILES[tile].bn);
+    const auto& t = W8_TILES[tile];
+    return a.k > 0 && w8_chunks_fit(a) && w8_spans_fit(a, t.bm, t.bn) && w8_launch_fits(a, t.bm, a.gated ? t.bn / 2 : t.bn, t.threads);
 }
 
 double w8_met(const W8Args& a) { return a.offsets ? a.experts * -expm1(-(double)a.rows / a.experts) : 1; }

@@ -1,4 +1,5 @@
-"""Which kernel of the layers with 8-bit weights runs, read from the kernel log; and every tile with both of its rings of stages."""
+"""Which kernel of the layers with 8-bit weights runs, read from the kernel log; every tile with both of its rings of stages, and
+the largest numbers of channels and tokens."""
 import numpy as np
 import pytest
 
@@ -158,3 +159,80 @@ def test_the_kernel_that_is_chosen(gpu, T, N, K, pin, many):
     lh.synchronize()
     assert log == names(pin, many)
     assert (Y.to_numpy() == FILL * FILL * K).all()
+
+
+# ---- the largest -------------------------------------------------------------------------------
+
+MOST = 2 ** 31 - 256
+
+
+def put(lh, at, a):
+    lh._lib.call("lava_hip_memcpy_h2d", at, a.ctypes.data, a.nbytes)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_the_most_channels(gpu, gated):
+    """One token, K = 16: more tiles of 64 x 64 than a launch holds, so a wider tile runs."""
+    lh = gpu
+    announce(f"{MOST} channels, gated={gated}")
+    K, cols = 16, MOST // 2 if gated else MOST
+    rng = np.random.default_rng(54)
+    seen = np.array([0, 1, cols // 2, cols - 130, cols - 2, cols - 1])
+    x, w = rng.integers(-127, 128, K).astype(np.int8), rng.integers(-127, 128, (seen.size, K)).astype(np.int8)
+    W, S, Y = lh.HIPDeviceArray("i8", (MOST * K,)), lh.HIPDeviceArray("f32", (MOST,)), lh.HIPDeviceArray("f16", (cols,))
+    X, one = up(lh, x), up(lh, np.float32([2.0 ** -6]))
+    try:
+        W.fill_bytes(0)
+        S.fill_bytes(0x3c)
+        Y.fill_bytes(FILL)
+        s = float(np.array([0x3c3c3c3c], np.uint32).view(np.float32)[0])
+        for n, row in zip(seen, w):
+            put(lh, W.ptr + int(n) * K, row)
+            if gated:
+                put(lh, W.ptr + int(n + cols) * K, w[0])
+        lh.synchronize()
+        layer = lh.w8_layer_raw(W.ptr, S.ptr, MOST, K, K, gated=gated)
+        _, log = ran(lh, 0, lambda: lh.w8a8_raw(layer, X.ptr, one.ptr, 1, K, "f16", Y.ptr, cols))
+        lh.synchronize()
+        assert log == names(4, True)
+        got = Y.to_numpy()
+    finally:
+        for a in (W, S, Y):
+            a.close()
+    sums = w.astype(np.float64) @ x * 2.0 ** -6 * s
+    want = sums * sums[0] if gated else sums
+    assert (np.abs(got[seen] - want) <= np.abs(want) * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25).all()
+    got[seen] = 0
+    assert not got.any()
+
+
+def test_the_most_tokens(gpu):
+    """One channel: only tiles of 256 rows fit a launch."""
+    lh = gpu
+    announce(f"{MOST} tokens")
+    K = 16
+    rng = np.random.default_rng(55)
+    seen = np.array([0, 1, MOST // 2, MOST - 257, MOST - 1])
+    x, w = rng.integers(-127, 128, (seen.size, K)).astype(np.int8), rng.integers(-127, 128, (1, K)).astype(np.int8)
+    X, S, Y = lh.HIPDeviceArray("i8", (MOST * K,)), lh.HIPDeviceArray("f32", (MOST,)), lh.HIPDeviceArray("f16", (MOST,))
+    W, one = up(lh, w), up(lh, np.float32([0.5]))
+    try:
+        X.fill_bytes(0)
+        S.fill_bytes(0x3c)
+        Y.fill_bytes(FILL)
+        s = float(np.array([0x3c3c3c3c], np.uint32).view(np.float32)[0])
+        for t, row in zip(seen, x):
+            put(lh, X.ptr + int(t) * K, row)
+        lh.synchronize()
+        layer = lh.w8_layer_raw(W.ptr, one.ptr, 1, K, K)
+        _, log = ran(lh, 0, lambda: lh.w8a8_raw(layer, X.ptr, S.ptr, MOST, K, "f16", Y.ptr, 1))
+        lh.synchronize()
+        assert log == names(7, True)
+        got = Y.to_numpy()
+    finally:
+        for a in (X, S, Y):
+            a.close()
+    want = x.astype(np.float64) @ w[0] * 0.5 * s
+    assert (np.abs(got[seen] - want) <= np.abs(want) * (2.0 ** -11 + 2.0 ** -20) + 2.0 ** -25).all()
+    got[seen] = 0
+    assert not got.any()
