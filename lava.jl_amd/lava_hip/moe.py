@@ -12,6 +12,7 @@ from typing import Optional
 from . import _lib
 from .device import HIPDeviceArray
 from .kernels import _DCODE
+from .paged import _fits_size
 from .w8a8 import W8Layer, _code, _cut, _fits, _matrix, _scales
 
 _SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
@@ -30,6 +31,7 @@ def moe_plan_raw(tokens: int, experts: int, top_k: int, offsets: int, order: int
                  workspace_bytes: int = 0) -> _lib.MoePlanDesc:
     _fits(64, tokens=tokens)
     _fits(32, experts=experts, top_k=top_k)
+    _fits_size(workspace_bytes=workspace_bytes)
     return _lib.MoePlanDesc(tokens, experts, top_k, offsets or None, order or None, workspace or None, workspace_bytes)
 
 

@@ -24,6 +24,13 @@ def _fits(bits: int, **values: int) -> None:
             raise ValueError(f"{name} = {x} does not fit {bits} bits")
 
 
+def _fits_size(**values: int) -> None:
+    """Refuses a number of bytes that a size_t would cut off, or take a negative one for the largest there is."""
+    for name, x in values.items():
+        if not 0 <= x < 2 ** 64:
+            raise ValueError(f"{name} = {x} is no size")
+
+
 def paged_cache_raw(dtype: str, k: int, v: int, head_dim: int, page_size: int, heads: int, pages: int,
                     strides: Sequence[int]) -> _lib.KVCacheDesc:
     """Pages of keys at `k` and of values at `v`, both with element strides of (E, L, H, P)."""
@@ -40,6 +47,7 @@ def paged_batch_raw(sequences: int, tokens: int, q_start: int, kv_len: int, tabl
     max_pages)."""
     _fits(32, sequences=sequences, max_pages=max_pages)
     _fits(64, tokens=tokens, max_q=max_q)
+    _fits_size(workspace_bytes=workspace_bytes)
     return _lib.KVBatchDesc(sequences, max_pages, tokens, max_q, q_start, kv_len, table, workspace or None,
                             workspace_bytes)
 
