@@ -25,12 +25,12 @@ def _fits(bits: int, **values: int) -> None:
 
 
 def _cut(*values: int) -> bool:
-    """Whether a 64-bit argument would be cut off: their bits together leave the range where one does, unless a negative one
-    hides it, which the library refuses."""
+    """Whether a 64-bit argument may be cut off: the bits of all together leave the range where one does, or are negative where one
+    is, which would hide it."""
     together = 0
     for x in values:
         together |= x
-    return not -2 ** 63 <= together < 2 ** 63
+    return not 0 <= together < 2 ** 63
 
 
 def _code(dtype: str) -> int:
