@@ -180,9 +180,8 @@ static int launch_quantize(const void* X, int8_t* Q, float* scale, int64_t k, in
         if (ch <= 1) go(quantize_rows_kernel<T, N, 1>, N);
         else if (ch <= 2) go(quantize_rows_kernel<T, N, 2>, N);
         else if (ch <= 3) go(quantize_rows_kernel<T, N, 3>, N);
-        else if (ch <= 4) go(quantize_rows_kernel<T, N, 4>, N);
-        else if (ch <= 6) go(quantize_rows_kernel<T, N, 6>, N);
-        else go(quantize_rows_kernel<T, N, 8>, N);
+        else if (N == 64 || ch <= 4) go(quantize_rows_kernel<T, N, 4>, N);   // 64 lanes have at most 2048 values
+        else if constexpr (N > 64) ch <= 6 ? go(quantize_rows_kernel<T, N, 6>, N) : go(quantize_rows_kernel<T, N, 8>, N);
     };
     if (threads == 64) by_ch(std::integral_constant<int, 64>{});
     else if (threads == 256) by_ch(std::integral_constant<int, 256>{});
