@@ -670,11 +670,13 @@ int lava_hip_paged_workspace_bytes(const lava_hip_kv_cache* cache, const lava_hi
  *   scale[t] = max |x| / 127, Q[t][j] = the integer nearest to 127 x / max |x| (ties to even; of the real quotient, so no
  * rounding of a quotient or of the scale moves it), row t of Q at Q + t * ldq.  A row of zeros gives zeros and a scale of 0; a
  * row that holds an infinity or NaN gives zeros and a scale of NaN, so that what is computed from it shows.  Q and scale
- * do not overlap X.  Columns of Q from k on are left as they are. */
+ * do not overlap X.  Columns of Q from k on are left as they are.  One launch, of fewer than 2^32 threads: more than 2^26 - 4 rows of 1
+ * to 2048 values, 2^24 - 1 of up to 16384 (of none, of more than 65536), 2^22 - 1 of the lengths between are LAVA_HIP_ERR_UNSUPPORTED. */
 int lava_hip_quantize_i8(int x_dtype, const void* X, int8_t* Q, float* scale, int64_t k, int64_t tokens, int64_t ldx,
                          int64_t ldq, void* stream);
 
-/* x / (1 + exp(-x)); lava_hip_w8_layer takes it beside LAVA_HIP_ACT_NONE to LAVA_HIP_ACT_GELU_ERF. */
+/* x / (1 + exp(-x)); lava_hip_w8_layer takes it beside LAVA_HIP_ACT_NONE to LAVA_HIP_ACT_GELU_ERF.  As the formulas have it, this one
+ * and both GELU give NaN at -infinity (RELU 0); their results below zero and above -2^-119 may come out as 0. */
 #define LAVA_HIP_ACT_SILU 4
 
 /* A linear layer with 8-bit weights, or one for each of several experts: weight j of channel n of expert e is
@@ -700,7 +702,8 @@ typedef struct lava_hip_w8_layer {
  * 32-bit floating point in the order written, whichever kernel runs: its choice changes no bit of Y.  The fast kernels take
  * k, ldx and ldw (and an expert_stride) that are multiples of 16 and 16-byte aligned X and w whose rows of a tile span less than
  * 2 GiB (all tokens, where a plan gathers them); any other layout runs on a generic one, also on matrix instructions.  One
- * launch, no workspace.  Y overlaps no other operand. */
+ * launch, no workspace; the generic kernel's holds 2^24 - 1 tiles of 128 x 128 of Y (128 x 64 where gated; of a plan, an expert's last
+ * is a whole one), more are LAVA_HIP_ERR_UNSUPPORTED.  Y overlaps no other operand. */
 int lava_hip_gemm_w8a8(const lava_hip_w8_layer* layer, const int8_t* X, const float* x_scale, int64_t tokens, int64_t ldx,
                        int y_dtype, void* Y, int64_t ldy, void* stream);
 
@@ -754,7 +757,8 @@ int lava_hip_moe_plan_workspace_bytes(int64_t tokens, int32_t experts, int32_t t
 int lava_hip_moe_route(const lava_hip_moe_router* router, int dtype, const void* logits, int64_t ldl, int64_t tokens,
                        int32_t* ids, float* weights, const lava_hip_moe_plan* plan, void* stream);
 
-/* Writes the plan of given ids, (top_k, tokens). */
+/* Writes the plan of given ids, (top_k, tokens).  Ids of no expert are negative where lava_hip_moe_combine gets them too: it does not
+ * know how many experts there are. */
 int lava_hip_moe_sort(const int32_t* ids, const lava_hip_moe_plan* plan, void* stream);
 
 /* The experts' layers on the rows of a plan.  Row i of a run is token order[i] / top_k of X, or with LAVA_HIP_X_SORTED row i of
@@ -769,7 +773,8 @@ int lava_hip_experts_w8a8(const lava_hip_moe_plan* plan, const lava_hip_w8_layer
 
 /* out[t] = base[t] + sum over j of weights[t * top_k + j] * Y[t * top_k + j], rows of n values of one type (F16, BF16 or F32), in
  * 32 bits in the order of j, rounded once.  base may be NULL, or out itself with the same stride; Y overlaps out nowhere.  A
- * negative id's row of Y is not read (its weight counts times 0: a weight of NaN shows); ids NULL: every row is read. */
+ * negative id's row of Y is not read (its weight counts times 0: a weight of NaN shows); any other id's is, and with ids NULL every
+ * row.  tokens * ceil(n / 2048) of 2^24 and more are LAVA_HIP_ERR_UNSUPPORTED. */
 int lava_hip_moe_combine(int dtype, const void* Y, int64_t ldy, const int32_t* ids, const float* weights, int64_t tokens,
                          int32_t top_k, int64_t n, const void* base, int64_t ldb, void* out, int64_t ldo, void* stream);
 

@@ -7,13 +7,14 @@
 // experts, and groups counted by their best, are then compared: p of two may be equal in 64 bits (sigmoids of 38 and 39).  With one,
 // and for groups counted by two, c = p + bias is taken in 32 bits first; where two that the choice tells apart lie nearer to each
 // other than c's rounding may move them, the wavefront's tokens are done again in 64.
-// Bound by issue: 8 ranks of 256 experts in 8 groups with a bias take 28 us for 16384 tokens (0.3 TB/s of logits), of which
-// the few that are done again are the last 7; one token 6.
+// Bound by issue: 8 ranks of 256 experts in 8 groups with a bias take 29 to 33 us for 16384 tokens (0.5 TB/s of logits), of which
+// the few that are done again are the last 7; a decode step's 64 tokens of 64 experts with their plan 8.8, one token 8.2.
 //
 // Sorting: workgroup b has tokens [b * span, (b + 1) * span), counts its assignments per expert, and in a second launch
 // (in the same one where a workgroup has all tokens) adds the counts of the lower workgroups and places its own in
 // order: a stable counting sort without global atomics, the same in every run.  Every workgroup looks at all the others' counts, which
-// are bytes where they fit: 16384 tokens, 8 of 256, the second launch 6.8 us, with counts of 32 bits 10.2.
+// are bytes where they fit: 16384 tokens, 8 of 256, the second launch 6.8 us, with counts of 32 bits, which given ids need as one may
+// come any number of times, 10.8 (and 2.5 for the counts; 64 tokens 3.9).
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -419,7 +420,8 @@ __global__ void __launch_bounds__(MOE_THREADS) moe_route_kernel(Router r, const 
         if (__ballot(!sure) != 0) choose<L, V, double>(r, x, bias, most, lane, sel, xs);
 
         // the weights, from the chosen logits; divided by their sum they are taken relative to the highest logit among them,
-        // so that p of far masked or shut out experts, below the least float, does not make 0 / 0
+        // so that p of far masked or shut out experts, below the least float, does not make 0 / 0.  In 32 bits, the type of the weights,
+        // whose last bit that costs (measured 6e-8 off, rounded once from 64 bits 3e-8)
         float weight[S], top = NONE, all = 0.f;
         if (r.bias) {
 #pragma unroll

@@ -30,7 +30,8 @@ __device__ __forceinline__ uint4 load16(const int8_t* row, int at, int k) {
 // Any layout: TILE rows x TILE channels a workgroup of 2 x 2 wavefronts, K bytes of K at a time through registers, which hold the next
 // ones during the MFMAs, and LDS.  Of a gated layer's channels each second block of 16 is the other half's, so that a lane holds a
 // column's gate and its factor.  Bound by the latency of one chunk of K in flight a workgroup and by rows that begin inside a
-// 16-byte word: 4096 x 4096 x 4095 150 us (917 TOP/s; of 4096 on the tiles 58), 16 rows x 14336 x 4095 22.8, one row x 4096 x 4095 18.
+// 16-byte word.  us with K = 4095 / the other kernels with 4096: 4096 x 4096 149 (922 TOP/s) / 60, 333 x 14336 70 / 31, 16 x 14336 22.4 /
+// 11.6, 1 x 4096 19.9 / 6.0.
 template <int TILE, int K>
 __global__ void __launch_bounds__(256) w8a8_generic_kernel(W8Args a, int tiles_n) {
     constexpr int PITCH = K + 16, F = TILE / 32;   // padded: the 16 rows of a fragment on distinct banks; fragments a wavefront

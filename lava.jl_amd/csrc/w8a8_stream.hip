@@ -4,8 +4,8 @@
 // A workgroup has 16 rows and 16 channels (of a gated layer a gate's and their factors) over all of K, so that 4096 channels are 256
 // workgroups.  Its wavefronts take 256 bytes of K in turn, whole lines of 8 channels a load (and rows of X, from L2), straight
 // to the MFMA operand's registers: no LDS, no barrier until the end, four chunks in flight a wavefront.  The wavefronts' sums are
-// added in LDS, in whole numbers, so in any order.  One row x 4096 x 4096: 5.6 us in a row of calls, 3.0 TB/s; x 4096 x 14336 11.6 us,
-// 5.1 TB/s.
+// added in LDS, in whole numbers, so in any order.  One row x 4096 x 4096, calls in a row: 5.5 to 6.0 us, 2.8 to 3.0 TB/s; x 4096 x 14336
+// 11.6 to 12.4, 4.7 to 5.1 TB/s.
 #include "lds_dma.hpp"
 #include "w8a8.hpp"
 

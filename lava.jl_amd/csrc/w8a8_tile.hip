@@ -10,10 +10,10 @@
 //  * a gated layer's tile has 16 channels of the gate and their 16 factors in turn, so that a lane has both of a column in its
 //    accumulators;
 //  * the sums go through LDS to lanes that have 8 columns of a row, which they finish, round to Y's type and store.
-// Measured: 8192 rows x 28672 gated channels x 4096 730 to 790 us (2440 to 2640 TOP/s) on 256 x 256 tiles, whose matrix cores are 0.66
+// Measured: 8192 rows x 28672 gated channels x 4096 735 to 825 us (770 in the middle, 2500 TOP/s) on 256 x 256 tiles, whose matrix cores are 0.66
 // busy at a clock that falls to 1.8 GHz under them (with 4 wavefronts of 128 x 128 each 0.57 and 1.9, 760 to 780 us; 16384 rows x 8192 x 1024
-// 181 us against 230); 16 rows x 14336 x 4096 11.6 us, 5.1 TB/s of weights; 64 tokens' 8 of 64 experts, gate and up of 2816 x 2048,
-// 64 us, 5.7 TB/s.  Between those, latency: of a tile's first requests and of its finish where K is short, of requests that miss
+// 181 us against 230); 16 rows x 14336 x 4096 11.6 us, 5.1 TB/s of weights; 32 tokens' 8 of 64 experts, gates and factors of 2816 x 2048,
+// 65 us, 5.6 TB/s; one token's 11.0, 4.2 TB/s.  Between those, latency: of a tile's first requests and of its finish where K is short, of requests that miss
 // L2 (two or three stages in flight a workgroup).
 #include <math.h>
 

@@ -116,7 +116,7 @@ def moe_route(ids: HIPDeviceArray, weights: HIPDeviceArray, router: MoeRouter, l
 
 
 def moe_sort(plan: MoePlan, ids: HIPDeviceArray, stream: Optional[int] = None) -> MoePlan:
-    """The plan of given ids (top_k, T); numbers outside [0, experts) are no expert."""
+    """The plan of given ids (top_k, T); numbers outside [0, experts) are no expert (negative ones, if `moe_combine` gets them too)."""
     _matrix("ids", ids, ("i32",), plan.top_k, plan.tokens)
     moe_sort_raw(ids.ptr, plan.desc, stream)
     return plan

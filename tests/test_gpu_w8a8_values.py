@@ -59,6 +59,20 @@ def test_gelu_erf_over_all_numbers(gpu):
     assert not bad.any(), f"{bad.sum()} of {bad.size}, x = {a[bad][0]}, off {off[bad][0] / (y[bad][0] * U)} half steps"
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_silu_and_gelu_tanh_over_their_range(gpu, act):
+    """Within the bound that the layers' tests use; results below zero and above -2^-119 may be 0: 1 / (1 + exp) is below the least
+    normal float from 2^126 on, times |x| of up to 88."""
+    lh = gpu
+    announce(f"{act} over its range")
+    a = everywhere()
+    a = np.concatenate((a[a < 400], np.linspace(14, 130, 100001).astype(np.float32)))
+    x = np.concatenate((-a, a))
+    off = np.abs(activation(lh, act, x).astype(np.float64) - ref.act(act, x.astype(np.float64)))
+    bad = ~(off <= ref.act_error(act, x.astype(np.float64), 0.0) + (x < 0) * 2.0 ** -119 + 2.0 ** -148)
+    assert not bad.any(), f"{bad.sum()} of {bad.size}, x = {x[bad][0]}, off {off[bad][0]}"
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu_tanh", "gelu_erf", "silu"])
 def test_activations_of_infinities_zeros_and_nan(gpu, act):
     """As their formulas have them: a product of -infinity with zero is NaN, and +infinity stays."""
